@@ -350,6 +350,46 @@ TRITEIA_HIP_API int triteia_hip_dense(const void* x, long x_stride, const void* 
 TRITEIA_HIP_API int triteia_hip_pack_2_4(const void* weight, const void* scales, void* qweight, void* meta, void* meta_raw, int prob_k,
                          int prob_m, int dev, void* stream);
 
+/* ---- The attention side of a serving step (no counterpart in the reference). ----
+ *
+ * A cache: cache_k, cache_v [n_pages, kv_heads, page, dim] of the activations' type (kind 0), or codes of int8 (1) or e4m3 (2) with 32-bit
+ * k_scale, v_scale [n_pages, kv_heads, page]; the elements of a row are adjacent.  `strides`, 12 numbers in host memory: (page, head, slot) of
+ * cache_k, of cache_v (in elements), of k_scale, of v_scale.  Pages of 16, 32, .. 1024 tokens; slot = page * (tokens of a page) + offset.  Rows
+ * start on 16 bytes (kind 1, 2 outside attention: 8).  Activations are fp16, or bf16 with bf16 = 1.
+ *
+ * Queries and keys [tokens, heads, dim] with token and head strides: normalised per head (x * rsqrt(mean(x^2) + eps) * norm, where the norm
+ * is not null), their first `rot` elements rotated by row positions[t] of table [limit, rot / 2, 2] (float: cos, sin; positions null: not
+ * rotated; outside the table: NaN), pairs (i, i + rot / 2) or, interleaved, (2 i, 2 i + 1).  Queries go to q_out [tokens, heads, dim]; keys
+ * to k_out likewise (strides and v null), or, with k_out null, keys and values into the cache at slots[t] (outside it: not written).  8-bit rows get the
+ * scale max|x| / 127 or max|x| / 448.  positions and slots are int32, or int64 with positions64, slots64.  dim a multiple of 8 up to 256, rot of 16;
+ * rows of q, k, v start on 16 bytes. */
+TRITEIA_HIP_API int triteia_hip_rotary_cache(const void* q, long q_token, long q_head, const void* k, long k_token, long k_head, const void* v, long v_token,
+                             long v_head, void* q_out, void* k_out, int tokens, int heads, int kv_heads, int dim, int rot, const void* positions,
+                             int positions64, const void* table, long limit, int interleaved, const void* q_norm, const void* k_norm, float eps,
+                             const void* slots, int slots64, const void* cache_k, const void* cache_v, const void* k_scale, const void* v_scale,
+                             const long* strides, int n_pages, int page, int kind, int bf16, int dev, void* stream);
+/* Rows of the cache at slots[t] as values: k_out, v_out [tokens, kv_heads, dim]; zeros where a slot lies outside the cache. */
+TRITEIA_HIP_API int triteia_hip_cache_read(const void* cache_k, const void* cache_v, const void* k_scale, const void* v_scale, const long* strides, int n_pages,
+                             int kv_heads, int page, int dim, int kind, const void* slots, int slots64, int tokens, void* k_out, void* v_out, int bf16,
+                             int dev, void* stream);
+
+/* The work list of a batch, once for a forward pass: int32 q_starts [n_seqs + 1] (where each sequence's new tokens begin) and kv_lens [n_seqs]
+ * (tokens of its context, the new ones last) on the device; max_q: no sequence brings more new tokens (it chooses kernels, results do not
+ * depend on it).  Tokens behind q_starts[n_seqs] get zeros.  Up to 4096 sequences.  Sizes of the plan and of an attention call's scratch, both 16-byte
+ * aligned, contents irrelevant on entry; 0: sizes that are refused. */
+TRITEIA_HIP_API size_t triteia_hip_attention_plan_bytes(int n_seqs, int n_tokens, int heads, int kv_heads, int max_q);
+TRITEIA_HIP_API size_t triteia_hip_attention_scratch_bytes(int n_seqs, int n_tokens, int heads, int kv_heads, int max_q, int dim);
+TRITEIA_HIP_API int triteia_hip_attention_plan(const void* q_starts, const void* kv_lens, int n_seqs, int n_tokens, int heads, int kv_heads, int max_q, int causal,
+                             int window, void* plan, size_t plan_bytes, int dev, void* stream);
+/* out [n_tokens, heads, dim] = softmax(scale q k^T) v over the pages of each token's sequence, on a plan made with the same numbers.  causal: the
+ * last new token sees the whole context, each one before it a token less; window > 0: the last `window` of those.  Head h reads head
+ * h / (heads / kv_heads) of the cache.  pages int32 [n_seqs, table_width] with a row stride; a row without tokens to see gives zeros.  dim 64 or 128,
+ * scale positive; a page's scales of one head are adjacent and 16-byte aligned. */
+TRITEIA_HIP_API int triteia_hip_paged_attention(const void* q, long q_token, long q_head, void* out, const void* cache_k, const void* cache_v, const void* k_scale,
+                             const void* v_scale, const long* strides, int n_pages, int page, int kind, const void* pages, long pages_seq, int table_width,
+                             const void* plan, size_t plan_bytes, int n_seqs, int n_tokens, int heads, int kv_heads, int dim, int max_q, int causal,
+                             int window, float scale, void* scratch, size_t scratch_bytes, int bf16, int dev, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

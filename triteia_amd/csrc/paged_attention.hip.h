@@ -1,0 +1,703 @@
+// Attention of new tokens over a paged cache: out = softmax(scale q K^T, masked) V, per head, on a plan's items (attention_plan.hip.h).
+//
+// Pages [n_pages, kv_heads, page, D] of the activations' type, or of int8 / e4m3 codes with a 32-bit scale per row.  Row r of a tile is
+// token r / group of its sequence and head r % group of the cache head's group; with causal its last token is the sequence's
+// newest, a window keeps the last `window` tokens.  Both kernels work on the transposed product:
+//   S^T = K Q^T        an MFMA with tokens of the cache down and rows across, so a lane holds scores of ONE row and the softmax needs
+//                      one or two lane exchanges;
+//   O^T = V^T P^T      whose operand P^T is, in the accumulator's own layout, what the lane holds already: the order of the tokens inside an
+//                      MFMA's K is free as long as V has the same, and ds_read_b64_tr_b16 (_b8) takes four (eight) rows of any addresses and
+//                      hands a lane one column of them.  P never leaves the registers.
+// Scores, running maxima and sums and the output's sums are 32 bits; P is rounded once to the activations' type for the MFMA.  The maximum is
+// a reference that is only moved (and the sums rescaled) when a score passes it by 2^kAttnSlack: P <= 2^8 is far from the types' ends.
+// Masked scores are -infinity ahead of the maximum; a row that sees nothing has a sum of zero and gives zeros.  What is masked for some rows of
+// a tile and holds an infinity or a NaN in V must not reach those rows by 0 * inf: see attn_split.
+#pragma once
+#include "attention_plan.hip.h"
+#include "kv_cache.hip.h"
+
+namespace triteia_hip {
+
+typedef float attn_f4 __attribute__((ext_vector_type(4)));
+typedef float attn_f16 __attribute__((ext_vector_type(16)));
+typedef short attn_s4 __attribute__((ext_vector_type(4)));
+typedef int attn_i2 __attribute__((ext_vector_type(2)));
+
+constexpr float kAttnNone = -1e30f;     // below every score: the maximum of nothing
+constexpr float kAttnSlack = 8.f;
+
+struct AttendArgs {
+  const void* q;
+  long q_token, q_head;
+  void* out;                            // [tokens, heads, D]
+  CachePart ck, cv;
+  const int* pages;
+  long pages_seq;                       // stride
+  int n_pages, table_width, page_shift;
+  int group, kv_heads, causal, window;
+  float scale_log2;                     // scale * log2(e)
+  const int* plan;
+  AttnList list;
+  int which;
+  float *part_o, *part_ml;              // [parts][kv_heads][rows][D], [parts][kv_heads][rows][2]
+};
+
+template <class T>
+struct AttnMma;
+template <>
+struct AttnMma<_Float16> {
+  typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+  static constexpr uint32_t kInf = 0x7c00;
+  static __device__ __forceinline__ attn_f4 m16(v8 a, v8 b, attn_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ attn_f16 m32(v8 a, v8 b, attn_f16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct AttnMma<__bf16> {
+  typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+  static constexpr uint32_t kInf = 0x7f80;
+  static __device__ __forceinline__ attn_f4 m16(v8 a, v8 b, attn_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ attn_f16 m32(v8 a, v8 b, attn_f16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+
+// V with its infinities and NaNs taken out (`finite`), and numbers in their places whose sums over the tokens that a row sees, at most 64 of
+// them at a time, say which there were: 1 an infinity, 128 a negative one, 16384 a NaN.
+template <class T>
+__device__ __forceinline__ void attn_split(kv8<T> v, kv8<T>* finite, kv8<T>* marks) {
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const T x = v[j];          // (a bit cast of the vector's element itself would be one of its first)
+    const uint32_t b = __builtin_bit_cast(uint16_t, x), mag = b & 0x7fffu;
+    (*finite)[j] = mag >= AttnMma<T>::kInf ? (T)0.f : x;
+    (*marks)[j] = mag > AttnMma<T>::kInf ? (T)16384.f : mag < AttnMma<T>::kInf ? (T)0.f : (b >> 15) ? (T)128.f : (T)1.f;
+  }
+}
+__device__ __forceinline__ float attn_marked(float sum) {      // what those infinities and NaNs add up to
+  const int n = (int)sum, nan = n >> 14, minus = (n >> 7) & 127, plus = n & 127;
+  return nan || (minus && plus) ? __builtin_nanf("") : minus ? -__builtin_inff() : plus ? __builtin_inff() : 0.f;
+}
+
+// 8 codes as 8 values of the activations' type, exactly
+template <class T, int KIND>
+__device__ __forceinline__ kv8<T> attn_values(kv_uint2 c) {
+  kv8<T> out;
+  typedef T t2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      t2 pair;
+      if constexpr (KIND == kCacheFp8) {
+        if constexpr (__is_same(T, _Float16)) pair = j ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[i], 1.f, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[i], 1.f, false);
+        else pair = j ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[i], 1.f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[i], 1.f, false);
+      } else if constexpr (__is_same(T, _Float16)) {
+        // (code + 128 in the low bits of 1024, and 1152 taken off)
+        const uint32_t w = __builtin_amdgcn_perm(0x64646464u, c[i] ^ 0x80808080u, j ? 0x04030402u : 0x04010400u);
+        pair = __builtin_bit_cast(t2, w) - t2{(T)1152.f, (T)1152.f};
+      } else {
+        pair = t2{(T)(float)(int)(int8_t)(c[i] >> (16 * j)), (T)(float)(int)(int8_t)(c[i] >> (16 * j + 8))};
+      }
+      out[4 * i + 2 * j] = pair.x, out[4 * i + 2 * j + 1] = pair.y;
+    }
+  }
+  return out;
+}
+
+template <class T>
+__device__ __forceinline__ kv8<T> attn_transposed(const uint8_t* lds, int first, int second) {    // four rows at each
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  const t4 a = __builtin_bit_cast(t4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) attn_s4*)(lds + first)));
+  const t4 b = __builtin_bit_cast(t4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) attn_s4*)(lds + second)));
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+__device__ __forceinline__ AttnItem attn_item(const AttendArgs& a, int i) {
+  const int* p = a.plan + a.list.items + 8L * i;
+  return AttnItem{p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]};
+}
+
+// the page of a token, kept inside the table and the cache
+__device__ __forceinline__ long attn_page(const AttendArgs& a, int seq, int token) {
+  const int at = min(token >> a.page_shift, a.table_width - 1);
+  return (long)min((uint32_t)a.pages[seq * a.pages_seq + at], (uint32_t)(a.n_pages - 1));
+}
+
+// Which tokens row `r` of a tile sees: lo <= token < hi.  Rows behind the last see all that the tile sees and are not stored.
+struct AttnRow {
+  int lo, hi, token, head;     // token of the sequence, head of the group
+  bool live;
+};
+__device__ __forceinline__ AttnRow attn_row(const AttendArgs& a, const AttnItem& it, int rows, int r) {
+  const long row = (long)it.tile * rows + r;
+  AttnRow x;
+  x.token = (int)(row / a.group), x.head = (int)(row - (long)x.token * a.group);
+  x.live = x.token < it.n_tokens;
+  const int position = it.kv_len - it.n_tokens + x.token;
+  x.hi = x.live && a.causal ? min(position + 1, it.kv_len) : it.kv_len;
+  x.lo = x.live && a.window > 0 ? position - a.window + 1 : 0;
+  if (!x.live) x.token = 0, x.head = 0;
+  return x;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// Few rows: a decode step's heads, a handful of tokens.  Bound by the cache's bytes.  A workgroup takes a share of one tile's tokens; each of
+// its four wavefronts walks sub-tiles of its own (8 KB of K and 8 KB of V: 32 tokens of 128 elements in 16 bits, 64 in 8) with the next one's whole rows
+// on their way in registers and this one's in LDS of its own, so that the loop has no barrier; maxima, sums and outputs are joined once at the end.
+// grid: list.max_items * kv_heads, block 256
+template <class T, int KIND, int D, int NQ>
+__global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
+  using M = AttnMma<T>;
+  using v8 = typename M::v8;
+  constexpr int kRowBytes = D * (KIND == kCacheSame ? 2 : 1), kChunks = kRowBytes / 16;
+  constexpr int kSub = 8192 / kRowBytes < 64 ? 8192 / kRowBytes : 64;
+  constexpr int kLoads = kSub * kChunks / 64, kLoadRows = 64 / kChunks;     // requests of a sub-tile, rows of each
+  constexpr int kGroups = kSub / 16, kGroupLoads = kLoads / kGroups;
+  constexpr int kRows = 16 * NQ, kKeyRows = 256 / kRowBytes;
+  constexpr int kTile = kSub * kRowBytes;
+  constexpr int kStride = D + 4;                                             // floats of a row where the wavefronts meet
+  constexpr int kMeet = 4 * kRows * kStride * 4;
+  constexpr int kLds = 4 * 2 * kTile > kMeet ? 4 * 2 * kTile : kMeet;
+  __shared__ alignas(16) uint8_t lds[kLds];
+  __shared__ float meet_m[4][kRows], meet_l[4][kRows];
+  const int index = blockIdx.x / a.kv_heads, head = blockIdx.x - index * a.kv_heads;
+  if (index >= a.plan[2 * a.which]) return;
+  const AttnItem it = attn_item(a, index);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, h = lane >> 4;
+  uint8_t* lds_k = lds + wave * 2 * kTile;
+  uint8_t* lds_v = lds_k + kTile;
+
+  v8 qf[NQ][D / 32];
+  int row_lo[NQ], row_hi[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; n++) {
+    const AttnRow r = attn_row(a, it, kRows, 16 * n + col);
+    row_lo[n] = r.lo, row_hi[n] = r.hi;
+    const T* src = static_cast<const T*>(a.q) + (it.q_start + r.token) * a.q_token + (head * a.group + r.head) * a.q_head;
+#pragma unroll
+    for (int s = 0; s < D / 32; s++) {
+      const int d = KIND == kCacheSame ? 32 * s + 8 * h : 64 * (s / 2) + 16 * h + 8 * (s % 2);
+      qf[n][s] = r.live ? *reinterpret_cast<const v8*>(src + d) : v8{0, 0, 0, 0, 0, 0, 0, 0};
+    }
+  }
+  // the tile's masks: no token ahead of `all_lo` or from `all_hi` on is hidden from some of its rows only
+  const AttnRow first = attn_row(a, it, kRows, 0);
+  const int last_row = (int)min((long)kRows, (long)it.n_tokens * a.group - (long)it.tile * kRows) - 1;
+  const AttnRow last = attn_row(a, it, kRows, last_row);
+  const int all_lo = last.lo, all_hi = first.hi;
+
+  const int n_sub = (it.kv_end - it.kv_begin + kSub - 1) / kSub;
+  kv_uint4 rk[kLoads], rv[kLoads];
+  attn_f4 ks[kGroups], vs[kGroups];
+  const int load_row = lane / kChunks, load_chunk = lane % kChunks;
+  auto request = [&](int t0) {
+#pragma unroll
+    for (int g = 0; g < kGroups; g++) {
+      const int token = min(t0 + 16 * g, (it.kv_end - 1) & ~15);
+      const long page = attn_page(a, it.seq, token);
+      const int slot = token & ((1 << a.page_shift) - 1);
+      const uint8_t* pk = static_cast<const uint8_t*>(a.ck.data) + (page * a.ck.page + head * a.ck.head + (slot + load_row) * a.ck.slot) * (kRowBytes / D) + 16 * load_chunk;
+      const uint8_t* pv = static_cast<const uint8_t*>(a.cv.data) + (page * a.cv.page + head * a.cv.head + (slot + load_row) * a.cv.slot) * (kRowBytes / D) + 16 * load_chunk;
+#pragma unroll
+      for (int j = 0; j < kGroupLoads; j++) {
+        rk[g * kGroupLoads + j] = *reinterpret_cast<const kv_uint4*>(pk + (long)j * kLoadRows * a.ck.slot * (kRowBytes / D));
+        rv[g * kGroupLoads + j] = *reinterpret_cast<const kv_uint4*>(pv + (long)j * kLoadRows * a.cv.slot * (kRowBytes / D));
+      }
+      if constexpr (KIND != kCacheSame) {
+        ks[g] = *reinterpret_cast<const attn_f4*>(a.ck.scale + page * a.ck.scale_page + head * a.ck.scale_head + slot + 4 * h);
+        vs[g] = *reinterpret_cast<const attn_f4*>(a.cv.scale + page * a.cv.scale_page + head * a.cv.scale_head + slot + 4 * h);
+      }
+    }
+  };
+  auto key_of = [](int row) { return (row / kKeyRows) & (kChunks - 1); };
+  auto key_of_v = [](int row) {
+    return KIND == kCacheSame ? (row / kKeyRows << 1) & (kChunks - 1) : ((row / kKeyRows) & (kChunks / 2 - 1)) | ((row >> 4) & 1) * (kChunks / 2);
+  };
+
+  attn_f4 o[NQ][D / 16];
+  float m[NQ], l[NQ], norm = 0.f;           // norm: of the scales of V, so that P times a scale stays inside fp16
+#pragma unroll
+  for (int n = 0; n < NQ; n++) {
+    m[n] = kAttnNone, l[n] = 0.f;
+#pragma unroll
+    for (int d = 0; d < D / 16; d++) o[n][d] = attn_f4{0.f, 0.f, 0.f, 0.f};
+  }
+  if (wave < n_sub) request(it.kv_begin + wave * kSub);
+  for (int sub = wave; sub < n_sub; sub += 4) {
+    const int t0 = it.kv_begin + sub * kSub;
+    if (t0 + kSub > it.kv_end) {             // tokens behind the last: whatever the page holds there must not meet a zero of P
+#pragma unroll
+      for (int j = 0; j < kLoads; j++)
+        if (t0 + j * kLoadRows + load_row >= it.kv_end) rv[j] = kv_uint4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int j = 0; j < kLoads; j++) {
+      const int row = j * kLoadRows + load_row;
+      *reinterpret_cast<kv_uint4*>(lds_k + row * kRowBytes + (load_chunk ^ key_of(row)) * 16) = rk[j];
+      *reinterpret_cast<kv_uint4*>(lds_v + row * kRowBytes + (load_chunk ^ key_of_v(row)) * 16) = rv[j];
+    }
+    attn_f4 ks_now[kGroups], vs_now[kGroups];
+    if constexpr (KIND != kCacheSame) {
+#pragma unroll
+      for (int g = 0; g < kGroups; g++) ks_now[g] = ks[g], vs_now[g] = vs[g];
+    }
+    if (sub + 4 < n_sub) request(t0 + 4 * kSub);
+
+    attn_f4 s[NQ][kGroups];
+#pragma unroll
+    for (int g = 0; g < kGroups; g++) {
+#pragma unroll
+      for (int n = 0; n < NQ; n++) s[n][g] = attn_f4{0.f, 0.f, 0.f, 0.f};
+      const int row = 16 * g + col;
+      if constexpr (KIND == kCacheSame) {
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) {
+          const v8 k = *reinterpret_cast<const v8*>(lds_k + row * kRowBytes + ((4 * i + h) ^ key_of(row)) * 16);
+#pragma unroll
+          for (int n = 0; n < NQ; n++) s[n][g] = M::m16(k, qf[n][i], s[n][g]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 64; i++) {
+          const kv_uint4 c = *reinterpret_cast<const kv_uint4*>(lds_k + row * kRowBytes + ((4 * i + h) ^ key_of(row)) * 16);
+          const v8 k0 = attn_values<T, KIND>(kv_uint2{c[0], c[1]}), k1 = attn_values<T, KIND>(kv_uint2{c[2], c[3]});
+#pragma unroll
+          for (int n = 0; n < NQ; n++) s[n][g] = M::m16(k1, qf[n][2 * i + 1], M::m16(k0, qf[n][2 * i], s[n][g]));
+        }
+      }
+    }
+    const bool edge = t0 < all_lo || t0 + kSub > min(all_hi, it.kv_end);
+    float grown = 1.f;                       // what the outputs are multiplied by for a larger norm
+    if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) {
+      float top = norm;
+#pragma unroll
+      for (int g = 0; g < kGroups; g++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (t0 + 16 * g + 4 * h + j < it.kv_end) top = fmaxf(top, vs_now[g][j]);
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      if (top > norm) grown = norm / top, norm = top;
+    }
+    v8 p[NQ][kSub / 32], seen[NQ][kSub / 32];
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+      float top = kAttnNone;
+#pragma unroll
+      for (int g = 0; g < kGroups; g++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          float x = s[n][g][j] * (KIND == kCacheSame ? a.scale_log2 : ks_now[g][j] * a.scale_log2);
+          const int token = t0 + 16 * g + 4 * h + j;
+          if (edge && (token < row_lo[n] || token >= min(row_hi[n], it.kv_end))) x = -__builtin_inff();
+          s[n][g][j] = x;
+          top = fmaxf(top, x);
+        }
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      float alpha = grown;
+      if (__any(top > m[n] + kAttnSlack)) {
+        const float next = fmaxf(m[n], top);
+        alpha *= __builtin_amdgcn_exp2f(m[n] - next);
+        l[n] *= __builtin_amdgcn_exp2f(m[n] - next);
+        m[n] = next;
+      }
+      if (__any(alpha != 1.f)) {
+#pragma unroll
+        for (int d = 0; d < D / 16; d++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) o[n][d][j] *= alpha;
+      }
+      const float inv = KIND != kCacheSame && __is_same(T, _Float16) ? 1.f / fmaxf(norm, 1e-30f) : 1.f;
+#pragma unroll
+      for (int g = 0; g < kGroups; g++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float e = __builtin_amdgcn_exp2f(s[n][g][j] - m[n]);
+          l[n] += e;
+          const int token = t0 + 16 * g + 4 * h + j;
+          const bool hidden = edge && (token < row_lo[n] || token >= min(row_hi[n], it.kv_end));
+          float w = e;
+          if constexpr (KIND != kCacheSame) w = hidden ? 0.f : e * (vs_now[g][j] * inv);
+          p[n][g / 2][4 * (g % 2) + j] = (T)w;
+          seen[n][g / 2][4 * (g % 2) + j] = hidden ? (T)0.f : (T)1.f;
+        }
+    }
+    // (a single limit for all rows, as one token's heads have, hides the same from all of them: V is zero there)
+    const bool mixed = edge && (t0 < all_lo || t0 + kSub > all_hi) && !(first.lo == last.lo && first.hi == last.hi && first.lo <= it.kv_begin && first.hi >= it.kv_end);
+    auto column = [&](int d, int b) {        // V of 32 tokens from 32 b on, as the MFMA's operand for columns 16 d ..
+      if constexpr (KIND == kCacheSame) {
+        const int row = 32 * b + 4 * h + col / 4, chunk = 2 * d + (col & 3) / 2, in = 8 * (col & 1);
+        return attn_transposed<T>(lds_v, row * kRowBytes + (chunk ^ key_of_v(row)) * 16 + in, (row + 16) * kRowBytes + (chunk ^ key_of_v(row + 16)) * 16 + in);
+      } else {
+        const int r = col / 2, row = 32 * b + 4 * h + (r & 3) + 16 * (r >> 2);
+        const attn_i2 c = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+            (__attribute__((address_space(3))) attn_i2*)(lds_v + row * kRowBytes + (d ^ key_of_v(row)) * 16 + 8 * (col & 1)));
+        return attn_values<T, KIND>(kv_uint2{(uint32_t)c.x, (uint32_t)c.y});
+      }
+    };
+#pragma unroll
+    for (int d = 0; d < D / 16; d++) {
+      attn_f4 marks[NQ];
+#pragma unroll
+      for (int n = 0; n < NQ; n++) marks[n] = attn_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int b = 0; b < kSub / 32; b++) {
+        v8 v = column(d, b), mark;
+        if (mixed) attn_split<T>(v, &v, &mark);
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+          o[n][d] = M::m16(v, p[n][b], o[n][d]);
+          if (mixed) marks[n] = M::m16(mark, seen[n][b], marks[n]);
+        }
+      }
+      if (mixed) {
+#pragma unroll
+        for (int n = 0; n < NQ; n++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) o[n][d][j] += attn_marked(marks[n][j]);
+      }
+    }
+  }
+
+  // the four wavefronts' results
+#pragma unroll
+  for (int n = 0; n < NQ; n++) {
+    l[n] += __shfl_xor(l[n], 16);
+    l[n] += __shfl_xor(l[n], 32);
+    if (h == 0) meet_m[wave][16 * n + col] = m[n], meet_l[wave][16 * n + col] = l[n];
+  }
+  __syncthreads();
+  float* meet = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int n = 0; n < NQ; n++) {
+    const int r = 16 * n + col;
+    const float top = fmaxf(fmaxf(meet_m[0][r], meet_m[1][r]), fmaxf(meet_m[2][r], meet_m[3][r]));
+    float f = __builtin_amdgcn_exp2f(m[n] - top);
+    if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) f *= norm;
+#pragma unroll
+    for (int d = 0; d < D / 16; d++) {
+      attn_f4 x = o[n][d];
+#pragma unroll
+      for (int j = 0; j < 4; j++) x[j] *= f;
+      *reinterpret_cast<attn_f4*>(meet + (wave * kRows + r) * kStride + 16 * d + 4 * h) = x;
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kRows * (D / 4); i += 256) {
+    const int r = i / (D / 4), d = 4 * (i % (D / 4));
+    if (r > last_row) break;
+    float top = fmaxf(fmaxf(meet_m[0][r], meet_m[1][r]), fmaxf(meet_m[2][r], meet_m[3][r])), sum = 0.f;
+    attn_f4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      sum += meet_l[w][r] * __builtin_amdgcn_exp2f(meet_m[w][r] - top);
+      x += *reinterpret_cast<const attn_f4*>(meet + (w * kRows + r) * kStride + d);
+    }
+    if (it.part < 0) {
+      const AttnRow row = attn_row(a, it, kRows, r);
+      typedef T t4 __attribute__((ext_vector_type(4)));
+      t4 y;
+#pragma unroll
+      for (int j = 0; j < 4; j++) y[j] = sum == 0.f ? (T)0.f : (T)(x[j] / sum);
+      *reinterpret_cast<t4*>(static_cast<T*>(a.out) + ((long)(it.q_start + row.token) * (a.kv_heads * a.group) + head * a.group + row.head) * D + d) = y;
+    } else {
+      const long at = ((long)it.part * a.kv_heads + head) * kRows + r;
+      *reinterpret_cast<attn_f4*>(a.part_o + at * D + d) = x;
+      if (d == 0) a.part_ml[2 * at] = top, a.part_ml[2 * at + 1] = sum;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// Many rows: prompts.  Bound by the matrix cores and the exponentials.  A workgroup takes 128 rows, 32 a wavefront (as columns of 32 x 32 x 16
+// MFMAs), and walks the share's tokens in blocks of 64 that all of it reads from LDS: two places, the next block on its way in registers,
+// one barrier a block.  Codes of 8 bits become values on their way to LDS.
+// grid: list.max_items * kv_heads, block 256
+template <class T, int KIND, int D>
+__global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a) {
+  using M = AttnMma<T>;
+  using v8 = typename M::v8;
+  constexpr int kRowBytes = 2 * D, kChunks = kRowBytes / 16, kKeyRows = 256 / kRowBytes;
+  constexpr int kTile = kAttnBlock * kRowBytes;
+  constexpr int kHeld = D * (KIND == kCacheSame ? 2 : 1), kHeldChunks = kHeld / 16;      // a row in the cache
+  constexpr int kLoads = 16 * kHeldChunks / 64, kLoadRows = 64 / kHeldChunks;            // of the wavefront's 16 tokens of a block
+  static_assert(kLoads >= 1, "16 tokens are a request at least");
+  __shared__ alignas(16) uint8_t lds[4 * kTile];                                         // K, V, K, V
+  __shared__ alignas(16) float scales[2][2][kAttnBlock];
+  __shared__ int odd[2][4];                                                              // infinities or NaNs among a wavefront's V
+  const int index = blockIdx.x / a.kv_heads, head = blockIdx.x - index * a.kv_heads;
+  if (index >= a.plan[2 * a.which]) return;
+  const AttnItem it = attn_item(a, index);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, h = lane >> 5;
+
+  const AttnRow mine = attn_row(a, it, kAttnTileRows, 32 * wave + col);
+  const T* q = static_cast<const T*>(a.q) + (it.q_start + mine.token) * a.q_token + (head * a.group + mine.head) * a.q_head;
+  v8 qf[D / 16];
+#pragma unroll
+  for (int s = 0; s < D / 16; s++) qf[s] = mine.live ? *reinterpret_cast<const v8*>(q + 16 * s + 8 * h) : v8{0, 0, 0, 0, 0, 0, 0, 0};
+  // the limits of the wavefront's and the tile's first and last rows: tokens between are the same for all of them
+  const int n_rows = (int)min((long)kAttnTileRows, (long)it.n_tokens * a.group - (long)it.tile * kAttnTileRows);
+  const int wave_last = min(32 * wave + 31, n_rows - 1);
+  const bool wave_live = 32 * wave < n_rows;
+  const AttnRow w0 = attn_row(a, it, kAttnTileRows, 32 * wave), w1 = attn_row(a, it, kAttnTileRows, max(wave_last, 0));
+  const AttnRow g0 = attn_row(a, it, kAttnTileRows, 0), g1 = attn_row(a, it, kAttnTileRows, n_rows - 1);
+
+  const int n_blocks = (it.kv_end - it.kv_begin + kAttnBlock - 1) / kAttnBlock;
+  kv_uint4 rk[kLoads], rv[kLoads];
+  float rs = 0.f;
+  const int load_row = lane / kHeldChunks, load_chunk = lane % kHeldChunks;
+  auto request = [&](int t0) {
+    const int token = min(t0 + 16 * wave, (it.kv_end - 1) & ~15);
+    const long page = attn_page(a, it.seq, token);
+    const int slot = token & ((1 << a.page_shift) - 1);
+    const uint8_t* pk = static_cast<const uint8_t*>(a.ck.data) + (page * a.ck.page + head * a.ck.head + (slot + load_row) * a.ck.slot) * (kHeld / D) + 16 * load_chunk;
+    const uint8_t* pv = static_cast<const uint8_t*>(a.cv.data) + (page * a.cv.page + head * a.cv.head + (slot + load_row) * a.cv.slot) * (kHeld / D) + 16 * load_chunk;
+#pragma unroll
+    for (int j = 0; j < kLoads; j++) {
+      rk[j] = *reinterpret_cast<const kv_uint4*>(pk + (long)j * kLoadRows * a.ck.slot * (kHeld / D));
+      rv[j] = *reinterpret_cast<const kv_uint4*>(pv + (long)j * kLoadRows * a.cv.slot * (kHeld / D));
+    }
+    if constexpr (KIND != kCacheSame) {
+      const int i = lane & 15;
+      rs = lane < 16 ? a.ck.scale[page * a.ck.scale_page + head * a.ck.scale_head + slot + i] * a.scale_log2
+                     : a.cv.scale[page * a.cv.scale_page + head * a.cv.scale_head + slot + i];
+    }
+  };
+  auto key_of = [](int row) { return (row / kKeyRows) & (kChunks - 1); };
+  auto key_of_v = [](int row) { return (row / kKeyRows << 2) & (kChunks - 1); };
+  // the registers' 16 tokens of the block at t0 into place `at`
+  auto keep = [&](int t0, int at) {
+    uint8_t* to_k = lds + at * 2 * kTile;
+    uint8_t* to_v = to_k + kTile;
+    if (t0 + kAttnBlock > it.kv_end) {       // tokens behind the last: whatever the page holds there must not meet a zero of P
+#pragma unroll
+      for (int j = 0; j < kLoads; j++)
+        if (t0 + 16 * wave + j * kLoadRows + load_row >= it.kv_end) rv[j] = kv_uint4{0, 0, 0, 0};
+    }
+    const bool edge = t0 < g1.lo || t0 + kAttnBlock > g0.hi;
+    bool strange = false;
+#pragma unroll
+    for (int j = 0; j < kLoads; j++) {
+      const int row = 16 * wave + j * kLoadRows + load_row;
+      if constexpr (KIND == kCacheSame) {
+        *reinterpret_cast<kv_uint4*>(to_k + row * kRowBytes + (load_chunk ^ key_of(row)) * 16) = rk[j];
+        *reinterpret_cast<kv_uint4*>(to_v + row * kRowBytes + (load_chunk ^ key_of_v(row)) * 16) = rv[j];
+        if (edge) {
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            strange |= (rv[j][i] & M::kInf) == M::kInf || (rv[j][i] >> 16 & M::kInf) == M::kInf;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          const int chunk = 2 * load_chunk + i;
+          *reinterpret_cast<v8*>(to_k + row * kRowBytes + (chunk ^ key_of(row)) * 16) = attn_values<T, KIND>(kv_uint2{rk[j][2 * i], rk[j][2 * i + 1]});
+          *reinterpret_cast<v8*>(to_v + row * kRowBytes + (chunk ^ key_of_v(row)) * 16) = attn_values<T, KIND>(kv_uint2{rv[j][2 * i], rv[j][2 * i + 1]});
+          if (KIND == kCacheFp8 && edge) {   // (e4m3 has one NaN and no infinity)
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+              for (int b = 0; b < 4; b++) strange |= (rv[j][2 * i + k] >> (8 * b) & 0x7f) == 0x7f;
+          }
+        }
+      }
+    }
+    const bool any = __any(strange);
+    if (lane == 0) odd[at][wave] = any;
+    if constexpr (KIND != kCacheSame) {
+      if (lane < 32) scales[at][lane / 16][16 * wave + (lane & 15)] = rs;
+    }
+  };
+
+  attn_f16 o[D / 32];
+#pragma unroll
+  for (int d = 0; d < D / 32; d++)
+#pragma unroll
+    for (int j = 0; j < 16; j++) o[d][j] = 0.f;
+  float m = kAttnNone, l = 0.f, norm = 0.f;
+
+  if (n_blocks > 0) {
+    request(it.kv_begin);
+    keep(it.kv_begin, 0);
+    if (n_blocks > 1) request(it.kv_begin + kAttnBlock);
+  }
+  __syncthreads();
+  for (int block = 0; block < n_blocks; block++) {
+    const int t0 = it.kv_begin + block * kAttnBlock, at = block & 1;
+    if (block + 1 < n_blocks) {
+      keep(t0 + kAttnBlock, at ^ 1);
+      if (block + 2 < n_blocks) request(t0 + 2 * kAttnBlock);
+    }
+    if (wave_live && t0 < min(w1.hi, it.kv_end) && t0 + kAttnBlock > w0.lo) {
+      const uint8_t* lds_k = lds + at * 2 * kTile;
+      const uint8_t* lds_v = lds_k + kTile;
+      attn_f16 s[2];
+#pragma unroll
+      for (int g = 0; g < 2; g++) {
+#pragma unroll
+        for (int j = 0; j < 16; j++) s[g][j] = 0.f;
+        const int row = 32 * g + col;
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) {
+          const v8 k = *reinterpret_cast<const v8*>(lds_k + row * kRowBytes + ((2 * i + h) ^ key_of(row)) * 16);
+          s[g] = M::m32(k, qf[i], s[g]);
+        }
+      }
+      const bool edge = t0 < w1.lo || t0 + kAttnBlock > min(w0.hi, it.kv_end);
+      float grown = 1.f;
+      if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) {
+        float top = t0 + lane < it.kv_end ? fmaxf(norm, scales[at][1][lane]) : norm;
+#pragma unroll
+        for (int d = 32; d > 0; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
+        if (top > norm) grown = norm / top, norm = top;
+      }
+      float top = kAttnNone;
+      const int lo = mine.lo - t0 - 4 * h, hi = min(mine.hi, it.kv_end) - t0 - 4 * h;
+#pragma unroll
+      for (int g = 0; g < 2; g++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+          const int token = 32 * g + 8 * (j / 4) + j % 4;
+          float x = s[g][j];
+          if constexpr (KIND != kCacheSame) x *= scales[at][0][token + 4 * h];
+          if (edge) x = token < lo || token >= hi ? -__builtin_inff() : x;
+          s[g][j] = x;
+          top = fmaxf(top, x);
+        }
+      if constexpr (KIND == kCacheSame) top = fmaxf(top * a.scale_log2, kAttnNone);
+      top = fmaxf(top, __shfl_xor(top, 32));
+      float alpha = grown;
+      if (__any(top > m + kAttnSlack)) {
+        const float next = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - next);
+        alpha *= f, l *= f, m = next;
+      }
+      if (__any(alpha != 1.f)) {
+#pragma unroll
+        for (int d = 0; d < D / 32; d++)
+#pragma unroll
+          for (int j = 0; j < 16; j++) o[d][j] *= alpha;
+      }
+      const float inv = KIND != kCacheSame && __is_same(T, _Float16) ? 1.f / fmaxf(norm, 1e-30f) : 1.f;
+      v8 p[4];
+#pragma unroll
+      for (int g = 0; g < 2; g++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+          const int token = 32 * g + 8 * (j / 4) + j % 4;
+          float e = __builtin_amdgcn_exp2f(KIND == kCacheSame ? __builtin_fmaf(s[g][j], a.scale_log2, -m) : s[g][j] - m);
+          l += e;
+          if constexpr (KIND != kCacheSame) {
+            e *= scales[at][1][token + 4 * h] * inv;
+            if (edge) e = token < lo || token >= hi ? 0.f : e;     // (a scale may be a NaN)
+          }
+          p[2 * g + j / 8][j % 8] = (T)e;
+        }
+      const int row = 4 * h + (lane & 15) / 4, in = 8 * (lane & 1);
+      auto column = [&](int d, int b) {      // V of 16 tokens from 16 b on, columns 32 d ..
+        const int chunk = 4 * d + 2 * (lane >> 4 & 1) + (lane & 3) / 2, r = 16 * b + row;
+        return attn_transposed<T>(lds_v, r * kRowBytes + (chunk ^ key_of_v(r)) * 16 + in, (r + 8) * kRowBytes + (chunk ^ key_of_v(r + 8)) * 16 + in);
+      };
+      if (edge && (odd[at][0] | odd[at][1] | odd[at][2] | odd[at][3])) {
+        v8 seen[4];
+#pragma unroll
+        for (int b = 0; b < 4; b++)
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            const int token = 16 * b + 8 * (j / 4) + j % 4;
+            seen[b][j] = token < lo || token >= hi ? (T)0.f : (T)1.f;
+          }
+#pragma unroll
+        for (int d = 0; d < D / 32; d++) {
+          attn_f16 marks;
+#pragma unroll
+          for (int j = 0; j < 16; j++) marks[j] = 0.f;
+#pragma unroll
+          for (int b = 0; b < 4; b++) {
+            v8 v = column(d, b), mark;
+            attn_split<T>(v, &v, &mark);
+            o[d] = M::m32(v, p[b], o[d]);
+            marks = M::m32(mark, seen[b], marks);
+          }
+#pragma unroll
+          for (int j = 0; j < 16; j++) o[d][j] += attn_marked(marks[j]);
+        }
+      } else {
+#pragma unroll
+        for (int d = 0; d < D / 32; d++)
+#pragma unroll
+          for (int b = 0; b < 4; b++) o[d] = M::m32(column(d, b), p[b], o[d]);
+      }
+    }
+    __syncthreads();
+  }
+  if (!mine.live || 32 * wave + col >= n_rows) return;
+  l += __shfl_xor(l, 32);
+  float f = 1.f;
+  if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) f = norm;
+  if (it.part < 0) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    f = l == 0.f ? 0.f : f / l;
+    T* out = static_cast<T*>(a.out) + ((long)(it.q_start + mine.token) * (a.kv_heads * a.group) + head * a.group + mine.head) * D + 4 * h;
+#pragma unroll
+    for (int d = 0; d < D / 32; d++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        t4 y;
+#pragma unroll
+        for (int j = 0; j < 4; j++) y[j] = (T)(o[d][4 * i + j] * f);
+        *reinterpret_cast<t4*>(out + 32 * d + 8 * i) = y;
+      }
+  } else {
+    const long at = ((long)it.part * a.kv_heads + head) * kAttnTileRows + 32 * wave + col;
+#pragma unroll
+    for (int d = 0; d < D / 32; d++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        attn_f4 y;
+#pragma unroll
+        for (int j = 0; j < 4; j++) y[j] = o[d][4 * i + j] * f;
+        *reinterpret_cast<attn_f4*>(a.part_o + at * D + 32 * d + 8 * i + 4 * h) = y;
+      }
+    if (h == 0) a.part_ml[2 * at] = m, a.part_ml[2 * at + 1] = l;
+  }
+}
+
+// Shares of one tile, added in their order.  grid (max_joins * kv_heads, rows / 16), block 256: a row's D / 4 lanes times the shares between them.
+template <class T, int D>
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
+  const int index = blockIdx.x / a.kv_heads, head = blockIdx.x - index * a.kv_heads;
+  if (index >= a.plan[2 * a.which + 1]) return;
+  const int* j = a.plan + a.list.joins + 8L * index;
+  const int q_start = j[0], n_tokens = j[1], tile = j[2], first = j[3], n_parts = j[4];
+  const int rows = a.list.rows;
+  constexpr int kLanes = D / 4, kPer = 256 / kLanes;
+  const int d = 4 * (threadIdx.x % kLanes);
+  for (int i = threadIdx.x / kLanes; i < 16; i += kPer) {
+    const int r = 16 * blockIdx.y + i;
+    const long row = (long)tile * rows + r;
+    const int token = (int)(row / a.group), g = (int)(row - (long)token * a.group);
+    if (token >= n_tokens) return;
+    const long step = (long)a.kv_heads * rows;
+    const long at = ((long)first * a.kv_heads + head) * rows + r;
+    float top = kAttnNone;
+    for (int p = 0; p < n_parts; p++) top = fmaxf(top, a.part_ml[2 * (at + p * step)]);
+    float sum = 0.f;
+    attn_f4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int p = 0; p < n_parts; p++) {
+      const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * (at + p * step)] - top);
+      sum += f * a.part_ml[2 * (at + p * step) + 1];
+      const attn_f4 y = *reinterpret_cast<const attn_f4*>(a.part_o + (at + p * step) * D + d);
+#pragma unroll
+      for (int k = 0; k < 4; k++) x[k] = __builtin_fmaf(y[k], f, x[k]);
+    }
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    t4 y;
+#pragma unroll
+    for (int k = 0; k < 4; k++) y[k] = sum == 0.f ? (T)0.f : (T)(x[k] / sum);
+    *reinterpret_cast<t4*>(static_cast<T*>(a.out) + ((long)(q_start + token) * (a.kv_heads * a.group) + head * a.group + g) * D + d) = y;
+  }
+}
+
+}  // namespace triteia_hip

@@ -8,6 +8,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 
 #include "dense_base.hip.h"
@@ -16,6 +17,7 @@
 #include "lora_mfma.hip.h"
 #include "lora_routed.hip.h"
 #include "pack.hip.h"
+#include "paged_attention.hip.h"
 #include "route_plan.hip.h"
 #include "sparse24_gemm.hip.h"
 #include "sparse24_ktile.hip.h"
@@ -2129,3 +2131,5 @@ int triteia_hip_pack_2_4(const void* weight, const void* scales, void* qweight, 
 }
 
 }  // extern "C"
+
+#include "attention_entry.hip.h"

@@ -69,6 +69,14 @@ SIGNATURES = {
     "triteia_hip_dense_tile": (_c_int, [_c_int] * 3),
     "triteia_hip_dense_scratch_bytes": (_c_sz, [_c_int] * 3),
     "triteia_hip_dense": (_c_int, [_c_vp, _c_long, _c_vp, _c_long, _c_vp] + [_c_int] * 3 + [_c_vp, _c_sz, _c_int, _c_vp]),
+    "triteia_hip_rotary_cache": (_c_int, [_c_vp, _c_long, _c_long] * 3 + [_c_vp] * 2 + [_c_int] * 5 + [_c_vp, _c_int, _c_vp, _c_long, _c_int]
+                                 + [_c_vp] * 2 + [_c_float, _c_vp, _c_int] + [_c_vp] * 5 + [_c_int] * 5 + [_c_vp]),
+    "triteia_hip_cache_read": (_c_int, [_c_vp] * 5 + [_c_int] * 5 + [_c_vp] + [_c_int] * 2 + [_c_vp] * 2 + [_c_int] * 2 + [_c_vp]),
+    "triteia_hip_attention_plan_bytes": (_c_sz, [_c_int] * 5),
+    "triteia_hip_attention_scratch_bytes": (_c_sz, [_c_int] * 6),
+    "triteia_hip_attention_plan": (_c_int, [_c_vp] * 2 + [_c_int] * 7 + [_c_vp, _c_sz, _c_int, _c_vp]),
+    "triteia_hip_paged_attention": (_c_int, [_c_vp, _c_long, _c_long] + [_c_vp] * 6 + [_c_int] * 3 + [_c_vp, _c_long, _c_int, _c_vp, _c_sz]
+                                    + [_c_int] * 8 + [_c_float, _c_vp, _c_sz] + [_c_int] * 2 + [_c_vp]),
     "triteia_hip_pack_2_4": (_c_int, [_c_vp] * 5 + [_c_int] * 3 + [_c_vp]),
 }
 
