@@ -43,8 +43,9 @@ CachePart cache_part(const void* data, const void* scale, const long* strides, c
 
 template <class T, int KIND, int LPR, int U>
 void launch_rotary(const RotaryArgs& a, int interleaved, hipStream_t stream) {
+  // small batches: a workgroup for every pass, so that all of them are on their way together; large ones: a workgroup walks whole tokens
   const int rows = a.heads + a.kv_heads * (a.v ? 2 : 1), per = 256 / LPR * U;
-  const dim3 grid((rows + per - 1) / per, a.tokens < 65535 ? a.tokens : 65535);
+  const dim3 grid(U == 1 ? (rows + per - 1) / per : 1, U == 1 ? a.tokens < 65535 ? a.tokens : 65535 : a.tokens < 2048 ? a.tokens : 2048);
   if (a.q_norm || a.k_norm) hipLaunchKernelGGL((rotary_cache_kernel<T, KIND, LPR, U, true>), grid, dim3(256), 0, stream, a, interleaved);
   else hipLaunchKernelGGL((rotary_cache_kernel<T, KIND, LPR, U, false>), grid, dim3(256), 0, stream, a, interleaved);
 }

@@ -23,6 +23,7 @@ enum CacheKind { kCacheSame = 0, kCacheInt8 = 1, kCacheFp8 = 2 };
 
 template <class T> using kv8 = T __attribute__((ext_vector_type(8)));
 typedef uint32_t kv_uint4 __attribute__((ext_vector_type(4)));
+typedef float kv_float4 __attribute__((ext_vector_type(4)));
 typedef uint32_t kv_uint2 __attribute__((ext_vector_type(2)));
 
 // Where row (page, head, slot) of a cache lies: offsets in elements (bytes in an 8-bit cache); the elements of a row are adjacent.
@@ -94,6 +95,21 @@ __device__ __forceinline__ void values_of(kv_uint2 c, float (&x)[8]) {
   }
 }
 
+template <int N> struct KvControl { static constexpr int value = N; };
+// The sum, or the largest, of a row's LPR lanes, in all of them: exchanges inside a quad, mirrors of 8 and of 16 lanes.
+template <int LPR, class V, class F>
+__device__ __forceinline__ V across_row(V v, F f) {
+  auto dpp = [](V x, auto control) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(control)::value, 0xf, 0xf, true));
+  };
+  v = f(v, dpp(v, KvControl<0xb1>{}));
+  v = f(v, dpp(v, KvControl<0x4e>{}));
+  v = f(v, dpp(v, KvControl<0x141>{}));
+  if constexpr (LPR >= 16) v = f(v, dpp(v, KvControl<0x140>{}));
+  if constexpr (LPR >= 32) v = f(v, __builtin_bit_cast(V, __shfl_xor(__builtin_bit_cast(int, v), 16)));
+  return v;
+}
+
 // One row of the cache: x[8] of each of the row's LPR lanes (`live`: the lane holds elements of the row).
 template <class T, int KIND, int LPR>
 __device__ __forceinline__ void cache_row(const CachePart& c, long page, long head, long slot, int e, bool live, const float (&x)[8]) {
@@ -108,8 +124,7 @@ __device__ __forceinline__ void cache_row(const CachePart& c, long page, long he
 #pragma unroll
     for (int j = 0; j < 8; j++) top = max(top, __builtin_bit_cast(uint32_t, x[j]) & 0x7fffffffu);
     if (!live) top = 0;
-#pragma unroll
-    for (int s = LPR / 2; s > 0; s /= 2) top = max(top, (uint32_t)__shfl_xor((int)top, s));
+    top = across_row<LPR>(top, [](uint32_t p, uint32_t q) { return max(p, q); });
     const float most = __builtin_bit_cast(float, top);
     float scale = most / (KIND == kCacheInt8 ? 127.f : 448.f), inv = 1.f / scale;
     if (most < 1e-30f) scale = 0.f, inv = 0.f;
@@ -127,97 +142,99 @@ __global__ __launch_bounds__(256) void rotary_cache_kernel(RotaryArgs a, int int
   const int lane = threadIdx.x % LPR, e = 8 * lane;
   const bool live = e < a.dim;
   const int n_rows = a.heads + a.kv_heads * (a.v ? 2 : 1);
-  for (long t = blockIdx.y; t < a.tokens; t += gridDim.y) {
-    const int row0 = blockIdx.x * (kRows * U) + threadIdx.x / LPR;
-    kv8<T> x[U];
+  const int half = a.rot / 2;
+  const bool turned = a.positions && e < a.rot, first = e < half;
+  const int across = interleaved || !turned ? lane : first ? lane + half / 8 : lane - half / 8;
+  const kv8<T> none = {0, 0, 0, 0, 0, 0, 0, 0};
+  kv8<T> w[2], wx[2];             // norm weights of this lane's elements and of those across, for q and k
+  if constexpr (NORM) {
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      const int r = row0 + u * kRows;
-      x[u] = kv8<T>{0, 0, 0, 0, 0, 0, 0, 0};
-      if (!live || r >= n_rows) continue;
-      const T* src = r < a.heads ? static_cast<const T*>(a.q) + t * a.q_token + r * a.q_head
-                     : r < a.heads + a.kv_heads ? static_cast<const T*>(a.k) + t * a.k_token + (r - a.heads) * a.k_head
-                                                : static_cast<const T*>(a.v) + t * a.v_token + (r - a.heads - a.kv_heads) * a.v_head;
-      x[u] = *reinterpret_cast<const kv8<T>*>(src + e);
+    for (int n = 0; n < 2; n++) {
+      const T* src = static_cast<const T*>(n ? a.k_norm : a.q_norm);
+      w[n] = src && live ? *reinterpret_cast<const kv8<T>*>(src + e) : none;
+      wx[n] = src && live ? *reinterpret_cast<const kv8<T>*>(src + 8 * across) : none;
+      if (interleaved) wx[n] = __builtin_shufflevector(w[n], w[n], 1, 0, 3, 2, 5, 4, 7, 6);
     }
+  }
+  for (long t = blockIdx.y; t < a.tokens; t += gridDim.y) {
     long page = 0, slot = -1;
     if (a.slots) {
       const long s = index_at(a.slots, a.slots64, t);
       if (s >= 0 && s < a.n_slots) page = s >> a.page_shift, slot = s & ((1 << a.page_shift) - 1);
     }
     // this lane's cos and sin: pairs e / 2 .. + 3 (interleaved) or e % (R / 2) .. + 7, minus in front of the sine of a pair's first element
-    const bool turned = a.positions && e < a.rot;
-    const int half = a.rot / 2;
-    const bool first = e < half;
     float c[8], s[8];
     if (turned) {
       const long p = index_at(a.positions, a.positions64, t);
       const bool inside = p >= 0 && p < a.limit;
-      const float* row = a.table + (inside ? p : 0) * a.rot;
       const int pair = interleaved ? e / 2 : first ? e : e - half;
-      const float outside = __builtin_nanf("");
+      const kv_float4* row = reinterpret_cast<const kv_float4*>(a.table + (inside ? p : 0) * a.rot + 2 * pair);
+      kv_float4 f[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) f[i] = i < 2 || !interleaved ? row[i] : kv_float4{0.f, 0.f, 0.f, 0.f};
+      if (!inside) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) f[i] = kv_float4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+      }
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        const int i = interleaved ? pair + j / 2 : pair + j;
-        c[j] = inside ? row[2 * i] : outside;
-        s[j] = inside ? row[2 * i + 1] : outside;
+        c[j] = interleaved ? f[j / 4][j / 2 % 2 * 2] : f[j / 2][j % 2 * 2];
+        s[j] = interleaved ? f[j / 4][j / 2 % 2 * 2 + 1] : f[j / 2][j % 2 * 2 + 1];
         if (interleaved ? j % 2 == 0 : first) s[j] = -s[j];
       }
     }
-    const int across = interleaved ? lane : !turned ? lane : first ? lane + half / 8 : lane - half / 8;
-    float w[2][8], wx[2][8];     // norm weights of this lane's elements and of those across, for q and k
-    if constexpr (NORM) {
+    for (int row0 = blockIdx.x * (kRows * U) + threadIdx.x / LPR; row0 < n_rows + (int)(threadIdx.x / LPR); row0 += gridDim.x * (kRows * U)) {
+      kv8<T> x[U];
 #pragma unroll
-      for (int n = 0; n < 2; n++) {
-        const T* src = static_cast<const T*>(n ? a.k_norm : a.q_norm);
+      for (int u = 0; u < U; u++) {
+        const int r = row0 + u * kRows;
+        const T* src = r < a.heads ? static_cast<const T*>(a.q) + t * a.q_token + r * a.q_head
+                       : r < a.heads + a.kv_heads ? static_cast<const T*>(a.k) + t * a.k_token + (r - a.heads) * a.k_head
+                                                  : static_cast<const T*>(a.v) + t * a.v_token + (r - a.heads - a.kv_heads) * a.v_head;
+        x[u] = live && r < n_rows ? *reinterpret_cast<const kv8<T>*>(src + e) : none;
+      }
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-          w[n][j] = src && live ? (float)src[e + j] : 1.f;
-          wx[n][j] = src && live ? (float)src[8 * across + j] : 1.f;
+      for (int u = 0; u < U; u++) {
+        const int r = row0 + u * kRows;
+        const bool is_q = r < a.heads, is_v = r >= a.heads + a.kv_heads;
+        float y[8], o[8];          // own elements, and those across
+        const kv_uint4 mine = __builtin_bit_cast(kv_uint4, x[u]);
+        kv8<T> xo;
+        if (interleaved) {
+          xo = __builtin_shufflevector(x[u], x[u], 1, 0, 3, 2, 5, 4, 7, 6);
+        } else {
+          kv_uint4 other;
+#pragma unroll
+          for (int i = 0; i < 4; i++) other[i] = (uint32_t)__shfl((int)mine[i], across, LPR);
+          xo = __builtin_bit_cast(kv8<T>, other);
         }
-      }
-    }
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      const int r = row0 + u * kRows;
-      const bool is_q = r < a.heads, is_v = r >= a.heads + a.kv_heads;
-      float y[8], o[8];          // own elements, and those across
-      const kv_uint4 mine = __builtin_bit_cast(kv_uint4, x[u]);
-      kv_uint4 other;
+        for (int j = 0; j < 8; j++) y[j] = (float)x[u][j], o[j] = (float)xo[j];
+        if constexpr (NORM) {
+          float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; i++) other[i] = (uint32_t)__shfl((int)mine[i], across, LPR);
-      const kv8<T> xo = __builtin_bit_cast(kv8<T>, other);
+          for (int j = 0; j < 8; j++) sum = __builtin_fmaf(y[j], y[j], sum);
+          sum = across_row<LPR>(sum, [](float p, float q) { return p + q; });
+          if (!is_v && (is_q ? a.q_norm : a.k_norm) != nullptr) {
+            const float f = __builtin_amdgcn_rsqf(sum / a.dim + a.eps);
+            const kv8<T> own = is_q ? w[0] : w[1], far = is_q ? wx[0] : wx[1];
 #pragma unroll
-      for (int j = 0; j < 8; j++) y[j] = (float)x[u][j], o[j] = interleaved ? (float)x[u][j ^ 1] : (float)xo[j];
-      if constexpr (NORM) {
-        float sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; j++) sum = __builtin_fmaf(y[j], y[j], sum);
-#pragma unroll
-        for (int d = LPR / 2; d > 0; d /= 2) sum += __shfl_xor(sum, d);
-        const bool normed = !is_v && (is_q ? a.q_norm : a.k_norm) != nullptr;
-        const float f = normed ? 1.f / __builtin_sqrtf(sum / a.dim + a.eps) : 1.f;
-        const int n = is_q ? 0 : 1;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const float wo = interleaved ? w[n][j ^ 1] : wx[n][j];
-          if (normed) y[j] = y[j] * f * w[n][j], o[j] = o[j] * f * wo;
+            for (int j = 0; j < 8; j++) y[j] = y[j] * f * (float)own[j], o[j] = o[j] * f * (float)far[j];
+          }
         }
-      }
-      if (turned && !is_v) {
+        if (turned && !is_v) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) y[j] = __builtin_fmaf(o[j], s[j], y[j] * c[j]);
-      }
-      const bool stored = live && r < n_rows;
-      if (r < n_rows && (is_q || a.k_out)) {
-        kv8<T> out;
+          for (int j = 0; j < 8; j++) y[j] = __builtin_fmaf(o[j], s[j], y[j] * c[j]);
+        }
+        if (r < n_rows && (is_q || a.k_out)) {
+          kv8<T> out;
 #pragma unroll
-        for (int j = 0; j < 8; j++) out[j] = (T)y[j];
-        T* dst = is_q ? static_cast<T*>(a.q_out) + (t * a.heads + r) * a.dim : static_cast<T*>(a.k_out) + (t * a.kv_heads + r - a.heads) * a.dim;
-        if (stored) *reinterpret_cast<kv8<T>*>(dst + e) = out;
-      } else if (r < n_rows && slot >= 0) {
-        const bool to_k = !is_v;
-        cache_row<T, KIND, LPR>(to_k ? a.ck : a.cv, page, to_k ? r - a.heads : r - a.heads - a.kv_heads, slot, e, live, y);
+          for (int j = 0; j < 8; j++) out[j] = (T)y[j];
+          T* dst = is_q ? static_cast<T*>(a.q_out) + (t * a.heads + r) * a.dim : static_cast<T*>(a.k_out) + (t * a.kv_heads + r - a.heads) * a.dim;
+          if (live) *reinterpret_cast<kv8<T>*>(dst + e) = out;
+        } else if (r < n_rows && slot >= 0) {
+          cache_row<T, KIND, LPR>(is_v ? a.cv : a.ck, page, is_v ? r - a.heads - a.kv_heads : r - a.heads, slot, e, live, y);
+        }
       }
     }
   }

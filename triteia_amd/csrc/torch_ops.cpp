@@ -18,6 +18,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/Event.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #define TORCH_CUDA_CPP_API TORCH_HIP_CPP_API   // (as the torch of this build names it, but for this header)
@@ -36,7 +37,7 @@ using at::Tensor;
 // path honours.  So may a transform's wrapper around a tensor, a dispatch mode and a trace: what they follow are torch's
 // operations, and a kernel launched from here would leave its result in them as a constant.
 struct Args {
-  static constexpr int kMax = 8;
+  static constexpr int kMax = 16;
   int n;
   const Tensor* tensors[kMax] = {};
   bool nones[kMax] = {};
@@ -432,9 +433,212 @@ PyObject* sparse(PyObject*, PyObject* const* v, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// --- the attention side: rotary positions, the paged cache, the attention over it ---
+
+// The arguments of these, which have numbers and truth values among them.  (Taken apart under the interpreter lock, as above.)
+struct MoreArgs : Args {
+  double numbers[kMax] = {};
+  bool given[kMax] = {};
+  at::ScalarType types[kMax] = {};
+  bool typed[kMax] = {};
+  MoreArgs(PyObject* const* values, Py_ssize_t count) : Args(values, count) {
+    for (int i = 0; i < n; i++) {
+      if (nones[i] || THPVariable_Check(values[i])) continue;
+      if (THPDtype_Check(values[i])) {
+        types[i] = reinterpret_cast<THPDtype*>(values[i])->scalar_type, typed[i] = true;
+        continue;
+      }
+      if (!PyLong_CheckExact(values[i]) && !PyFloat_CheckExact(values[i]) && !PyBool_Check(values[i])) continue;
+      numbers[i] = PyFloat_AsDouble(values[i]);
+      given[i] = !PyErr_Occurred();
+      PyErr_Clear();
+    }
+  }
+  bool whole(int i, double most = 2147483647.0) const { return i < n && given[i] && numbers[i] >= 0 && numbers[i] <= most && numbers[i] == (double)(int64_t)numbers[i]; }
+  int integer(int i) const { return (int)numbers[i]; }
+  bool maybe(int i) const { return none(i) || tensor(i); }
+  const Tensor* get(int i) const { return none(i) ? nullptr : tensors[i]; }
+  // a plain tensor of the GPU that records no gradient
+  bool plain(int i, const Tensor& ref) const {
+    return tensor(i) && (*this)[i].is_cuda() && (*this)[i].device() == ref.device() && (*this)[i].layout() == at::kStrided && !(*this)[i].is_neg() &&
+           !((*this)[i].requires_grad() && at::GradMode::is_enabled()) && !(*this)[i]._fw_grad(0).defined();
+  }
+};
+
+bool half_type(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
+const void* data(const Tensor* t) { return t ? t->data_ptr() : nullptr; }
+bool index_vector(const Tensor& t, int64_t count) {
+  return t.dim() == 1 && t.size(0) == count && t.is_contiguous() && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong);
+}
+// [tokens, heads, dim] that can be read 16 bytes at a time
+bool rows_ok(const Tensor& t, at::ScalarType type, int64_t tokens, int64_t dim) {
+  return t.dim() == 3 && t.scalar_type() == type && t.size(0) == tokens && t.size(2) == dim && t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
+         t.stride(0) >= 0 && t.stride(1) >= 0 && aligned(t);
+}
+
+// The four tensors of a PagedCache, which has checked them; what a program may have done to them since is checked again by the library.
+struct Cache {
+  const Tensor *k, *v, *ks, *vs;
+  long strides[12];
+  int n_pages, heads, page, dim, kind;
+  at::ScalarType type;
+  bool ok = false;
+  Cache(const MoreArgs& a, int i) {
+    if (!a.tensor(i) || !a.tensor(i + 1) || !a.maybe(i + 2) || !a.maybe(i + 3) || a.none(i + 2) != a.none(i + 3)) return;
+    k = a.get(i), v = a.get(i + 1), ks = a.get(i + 2), vs = a.get(i + 3);
+    if (k->dim() != 4 || v->dim() != 4 || v->sizes() != k->sizes() || !a.plain(i, *k) || !a.plain(i + 1, *k) || v->scalar_type() != k->scalar_type() ||
+        !sizes_ok({k->size(0), k->size(1), k->size(2), k->size(3)}) || k->size(0) * k->size(2) > 0x7fffffff)
+      return;
+    type = k->scalar_type();
+    kind = half_type(type) ? 0 : type == at::kChar ? 1 : type == at::kFloat8_e4m3fn ? 2 : 3;
+    if (kind == 3 || (kind == 0) != (ks == nullptr)) return;
+    for (int j = 0; j < 3; j++) strides[j] = k->stride(j), strides[3 + j] = v->stride(j);
+    for (int j = 0; j < 6; j++) strides[6 + j] = 0;
+    if (k->stride(3) != 1 || v->stride(3) != 1) return;
+    if (kind) {
+      if (!a.plain(i + 2, *k) || !a.plain(i + 3, *k)) return;
+      for (const Tensor* t : {ks, vs})
+        if (t->scalar_type() != at::kFloat || t->dim() != 3 || t->sizes() != k->sizes().slice(0, 3)) return;
+      for (int j = 0; j < 3; j++) strides[6 + j] = ks->stride(j), strides[9 + j] = vs->stride(j);
+    }
+    n_pages = (int)k->size(0), heads = (int)k->size(1), page = (int)k->size(2), dim = (int)k->size(3);
+    ok = true;
+  }
+  bool takes(at::ScalarType t) const { return half_type(t) && (kind != 0 || t == type); }
+};
+
+struct Outputs {
+  bool done = false;
+  Tensor first, second;
+};
+
+// rotary(q or None, k, v or None, positions or None, table or None, cache k, v and scales (or four None), slots or None, interleaved, norms or None, eps)
+Outputs rotary_cache(const MoreArgs& a) {
+  if (a.n != 14 || !a.tensor(1) || !a.maybe(0) || !a.maybe(2) || !a.maybe(3) || !a.maybe(4) || !a.maybe(9) || !a.whole(10, 1) || !a.maybe(11) || !a.maybe(12) || !a.given[13]) return {};
+  const Tensor& k = a[1];
+  if (!k.is_cuda() || k.dim() != 3 || !half_type(k.scalar_type())) return {};
+  const bool to_cache = !a.none(5);
+  const int64_t tokens = k.size(0), kv_heads = k.size(1), dim = k.size(2);
+  for (int i : {0, 1, 2, 3, 4, 9, 11, 12})
+    if (a.tensor(i) && !a.plain(i, k)) return {};
+  if (!sizes_ok({tokens, kv_heads, dim}) || dim % 8 != 0 || dim > 256) return {};
+  for (int i : {0, 1, 2})
+    if (a.tensor(i) && !rows_ok(a[i], k.scalar_type(), tokens, dim)) return {};
+  const int64_t heads = a.none(0) ? 0 : a[0].size(1);
+  if (heads > 65536 || kv_heads > 65536 || a.none(2) == to_cache || a.none(9) == to_cache || a.none(3) != a.none(4)) return {};
+  int64_t limit = 0, rot = 0;
+  if (!a.none(3)) {
+    const Tensor& t = a[4];
+    if (!index_vector(a[3], tokens) || t.scalar_type() != at::kFloat || t.dim() != 3 || t.size(2) != 2 || !t.is_contiguous() || !aligned(t)) return {};
+    limit = t.size(0), rot = 2 * t.size(1);
+    if (limit < 1 || rot < 16 || rot % 16 != 0 || rot > dim) return {};
+  }
+  for (int i : {11, 12})
+    if (a.tensor(i) && (a[i].dim() != 1 || a[i].size(0) != dim || a[i].scalar_type() != k.scalar_type() || !a[i].is_contiguous())) return {};
+  const Cache c(a, 5);
+  if (to_cache && (!c.ok || !c.takes(k.scalar_type()) || c.k->device() != k.device() || c.heads != kv_heads || c.dim != dim || a[2].size(1) != kv_heads || !index_vector(a[9], tokens))) return {};
+  const Place at_(k);
+  Outputs out;
+  if (heads) out.first = at::empty({tokens, heads, dim}, k.options());
+  if (!to_cache) out.second = at::empty({tokens, kv_heads, dim}, k.options());
+  const Tensor *q = a.get(0), *v = a.get(2), *slots = a.get(9);
+  auto stride = [](const Tensor* t, int i) -> long { return t ? t->stride(i) : 0; };
+  out.done = launched(triteia_hip_rotary_cache(
+      data(q), stride(q, 0), stride(q, 1), data(&k), k.stride(0), k.stride(1), data(v), stride(v, 0), stride(v, 1), heads ? out.first.data_ptr() : nullptr,
+      to_cache ? nullptr : out.second.data_ptr(), tokens, heads, kv_heads, dim, rot, data(a.get(3)), !a.none(3) && a[3].scalar_type() == at::kLong,
+      data(a.get(4)), limit, a.integer(10), data(a.get(11)), data(a.get(12)), (float)a.numbers[13], data(slots), slots && slots->scalar_type() == at::kLong,
+      to_cache ? data(c.k) : nullptr, to_cache ? data(c.v) : nullptr, to_cache ? data(c.ks) : nullptr, to_cache ? data(c.vs) : nullptr,
+      to_cache ? c.strides : nullptr, to_cache ? c.n_pages : 0, to_cache ? c.page : 0, to_cache ? c.kind : 0, k.scalar_type() == at::kBFloat16, at_.dev, at_.handle()));
+  return out;
+}
+
+// cache_read(cache k, v, scales, slots, dtype)
+Outputs cache_read(const MoreArgs& a) {
+  if (a.n != 6 || !a.tensor(4) || !a.typed[5]) return {};
+  const Cache c(a, 0);
+  if (!c.ok || !c.takes(a.types[5]) || !a.plain(4, *c.k) || a[4].dim() != 1 || !index_vector(a[4], a[4].size(0)) || !sizes_ok({a[4].size(0)})) return {};
+  const Place at_(*c.k);
+  Outputs out;
+  const int64_t tokens = a[4].size(0);
+  out.first = at::empty({tokens, c.heads, c.dim}, c.k->options().dtype(a.types[5]));
+  out.second = at::empty({tokens, c.heads, c.dim}, c.k->options().dtype(a.types[5]));
+  out.done = launched(triteia_hip_cache_read(data(c.k), data(c.v), data(c.ks), data(c.vs), c.strides, c.n_pages, c.heads, c.page, c.dim, c.kind, data(&a[4]),
+                                             a[4].scalar_type() == at::kLong, tokens, out.first.data_ptr(), out.second.data_ptr(), a.types[5] == at::kBFloat16,
+                                             at_.dev, at_.handle()));
+  return out;
+}
+
+// attention_plan(q_starts, kv_lens, tokens, heads, heads of the cache, max_q, causal, window)
+Outputs attention_plan(const MoreArgs& a) {
+  if (a.n != 8 || !a.tensor(0) || !a.tensor(1) || !a.whole(6, 1)) return {};
+  for (int i : {2, 3, 4, 5, 7})
+    if (!a.whole(i)) return {};
+  const Tensor &starts = a[0], &lens = a[1];
+  if (!starts.is_cuda() || !a.plain(0, starts) || !a.plain(1, starts) || !dense_on(starts, starts, at::kInt, 1) || !dense_on(lens, starts, at::kInt, 1) ||
+      starts.size(0) != lens.size(0) + 1 || starts.size(0) > 0x7fffffff)
+    return {};
+  const int seqs = (int)lens.size(0), tokens = a.integer(2), heads = a.integer(3), kv_heads = a.integer(4), most = a.integer(5);
+  const size_t bytes = triteia_hip_attention_plan_bytes(seqs, tokens, heads, kv_heads, most);
+  if (bytes == 0) return {};
+  const Place at_(starts);
+  Outputs out;
+  out.first = at::empty({(int64_t)bytes}, starts.options().dtype(at::kByte));
+  out.done = launched(triteia_hip_attention_plan(starts.data_ptr(), lens.data_ptr(), seqs, tokens, heads, kv_heads, most, a.integer(6), a.integer(7),
+                                                 out.first.data_ptr(), bytes, at_.dev, at_.handle()));
+  return out;
+}
+
+// paged_attention(q, cache k, v, scales, pages, plan, sequences, heads of the plan, its max_q, causal, window, scale)
+Outputs paged_attention(const MoreArgs& a) {
+  if (a.n != 13 || !a.tensor(0) || !a.tensor(5) || !a.tensor(6) || !a.given[12] || !a.whole(10, 1)) return {};
+  for (int i : {7, 8, 9, 11})
+    if (!a.whole(i)) return {};
+  const Tensor &q = a[0], &pages = a[5], &plan = a[6];
+  const Cache c(a, 1);
+  if (!c.ok || !c.takes(q.scalar_type()) || q.dim() != 3 || !a.plain(0, *c.k) || !a.plain(5, *c.k) || !a.plain(6, *c.k)) return {};
+  const int64_t tokens = q.size(0), heads = a.integer(8), seqs = a.integer(7);
+  if (!sizes_ok({tokens, heads, seqs}) || !rows_ok(q, q.scalar_type(), tokens, c.dim) || q.size(1) != heads || pages.scalar_type() != at::kInt || pages.dim() != 2 ||
+      pages.size(0) != seqs || !sizes_ok({pages.size(1)}) || pages.stride(1) != 1 || pages.stride(0) < 0 || !dense_on(plan, q, at::kByte, 1))
+    return {};
+  const size_t bytes = triteia_hip_attention_scratch_bytes(seqs, tokens, heads, c.heads, a.integer(9), c.dim);
+  if (bytes == 0) return {};
+  const Place at_(q);
+  Outputs out;
+  out.first = at::empty({tokens, heads, c.dim}, q.options());
+  const Tensor scratch = scratch_bytes(bytes, q);
+  out.done = launched(triteia_hip_paged_attention(
+      q.data_ptr(), q.stride(0), q.stride(1), out.first.data_ptr(), data(c.k), data(c.v), data(c.ks), data(c.vs), c.strides, c.n_pages, c.page, c.kind,
+      pages.data_ptr(), pages.stride(0), pages.size(1), plan.data_ptr(), plan.numel(), seqs, tokens, heads, c.heads, c.dim, a.integer(9), a.integer(10),
+      a.integer(11), (float)a.numbers[12], scratch.data_ptr(), bytes, q.scalar_type() == at::kBFloat16, at_.dev, at_.handle()));
+  return out;
+}
+
+// One output as a tensor, two (and a missing first) as a tuple.
+template <Outputs (*F)(const MoreArgs&), bool PAIR>
+PyObject* call_more(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const MoreArgs a(v, n);
+  Outputs out;
+  {
+    const WithoutGil released;
+    out = F(a);
+  }
+  if (!out.done) Py_RETURN_NONE;
+  if (!PAIR) return THPVariable_Wrap(std::move(out.first));
+  auto one = [](Tensor&& t) -> PyObject* {
+    if (!t.defined()) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(t));
+  };
+  PyObject* first = one(std::move(out.first));
+  return Py_BuildValue("(NN)", first, one(std::move(out.second)));
+  END_HANDLE_TH_ERRORS
+}
+
 #define METHOD(NAME_, FN_) {NAME_, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(FN_)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD("matmul", (call<matmul>)), METHOD("bmm", (call<bmm>)), METHOD("sbmm", (call<sbmm>)), METHOD("lora", (call<lora>)), METHOD("ldmm", (call<ldmm>)),
-                         METHOD("pack", pack), METHOD("sparse", sparse), {nullptr, nullptr, 0, nullptr}};
+                         METHOD("pack", pack), METHOD("sparse", sparse), METHOD("rotary_cache", (call_more<rotary_cache, true>)),
+                         METHOD("cache_read", (call_more<cache_read, true>)), METHOD("attention_plan", (call_more<attention_plan, false>)),
+                         METHOD("paged_attention", (call_more<paged_attention, false>)), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "triteia_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -5,6 +5,7 @@ import ctypes
 import torch
 
 from . import _ffi
+from ._native import native
 
 _DTYPES = (torch.float16, torch.bfloat16)
 CACHE_KINDS = {torch.float16: 0, torch.bfloat16: 0, torch.int8: 1, torch.float8_e4m3fn: 2}
@@ -103,6 +104,9 @@ class PagedCache:
 
 def rotary_cache(q, k, v, positions, table, cache, slots, interleaved=False, q_norm=None, k_norm=None, eps=1e-6):
     """The one launch behind ops.rotary, ops.rotary_cache_write and ops.cache_write: (q, k) of the outputs, None where there is none."""
+    out = native().rotary_cache(q, k, v, positions, table, *(cache._tensors if cache is not None else (None,) * 4), slots, interleaved, q_norm, k_norm, eps)
+    if out is not None:
+        return out
     device = _require(q=q, k=k, v=v, positions=positions, table=table, slots=slots, q_norm=q_norm, k_norm=k_norm)
     like = k if k is not None else q
     tokens, dim, dtype = like.shape[0], like.shape[-1], like.dtype
@@ -150,6 +154,9 @@ def rotary_cache(q, k, v, positions, table, cache, slots, interleaved=False, q_n
 
 def cache_read(cache, slots, dtype):
     """(k, v) [len(slots), kv_heads, dim] of the cache's rows at `slots`; zeros where a slot lies outside the cache."""
+    out = native().cache_read(*cache._tensors, slots, dtype)
+    if out is not None:
+        return out
     _require(cache.device, slots=slots)
     cache._activations(dtype)
     slots = _integers("slots", slots, slots.shape[0] if slots.dim() else None)
@@ -169,6 +176,10 @@ class AttentionPlan:
 
 
 def attention_plan(q_starts, kv_lens, n_tokens, heads, kv_heads, max_q=None, causal=True, window=0):
+    max_q = n_tokens if max_q is None else max_q
+    buffer = native().attention_plan(q_starts, kv_lens, n_tokens, heads, kv_heads, max_q, causal, window)
+    if buffer is not None:
+        return AttentionPlan(buffer, kv_lens.shape[0], n_tokens, heads, kv_heads, max_q, bool(causal), window)
     device = _require(q_starts=q_starts, kv_lens=kv_lens)
     for name, t in (("q_starts", q_starts), ("kv_lens", kv_lens)):
         if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
@@ -176,8 +187,7 @@ def attention_plan(q_starts, kv_lens, n_tokens, heads, kv_heads, max_q=None, cau
     n_seqs = kv_lens.shape[0]
     if q_starts.shape[0] != n_seqs + 1:
         raise RuntimeError(f"q_starts must have {n_seqs + 1} entries for {n_seqs} sequences, got {q_starts.shape[0]}")
-    max_q = n_tokens if max_q is None else int(max_q)
-    sizes = (n_seqs, int(n_tokens), int(heads), int(kv_heads), max_q)
+    sizes = (n_seqs, int(n_tokens), int(heads), int(kv_heads), int(max_q))
     nbytes = _ffi.lib().triteia_hip_attention_plan_bytes(*sizes)
     if nbytes == 0:
         raise RuntimeError(_ffi.last_error())
@@ -188,6 +198,10 @@ def attention_plan(q_starts, kv_lens, n_tokens, heads, kv_heads, max_q=None, cau
 
 
 def paged_attention(q, cache, pages, plan, scale):
+    if isinstance(q, torch.Tensor) and q.dim() == 3 and q.shape[0] == plan.n_tokens and cache.kv_heads == plan.kv_heads:
+        out = native().paged_attention(q, *cache._tensors, pages, plan.buffer, plan.n_seqs, plan.heads, plan.max_q, plan.causal, plan.window, scale)
+        if out is not None:
+            return out
     device = _require(cache.device, q=q, pages=pages, plan=plan.buffer)
     cache._activations(q.dtype)
     q = _rows("q", q, plan.heads, cache.dim)
