@@ -11,7 +11,8 @@
 // Scores, running maxima and sums and the output's sums are 32 bits; P is rounded once to the activations' type for the MFMA.  The maximum is
 // a reference that is only moved (and the sums rescaled) when a score passes it by 2^kAttnSlack: P <= 2^8 is far from the types' ends.
 // Masked scores are -infinity ahead of the maximum; a row that sees nothing has a sum of zero and gives zeros.  What is masked for some rows of
-// a tile and holds an infinity or a NaN in V must not reach those rows by 0 * inf: see attn_split.
+// a tile and holds an infinity or a NaN in V must not reach those rows by 0 * inf: blocks on such an edge enter LDS without them (attn_clean),
+// and the rows that see them get them added one by one (attn_strange).
 #pragma once
 #include "attention_plan.hip.h"
 #include "kv_cache.hip.h"
@@ -59,21 +60,37 @@ struct AttnMma<__bf16> {
   static __device__ __forceinline__ attn_f16 m32(v8 a, v8 b, attn_f16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 
-// V with its infinities and NaNs taken out (`finite`), and numbers in their places whose sums over the tokens that a row sees, at most 64 of
-// them at a time, say which there were: 1 an infinity, 128 a negative one, 16384 a NaN.
-template <class T>
-__device__ __forceinline__ void attn_split(kv8<T> v, kv8<T>* finite, kv8<T>* marks) {
+// 16 bytes of V without their infinities and NaNs; whether there were any.
+template <class T, int KIND>
+__device__ __forceinline__ bool attn_clean(kv_uint4* v) {
+  bool found = false;
+  if constexpr (KIND != kCacheInt8) {
+    constexpr uint32_t bits = KIND == kCacheSame ? 16 : 8, magnitude = KIND == kCacheSame ? 0x7fff : 0x7f;
+    constexpr uint32_t least = KIND == kCacheSame ? AttnMma<T>::kInf : 0x7f;       // (e4m3 has one NaN and no infinity)
 #pragma unroll
-  for (int j = 0; j < 8; j++) {
-    const T x = v[j];          // (a bit cast of the vector's element itself would be one of its first)
-    const uint32_t b = __builtin_bit_cast(uint16_t, x), mag = b & 0x7fffu;
-    (*finite)[j] = mag >= AttnMma<T>::kInf ? (T)0.f : x;
-    (*marks)[j] = mag > AttnMma<T>::kInf ? (T)16384.f : mag < AttnMma<T>::kInf ? (T)0.f : (b >> 15) ? (T)128.f : (T)1.f;
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (uint32_t at = 0; at < 32; at += bits)
+        if (((*v)[i] >> at & magnitude) >= least) (*v)[i] &= ~(((magnitude << 1) + 1) << at), found = true;
   }
+  return found;
 }
-__device__ __forceinline__ float attn_marked(float sum) {      // what those infinities and NaNs add up to
-  const int n = (int)sum, nan = n >> 14, minus = (n >> 7) & 127, plus = n & 127;
-  return nan || (minus && plus) ? __builtin_nanf("") : minus ? -__builtin_inff() : plus ? __builtin_inff() : 0.f;
+
+// What attn_clean took out, for rows that see it: V's infinities and NaNs among four elements of a token's row, zeros for all that is finite.
+template <class T, int KIND>
+__device__ __forceinline__ attn_f4 attn_strange(const CachePart& c, long page, int head, int slot, int d) {
+  attn_f4 x = {0.f, 0.f, 0.f, 0.f};
+  const long at = page * c.page + head * c.head + slot * c.slot + d;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    if constexpr (KIND == kCacheSame) {
+      const float v = (float)static_cast<const T*>(c.data)[at + j];
+      if (!(__builtin_fabsf(v) < __builtin_inff())) x[j] = v;
+    } else if constexpr (KIND == kCacheFp8) {
+      if ((static_cast<const uint8_t*>(c.data)[at + j] & 0x7f) == 0x7f) x[j] = __builtin_nanf("");
+    }
+  }
+  return x;
 }
 
 // 8 codes as 8 values of the activations' type, exactly
@@ -148,7 +165,7 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
   using M = AttnMma<T>;
   using v8 = typename M::v8;
   constexpr int kRowBytes = D * (KIND == kCacheSame ? 2 : 1), kChunks = kRowBytes / 16;
-  constexpr int kSub = 8192 / kRowBytes < 64 ? 8192 / kRowBytes : 64;
+  constexpr int kSub = KIND != kCacheSame && NQ == 2 ? 32 : 8192 / kRowBytes < 64 ? 8192 / kRowBytes : 64;   // (two tiles of rows fill the registers)
   constexpr int kLoads = kSub * kChunks / 64, kLoadRows = 64 / kChunks;     // requests of a sub-tile, rows of each
   constexpr int kGroups = kSub / 16, kGroupLoads = kLoads / kGroups;
   constexpr int kRows = 16 * NQ, kKeyRows = 256 / kRowBytes;
@@ -158,6 +175,7 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
   constexpr int kLds = 4 * 2 * kTile > kMeet ? 4 * 2 * kTile : kMeet;
   __shared__ alignas(16) uint8_t lds[kLds];
   __shared__ float meet_m[4][kRows], meet_l[4][kRows];
+  __shared__ alignas(16) float scales[KIND == kCacheSame ? 1 : 4][2][kSub];
   const int index = blockIdx.x / a.kv_heads, head = blockIdx.x - index * a.kv_heads;
   if (index >= a.plan[2 * a.which]) return;
   const AttnItem it = attn_item(a, index);
@@ -187,9 +205,10 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
 
   const int n_sub = (it.kv_end - it.kv_begin + kSub - 1) / kSub;
   kv_uint4 rk[kLoads], rv[kLoads];
-  attn_f4 ks[kGroups], vs[kGroups];
+  float ks = 0.f, vs = 0.f;                 // scales of token `lane` of the sub-tile
   const int load_row = lane / kChunks, load_chunk = lane % kChunks;
   auto request = [&](int t0) {
+    long at_k = 0, at_v = 0;
 #pragma unroll
     for (int g = 0; g < kGroups; g++) {
       const int token = min(t0 + 16 * g, (it.kv_end - 1) & ~15);
@@ -202,10 +221,11 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
         rk[g * kGroupLoads + j] = *reinterpret_cast<const kv_uint4*>(pk + (long)j * kLoadRows * a.ck.slot * (kRowBytes / D));
         rv[g * kGroupLoads + j] = *reinterpret_cast<const kv_uint4*>(pv + (long)j * kLoadRows * a.cv.slot * (kRowBytes / D));
       }
-      if constexpr (KIND != kCacheSame) {
-        ks[g] = *reinterpret_cast<const attn_f4*>(a.ck.scale + page * a.ck.scale_page + head * a.ck.scale_head + slot + 4 * h);
-        vs[g] = *reinterpret_cast<const attn_f4*>(a.cv.scale + page * a.cv.scale_page + head * a.cv.scale_head + slot + 4 * h);
-      }
+      if (KIND != kCacheSame && lane / 16 == g)
+        at_k = page * a.ck.scale_page + head * a.ck.scale_head + slot + col, at_v = page * a.cv.scale_page + head * a.cv.scale_head + slot + col;
+    }
+    if constexpr (KIND != kCacheSame) {
+      if (lane < kSub) ks = a.ck.scale[at_k] * a.scale_log2, vs = a.cv.scale[at_v];
     }
   };
   auto key_of = [](int row) { return (row / kKeyRows) & (kChunks - 1); };
@@ -229,16 +249,28 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
       for (int j = 0; j < kLoads; j++)
         if (t0 + j * kLoadRows + load_row >= it.kv_end) rv[j] = kv_uint4{0, 0, 0, 0};
     }
+    // a block with tokens that some of its rows see and others do not
+    const bool edge = t0 < all_lo || t0 + kSub > min(all_hi, it.kv_end);
+    bool strange = false;
+    if (t0 < all_lo || (t0 + kSub > all_hi && all_hi < it.kv_end)) {
+#pragma unroll
+      for (int j = 0; j < kLoads; j++) strange |= attn_clean<T, KIND>(&rv[j]);
+      strange = __any(strange);
+    }
 #pragma unroll
     for (int j = 0; j < kLoads; j++) {
       const int row = j * kLoadRows + load_row;
       *reinterpret_cast<kv_uint4*>(lds_k + row * kRowBytes + (load_chunk ^ key_of(row)) * 16) = rk[j];
       *reinterpret_cast<kv_uint4*>(lds_v + row * kRowBytes + (load_chunk ^ key_of_v(row)) * 16) = rv[j];
     }
-    attn_f4 ks_now[kGroups], vs_now[kGroups];
     if constexpr (KIND != kCacheSame) {
+      if (lane < kSub) scales[wave][0][lane] = ks, scales[wave][1][lane] = vs;
+    }
+    float norm_now = norm;                   // the largest scale of V so far
+    if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) {
+      if (lane < kSub && t0 + lane < it.kv_end) norm_now = fmaxf(norm, vs);
 #pragma unroll
-      for (int g = 0; g < kGroups; g++) ks_now[g] = ks[g], vs_now[g] = vs[g];
+      for (int d = 32; d > 0; d /= 2) norm_now = fmaxf(norm_now, __shfl_xor(norm_now, d));
     }
     if (sub + 4 < n_sub) request(t0 + 4 * kSub);
 
@@ -265,20 +297,11 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
         }
       }
     }
-    const bool edge = t0 < all_lo || t0 + kSub > min(all_hi, it.kv_end);
     float grown = 1.f;                       // what the outputs are multiplied by for a larger norm
     if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) {
-      float top = norm;
-#pragma unroll
-      for (int g = 0; g < kGroups; g++)
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-          if (t0 + 16 * g + 4 * h + j < it.kv_end) top = fmaxf(top, vs_now[g][j]);
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      if (top > norm) grown = norm / top, norm = top;
+      if (norm_now > norm) grown = norm / norm_now, norm = norm_now;
     }
-    v8 p[NQ][kSub / 32], seen[NQ][kSub / 32];
+    v8 p[NQ][kSub / 32];
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
       float top = kAttnNone;
@@ -286,7 +309,7 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
       for (int g = 0; g < kGroups; g++)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          float x = s[n][g][j] * (KIND == kCacheSame ? a.scale_log2 : ks_now[g][j] * a.scale_log2);
+          float x = s[n][g][j] * (KIND == kCacheSame ? a.scale_log2 : scales[wave][0][16 * g + 4 * h + j]);
           const int token = t0 + 16 * g + 4 * h + j;
           if (edge && (token < row_lo[n] || token >= min(row_hi[n], it.kv_end))) x = -__builtin_inff();
           s[n][g][j] = x;
@@ -315,15 +338,14 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
           const float e = __builtin_amdgcn_exp2f(s[n][g][j] - m[n]);
           l[n] += e;
           const int token = t0 + 16 * g + 4 * h + j;
-          const bool hidden = edge && (token < row_lo[n] || token >= min(row_hi[n], it.kv_end));
           float w = e;
-          if constexpr (KIND != kCacheSame) w = hidden ? 0.f : e * (vs_now[g][j] * inv);
+          if constexpr (KIND != kCacheSame) {        // (a scale may be a NaN)
+            w = e * (scales[wave][1][16 * g + 4 * h + j] * inv);
+            if (edge && (token < row_lo[n] || token >= min(row_hi[n], it.kv_end))) w = 0.f;
+          }
           p[n][g / 2][4 * (g % 2) + j] = (T)w;
-          seen[n][g / 2][4 * (g % 2) + j] = hidden ? (T)0.f : (T)1.f;
         }
     }
-    // (a single limit for all rows, as one token's heads have, hides the same from all of them: V is zero there)
-    const bool mixed = edge && (t0 < all_lo || t0 + kSub > all_hi) && !(first.lo == last.lo && first.hi == last.hi && first.lo <= it.kv_begin && first.hi >= it.kv_end);
     auto column = [&](int d, int b) {        // V of 32 tokens from 32 b on, as the MFMA's operand for columns 16 d ..
       if constexpr (KIND == kCacheSame) {
         const int row = 32 * b + 4 * h + col / 4, chunk = 2 * d + (col & 3) / 2, in = 8 * (col & 1);
@@ -336,25 +358,24 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
       }
     };
 #pragma unroll
-    for (int d = 0; d < D / 16; d++) {
-      attn_f4 marks[NQ];
-#pragma unroll
-      for (int n = 0; n < NQ; n++) marks[n] = attn_f4{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < D / 16; d++)
 #pragma unroll
       for (int b = 0; b < kSub / 32; b++) {
-        v8 v = column(d, b), mark;
-        if (mixed) attn_split<T>(v, &v, &mark);
+        const v8 v = column(d, b);
 #pragma unroll
-        for (int n = 0; n < NQ; n++) {
-          o[n][d] = M::m16(v, p[n][b], o[n][d]);
-          if (mixed) marks[n] = M::m16(mark, seen[n][b], marks[n]);
-        }
+        for (int n = 0; n < NQ; n++) o[n][d] = M::m16(v, p[n][b], o[n][d]);
       }
-      if (mixed) {
+    if (strange) {
+#pragma unroll 1
+      for (int token = max(t0, 0); token < min(t0 + kSub, it.kv_end); token++) {
+        const long page = attn_page(a, it.seq, token);
 #pragma unroll
-        for (int n = 0; n < NQ; n++)
+        for (int d = 0; d < D / 16; d++) {
+          const attn_f4 x = attn_strange<T, KIND>(a.cv, page, head, token & ((1 << a.page_shift) - 1), 16 * d + 4 * h);
 #pragma unroll
-          for (int j = 0; j < 4; j++) o[n][d][j] += attn_marked(marks[n][j]);
+          for (int n = 0; n < NQ; n++)
+            if (token >= row_lo[n] && token < row_hi[n]) o[n][d] += x;
+        }
       }
     }
   }
@@ -475,31 +496,23 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a) {
       for (int j = 0; j < kLoads; j++)
         if (t0 + 16 * wave + j * kLoadRows + load_row >= it.kv_end) rv[j] = kv_uint4{0, 0, 0, 0};
     }
-    const bool edge = t0 < g1.lo || t0 + kAttnBlock > g0.hi;
     bool strange = false;
+    if (t0 < g1.lo || t0 + kAttnBlock > g0.hi) {
+#pragma unroll
+      for (int j = 0; j < kLoads; j++) strange |= attn_clean<T, KIND>(&rv[j]);
+    }
 #pragma unroll
     for (int j = 0; j < kLoads; j++) {
       const int row = 16 * wave + j * kLoadRows + load_row;
       if constexpr (KIND == kCacheSame) {
         *reinterpret_cast<kv_uint4*>(to_k + row * kRowBytes + (load_chunk ^ key_of(row)) * 16) = rk[j];
         *reinterpret_cast<kv_uint4*>(to_v + row * kRowBytes + (load_chunk ^ key_of_v(row)) * 16) = rv[j];
-        if (edge) {
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            strange |= (rv[j][i] & M::kInf) == M::kInf || (rv[j][i] >> 16 & M::kInf) == M::kInf;
-        }
       } else {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
           const int chunk = 2 * load_chunk + i;
           *reinterpret_cast<v8*>(to_k + row * kRowBytes + (chunk ^ key_of(row)) * 16) = attn_values<T, KIND>(kv_uint2{rk[j][2 * i], rk[j][2 * i + 1]});
           *reinterpret_cast<v8*>(to_v + row * kRowBytes + (chunk ^ key_of_v(row)) * 16) = attn_values<T, KIND>(kv_uint2{rv[j][2 * i], rv[j][2 * i + 1]});
-          if (KIND == kCacheFp8 && edge) {   // (e4m3 has one NaN and no infinity)
-#pragma unroll
-            for (int k = 0; k < 2; k++)
-#pragma unroll
-              for (int b = 0; b < 4; b++) strange |= (rv[j][2 * i + k] >> (8 * b) & 0x7f) == 0x7f;
-          }
         }
       }
     }
@@ -509,6 +522,12 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a) {
       if (lane < 32) scales[at][lane / 16][16 * wave + (lane & 15)] = rs;
     }
   };
+
+  // where a lane's K operand (row `col`, 16-byte piece h) and V operand (row 4 h + lane % 16 / 4, columns 16 (lane / 16 % 2) + 4 (lane % 4) ..) lie: piece 2 i
+  // + h of K and 4 d + .. of V are an exclusive or away, other rows an offset, since the keys repeat every 16 rows (of V every 4)
+  const int v_row = 4 * h + (lane & 15) / 4;
+  const uint32_t lane_k = col * kRowBytes + (h ^ key_of(col)) * 16;
+  const uint32_t lane_v = v_row * kRowBytes + ((2 * (lane >> 4 & 1) + (lane & 3) / 2) ^ key_of_v(v_row)) * 16 + 8 * (lane & 1);
 
   attn_f16 o[D / 32];
 #pragma unroll
@@ -530,20 +549,18 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a) {
       if (block + 2 < n_blocks) request(t0 + 2 * kAttnBlock);
     }
     if (wave_live && t0 < min(w1.hi, it.kv_end) && t0 + kAttnBlock > w0.lo) {
-      const uint8_t* lds_k = lds + at * 2 * kTile;
-      const uint8_t* lds_v = lds_k + kTile;
+      // (one lane constant each, kept from being spread over a register for every address)
+      uint32_t at_k = at * 2 * kTile + lane_k, at_v = at * 2 * kTile + kTile + lane_v;
+      asm volatile("" : "+v"(at_k), "+v"(at_v));
       attn_f16 s[2];
 #pragma unroll
-      for (int g = 0; g < 2; g++) {
+      for (int g = 0; g < 2; g++)
 #pragma unroll
         for (int j = 0; j < 16; j++) s[g][j] = 0.f;
-        const int row = 32 * g + col;
 #pragma unroll
-        for (int i = 0; i < D / 16; i++) {
-          const v8 k = *reinterpret_cast<const v8*>(lds_k + row * kRowBytes + ((2 * i + h) ^ key_of(row)) * 16);
-          s[g] = M::m32(k, qf[i], s[g]);
-        }
-      }
+      for (int i = 0; i < D / 16; i++)
+#pragma unroll
+        for (int g = 0; g < 2; g++) s[g] = M::m32(*reinterpret_cast<const v8*>(lds + (at_k ^ (32 * i)) + 32 * g * kRowBytes), qf[i], s[g]);
       const bool edge = t0 < w1.lo || t0 + kAttnBlock > min(w0.hi, it.kv_end);
       float grown = 1.f;
       if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) {
@@ -593,40 +610,27 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a) {
           }
           p[2 * g + j / 8][j % 8] = (T)e;
         }
-      const int row = 4 * h + (lane & 15) / 4, in = 8 * (lane & 1);
       auto column = [&](int d, int b) {      // V of 16 tokens from 16 b on, columns 32 d ..
-        const int chunk = 4 * d + 2 * (lane >> 4 & 1) + (lane & 3) / 2, r = 16 * b + row;
-        return attn_transposed<T>(lds_v, r * kRowBytes + (chunk ^ key_of_v(r)) * 16 + in, (r + 8) * kRowBytes + (chunk ^ key_of_v(r + 8)) * 16 + in);
+        return attn_transposed<T>(lds, (at_v ^ (64 * d)) + 16 * b * kRowBytes, (at_v ^ (64 * d)) + (16 * b + 8) * kRowBytes);
       };
-      if (edge && (odd[at][0] | odd[at][1] | odd[at][2] | odd[at][3])) {
-        v8 seen[4];
 #pragma unroll
-        for (int b = 0; b < 4; b++)
+      for (int d = 0; d < D / 32; d++)
 #pragma unroll
-          for (int j = 0; j < 8; j++) {
-            const int token = 16 * b + 8 * (j / 4) + j % 4;
-            seen[b][j] = token < lo || token >= hi ? (T)0.f : (T)1.f;
-          }
+        for (int b = 0; b < 4; b++) o[d] = M::m32(column(d, b), p[b], o[d]);
+      if ((t0 < g1.lo || t0 + kAttnBlock > g0.hi) && (odd[at][0] | odd[at][1] | odd[at][2] | odd[at][3])) {
+#pragma unroll 1
+        for (int token = t0; token < min(t0 + kAttnBlock, it.kv_end); token++) {
+          const long page = attn_page(a, it.seq, token);
+          const bool sees = token >= mine.lo && token < mine.hi;
 #pragma unroll
-        for (int d = 0; d < D / 32; d++) {
-          attn_f16 marks;
+          for (int d = 0; d < D / 32; d++)
 #pragma unroll
-          for (int j = 0; j < 16; j++) marks[j] = 0.f;
+            for (int i = 0; i < 4; i++) {
+              const attn_f4 x = attn_strange<T, KIND>(a.cv, page, head, token & ((1 << a.page_shift) - 1), 32 * d + 8 * i + 4 * h);
 #pragma unroll
-          for (int b = 0; b < 4; b++) {
-            v8 v = column(d, b), mark;
-            attn_split<T>(v, &v, &mark);
-            o[d] = M::m32(v, p[b], o[d]);
-            marks = M::m32(mark, seen[b], marks);
-          }
-#pragma unroll
-          for (int j = 0; j < 16; j++) o[d][j] += attn_marked(marks[j]);
+              for (int j = 0; j < 4; j++) o[d][4 * i + j] += sees ? x[j] : 0.f;
+            }
         }
-      } else {
-#pragma unroll
-        for (int d = 0; d < D / 32; d++)
-#pragma unroll
-          for (int b = 0; b < 4; b++) o[d] = M::m32(column(d, b), p[b], o[d]);
       }
     }
     __syncthreads();
