@@ -98,7 +98,7 @@ struct ReadLaunch {
 };
 
 template <class T, int KIND, int D>
-void launch_attend(AttendArgs a, const AttnLayout& layout, float* scratch, bool cut, hipStream_t stream) {
+void launch_attend(AttendArgs a, const AttnLayout& layout, float* scratch, long table_tokens, hipStream_t stream) {
   for (int which = 0; which < 2; which++) {
     const AttnList& l = layout.list[which];
     if (l.max_items == 0) continue;
@@ -108,21 +108,22 @@ void launch_attend(AttendArgs a, const AttnLayout& layout, float* scratch, bool 
     scratch = a.part_ml + 2L * l.max_items * a.kv_heads * l.rows;
     const dim3 grid((unsigned)((long)l.max_items * a.kv_heads));
     if (which == 1) hipLaunchKernelGGL((attend_tile_kernel<T, KIND, D>), grid, dim3(256), 0, stream, a);
-    else if (l.rows == 16) hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 1>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 2>), grid, dim3(256), 0, stream, a);
-    if (cut) hipLaunchKernelGGL((attend_join_kernel<T, D>), dim3(l.max_joins * a.kv_heads, l.rows / 16), dim3(256), 0, stream, a);
+    else if (l.rows == 16) hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 1>), grid, dim3(64 * kAttnWaves), 0, stream, a);
+    else hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 2>), grid, dim3(64 * kAttnWaves), 0, stream, a);
+    // (no sequence is longer than its pages)
+    if (table_tokens > (long)l.min_blocks * kAttnBlock) hipLaunchKernelGGL((attend_join_kernel<T, D>), dim3(l.max_joins * a.kv_heads, l.rows / 16), dim3(1024), 0, stream, a);
   }
 }
 struct AttendLaunch {
   const AttendArgs& a;
   const AttnLayout& layout;
   float* scratch;
-  bool cut;
+  long table_tokens;
   int dim;
   hipStream_t stream;
   template <class T, int KIND> void operator()() {
-    if (dim == 64) launch_attend<T, KIND, 64>(a, layout, scratch, cut, stream);
-    else launch_attend<T, KIND, 128>(a, layout, scratch, cut, stream);
+    if (dim == 64) launch_attend<T, KIND, 64>(a, layout, scratch, table_tokens, stream);
+    else launch_attend<T, KIND, 128>(a, layout, scratch, table_tokens, stream);
   }
 };
 
@@ -258,11 +259,9 @@ int triteia_hip_paged_attention(const void* q, long q_token, long q_head, void* 
   a.pages = static_cast<const int*>(pages), a.pages_seq = pages_seq, a.n_pages = n_pages, a.table_width = table_width, a.page_shift = page_shift_of(page);
   a.group = heads / kv_heads, a.kv_heads = kv_heads, a.causal = causal, a.window = window, a.scale_log2 = scale * 1.44269504088896340736f;
   a.plan = static_cast<const int*>(plan);
-  // (no sequence is longer than its pages; a list's shares are `min_blocks` long at least)
-  const bool cut = (long)table_width * page > (long)l.list[0].min_blocks * kAttnBlock;
   DeviceGuard g(dev);
   if (!g.ok) return fail(TRITEIA_HIP_ERR_RUNTIME, "cannot select device %d", dev);
-  by_types(bf16, kind, AttendLaunch{a, l, static_cast<float*>(scratch), cut, dim, static_cast<hipStream_t>(stream)});
+  by_types(bf16, kind, AttendLaunch{a, l, static_cast<float*>(scratch), (long)table_width * page, dim, static_cast<hipStream_t>(stream)});
   return check_launch("paged attention");
 }
 

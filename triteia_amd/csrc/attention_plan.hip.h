@@ -6,8 +6,10 @@
 // 64-token blocks, so that every list has work for the whole chip; a share's result goes to scratch and a tile's shares are joined by a launch behind.
 // Lengths stay on the device: what the host knows are upper bounds, from which it sizes the lists and the grids.
 //
-// One workgroup: sequences are counted and scanned in LDS, a thread finds the sequence of a tile by a binary search.  Tokens behind the last
-// sequence get tiles without keys, whose rows are zeros.  Every number read from the device is clamped, so that no list passes its end.
+// One workgroup of two wavefronts, a list each, so that nothing but the sequences' lengths in LDS is waited for: sums over the lanes, a lane finds the
+// sequence of a tile by a binary search.  Tokens behind the last sequence get tiles without keys, whose rows are zeros.  Every number read from the
+// device is clamped, so that no list passes its end.
+// A step's batch of 26 sequences 14.2 us with a workgroup of 1024 threads on one list after the other -> PLANUS.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -17,7 +19,7 @@ namespace triteia_hip {
 constexpr int kAttnBlock = 64;         // tokens of a block: shares begin and end on its multiples
 constexpr int kAttnTileRows = 128;     // rows of a tile of the long list
 constexpr int kAttnMaxSeqs = 4096;
-constexpr int kAttnPlanThreads = 1024;
+constexpr int kAttnPlanThreads = 128;
 
 // One share of one tile.
 struct AttnItem {
@@ -52,7 +54,7 @@ inline AttnLayout attn_layout(int n_seqs, int n_tokens, int heads, int kv_heads,
   AttnList &s = a.list[0], &l = a.list[1];
   s.rows = only_short ? (most <= 16 ? 16 : 32) : a.group <= 16 ? 16 : 32;
   a.short_rows = only_short ? 0x7fffffff : s.rows;
-  s.aim = 1024, s.min_blocks = 4, l.aim = 512, l.min_blocks = 8;
+  s.aim = 512, s.min_blocks = 16, l.aim = 512, l.min_blocks = 8;
   l.rows = kAttnTileRows;
   const long s_tiles = only_short ? live + rows / s.rows : live, l_tiles = only_short ? 0 : live + rows / l.rows;
   s.max_joins = s.aim / kv_heads + 1, l.max_joins = only_short ? 0 : l.aim / kv_heads + 1;
@@ -66,37 +68,22 @@ inline AttnLayout attn_layout(int n_seqs, int n_tokens, int heads, int kv_heads,
   return a;
 }
 
-__device__ __forceinline__ int attn_scan(int v, int* lds, int* total) {     // exclusive sum over the workgroup
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// Exclusive sums over a wavefront's lanes, and the total.
+__device__ __forceinline__ int attn_scan(int v, int* total) {
+  const int lane = threadIdx.x & 63;
   int x = v;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
     const int y = __shfl_up(x, d);
     if (lane >= d) x += y;
   }
-  __syncthreads();
-  if (lane == 63) lds[wave] = x;
-  __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kAttnPlanThreads / 64; w++) {
-    if (w < wave) before += lds[w];
-    all += lds[w];
-  }
-  *total = all;
-  return before + x - v;
+  *total = __shfl(x, 63);
+  return x - v;
 }
 
 struct AttnSeq {
   int start, n, kv;
 };
-__device__ __forceinline__ AttnSeq attn_seq(const int* q_starts, const int* kv_lens, int b, const AttnLayout& a) {
-  const int lo = max(0, min(q_starts[b], a.n_tokens));
-  if (b == a.n_seqs) return {lo, a.n_tokens - lo, 0};
-  const int hi = max(lo, min(q_starts[b + 1], a.n_tokens));
-  return {lo, hi - lo, max(kv_lens[b], 0)};
-}
-
 // the tokens of the cache that some row of a tile sees, its beginning on a whole block
 __device__ __forceinline__ void attn_range(const AttnSeq& s, int tile, int rows, const AttnLayout& a, int* lo, int* hi) {
   const long row = (long)tile * rows;
@@ -109,84 +96,92 @@ __device__ __forceinline__ void attn_range(const AttnSeq& s, int tile, int rows,
 
 // grid 1, block kAttnPlanThreads
 __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const int* q_starts, const int* kv_lens, AttnLayout a, int* plan) {
-  __shared__ int starts[kAttnMaxSeqs + 2];       // tiles ahead of each sequence
-  __shared__ int lds[kAttnPlanThreads / 64];
-  __shared__ int end[2];                         // items and joins that have a place (all, but for offsets that do not ascend)
-  for (int which = 0; which < 2; which++) {
-    const AttnList& l = a.list[which];
-    if (l.max_items == 0) {
-      if (threadIdx.x == 0) plan[2 * which] = 0, plan[2 * which + 1] = 0;
-      continue;
-    }
-    int tiles = 0;
-    for (int b0 = 0; b0 <= a.n_seqs; b0 += kAttnPlanThreads) {
-      const int b = b0 + threadIdx.x;
-      int mine = 0;
-      if (b <= a.n_seqs) {
-        const long rows = (long)attn_seq(q_starts, kv_lens, b, a).n * a.group;
-        if ((rows <= a.short_rows) == (which == 0)) mine = (int)((rows + l.rows - 1) / l.rows);
-      }
-      int all;
-      const int before = attn_scan(mine, lds, &all);
-      if (b <= a.n_seqs) starts[b] = tiles + before;
-      tiles += all;
-    }
-    __syncthreads();
-    auto find = [&](int i) {                     // the last sequence that starts at or ahead of tile i
-      int lo = 0, hi = a.n_seqs;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (starts[mid] <= i) lo = mid; else hi = mid - 1;
-      }
-      return lo;
-    };
-    long work = 0;
-    for (int i = threadIdx.x; i < tiles; i += kAttnPlanThreads) {
-      const int b = find(i);
-      int lo, hi;
-      attn_range(attn_seq(q_starts, kv_lens, b, a), i - starts[b], l.rows, a, &lo, &hi);
-      work += (hi - lo + kAttnBlock - 1) / kAttnBlock;
-    }
-    if (threadIdx.x == 0) end[0] = l.max_items, end[1] = l.max_joins;
-    int total;
-    attn_scan((int)min(work, 0x7fffffffL / kAttnPlanThreads), lds, &total);
-    // enough tiles for the chip: none is cut
-    int share = 0x7fffffff;
-    if ((long)tiles * a.kv_heads < l.aim) share = (int)max((long)l.min_blocks, ((long)total * a.kv_heads + l.aim - 1) / l.aim);
-    int n_items = 0, n_joins = 0, n_parts = 0;
-    for (int i0 = 0; i0 < tiles; i0 += kAttnPlanThreads) {
-      const int i = tiles - 1 - (i0 + (int)threadIdx.x);      // (a sequence's last tile, the longest, first)
-      int splits = 0, lo = 0, hi = 0, per = 0, b = 0;
-      AttnSeq s = {0, 0, 0};
-      if (i >= 0) {
-        b = find(i);
-        s = attn_seq(q_starts, kv_lens, b, a);
-        attn_range(s, i - starts[b], l.rows, a, &lo, &hi);
-        const int blocks = (hi - lo + kAttnBlock - 1) / kAttnBlock;
-        splits = max(1, (int)(((long)blocks + share - 1) / share));
-        per = (blocks + splits - 1) / splits;
-        splits = per > 0 ? max(1, (blocks + per - 1) / per) : 1;
-      }
-      int all_items, all_joins, all_parts;
-      const int item = n_items + attn_scan(splits, lds, &all_items);
-      const int join = n_joins + attn_scan(splits > 1, lds, &all_joins);
-      const int part = n_parts + attn_scan(splits > 1 ? splits : 0, lds, &all_parts);
-      if (i >= 0 && (item + splits > l.max_items || (splits > 1 && join >= l.max_joins))) {
-        atomicMin(&end[0], item);
-        atomicMin(&end[1], join);
-      } else if (i >= 0) {
-        const int tile = i - starts[b];
-        AttnItem* out = reinterpret_cast<AttnItem*>(plan + l.items) + item;
-        for (int p = 0; p < splits; p++)
-          out[p] = AttnItem{b, s.start, s.n, s.kv, tile, lo + p * per * kAttnBlock, splits == 1 ? hi : min(hi, lo + (p + 1) * per * kAttnBlock), splits == 1 ? -1 : part + p};
-        if (splits > 1) reinterpret_cast<AttnJoin*>(plan + l.joins)[join] = AttnJoin{s.start, s.n, tile, part, splits, {0, 0, 0}};
-      }
-      n_items += all_items, n_joins += all_joins, n_parts += all_parts;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) plan[2 * which] = min(n_items, end[0]), plan[2 * which + 1] = min(n_joins, end[1]);
-    __syncthreads();
+  __shared__ int start[kAttnMaxSeqs + 1], count[kAttnMaxSeqs + 1], context[kAttnMaxSeqs + 1];
+  __shared__ int tiles_ahead[2][kAttnMaxSeqs + 1];       // of each sequence, in each list
+  for (int b = threadIdx.x; b <= a.n_seqs; b += kAttnPlanThreads) {
+    const bool rest = b == a.n_seqs;
+    const int lo = max(0, min(q_starts[b], a.n_tokens)), hi = rest ? a.n_tokens : max(lo, min(q_starts[b + 1], a.n_tokens));
+    start[b] = lo, count[b] = hi - lo, context[b] = rest ? 0 : max(kv_lens[b], 0);
   }
+  __syncthreads();
+  const int which = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const AttnList& l = a.list[which];
+  if (l.max_items == 0) {
+    if (lane < 2) plan[2 * which + lane] = 0;
+    return;
+  }
+  int* ahead = tiles_ahead[which];
+  int tiles = 0;
+  for (int b0 = 0; b0 <= a.n_seqs; b0 += 64) {
+    const int b = b0 + lane;
+    int mine = 0;
+    if (b <= a.n_seqs) {
+      const long rows = (long)count[b] * a.group;
+      if ((rows <= a.short_rows) == (which == 0)) mine = (int)((rows + l.rows - 1) / l.rows);
+    }
+    int all;
+    const int before = attn_scan(mine, &all);
+    if (b <= a.n_seqs) ahead[b] = tiles + before;
+    tiles += all;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");        // (the wavefront's own list: its lanes run together)
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+  struct Tile {
+    int seq, tile, lo, hi, blocks;
+    AttnSeq s;
+  };
+  auto at = [&](int i) {
+    int lo = 0, hi = a.n_seqs;                                   // the last sequence that starts at or ahead of tile i
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (ahead[mid] <= i) lo = mid; else hi = mid - 1;
+    }
+    Tile t;
+    t.seq = lo, t.tile = i - ahead[lo], t.s = {start[lo], count[lo], context[lo]};
+    attn_range(t.s, t.tile, l.rows, a, &t.lo, &t.hi);
+    t.blocks = (t.hi - t.lo + kAttnBlock - 1) / kAttnBlock;
+    return t;
+  };
+  // enough tiles for the chip: none is cut
+  int share = 0x7fffffff;
+  if ((long)tiles * a.kv_heads < l.aim) {
+    long work = 0;
+    for (int i0 = 0; i0 < tiles; i0 += 64) work += i0 + lane < tiles ? at(i0 + lane).blocks : 0;
+    int total;
+    attn_scan((int)min(work, 0x7fffffffL / 64), &total);
+    share = (int)max((long)l.min_blocks, ((long)total * a.kv_heads + l.aim - 1) / l.aim);
+  }
+  int n_items = 0, n_joins = 0, n_parts = 0;
+  int end_items = l.max_items, end_joins = l.max_joins;          // (all have a place, but for offsets that do not ascend)
+  for (int i0 = 0; i0 < tiles; i0 += 64) {
+    const int i = tiles - 1 - (i0 + lane);                       // (a sequence's last tile, the longest, first)
+    int splits = 0, per = 0;
+    Tile t = {};
+    if (i >= 0) {
+      t = at(i);
+      splits = max(1, (int)(((long)t.blocks + share - 1) / share));
+      per = (t.blocks + splits - 1) / splits;
+      splits = per > 0 ? max(1, (t.blocks + per - 1) / per) : 1;
+    }
+    int all_items, all_joins, all_parts;
+    const int item = n_items + attn_scan(splits, &all_items);
+    const int join = n_joins + attn_scan(splits > 1, &all_joins);
+    const int part = n_parts + attn_scan(splits > 1 ? splits : 0, &all_parts);
+    if (i >= 0 && (item + splits > l.max_items || (splits > 1 && join >= l.max_joins))) {
+      end_items = min(end_items, item), end_joins = min(end_joins, join);
+    } else if (i >= 0) {
+      AttnItem* out = reinterpret_cast<AttnItem*>(plan + l.items) + item;
+      for (int p = 0; p < splits; p++)
+        out[p] = AttnItem{t.seq, t.s.start, t.s.n, t.s.kv, t.tile, t.lo + p * per * kAttnBlock, splits == 1 ? t.hi : min(t.hi, t.lo + (p + 1) * per * kAttnBlock),
+                          splits == 1 ? -1 : part + p};
+      if (splits > 1) reinterpret_cast<AttnJoin*>(plan + l.joins)[join] = AttnJoin{t.s.start, t.s.n, t.tile, part, splits, {0, 0, 0}};
+    }
+    n_items += all_items, n_joins += all_joins, n_parts += all_parts;
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d /= 2) end_items = min(end_items, __shfl_xor(end_items, d)), end_joins = min(end_joins, __shfl_xor(end_joins, d));
+  if (lane == 0) plan[2 * which] = min(n_items, end_items), plan[2 * which + 1] = min(n_joins, end_joins);
 }
 
 }  // namespace triteia_hip

@@ -24,6 +24,7 @@ typedef float attn_f16 __attribute__((ext_vector_type(16)));
 typedef short attn_s4 __attribute__((ext_vector_type(4)));
 typedef int attn_i2 __attribute__((ext_vector_type(2)));
 
+constexpr int kAttnWaves = 8;             // of a workgroup with few rows
 constexpr float kAttnNone = -1e30f;     // below every score: the maximum of nothing
 constexpr float kAttnSlack = 8.f;
 
@@ -157,11 +158,11 @@ __device__ __forceinline__ AttnRow attn_row(const AttendArgs& a, const AttnItem&
 
 // ---------------------------------------------------------------------------------------------------------------------------------
 // Few rows: a decode step's heads, a handful of tokens.  Bound by the cache's bytes.  A workgroup takes a share of one tile's tokens; each of
-// its four wavefronts walks sub-tiles of its own (8 KB of K and 8 KB of V: 32 tokens of 128 elements in 16 bits, 64 in 8) with the next one's whole rows
+// its eight wavefronts walks sub-tiles of its own (8 KB of K and 8 KB of V: 32 tokens of 128 elements in 16 bits, 64 in 8) with the next one's whole rows
 // on their way in registers and this one's in LDS of its own, so that the loop has no barrier; maxima, sums and outputs are joined once at the end.
-// grid: list.max_items * kv_heads, block 256
+// grid: list.max_items * kv_heads, block 64 kAttnWaves
 template <class T, int KIND, int D, int NQ>
-__global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
+__global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendArgs a) {
   using M = AttnMma<T>;
   using v8 = typename M::v8;
   constexpr int kRowBytes = D * (KIND == kCacheSame ? 2 : 1), kChunks = kRowBytes / 16;
@@ -171,14 +172,14 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
   constexpr int kRows = 16 * NQ, kKeyRows = 256 / kRowBytes;
   constexpr int kTile = kSub * kRowBytes;
   constexpr int kStride = D + 4;                                             // floats of a row where the wavefronts meet
-  constexpr int kMeet = 4 * kRows * kStride * 4;
-  constexpr int kLds = 4 * 2 * kTile > kMeet ? 4 * 2 * kTile : kMeet;
+  constexpr int kMeet = kAttnWaves / 2 * kRows * kStride * 4;
+  constexpr int kLds = kAttnWaves * 2 * kTile > kMeet ? kAttnWaves * 2 * kTile : kMeet;
   __shared__ alignas(16) uint8_t lds[kLds];
-  __shared__ float meet_m[4][kRows], meet_l[4][kRows];
-  __shared__ alignas(16) float scales[KIND == kCacheSame ? 1 : 4][2][kSub];
+  __shared__ float meet_m[kAttnWaves][kRows], meet_l[kAttnWaves][kRows];
+  __shared__ alignas(16) float scales[KIND == kCacheSame ? 1 : kAttnWaves][2][kSub];
   const int index = blockIdx.x / a.kv_heads, head = blockIdx.x - index * a.kv_heads;
+  const AttnItem it = attn_item(a, index);        // (requested together with the number of items)
   if (index >= a.plan[2 * a.which]) return;
-  const AttnItem it = attn_item(a, index);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, h = lane >> 4;
   uint8_t* lds_k = lds + wave * 2 * kTile;
@@ -242,7 +243,7 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
     for (int d = 0; d < D / 16; d++) o[n][d] = attn_f4{0.f, 0.f, 0.f, 0.f};
   }
   if (wave < n_sub) request(it.kv_begin + wave * kSub);
-  for (int sub = wave; sub < n_sub; sub += 4) {
+  for (int sub = wave; sub < n_sub; sub += kAttnWaves) {
     const int t0 = it.kv_begin + sub * kSub;
     if (t0 + kSub > it.kv_end) {             // tokens behind the last: whatever the page holds there must not meet a zero of P
 #pragma unroll
@@ -272,7 +273,7 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
 #pragma unroll
       for (int d = 32; d > 0; d /= 2) norm_now = fmaxf(norm_now, __shfl_xor(norm_now, d));
     }
-    if (sub + 4 < n_sub) request(t0 + 4 * kSub);
+    if (sub + kAttnWaves < n_sub) request(t0 + kAttnWaves * kSub);
 
     attn_f4 s[NQ][kGroups];
 #pragma unroll
@@ -380,7 +381,7 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
     }
   }
 
-  // the four wavefronts' results
+  // the wavefronts' results: the upper half's go to LDS and are taken in by the lower half, whose go there in turn
 #pragma unroll
   for (int n = 0; n < NQ; n++) {
     l[n] += __shfl_xor(l[n], 16);
@@ -391,29 +392,41 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
   float* meet = reinterpret_cast<float*>(lds);
 #pragma unroll
   for (int n = 0; n < NQ; n++) {
-    const int r = 16 * n + col;
-    const float top = fmaxf(fmaxf(meet_m[0][r], meet_m[1][r]), fmaxf(meet_m[2][r], meet_m[3][r]));
+    float top = kAttnNone;
+#pragma unroll
+    for (int w = 0; w < kAttnWaves; w++) top = fmaxf(top, meet_m[w][16 * n + col]);
     float f = __builtin_amdgcn_exp2f(m[n] - top);
     if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) f *= norm;
 #pragma unroll
-    for (int d = 0; d < D / 16; d++) {
-      attn_f4 x = o[n][d];
+    for (int d = 0; d < D / 16; d++)
 #pragma unroll
-      for (int j = 0; j < 4; j++) x[j] *= f;
-      *reinterpret_cast<attn_f4*>(meet + (wave * kRows + r) * kStride + 16 * d + 4 * h) = x;
-    }
+      for (int j = 0; j < 4; j++) o[n][d][j] *= f;
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < kRows * (D / 4); i += 256) {
+#pragma unroll
+  for (int upper = 1; upper >= 0; upper--) {
+    if ((wave >= kAttnWaves / 2) == (upper == 1)) {
+#pragma unroll
+      for (int n = 0; n < NQ; n++)
+#pragma unroll
+        for (int d = 0; d < D / 16; d++) {
+          attn_f4* to = reinterpret_cast<attn_f4*>(meet + (wave % (kAttnWaves / 2) * kRows + 16 * n + col) * kStride + 16 * d + 4 * h);
+          if (!upper) o[n][d] += *to;
+          *to = o[n][d];
+        }
+    }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < kRows * (D / 4); i += 64 * kAttnWaves) {
     const int r = i / (D / 4), d = 4 * (i % (D / 4));
     if (r > last_row) break;
-    float top = fmaxf(fmaxf(meet_m[0][r], meet_m[1][r]), fmaxf(meet_m[2][r], meet_m[3][r])), sum = 0.f;
+    float top = kAttnNone, sum = 0.f;
     attn_f4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < 4; w++) {
-      sum += meet_l[w][r] * __builtin_amdgcn_exp2f(meet_m[w][r] - top);
-      x += *reinterpret_cast<const attn_f4*>(meet + (w * kRows + r) * kStride + d);
-    }
+    for (int w = 0; w < kAttnWaves; w++) top = fmaxf(top, meet_m[w][r]);
+#pragma unroll
+    for (int w = 0; w < kAttnWaves; w++) sum += meet_l[w][r] * __builtin_amdgcn_exp2f(meet_m[w][r] - top);
+#pragma unroll
+    for (int w = 0; w < kAttnWaves / 2; w++) x += *reinterpret_cast<const attn_f4*>(meet + (w * kRows + r) * kStride + d);
     if (it.part < 0) {
       const AttnRow row = attn_row(a, it, kRows, r);
       typedef T t4 __attribute__((ext_vector_type(4)));
@@ -447,8 +460,8 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a) {
   __shared__ alignas(16) float scales[2][2][kAttnBlock];
   __shared__ int odd[2][4];                                                              // infinities or NaNs among a wavefront's V
   const int index = blockIdx.x / a.kv_heads, head = blockIdx.x - index * a.kv_heads;
-  if (index >= a.plan[2 * a.which]) return;
   const AttnItem it = attn_item(a, index);
+  if (index >= a.plan[2 * a.which]) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, h = lane >> 5;
 
@@ -667,41 +680,52 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a) {
   }
 }
 
-// Shares of one tile, added in their order.  grid (max_joins * kv_heads, rows / 16), block 256: a row's D / 4 lanes times the shares between them.
+// Shares of one tile.  D / 4 lanes hold a row; 16 rows at a time (or as many as there are, rounded up to a power of two) and, between them, the shares: a
+// group of lanes adds every n-th share, the groups' sums are added in their order.  grid (max_joins * kv_heads, rows / 16), block 1024
 template <class T, int D>
-__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
+__global__ __launch_bounds__(1024) void attend_join_kernel(AttendArgs a) {
+  constexpr int kLanes = D / 4, kGroups = 1024 / kLanes;
+  __shared__ attn_f4 sums[1024];
+  __shared__ float totals[kGroups];
   const int index = blockIdx.x / a.kv_heads, head = blockIdx.x - index * a.kv_heads;
-  if (index >= a.plan[2 * a.which + 1]) return;
   const int* j = a.plan + a.list.joins + 8L * index;
   const int q_start = j[0], n_tokens = j[1], tile = j[2], first = j[3], n_parts = j[4];
-  const int rows = a.list.rows;
-  constexpr int kLanes = D / 4, kPer = 256 / kLanes;
-  const int d = 4 * (threadIdx.x % kLanes);
-  for (int i = threadIdx.x / kLanes; i < 16; i += kPer) {
-    const int r = 16 * blockIdx.y + i;
-    const long row = (long)tile * rows + r;
-    const int token = (int)(row / a.group), g = (int)(row - (long)token * a.group);
-    if (token >= n_tokens) return;
-    const long step = (long)a.kv_heads * rows;
-    const long at = ((long)first * a.kv_heads + head) * rows + r;
-    float top = kAttnNone;
-    for (int p = 0; p < n_parts; p++) top = fmaxf(top, a.part_ml[2 * (at + p * step)]);
-    float sum = 0.f;
-    attn_f4 x = {0.f, 0.f, 0.f, 0.f};
+  if (index >= a.plan[2 * a.which + 1]) return;
+  const int rows = a.list.rows, r0 = 16 * blockIdx.y;
+  const int live = (int)min(16L, (long)n_tokens * a.group - (long)tile * rows - r0);
+  if (live <= 0) return;
+  int wide = 1;                                  // rows side by side
+  while (wide < live) wide *= 2;
+  const int group = threadIdx.x / kLanes, d = 4 * (threadIdx.x % kLanes), i = group % wide, n = kGroups / wide;
+  const long step = (long)a.kv_heads * rows, at = ((long)first * a.kv_heads + head) * rows + r0 + min(i, live - 1);
+  float top = kAttnNone, sum = 0.f;
 #pragma unroll 4
-    for (int p = 0; p < n_parts; p++) {
-      const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * (at + p * step)] - top);
-      sum += f * a.part_ml[2 * (at + p * step) + 1];
-      const attn_f4 y = *reinterpret_cast<const attn_f4*>(a.part_o + (at + p * step) * D + d);
+  for (int p = 0; p < n_parts; p++) top = fmaxf(top, a.part_ml[2 * (at + p * step)]);
+  attn_f4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int p = group / wide; p < n_parts; p += n) {
+    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * (at + p * step)] - top);
+    sum += f * a.part_ml[2 * (at + p * step) + 1];
+    const attn_f4 y = *reinterpret_cast<const attn_f4*>(a.part_o + (at + p * step) * D + d);
 #pragma unroll
-      for (int k = 0; k < 4; k++) x[k] = __builtin_fmaf(y[k], f, x[k]);
-    }
-    typedef T t4 __attribute__((ext_vector_type(4)));
-    t4 y;
-#pragma unroll
-    for (int k = 0; k < 4; k++) y[k] = sum == 0.f ? (T)0.f : (T)(x[k] / sum);
-    *reinterpret_cast<t4*>(static_cast<T*>(a.out) + ((long)(q_start + token) * (a.kv_heads * a.group) + head * a.group + g) * D + d) = y;
+    for (int k = 0; k < 4; k++) x[k] = __builtin_fmaf(y[k], f, x[k]);
   }
+  sums[threadIdx.x] = x;
+  if (d == 0) totals[group] = sum;
+  __syncthreads();
+  if (group >= live) return;
+  x = sums[threadIdx.x], sum = totals[group];
+  for (int g = 1; g < n; g++) {
+    x += sums[threadIdx.x + g * wide * kLanes];
+    sum += totals[group + g * wide];
+  }
+  const long row = (long)tile * rows + r0 + group;
+  const int token = (int)(row / a.group), g = (int)(row - (long)token * a.group);
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  t4 y;
+#pragma unroll
+  for (int k = 0; k < 4; k++) y[k] = sum == 0.f ? (T)0.f : (T)(x[k] / sum);
+  *reinterpret_cast<t4*>(static_cast<T*>(a.out) + ((long)(q_start + token) * (a.kv_heads * a.group) + head * a.group + g) * D + d) = y;
 }
 
 }  // namespace triteia_hip
