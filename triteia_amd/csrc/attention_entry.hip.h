@@ -133,6 +133,7 @@ int check_batch(const char* what, int n_seqs, int n_tokens, int heads, int kv_he
                 window, kAttnMaxSeqs);
   if (heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || heads > 1024)
     return fail(TRITEIA_HIP_ERR_PROB_SHAPE, "%s: %d heads over %d heads of the cache: a multiple, up to 1024", what, heads, kv_heads);
+  if ((long)n_tokens * (heads / kv_heads) > (1L << 30)) return fail(TRITEIA_HIP_ERR_PROB_SHAPE, "%s: %d tokens of %d heads are too many", what, n_tokens, heads);
   if (window > 0 && !causal) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: a window needs causal", what);
   const AttnLayout l = attn_layout(n_seqs, n_tokens, heads, kv_heads, max_q, causal, window);
   for (const AttnList& x : l.list)
@@ -244,6 +245,7 @@ int triteia_hip_paged_attention(const void* q, long q_token, long q_head, void* 
   const long size = kind == kCacheSame ? 2 : 1;
   for (const CachePart* p : {&a.ck, &a.cv}) {
     if (!strides_ok({p->page, p->head, p->slot}, size, 16)) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: a cache's rows need 16-byte alignment", what);
+    if (p->slot * size > (1L << 26)) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: rows of a page %ld elements apart are too far", what, p->slot);
     if (kind != kCacheSame && (!aligned16(p->scale) || p->scale_slot != 1 || !strides_ok({p->scale_page, p->scale_head}, 4, 16)))
       return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: a page's scales of one head have to be adjacent and 16-byte aligned", what);
   }

@@ -18,6 +18,8 @@ namespace triteia_hip {
 
 constexpr int kAttnBlock = 64;         // tokens of a block: shares begin and end on its multiples
 constexpr int kAttnTileRows = 128;     // rows of a tile of the long list
+constexpr int kAttnRounds = 4;         // lists of this many rounds of workgroups and more are not cut
+constexpr int kAttnSorted = 256;       // lists of up to this many tiles begin with the longest
 constexpr int kAttnMaxSeqs = 4096;
 constexpr int kAttnPlanThreads = 128;
 
@@ -34,7 +36,7 @@ struct AttnList {
   int rows;              // rows of a tile
   int max_items, max_joins;
   long items, joins;     // where they start in the plan, in ints
-  int aim, min_blocks;   // shares that a list of few tiles is cut into (all heads), and the least length of one
+  int slots, min_blocks; // workgroups that run side by side, and the least length of a share
 };
 
 struct AttnLayout {
@@ -54,10 +56,10 @@ inline AttnLayout attn_layout(int n_seqs, int n_tokens, int heads, int kv_heads,
   AttnList &s = a.list[0], &l = a.list[1];
   s.rows = only_short ? (most <= 16 ? 16 : 32) : a.group <= 16 ? 16 : 32;
   a.short_rows = only_short ? 0x7fffffff : s.rows;
-  s.aim = 512, s.min_blocks = 16, l.aim = 512, l.min_blocks = 8;
+  s.slots = 256, s.min_blocks = 16, l.slots = 512, l.min_blocks = 8;
   l.rows = kAttnTileRows;
   const long s_tiles = only_short ? live + rows / s.rows : live, l_tiles = only_short ? 0 : live + rows / l.rows;
-  s.max_joins = s.aim / kv_heads + 1, l.max_joins = only_short ? 0 : l.aim / kv_heads + 1;
+  s.max_joins = kAttnRounds * s.slots / kv_heads + 1, l.max_joins = only_short ? 0 : kAttnRounds * l.slots / kv_heads + 1;
   s.max_items = (int)(s_tiles + s.max_joins), l.max_items = (int)(l_tiles + l.max_joins);
   long at = 8;
   for (AttnList& x : a.list) {
@@ -86,8 +88,8 @@ struct AttnSeq {
 };
 // the tokens of the cache that some row of a tile sees, its beginning on a whole block
 __device__ __forceinline__ void attn_range(const AttnSeq& s, int tile, int rows, const AttnLayout& a, int* lo, int* hi) {
-  const long row = (long)tile * rows;
-  const int t0 = (int)(row / a.group), t1 = min(s.n - 1, (int)((row + rows - 1) / a.group));
+  const uint32_t row = (uint32_t)tile * rows;            // (tokens times heads of a group are below 2^31)
+  const int t0 = (int)(row / (uint32_t)a.group), t1 = min(s.n - 1, (int)((row + rows - 1) / (uint32_t)a.group));
   const long before = (long)s.kv - s.n;
   *hi = a.causal ? (int)max(0L, before + t1 + 1) : s.kv;
   *lo = a.window > 0 ? (int)max(0L, before + t0 - a.window + 1) / kAttnBlock * kAttnBlock : 0;
@@ -98,6 +100,7 @@ __device__ __forceinline__ void attn_range(const AttnSeq& s, int tile, int rows,
 __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const int* q_starts, const int* kv_lens, AttnLayout a, int* plan) {
   __shared__ int start[kAttnMaxSeqs + 1], count[kAttnMaxSeqs + 1], context[kAttnMaxSeqs + 1];
   __shared__ int tiles_ahead[2][kAttnMaxSeqs + 1];       // of each sequence, in each list
+  __shared__ int order[2][kAttnSorted];
   for (int b = threadIdx.x; b <= a.n_seqs; b += kAttnPlanThreads) {
     const bool rest = b == a.n_seqs;
     const int lo = max(0, min(q_starts[b], a.n_tokens)), hi = rest ? a.n_tokens : max(lo, min(q_starts[b + 1], a.n_tokens));
@@ -143,19 +146,56 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const 
     t.blocks = (t.hi - t.lo + kAttnBlock - 1) / kAttnBlock;
     return t;
   };
-  // enough tiles for the chip: none is cut
+  // Few tiles: the least share with which all shares still run in as many rounds as the tiles would.
   int share = 0x7fffffff;
-  if ((long)tiles * a.kv_heads < l.aim) {
+  const long units = (long)tiles * a.kv_heads;
+  if (units < (long)kAttnRounds * l.slots) {
+    const int most = (int)((units + l.slots - 1) / l.slots * l.slots / a.kv_heads);        // shares of one head
     long work = 0;
     for (int i0 = 0; i0 < tiles; i0 += 64) work += i0 + lane < tiles ? at(i0 + lane).blocks : 0;
     int total;
     attn_scan((int)min(work, 0x7fffffffL / 64), &total);
-    share = (int)max((long)l.min_blocks, ((long)total * a.kv_heads + l.aim - 1) / l.aim);
+    total = __builtin_amdgcn_readfirstlane(total);
+    share = max(l.min_blocks, (total + most - 1) / max(most, 1));
+    while (true) {
+      int shares = 0;
+      for (int i0 = 0; i0 < tiles; i0 += 64) {
+        int sum;
+        attn_scan(i0 + lane < tiles ? max(1, (at(i0 + lane).blocks + share - 1) / share) : 0, &sum);
+        shares += sum;
+      }
+      if (__builtin_amdgcn_readfirstlane(shares) <= most || share > total) break;
+      share += (share + 7) / 8;
+    }
+  }
+  // longest first, so that the last workgroups to run are short ones
+  if (tiles <= kAttnSorted) {
+    int mine[kAttnSorted / 64], place[kAttnSorted / 64];
+#pragma unroll
+    for (int k = 0; k < kAttnSorted / 64; k++) {
+      const int i = 64 * k + lane;
+      mine[k] = i < tiles ? at(i).blocks : -1, place[k] = 0;
+    }
+#pragma unroll
+    for (int k = 0; k < kAttnSorted / 64; k++) {
+      for (int i = 64 * k; i < min(tiles, 64 * k + 64); i++) {
+        const int other = __builtin_amdgcn_readlane(mine[k], i & 63);
+#pragma unroll
+        for (int n = 0; n < kAttnSorted / 64; n++) place[n] += other > mine[n] || (other == mine[n] && i < 64 * n + lane);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAttnSorted / 64; k++)
+      if (64 * k + lane < tiles) order[which][place[k]] = 64 * k + lane;
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
   }
   int n_items = 0, n_joins = 0, n_parts = 0;
   int end_items = l.max_items, end_joins = l.max_joins;          // (all have a place, but for offsets that do not ascend)
   for (int i0 = 0; i0 < tiles; i0 += 64) {
-    const int i = tiles - 1 - (i0 + lane);                       // (a sequence's last tile, the longest, first)
+    // (of long lists a sequence's last tile, its longest, first)
+    const int i = i0 + lane >= tiles ? -1 : tiles <= kAttnSorted ? order[which][i0 + lane] : tiles - 1 - (i0 + lane);
     int splits = 0, per = 0;
     Tile t = {};
     if (i >= 0) {

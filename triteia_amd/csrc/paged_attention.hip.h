@@ -44,6 +44,18 @@ struct AttendArgs {
   float *part_o, *part_ml;              // [parts][kv_heads][rows][D], [parts][kv_heads][rows][2]
 };
 
+// The largest over lanes 32 apart, or 16 and 32 apart, in all of them: whole rows of lanes trade places on the vector ALU.
+__device__ __forceinline__ float attn_max32(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  const uint32_t lo = r[0], hi = r[1];
+  return fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+}
+__device__ __forceinline__ float attn_max16(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  const uint32_t lo = r[0], hi = r[1];
+  return attn_max32(fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi)));
+}
+
 template <class T>
 struct AttnMma;
 template <>
@@ -64,17 +76,20 @@ struct AttnMma<__bf16> {
 // 16 bytes of V without their infinities and NaNs; whether there were any.
 template <class T, int KIND>
 __device__ __forceinline__ bool attn_clean(kv_uint4* v) {
-  bool found = false;
+  uint32_t found = 0;
   if constexpr (KIND != kCacheInt8) {
-    constexpr uint32_t bits = KIND == kCacheSame ? 16 : 8, magnitude = KIND == kCacheSame ? 0x7fff : 0x7f;
-    constexpr uint32_t least = KIND == kCacheSame ? AttnMma<T>::kInf : 0x7f;       // (e4m3 has one NaN and no infinity)
+    // magnitudes from the least that is no number on carry into the sign's place (e4m3 has one NaN and no infinity)
+    constexpr uint32_t magnitude = KIND == kCacheSame ? 0x7fff7fffu : 0x7f7f7f7fu, sign = ~magnitude;
+    constexpr uint32_t carry = KIND == kCacheSame ? (0x8000u - AttnMma<T>::kInf) * 0x00010001u : 0x01010101u;
+    constexpr int bits = KIND == kCacheSame ? 15 : 7;
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-      for (uint32_t at = 0; at < 32; at += bits)
-        if (((*v)[i] >> at & magnitude) >= least) (*v)[i] &= ~(((magnitude << 1) + 1) << at), found = true;
+    for (int i = 0; i < 4; i++) {
+      const uint32_t odd = (((*v)[i] & magnitude) + carry) & sign;
+      (*v)[i] &= ~(odd | (odd - (odd >> bits)));
+      found |= odd;
+    }
   }
-  return found;
+  return found != 0;
 }
 
 // What attn_clean took out, for rows that see it: V's infinities and NaNs among four elements of a token's row, zeros for all that is finite.
@@ -134,10 +149,22 @@ __device__ __forceinline__ AttnItem attn_item(const AttendArgs& a, int i) {
 }
 
 // the page of a token, kept inside the table and the cache
-__device__ __forceinline__ long attn_page(const AttendArgs& a, int seq, int token) {
+__device__ __forceinline__ int attn_page(const AttendArgs& a, int seq, int token) {
   const int at = min(token >> a.page_shift, a.table_width - 1);
-  return (long)min((uint32_t)a.pages[seq * a.pages_seq + at], (uint32_t)(a.n_pages - 1));
+  return (int)min((uint32_t)a.pages[seq * a.pages_seq + at], (uint32_t)(a.n_pages - 1));
 }
+
+// One head's keys or values: where the 16 tokens of a group start is the same for all lanes, a lane's own offset from there has 32 bits.
+struct AttnHeld {
+  const uint8_t* head;
+  long page, slot;               // strides in bytes
+  uint32_t lane;
+  __device__ __forceinline__ AttnHeld(const CachePart& c, int h, int size, int row, int piece)
+      : head(static_cast<const uint8_t*>(c.data) + h * c.head * size), page(c.page * size), slot(c.slot * size), lane((uint32_t)(row * slot) + 16 * piece) {}
+  __device__ __forceinline__ kv_uint4 at(long p, int first, int row) const {
+    return *reinterpret_cast<const kv_uint4*>(head + p * page + (first + row) * slot + lane);
+  }
+};
 
 // Which tokens row `r` of a tile sees: lo <= token < hi.  Rows behind the last see all that the tile sees and are not stored.
 struct AttnRow {
@@ -145,9 +172,9 @@ struct AttnRow {
   bool live;
 };
 __device__ __forceinline__ AttnRow attn_row(const AttendArgs& a, const AttnItem& it, int rows, int r) {
-  const long row = (long)it.tile * rows + r;
+  const uint32_t row = (uint32_t)it.tile * rows + r;       // (tokens times heads of a group are below 2^31)
   AttnRow x;
-  x.token = (int)(row / a.group), x.head = (int)(row - (long)x.token * a.group);
+  x.token = (int)(row / (uint32_t)a.group), x.head = (int)(row - (uint32_t)x.token * a.group);
   x.live = x.token < it.n_tokens;
   const int position = it.kv_len - it.n_tokens + x.token;
   x.hi = x.live && a.causal ? min(position + 1, it.kv_len) : it.kv_len;
@@ -185,6 +212,48 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendA
   uint8_t* lds_k = lds + wave * 2 * kTile;
   uint8_t* lds_v = lds_k + kTile;
 
+  const int n_sub = (it.kv_end - it.kv_begin + kSub - 1) / kSub;
+  kv_uint4 rk[kLoads], rv[kLoads];
+  float ks = 0.f, vs = 0.f;                 // scales of token `lane` of the sub-tile
+  const int load_row = lane / kChunks, load_chunk = lane % kChunks;
+  const int page_mask = (1 << a.page_shift) - 1;
+  const AttnHeld held_k(a.ck, head, kRowBytes / D, load_row, load_chunk), held_v(a.cv, head, kRowBytes / D, load_row, load_chunk);
+  const float *scale_k = a.ck.scale + head * a.ck.scale_head, *scale_v = a.cv.scale + head * a.cv.scale_head;
+  // A lane fetches the page of one 16-token group of the wavefront's next sub-tiles: kIds sub-tiles' pages are one request, a request ahead.
+  constexpr int kIds = 64 / kGroups;
+  auto pages_from = [&](int i) {
+    const long token = it.kv_begin + (wave + (long)kAttnWaves * (i + lane / kGroups)) * kSub + 16 * (lane % kGroups);
+    return attn_page(a, it.seq, (int)min(token, (long)it.kv_end - 1));
+  };
+  int ids = n_sub > wave ? pages_from(0) : 0, next_ids = n_sub > wave + kAttnWaves * kIds ? pages_from(kIds) : 0;
+  auto request = [&](int i) {                // the wavefront's i-th sub-tile
+    const int t0 = it.kv_begin + (wave + kAttnWaves * i) * kSub;
+    if (i > 0 && i % kIds == 0) {
+      ids = next_ids;
+      if (wave + kAttnWaves * (i + kIds) < n_sub) next_ids = pages_from(i + kIds);
+    }
+#pragma unroll
+    for (int g = 0; g < kGroups; g++) {
+      const long page = __builtin_amdgcn_readlane(ids, i % kIds * kGroups + g);
+      const int slot = min(t0 + 16 * g, (it.kv_end - 1) & ~15) & page_mask;
+#pragma unroll
+      for (int j = 0; j < kGroupLoads; j++) {
+        rk[g * kGroupLoads + j] = held_k.at(page, slot, j * kLoadRows);
+        rv[g * kGroupLoads + j] = held_v.at(page, slot, j * kLoadRows);
+      }
+    }
+    if constexpr (KIND != kCacheSame) {
+      const long page = __shfl(ids, i % kIds * kGroups + lane / 16);
+      const int slot = (min(t0 + 16 * (lane / 16), (it.kv_end - 1) & ~15) & page_mask) + col;
+      if (lane < kSub) ks = scale_k[page * a.ck.scale_page + slot] * a.scale_log2, vs = scale_v[page * a.cv.scale_page + slot];
+    }
+  };
+  auto key_of = [](int row) { return (row / kKeyRows) & (kChunks - 1); };
+  auto key_of_v = [](int row) {
+    return KIND == kCacheSame ? (row / kKeyRows << 1) & (kChunks - 1) : ((row / kKeyRows) & (kChunks / 2 - 1)) | ((row >> 4) & 1) * (kChunks / 2);
+  };
+
+  if (wave < n_sub) request(0);
   v8 qf[NQ][D / 32];
   int row_lo[NQ], row_hi[NQ];
 #pragma unroll
@@ -200,39 +269,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendA
   }
   // the tile's masks: no token ahead of `all_lo` or from `all_hi` on is hidden from some of its rows only
   const AttnRow first = attn_row(a, it, kRows, 0);
-  const int last_row = (int)min((long)kRows, (long)it.n_tokens * a.group - (long)it.tile * kRows) - 1;
+  const int last_row = min(kRows, it.n_tokens * a.group - it.tile * kRows) - 1;
   const AttnRow last = attn_row(a, it, kRows, last_row);
   const int all_lo = last.lo, all_hi = first.hi;
-
-  const int n_sub = (it.kv_end - it.kv_begin + kSub - 1) / kSub;
-  kv_uint4 rk[kLoads], rv[kLoads];
-  float ks = 0.f, vs = 0.f;                 // scales of token `lane` of the sub-tile
-  const int load_row = lane / kChunks, load_chunk = lane % kChunks;
-  auto request = [&](int t0) {
-    long at_k = 0, at_v = 0;
-#pragma unroll
-    for (int g = 0; g < kGroups; g++) {
-      const int token = min(t0 + 16 * g, (it.kv_end - 1) & ~15);
-      const long page = attn_page(a, it.seq, token);
-      const int slot = token & ((1 << a.page_shift) - 1);
-      const uint8_t* pk = static_cast<const uint8_t*>(a.ck.data) + (page * a.ck.page + head * a.ck.head + (slot + load_row) * a.ck.slot) * (kRowBytes / D) + 16 * load_chunk;
-      const uint8_t* pv = static_cast<const uint8_t*>(a.cv.data) + (page * a.cv.page + head * a.cv.head + (slot + load_row) * a.cv.slot) * (kRowBytes / D) + 16 * load_chunk;
-#pragma unroll
-      for (int j = 0; j < kGroupLoads; j++) {
-        rk[g * kGroupLoads + j] = *reinterpret_cast<const kv_uint4*>(pk + (long)j * kLoadRows * a.ck.slot * (kRowBytes / D));
-        rv[g * kGroupLoads + j] = *reinterpret_cast<const kv_uint4*>(pv + (long)j * kLoadRows * a.cv.slot * (kRowBytes / D));
-      }
-      if (KIND != kCacheSame && lane / 16 == g)
-        at_k = page * a.ck.scale_page + head * a.ck.scale_head + slot + col, at_v = page * a.cv.scale_page + head * a.cv.scale_head + slot + col;
-    }
-    if constexpr (KIND != kCacheSame) {
-      if (lane < kSub) ks = a.ck.scale[at_k] * a.scale_log2, vs = a.cv.scale[at_v];
-    }
-  };
-  auto key_of = [](int row) { return (row / kKeyRows) & (kChunks - 1); };
-  auto key_of_v = [](int row) {
-    return KIND == kCacheSame ? (row / kKeyRows << 1) & (kChunks - 1) : ((row / kKeyRows) & (kChunks / 2 - 1)) | ((row >> 4) & 1) * (kChunks / 2);
-  };
 
   attn_f4 o[NQ][D / 16];
   float m[NQ], l[NQ], norm = 0.f;           // norm: of the scales of V, so that P times a scale stays inside fp16
@@ -242,7 +281,6 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendA
 #pragma unroll
     for (int d = 0; d < D / 16; d++) o[n][d] = attn_f4{0.f, 0.f, 0.f, 0.f};
   }
-  if (wave < n_sub) request(it.kv_begin + wave * kSub);
   for (int sub = wave; sub < n_sub; sub += kAttnWaves) {
     const int t0 = it.kv_begin + sub * kSub;
     if (t0 + kSub > it.kv_end) {             // tokens behind the last: whatever the page holds there must not meet a zero of P
@@ -270,10 +308,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendA
     float norm_now = norm;                   // the largest scale of V so far
     if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) {
       if (lane < kSub && t0 + lane < it.kv_end) norm_now = fmaxf(norm, vs);
-#pragma unroll
-      for (int d = 32; d > 0; d /= 2) norm_now = fmaxf(norm_now, __shfl_xor(norm_now, d));
+      norm_now = attn_max16(across_row<16>(norm_now, [](float p, float q) { return fmaxf(p, q); }));
     }
-    if (sub + kAttnWaves < n_sub) request(t0 + kAttnWaves * kSub);
+    if (sub + kAttnWaves < n_sub) request((sub - wave) / kAttnWaves + 1);
 
     attn_f4 s[NQ][kGroups];
 #pragma unroll
@@ -310,14 +347,21 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendA
       for (int g = 0; g < kGroups; g++)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          float x = s[n][g][j] * (KIND == kCacheSame ? a.scale_log2 : scales[wave][0][16 * g + 4 * h + j]);
-          const int token = t0 + 16 * g + 4 * h + j;
-          if (edge && (token < row_lo[n] || token >= min(row_hi[n], it.kv_end))) x = -__builtin_inff();
-          s[n][g][j] = x;
-          top = fmaxf(top, x);
+          s[n][g][j] *= KIND == kCacheSame ? a.scale_log2 : scales[wave][0][16 * g + 4 * h + j];
+          top = fmaxf(top, s[n][g][j]);
         }
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
+      const int lo = row_lo[n] - t0 - 4 * h, hi = min(row_hi[n], it.kv_end) - t0 - 4 * h;
+      if (edge) {
+        top = kAttnNone;
+#pragma unroll
+        for (int g = 0; g < kGroups; g++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            s[n][g][j] = 16 * g + j < lo || 16 * g + j >= hi ? -__builtin_inff() : s[n][g][j];
+            top = fmaxf(top, s[n][g][j]);
+          }
+      }
+      top = attn_max16(top);
       float alpha = grown;
       if (__any(top > m[n] + kAttnSlack)) {
         const float next = fmaxf(m[n], top);
@@ -338,14 +382,18 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendA
         for (int j = 0; j < 4; j++) {
           const float e = __builtin_amdgcn_exp2f(s[n][g][j] - m[n]);
           l[n] += e;
-          const int token = t0 + 16 * g + 4 * h + j;
-          float w = e;
-          if constexpr (KIND != kCacheSame) {        // (a scale may be a NaN)
-            w = e * (scales[wave][1][16 * g + 4 * h + j] * inv);
-            if (edge && (token < row_lo[n] || token >= min(row_hi[n], it.kv_end))) w = 0.f;
-          }
-          p[n][g / 2][4 * (g % 2) + j] = (T)w;
+          s[n][g][j] = KIND == kCacheSame ? e : e * (scales[wave][1][16 * g + 4 * h + j] * inv);
         }
+      if (KIND != kCacheSame && edge) {              // (a scale may be a NaN)
+#pragma unroll
+        for (int g = 0; g < kGroups; g++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) s[n][g][j] = 16 * g + j < lo || 16 * g + j >= hi ? 0.f : s[n][g][j];
+      }
+#pragma unroll
+      for (int g = 0; g < kGroups; g++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) p[n][g / 2][4 * (g % 2) + j] = (T)s[n][g][j];
     }
     auto column = [&](int d, int b) {        // V of 32 tokens from 32 b on, as the MFMA's operand for columns 16 d ..
       if constexpr (KIND == kCacheSame) {
@@ -381,7 +429,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendA
     }
   }
 
-  // the wavefronts' results: the upper half's go to LDS and are taken in by the lower half, whose go there in turn
+  // the wavefronts' results: through LDS, the upper half's taken in by the lower half
 #pragma unroll
   for (int n = 0; n < NQ; n++) {
     l[n] += __shfl_xor(l[n], 16);
@@ -402,19 +450,24 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendA
 #pragma unroll
       for (int j = 0; j < 4; j++) o[n][d][j] *= f;
   }
+  // (rows that fill half a tile at most, as a decode step's of up to 8 heads do: all eight at once)
+  const bool once = last_row < kRows / 2;
+  const int met = once ? kAttnWaves : kAttnWaves / 2, met_rows = once ? kRows / 2 : kRows;
 #pragma unroll
   for (int upper = 1; upper >= 0; upper--) {
-    if ((wave >= kAttnWaves / 2) == (upper == 1)) {
+    if (once ? upper == 1 : (wave >= kAttnWaves / 2) == (upper == 1)) {
 #pragma unroll
       for (int n = 0; n < NQ; n++)
 #pragma unroll
         for (int d = 0; d < D / 16; d++) {
-          attn_f4* to = reinterpret_cast<attn_f4*>(meet + (wave % (kAttnWaves / 2) * kRows + 16 * n + col) * kStride + 16 * d + 4 * h);
+          attn_f4* to = reinterpret_cast<attn_f4*>(meet + (wave % met * met_rows + 16 * n + col) * kStride + 16 * d + 4 * h);
+          if (16 * n + col > last_row) continue;
           if (!upper) o[n][d] += *to;
           *to = o[n][d];
         }
     }
     __syncthreads();
+    if (once) break;
   }
   for (int i = threadIdx.x; i < kRows * (D / 4); i += 64 * kAttnWaves) {
     const int r = i / (D / 4), d = 4 * (i % (D / 4));
@@ -426,7 +479,11 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendA
 #pragma unroll
     for (int w = 0; w < kAttnWaves; w++) sum += meet_l[w][r] * __builtin_amdgcn_exp2f(meet_m[w][r] - top);
 #pragma unroll
-    for (int w = 0; w < kAttnWaves / 2; w++) x += *reinterpret_cast<const attn_f4*>(meet + (w * kRows + r) * kStride + d);
+    for (int w = 0; w < kAttnWaves / 2; w++) x += *reinterpret_cast<const attn_f4*>(meet + (w * met_rows + r) * kStride + d);
+    if (once) {
+#pragma unroll
+      for (int w = kAttnWaves / 2; w < kAttnWaves; w++) x += *reinterpret_cast<const attn_f4*>(meet + (w * met_rows + r) * kStride + d);
+    }
     if (it.part < 0) {
       const AttnRow row = attn_row(a, it, kRows, r);
       typedef T t4 __attribute__((ext_vector_type(4)));
@@ -465,39 +522,47 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, h = lane >> 5;
 
+  const int n_blocks = (it.kv_end - it.kv_begin + kAttnBlock - 1) / kAttnBlock;
+  kv_uint4 rk[kLoads], rv[kLoads];
+  float rs = 0.f;
+  const int load_row = lane / kHeldChunks, load_chunk = lane % kHeldChunks;
+  const int page_mask = (1 << a.page_shift) - 1;
+  const AttnHeld held_k(a.ck, head, kHeld / D, load_row, load_chunk), held_v(a.cv, head, kHeld / D, load_row, load_chunk);
+  const float *scale_k = a.ck.scale + head * a.ck.scale_head, *scale_v = a.cv.scale + head * a.cv.scale_head;
+  // a lane fetches the page of the wavefront's 16 tokens of one of the next 64 blocks
+  auto pages_from = [&](int i) {
+    const long token = it.kv_begin + (long)(i + lane) * kAttnBlock + 16 * wave;
+    return attn_page(a, it.seq, (int)min(token, (long)it.kv_end - 1));
+  };
+  int ids = n_blocks > 0 ? pages_from(0) : 0, next_ids = n_blocks > 64 ? pages_from(64) : 0;
+  auto request = [&](int i) {
+    if (i > 0 && i % 64 == 0) {
+      ids = next_ids;
+      if (n_blocks > i + 64) next_ids = pages_from(i + 64);
+    }
+    const long page = __builtin_amdgcn_readlane(ids, i % 64);
+    const int slot = min(it.kv_begin + i * kAttnBlock + 16 * wave, (it.kv_end - 1) & ~15) & page_mask;
+#pragma unroll
+    for (int j = 0; j < kLoads; j++) {
+      rk[j] = held_k.at(page, slot, j * kLoadRows);
+      rv[j] = held_v.at(page, slot, j * kLoadRows);
+    }
+    if constexpr (KIND != kCacheSame)
+      rs = lane < 16 ? scale_k[page * a.ck.scale_page + slot + lane] * a.scale_log2 : scale_v[page * a.cv.scale_page + slot + (lane & 15)];
+  };
+  if (n_blocks > 0) request(0);
   const AttnRow mine = attn_row(a, it, kAttnTileRows, 32 * wave + col);
   const T* q = static_cast<const T*>(a.q) + (it.q_start + mine.token) * a.q_token + (head * a.group + mine.head) * a.q_head;
   v8 qf[D / 16];
 #pragma unroll
   for (int s = 0; s < D / 16; s++) qf[s] = mine.live ? *reinterpret_cast<const v8*>(q + 16 * s + 8 * h) : v8{0, 0, 0, 0, 0, 0, 0, 0};
   // the limits of the wavefront's and the tile's first and last rows: tokens between are the same for all of them
-  const int n_rows = (int)min((long)kAttnTileRows, (long)it.n_tokens * a.group - (long)it.tile * kAttnTileRows);
+  const int n_rows = min(kAttnTileRows, it.n_tokens * a.group - it.tile * kAttnTileRows);
   const int wave_last = min(32 * wave + 31, n_rows - 1);
   const bool wave_live = 32 * wave < n_rows;
   const AttnRow w0 = attn_row(a, it, kAttnTileRows, 32 * wave), w1 = attn_row(a, it, kAttnTileRows, max(wave_last, 0));
   const AttnRow g0 = attn_row(a, it, kAttnTileRows, 0), g1 = attn_row(a, it, kAttnTileRows, n_rows - 1);
 
-  const int n_blocks = (it.kv_end - it.kv_begin + kAttnBlock - 1) / kAttnBlock;
-  kv_uint4 rk[kLoads], rv[kLoads];
-  float rs = 0.f;
-  const int load_row = lane / kHeldChunks, load_chunk = lane % kHeldChunks;
-  auto request = [&](int t0) {
-    const int token = min(t0 + 16 * wave, (it.kv_end - 1) & ~15);
-    const long page = attn_page(a, it.seq, token);
-    const int slot = token & ((1 << a.page_shift) - 1);
-    const uint8_t* pk = static_cast<const uint8_t*>(a.ck.data) + (page * a.ck.page + head * a.ck.head + (slot + load_row) * a.ck.slot) * (kHeld / D) + 16 * load_chunk;
-    const uint8_t* pv = static_cast<const uint8_t*>(a.cv.data) + (page * a.cv.page + head * a.cv.head + (slot + load_row) * a.cv.slot) * (kHeld / D) + 16 * load_chunk;
-#pragma unroll
-    for (int j = 0; j < kLoads; j++) {
-      rk[j] = *reinterpret_cast<const kv_uint4*>(pk + (long)j * kLoadRows * a.ck.slot * (kHeld / D));
-      rv[j] = *reinterpret_cast<const kv_uint4*>(pv + (long)j * kLoadRows * a.cv.slot * (kHeld / D));
-    }
-    if constexpr (KIND != kCacheSame) {
-      const int i = lane & 15;
-      rs = lane < 16 ? a.ck.scale[page * a.ck.scale_page + head * a.ck.scale_head + slot + i] * a.scale_log2
-                     : a.cv.scale[page * a.cv.scale_page + head * a.cv.scale_head + slot + i];
-    }
-  };
   auto key_of = [](int row) { return (row / kKeyRows) & (kChunks - 1); };
   auto key_of_v = [](int row) { return (row / kKeyRows << 2) & (kChunks - 1); };
   // the registers' 16 tokens of the block at t0 into place `at`
@@ -550,16 +615,15 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a) {
   float m = kAttnNone, l = 0.f, norm = 0.f;
 
   if (n_blocks > 0) {
-    request(it.kv_begin);
     keep(it.kv_begin, 0);
-    if (n_blocks > 1) request(it.kv_begin + kAttnBlock);
+    if (n_blocks > 1) request(1);
   }
   __syncthreads();
   for (int block = 0; block < n_blocks; block++) {
     const int t0 = it.kv_begin + block * kAttnBlock, at = block & 1;
     if (block + 1 < n_blocks) {
       keep(t0 + kAttnBlock, at ^ 1);
-      if (block + 2 < n_blocks) request(t0 + 2 * kAttnBlock);
+      if (block + 2 < n_blocks) request(block + 2);
     }
     if (wave_live && t0 < min(w1.hi, it.kv_end) && t0 + kAttnBlock > w0.lo) {
       // (one lane constant each, kept from being spread over a register for every address)
@@ -578,8 +642,7 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a) {
       float grown = 1.f;
       if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) {
         float top = t0 + lane < it.kv_end ? fmaxf(norm, scales[at][1][lane]) : norm;
-#pragma unroll
-        for (int d = 32; d > 0; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
+        top = attn_max16(across_row<16>(top, [](float p, float q) { return fmaxf(p, q); }));
         if (top > norm) grown = norm / top, norm = top;
       }
       float top = kAttnNone;
@@ -588,15 +651,22 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a) {
       for (int g = 0; g < 2; g++)
 #pragma unroll
         for (int j = 0; j < 16; j++) {
-          const int token = 32 * g + 8 * (j / 4) + j % 4;
-          float x = s[g][j];
-          if constexpr (KIND != kCacheSame) x *= scales[at][0][token + 4 * h];
-          if (edge) x = token < lo || token >= hi ? -__builtin_inff() : x;
-          s[g][j] = x;
-          top = fmaxf(top, x);
+          if constexpr (KIND != kCacheSame) s[g][j] *= scales[at][0][32 * g + 8 * (j / 4) + j % 4 + 4 * h];
+          top = fmaxf(top, s[g][j]);
         }
+      if (edge) {
+        top = kAttnNone;
+#pragma unroll
+        for (int g = 0; g < 2; g++)
+#pragma unroll
+          for (int j = 0; j < 16; j++) {
+            const int token = 32 * g + 8 * (j / 4) + j % 4;
+            s[g][j] = token < lo || token >= hi ? -__builtin_inff() : s[g][j];
+            top = fmaxf(top, s[g][j]);
+          }
+      }
       if constexpr (KIND == kCacheSame) top = fmaxf(top * a.scale_log2, kAttnNone);
-      top = fmaxf(top, __shfl_xor(top, 32));
+      top = attn_max32(top);
       float alpha = grown;
       if (__any(top > m + kAttnSlack)) {
         const float next = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - next);
@@ -614,15 +684,23 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a) {
       for (int g = 0; g < 2; g++)
 #pragma unroll
         for (int j = 0; j < 16; j++) {
-          const int token = 32 * g + 8 * (j / 4) + j % 4;
-          float e = __builtin_amdgcn_exp2f(KIND == kCacheSame ? __builtin_fmaf(s[g][j], a.scale_log2, -m) : s[g][j] - m);
+          const float e = __builtin_amdgcn_exp2f(KIND == kCacheSame ? __builtin_fmaf(s[g][j], a.scale_log2, -m) : s[g][j] - m);
           l += e;
-          if constexpr (KIND != kCacheSame) {
-            e *= scales[at][1][token + 4 * h] * inv;
-            if (edge) e = token < lo || token >= hi ? 0.f : e;     // (a scale may be a NaN)
-          }
-          p[2 * g + j / 8][j % 8] = (T)e;
+          s[g][j] = KIND == kCacheSame ? e : e * (scales[at][1][32 * g + 8 * (j / 4) + j % 4 + 4 * h] * inv);
         }
+      if (KIND != kCacheSame && edge) {              // (a scale may be a NaN)
+#pragma unroll
+        for (int g = 0; g < 2; g++)
+#pragma unroll
+          for (int j = 0; j < 16; j++) {
+            const int token = 32 * g + 8 * (j / 4) + j % 4;
+            s[g][j] = token < lo || token >= hi ? 0.f : s[g][j];
+          }
+      }
+#pragma unroll
+      for (int g = 0; g < 2; g++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) p[2 * g + j / 8][j % 8] = (T)s[g][j];
       auto column = [&](int d, int b) {      // V of 16 tokens from 16 b on, columns 32 d ..
         return attn_transposed<T>(lds, (at_v ^ (64 * d)) + 16 * b * kRowBytes, (at_v ^ (64 * d)) + (16 * b + 8) * kRowBytes);
       };
