@@ -3,6 +3,8 @@
 
 namespace {
 
+constexpr int kRotaryWalks = 65535;    // (what a grid takes along its second dimension)
+
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // rows of `dim` adjacent elements of `size` bytes, `align` of them at a time
@@ -43,32 +45,34 @@ CachePart cache_part(const void* data, const void* scale, const long* strides, c
 
 template <class T, int KIND, int LPR, int U>
 void launch_rotary(const RotaryArgs& a, int interleaved, hipStream_t stream) {
-  // small batches: a workgroup for every pass, so that all of them are on their way together; large ones: a workgroup walks whole tokens
-  const int rows = a.heads + a.kv_heads * (a.v ? 2 : 1), per = 256 / LPR * U;
-  const dim3 grid(U == 1 ? (rows + per - 1) / per : 1, U == 1 ? a.tokens < 65535 ? a.tokens : 65535 : a.tokens < 2048 ? a.tokens : 2048);
+  const dim3 grid((RotaryPasses(a, 256 / LPR).all() + U - 1) / U, a.tokens < kRotaryWalks ? a.tokens : kRotaryWalks);
   if (a.q_norm || a.k_norm) hipLaunchKernelGGL((rotary_cache_kernel<T, KIND, LPR, U, true>), grid, dim3(256), 0, stream, a, interleaved);
   else hipLaunchKernelGGL((rotary_cache_kernel<T, KIND, LPR, U, false>), grid, dim3(256), 0, stream, a, interleaved);
 }
+template <class T, int KIND, int LPR>
+void launch_rotary(const RotaryArgs& a, int interleaved, hipStream_t stream) {
+  // small batches: a workgroup for every pass of 256 lanes; once that would be more than two for every CU, one for six of them
+  if ((long)RotaryPasses(a, 256 / LPR).all() * a.tokens > 512) launch_rotary<T, KIND, LPR, 6>(a, interleaved, stream);
+  else launch_rotary<T, KIND, LPR, 1>(a, interleaved, stream);
+}
 template <class T, int KIND>
 void launch_rotary_lanes(const RotaryArgs& a, int interleaved, hipStream_t stream) {
-  // four rows a lane once a pass of single rows would be more than two workgroups for every CU
-  const long rows = a.heads + a.kv_heads * (a.v ? 2 : 1);
-  const int lanes = a.dim <= 64 ? 8 : a.dim <= 128 ? 16 : 32;
-  const bool many = rows * a.tokens * lanes > 512L * 256;
-  if (lanes == 8) many ? launch_rotary<T, KIND, 8, 4>(a, interleaved, stream) : launch_rotary<T, KIND, 8, 1>(a, interleaved, stream);
-  else if (lanes == 16) many ? launch_rotary<T, KIND, 16, 4>(a, interleaved, stream) : launch_rotary<T, KIND, 16, 1>(a, interleaved, stream);
-  else many ? launch_rotary<T, KIND, 32, 4>(a, interleaved, stream) : launch_rotary<T, KIND, 32, 1>(a, interleaved, stream);
+  if (a.dim <= 64) launch_rotary<T, KIND, 8>(a, interleaved, stream);
+  else if (a.dim <= 128) launch_rotary<T, KIND, 16>(a, interleaved, stream);
+  else launch_rotary<T, KIND, 32>(a, interleaved, stream);
 }
 
+template <class T, int KIND, int LPR, int U>
+void launch_read_tiles(const CacheReadArgs& a, hipStream_t stream) {
+  constexpr long tokens = 256 / LPR * U / 4;
+  const dim3 grid((unsigned)((a.tokens + tokens - 1) / tokens * ((a.kv_heads + 3) / 4)), 2);
+  hipLaunchKernelGGL((cache_read_kernel<T, KIND, LPR, U>), grid, dim3(256), 0, stream, a);
+}
 template <class T, int KIND>
 void launch_read(const CacheReadArgs& a, hipStream_t stream) {
-  const long rows = (long)a.tokens * a.kv_heads;
-  const int lanes = a.dim <= 64 ? 8 : a.dim <= 128 ? 16 : 32;
-  const long per = 256 / lanes * 4;
-  const dim3 grid((unsigned)((rows + per - 1) / per), 2);
-  if (lanes == 8) hipLaunchKernelGGL((cache_read_kernel<T, KIND, 8, 4>), grid, dim3(256), 0, stream, a);
-  else if (lanes == 16) hipLaunchKernelGGL((cache_read_kernel<T, KIND, 16, 4>), grid, dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((cache_read_kernel<T, KIND, 32, 4>), grid, dim3(256), 0, stream, a);
+  if (a.dim <= 64) launch_read_tiles<T, KIND, 8, 4>(a, stream);
+  else if (a.dim <= 128) launch_read_tiles<T, KIND, 16, 4>(a, stream);
+  else launch_read_tiles<T, KIND, 32, 4>(a, stream);
 }
 
 // the activations' type and what the cache holds, as template arguments
@@ -104,14 +108,14 @@ void launch_attend(AttendArgs a, const AttnLayout& layout, float* scratch, long 
     if (l.max_items == 0) continue;
     a.list = l, a.which = which;
     a.part_o = scratch;
-    a.part_ml = scratch + (long)l.max_items * a.kv_heads * l.rows * D;
-    scratch = a.part_ml + 2L * l.max_items * a.kv_heads * l.rows;
+    a.part_ml = scratch + (long)l.max_parts * a.kv_heads * l.rows * D;
+    scratch = a.part_ml + 2L * l.max_parts * a.kv_heads * l.rows;
     const dim3 grid((unsigned)((long)l.max_items * a.kv_heads));
     if (which == 1) hipLaunchKernelGGL((attend_tile_kernel<T, KIND, D>), grid, dim3(256), 0, stream, a);
     else if (l.rows == 16) hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 1>), grid, dim3(64 * kAttnWaves), 0, stream, a);
     else hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 2>), grid, dim3(64 * kAttnWaves), 0, stream, a);
     // (no sequence is longer than its pages)
-    if (table_tokens > (long)l.min_blocks * kAttnBlock) hipLaunchKernelGGL((attend_join_kernel<T, D>), dim3(l.max_joins * a.kv_heads, l.rows / 16), dim3(1024), 0, stream, a);
+    if (l.max_joins > 0 && table_tokens > (long)l.min_blocks * kAttnBlock) hipLaunchKernelGGL((attend_join_kernel<T, D>), dim3(l.max_joins * a.kv_heads, l.rows / 16), dim3(1024), 0, stream, a);
   }
 }
 struct AttendLaunch {
@@ -167,13 +171,13 @@ int triteia_hip_rotary_cache(const void* q, long q_token, long q_head, const voi
   }
   if (tokens == 0 || (heads == 0 && kv_heads == 0)) return TRITEIA_HIP_OK;
   if ((heads && (!q || !q_out)) || (kv_heads && !k) || (to_cache ? !v || !slots || k_out : kv_heads && !k_out)) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: null tensor pointer", what);
-  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(q_out) || !aligned16(k_out) || !aligned16(table) ||
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(q_out) || !aligned16(k_out) || !aligned16(table) || !aligned16(q_norm) || !aligned16(k_norm) ||
       !strides_ok({q_token, q_head, k_token, k_head, v_token, v_head}, 2, 16))
-    return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: rows need 16-byte alignment", what);
+    return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: rows, table and norms need 16-byte alignment", what);
   a.q = q, a.k = k, a.v = v, a.q_token = q_token, a.q_head = q_head, a.k_token = k_token, a.k_head = k_head, a.v_token = v_token, a.v_head = v_head;
   a.q_out = q_out, a.k_out = k_out, a.tokens = tokens, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim, a.rot = rot;
   a.positions = positions, a.positions64 = positions64, a.table = static_cast<const float*>(table), a.limit = limit;
-  a.q_norm = q_norm, a.k_norm = k_norm, a.eps = eps;
+  a.q_norm = q_norm, a.k_norm = k_norm, a.eps = eps, a.inv_dim = 1.f / dim;
   DeviceGuard g(dev);
   if (!g.ok) return fail(TRITEIA_HIP_ERR_RUNTIME, "cannot select device %d", dev);
   by_types(bf16, to_cache ? kind : kCacheSame, RotaryLaunch{a, interleaved, static_cast<hipStream_t>(stream)});
@@ -189,7 +193,7 @@ int triteia_hip_cache_read(const void* cache_k, const void* cache_v, const void*
   a.ck = cache_part(cache_k, k_scale, strides, strides + 6);
   a.cv = cache_part(cache_v, v_scale, strides + 3, strides + 9);
   if (const int e = check_cache(what, a.ck, a.cv, n_pages, kv_heads, page, dim, kind)) return e;
-  if (tokens < 0 || (long)tokens * kv_heads > (1L << 36)) return fail(TRITEIA_HIP_ERR_PROB_SHAPE, "%s: %d tokens of %d heads", what, tokens, kv_heads);
+  if (tokens < 0 || (long)tokens * kv_heads > (1L << 31)) return fail(TRITEIA_HIP_ERR_PROB_SHAPE, "%s: %d tokens of %d heads", what, tokens, kv_heads);
   if (tokens == 0) return TRITEIA_HIP_OK;
   if (!slots || !k_out || !v_out) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: null tensor pointer", what);
   if (!aligned16(k_out) || !aligned16(v_out)) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: outputs need 16-byte alignment", what);
@@ -210,7 +214,7 @@ size_t triteia_hip_attention_scratch_bytes(int n_seqs, int n_tokens, int heads, 
   if (check_batch("paged_attention", n_seqs, n_tokens, heads, kv_heads, max_q, 1, 0)) return 0;
   const AttnLayout l = attn_layout(n_seqs, n_tokens, heads, kv_heads, max_q, 1, 0);
   size_t bytes = 0;
-  for (const AttnList& x : l.list) bytes += 4 * (size_t)x.max_items * kv_heads * x.rows * (dim + 2);
+  for (const AttnList& x : l.list) bytes += 4 * (size_t)x.max_parts * kv_heads * x.rows * (dim + 2);
   return bytes;
 }
 

@@ -18,7 +18,6 @@ namespace triteia_hip {
 
 constexpr int kAttnBlock = 64;         // tokens of a block: shares begin and end on its multiples
 constexpr int kAttnTileRows = 128;     // rows of a tile of the long list
-constexpr int kAttnRounds = 4;         // lists of this many rounds of workgroups and more are not cut
 constexpr int kAttnSorted = 256;       // lists of up to this many tiles begin with the longest
 constexpr int kAttnMaxSeqs = 4096;
 constexpr int kAttnPlanThreads = 128;
@@ -37,6 +36,8 @@ struct AttnList {
   int max_items, max_joins;
   long items, joins;     // where they start in the plan, in ints
   int slots, min_blocks; // workgroups that run side by side, and the least length of a share
+  int rounds;            // lists of this many rounds of workgroups and more are not cut
+  int max_parts;
 };
 
 struct AttnLayout {
@@ -56,11 +57,18 @@ inline AttnLayout attn_layout(int n_seqs, int n_tokens, int heads, int kv_heads,
   AttnList &s = a.list[0], &l = a.list[1];
   s.rows = only_short ? (most <= 16 ? 16 : 32) : a.group <= 16 ? 16 : 32;
   a.short_rows = only_short ? 0x7fffffff : s.rows;
-  s.slots = 256, s.min_blocks = 16, l.slots = 512, l.min_blocks = 8;
+  s.slots = 256, s.min_blocks = 16, s.rounds = 4, l.slots = 512, l.min_blocks = 8, l.rounds = 2;
   l.rows = kAttnTileRows;
-  const long s_tiles = only_short ? live + rows / s.rows : live, l_tiles = only_short ? 0 : live + rows / l.rows;
-  s.max_joins = kAttnRounds * s.slots / kv_heads + 1, l.max_joins = only_short ? 0 : kAttnRounds * l.slots / kv_heads + 1;
-  s.max_items = (int)(s_tiles + s.max_joins), l.max_items = (int)(l_tiles + l.max_joins);
+  const long tiles[2] = {only_short ? live + rows / s.rows : live, only_short ? 0 : live + rows / l.rows};
+  for (int which = 0; which < 2; which++) {
+    AttnList& x = a.list[which];
+    // (as the kernel cuts them: into the shares of whole rounds of workgroups; a cut tile has two at least)
+    const long units = tiles[which] * kv_heads, whole = units < (long)x.rounds * x.slots ? units : (long)x.rounds * x.slots;
+    const long shares = (whole + x.slots - 1) / x.slots * x.slots / kv_heads;
+    x.max_joins = (int)(tiles[which] < shares / 2 ? tiles[which] : shares / 2);
+    x.max_parts = (int)(tiles[which] > 0 ? shares : 0);
+    x.max_items = (int)(tiles[which] > shares ? tiles[which] : shares);
+  }
   long at = 8;
   for (AttnList& x : a.list) {
     x.items = at, at += 8L * x.max_items;
@@ -149,7 +157,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const 
   // Few tiles: the least share with which all shares still run in as many rounds as the tiles would.
   int share = 0x7fffffff;
   const long units = (long)tiles * a.kv_heads;
-  if (units < (long)kAttnRounds * l.slots) {
+  if (units < (long)l.rounds * l.slots) {
     const int most = (int)((units + l.slots - 1) / l.slots * l.slots / a.kv_heads);        // shares of one head
     long work = 0;
     for (int i0 = 0; i0 < tiles; i0 += 64) work += i0 + lane < tiles ? at(i0 + lane).blocks : 0;

@@ -43,7 +43,7 @@ struct RotaryArgs {
   const float* table;           // [limit, rot / 2, 2]
   long limit;
   const void *q_norm, *k_norm;  // null: none
-  float eps;
+  float eps, inv_dim;
   const void* slots;
   int positions64, slots64;
   int page_shift;
@@ -53,6 +53,12 @@ struct RotaryArgs {
 
 __device__ __forceinline__ long index_at(const void* p, int wide, long i) {
   return wide ? static_cast<const int64_t*>(p)[i] : (long)static_cast<const int32_t*>(p)[i];
+}
+// The same for an index that all lanes share, from memory that the kernel does not write: a scalar load.
+__device__ __forceinline__ long shared_index_at(const void* p, int wide, long i) {
+  typedef const __attribute__((address_space(4))) int64_t* Wide;
+  typedef const __attribute__((address_space(4))) int32_t* Narrow;
+  return wide ? reinterpret_cast<Wide>(reinterpret_cast<uintptr_t>(p))[i] : (long)reinterpret_cast<Narrow>(reinterpret_cast<uintptr_t>(p))[i];
 }
 
 // 8 values as codes of the row's scale; inv = 1 / scale
@@ -135,108 +141,135 @@ __device__ __forceinline__ void cache_row(const CachePart& c, long page, long he
   }
 }
 
-// grid (chunks of a token's rows, tokens), block 256.  A token's rows: heads of q, heads of k, heads of v.
+// Passes of 256 / LPR rows over a token's heads of q, of k and of v, none of two kinds.
+struct RotaryPasses {
+  int q, k, v;
+  __host__ __device__ RotaryPasses(const RotaryArgs& a, int rows) : q((a.heads + rows - 1) / rows), k((a.kv_heads + rows - 1) / rows), v(a.v ? k : 0) {}
+  __host__ __device__ int all() const { return q + k + v; }
+};
+
+__device__ __forceinline__ void kv_to_lds(const void* src, void* dst) {      // 16 bytes a lane, to dst + 16 lane
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(uintptr_t)src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+}
+
+// grid (passes of a token / U, tokens), block 256; with fewer workgroups than tokens they walk them.  The rows of U passes are requested together, by
+// direct loads to LDS, and worked on one after the other: held in registers the compiler runs them side by side in 120 to 220 of these, and the
+// wavefronts that are missing then cost more.  A wavefront reads what it has loaded itself, the element across a pair from its neighbour's place.  What does not depend on the row is multiplied first: cos and sin with the norm's weights, once for q and once for k of a token.
 template <class T, int KIND, int LPR, int U, bool NORM>
 __global__ __launch_bounds__(256) void rotary_cache_kernel(RotaryArgs a, int interleaved) {
   constexpr int kRows = 256 / LPR;                 // rows of a pass
-  const int lane = threadIdx.x % LPR, e = 8 * lane;
+  const int lane = threadIdx.x % LPR, e = 8 * lane, row = threadIdx.x / LPR;
   const bool live = e < a.dim;
-  const int n_rows = a.heads + a.kv_heads * (a.v ? 2 : 1);
+  const RotaryPasses passes(a, kRows);
   const int half = a.rot / 2;
   const bool turned = a.positions && e < a.rot, first = e < half;
   const int across = interleaved || !turned ? lane : first ? lane + half / 8 : lane - half / 8;
+  const int pair = interleaved ? e / 2 : first ? e : e - half;      // of this lane's first element
   const kv8<T> none = {0, 0, 0, 0, 0, 0, 0, 0};
-  kv8<T> w[2], wx[2];             // norm weights of this lane's elements and of those across, for q and k
-  if constexpr (NORM) {
-#pragma unroll
-    for (int n = 0; n < 2; n++) {
-      const T* src = static_cast<const T*>(n ? a.k_norm : a.q_norm);
-      w[n] = src && live ? *reinterpret_cast<const kv8<T>*>(src + e) : none;
-      wx[n] = src && live ? *reinterpret_cast<const kv8<T>*>(src + 8 * across) : none;
-      if (interleaved) wx[n] = __builtin_shufflevector(w[n], w[n], 1, 0, 3, 2, 5, 4, 7, 6);
-    }
-  }
+  __shared__ kv8<T> xs[U][256];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), beside = (int)threadIdx.x - lane + across;
+  __shared__ kv8<T> weights[2][LPR];
+  bool settled = !NORM;
   for (long t = blockIdx.y; t < a.tokens; t += gridDim.y) {
-    long page = 0, slot = -1;
-    if (a.slots) {
-      const long s = index_at(a.slots, a.slots64, t);
-      if (s >= 0 && s < a.n_slots) page = s >> a.page_shift, slot = s & ((1 << a.page_shift) - 1);
-    }
-    // this lane's cos and sin: pairs e / 2 .. + 3 (interleaved) or e % (R / 2) .. + 7, minus in front of the sine of a pair's first element
-    float c[8], s[8];
+    const long position = a.positions ? shared_index_at(a.positions, a.positions64, t) : 0, to = a.slots ? shared_index_at(a.slots, a.slots64, t) : -1;
+    auto request = [&](int pass, int u) {
+      const T* src;
+      int head = row;
+      long step;
+      if (pass < passes.q) src = static_cast<const T*>(a.q) + t * a.q_token, step = a.q_head, head += pass * kRows;
+      else if (pass < passes.q + passes.k) src = static_cast<const T*>(a.k) + t * a.k_token, step = a.k_head, head += (pass - passes.q) * kRows;
+      else src = static_cast<const T*>(a.v) + t * a.v_token, step = a.v_head, head += (pass - passes.q - passes.k) * kRows;
+      if (live && head < (pass < passes.q ? a.heads : a.kv_heads)) kv_to_lds(src + head * step + e, &xs[u][64 * wave]);
+    };
+    const int pass0 = blockIdx.x * U, n = min(U, passes.all() - pass0);
+    for (int u = 0; u < n; u++) request(pass0 + u, u);
+    kv_float4 f[4];                 // cos and sin of this lane's pairs: 4 of them (interleaved) or 8
+    const bool inside = position >= 0 && position < a.limit;
     if (turned) {
-      const long p = index_at(a.positions, a.positions64, t);
-      const bool inside = p >= 0 && p < a.limit;
-      const int pair = interleaved ? e / 2 : first ? e : e - half;
-      const kv_float4* row = reinterpret_cast<const kv_float4*>(a.table + (inside ? p : 0) * a.rot + 2 * pair);
-      kv_float4 f[4];
+      const kv_float4* at = reinterpret_cast<const kv_float4*>(a.table + (inside ? position : 0) * a.rot + 2 * pair);
 #pragma unroll
-      for (int i = 0; i < 4; i++) f[i] = i < 2 || !interleaved ? row[i] : kv_float4{0.f, 0.f, 0.f, 0.f};
-      if (!inside) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) f[i] = kv_float4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
-      }
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        c[j] = interleaved ? f[j / 4][j / 2 % 2 * 2] : f[j / 2][j % 2 * 2];
-        s[j] = interleaved ? f[j / 4][j / 2 % 2 * 2 + 1] : f[j / 2][j % 2 * 2 + 1];
-        if (interleaved ? j % 2 == 0 : first) s[j] = -s[j];
-      }
+      for (int i = 0; i < 4; i++) f[i] = at[i < 2 || !interleaved ? i : 0];
     }
-    for (int row0 = blockIdx.x * (kRows * U) + threadIdx.x / LPR; row0 < n_rows + (int)(threadIdx.x / LPR); row0 += gridDim.x * (kRows * U)) {
-      kv8<T> x[U];
-#pragma unroll
-      for (int u = 0; u < U; u++) {
-        const int r = row0 + u * kRows;
-        const T* src = r < a.heads ? static_cast<const T*>(a.q) + t * a.q_token + r * a.q_head
-                       : r < a.heads + a.kv_heads ? static_cast<const T*>(a.k) + t * a.k_token + (r - a.heads) * a.k_head
-                                                  : static_cast<const T*>(a.v) + t * a.v_token + (r - a.heads - a.kv_heads) * a.v_head;
-        x[u] = live && r < n_rows ? *reinterpret_cast<const kv8<T>*>(src + e) : none;
+    if (!settled) {                 // (behind the requests of the first token)
+      for (int i = threadIdx.x; i < 2 * LPR; i += 256) {
+        const T* src = static_cast<const T*>(i < LPR ? a.q_norm : a.k_norm);
+        if (src && 8 * (i % LPR) < a.dim) weights[i / LPR][i % LPR] = *reinterpret_cast<const kv8<T>*>(src + 8 * (i % LPR));
       }
+      __syncthreads();
+      settled = true;
+    }
+    const bool kept = to >= 0 && to < a.n_slots;
+    const long page = kept ? to >> a.page_shift : 0, slot = kept ? to & ((1 << a.page_shift) - 1) : -1;
+    float c[8], s[8];               // what this lane's elements and those across are multiplied by
+    int kind = -1;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll 1
+    for (int u = 0; u < n; u++) {
+      const int pass = pass0 + u;
+      const kv8<T> x = live ? xs[u][threadIdx.x] : none;
+      const int now = pass < passes.q ? 0 : pass < passes.q + passes.k ? 1 : 2;
+      const int head = row + kRows * (pass - (now == 0 ? 0 : now == 1 ? passes.q : passes.q + passes.k));
+      const T* weight = static_cast<const T*>(now == 0 ? a.q_norm : a.k_norm);
+      float y[8];
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        const int r = row0 + u * kRows;
-        const bool is_q = r < a.heads, is_v = r >= a.heads + a.kv_heads;
-        float y[8], o[8];          // own elements, and those across
-        const kv_uint4 mine = __builtin_bit_cast(kv_uint4, x[u]);
-        kv8<T> xo;
-        if (interleaved) {
-          xo = __builtin_shufflevector(x[u], x[u], 1, 0, 3, 2, 5, 4, 7, 6);
-        } else {
-          kv_uint4 other;
+      for (int j = 0; j < 8; j++) y[j] = (float)x[j];
+      if (now != 2) {
+        if (now != kind) {
+          kind = now;
+          if (turned && interleaved) {
 #pragma unroll
-          for (int i = 0; i < 4; i++) other[i] = (uint32_t)__shfl((int)mine[i], across, LPR);
-          xo = __builtin_bit_cast(kv8<T>, other);
+            for (int j = 0; j < 8; j++) c[j] = f[j / 4][j / 2 % 2 * 2], s[j] = j % 2 ? f[j / 4][j / 2 % 2 * 2 + 1] : -f[j / 4][j / 2 % 2 * 2 + 1];
+          } else if (turned) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) c[j] = f[j / 2][j % 2 * 2], s[j] = first ? -f[j / 2][j % 2 * 2 + 1] : f[j / 2][j % 2 * 2 + 1];
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) c[j] = 1.f, s[j] = 0.f;
+          }
+          if (turned && !inside) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) c[j] = __builtin_nanf("");
+          }
+          if (NORM && weight && live) {
+            const kv8<T> w = weights[now][lane], wx = weights[now][across], wi = __builtin_shufflevector(w, w, 1, 0, 3, 2, 5, 4, 7, 6);
+#pragma unroll
+            for (int j = 0; j < 8; j++) c[j] *= (float)w[j], s[j] *= interleaved ? (float)wi[j] : (float)wx[j];
+          }
         }
+        float z[8];
+        if (interleaved) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) y[j] = (float)x[u][j], o[j] = (float)xo[j];
-        if constexpr (NORM) {
+          for (int j = 0; j < 8; j++) z[j] = turned ? y[j ^ 1] : 0.f;
+        } else {
+          const kv8<T> far = turned ? xs[u][beside] : none;                // (zero times an infinity would be a NaN)
+#pragma unroll
+          for (int j = 0; j < 8; j++) z[j] = (float)far[j];
+        }
+        float norm = 1.f;
+        if (NORM && weight) {
           float sum = 0.f;
 #pragma unroll
           for (int j = 0; j < 8; j++) sum = __builtin_fmaf(y[j], y[j], sum);
           sum = across_row<LPR>(sum, [](float p, float q) { return p + q; });
-          if (!is_v && (is_q ? a.q_norm : a.k_norm) != nullptr) {
-            const float f = __builtin_amdgcn_rsqf(sum / a.dim + a.eps);
-            const kv8<T> own = is_q ? w[0] : w[1], far = is_q ? wx[0] : wx[1];
-#pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = y[j] * f * (float)own[j], o[j] = o[j] * f * (float)far[j];
-          }
+          norm = __builtin_amdgcn_rsqf(__builtin_fmaf(sum, a.inv_dim, a.eps));
         }
-        if (turned && !is_v) {
 #pragma unroll
-          for (int j = 0; j < 8; j++) y[j] = __builtin_fmaf(o[j], s[j], y[j] * c[j]);
-        }
-        if (r < n_rows && (is_q || a.k_out)) {
-          kv8<T> out;
-#pragma unroll
-          for (int j = 0; j < 8; j++) out[j] = (T)y[j];
-          T* dst = is_q ? static_cast<T*>(a.q_out) + (t * a.heads + r) * a.dim : static_cast<T*>(a.k_out) + (t * a.kv_heads + r - a.heads) * a.dim;
-          if (live) *reinterpret_cast<kv8<T>*>(dst + e) = out;
-        } else if (r < n_rows && slot >= 0) {
-          cache_row<T, KIND, LPR>(is_v ? a.cv : a.ck, page, is_v ? r - a.heads - a.kv_heads : r - a.heads, slot, e, live, y);
+        for (int j = 0; j < 8; j++) {
+          y[j] = __builtin_fmaf(z[j], s[j], y[j] * c[j]);
+          if (NORM && weight) y[j] *= norm;
         }
       }
+      if (now == 0 || a.k_out) {
+        kv8<T> out;
+#pragma unroll
+        for (int j = 0; j < 8; j++) out[j] = (T)y[j];
+        T* dst = now == 0 ? static_cast<T*>(a.q_out) + (t * a.heads + head) * a.dim : static_cast<T*>(a.k_out) + (t * a.kv_heads + head) * a.dim;
+        if (live && head < (now == 0 ? a.heads : a.kv_heads)) *reinterpret_cast<kv8<T>*>(dst + e) = out;
+      } else if (slot >= 0 && head < a.kv_heads) {
+        cache_row<T, KIND, LPR>(now == 2 ? a.cv : a.ck, page, head, slot, e, live, y);
+      }
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                      // (the next token's rows go where these were read)
   }
 }
 
@@ -248,26 +281,27 @@ struct CacheReadArgs {
   long n_slots;
 };
 
-// grid (chunks of rows, 2: keys, values), block 256; rows in the order of the output (token, head).  A slot outside the cache gives zeros.
+// grid (tiles, 2: keys, values), block 256.  A tile is 4 heads of adjacent tokens, whose rows of a head lie side by side in a page.  A slot
+// outside the cache gives zeros.
 template <class T, int KIND, int LPR, int U>
 __global__ __launch_bounds__(256) void cache_read_kernel(CacheReadArgs a) {
-  constexpr int kRows = 256 / LPR;
+  constexpr int kRows = 256 / LPR, kTokens = kRows * U / 4;
   const int e = 8 * (threadIdx.x % LPR);
   const CachePart& c = blockIdx.y ? a.cv : a.ck;
   T* out = static_cast<T*>(blockIdx.y ? a.v_out : a.k_out);
-  const long n_rows = (long)a.tokens * a.kv_heads;
-  const long row0 = (long)blockIdx.x * (kRows * U) + threadIdx.x / LPR;
-  if (e >= a.dim) return;
+  const uint32_t heads4 = ((uint32_t)a.kv_heads + 3) / 4, tile = blockIdx.x / heads4;
+  const int row0 = threadIdx.x / LPR;
+  const int head = 4 * (int)(blockIdx.x - tile * heads4) + row0 % 4;
+  if (e >= a.dim || head >= a.kv_heads) return;
+  const long t0 = (long)tile * kTokens + row0 / 4;
   kv8<T> x[U];
   kv_uint2 code[U];
   float scale[U];
   bool inside[U];
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    const long r = row0 + u * kRows;
-    const uint32_t t = (uint32_t)((uint64_t)(r < n_rows ? r : n_rows - 1) / (uint32_t)a.kv_heads);
-    const long head = (r < n_rows ? r : n_rows - 1) - (long)t * a.kv_heads;
-    const long s = index_at(a.slots, a.slots64, t);
+    const long t = t0 + u * (kRows / 4);
+    const long s = t < a.tokens ? index_at(a.slots, a.slots64, t) : -1;
     inside[u] = s >= 0 && s < a.n_slots;
     const long page = inside[u] ? s >> a.page_shift : 0, slot = inside[u] ? s & ((1 << a.page_shift) - 1) : 0;
     const long at = page * c.page + head * c.head + slot * c.slot + e;
@@ -280,8 +314,8 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheReadArgs a) {
   }
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    const long r = row0 + u * kRows;
-    if (r >= n_rows) return;
+    const long t = t0 + u * (kRows / 4);
+    if (t >= a.tokens) return;
     if constexpr (KIND != kCacheSame) {
       float y[8];
       values_of<KIND>(code[u], y);
@@ -289,7 +323,7 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheReadArgs a) {
       for (int j = 0; j < 8; j++) x[u][j] = (T)(y[j] * scale[u]);
     }
     if (!inside[u]) x[u] = kv8<T>{0, 0, 0, 0, 0, 0, 0, 0};
-    *reinterpret_cast<kv8<T>*>(out + r * a.dim + e) = x[u];
+    *reinterpret_cast<kv8<T>*>(out + (t * a.kv_heads + head) * a.dim + e) = x[u];
   }
 }
 

@@ -245,7 +245,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendA
     if constexpr (KIND != kCacheSame) {
       const long page = __shfl(ids, i % kIds * kGroups + lane / 16);
       const int slot = (min(t0 + 16 * (lane / 16), (it.kv_end - 1) & ~15) & page_mask) + col;
-      if (lane < kSub) ks = scale_k[page * a.ck.scale_page + slot] * a.scale_log2, vs = scale_v[page * a.cv.scale_page + slot];
+      if (lane < kSub) ks = scale_k[page * a.ck.scale_page + slot], vs = scale_v[page * a.cv.scale_page + slot];
     }
   };
   auto key_of = [](int row) { return (row / kKeyRows) & (kChunks - 1); };
@@ -303,7 +303,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendA
       *reinterpret_cast<kv_uint4*>(lds_v + row * kRowBytes + (load_chunk ^ key_of_v(row)) * 16) = rv[j];
     }
     if constexpr (KIND != kCacheSame) {
-      if (lane < kSub) scales[wave][0][lane] = ks, scales[wave][1][lane] = vs;
+      if (lane < kSub) scales[wave][0][lane] = ks * a.scale_log2, scales[wave][1][lane] = vs;
     }
     float norm_now = norm;                   // the largest scale of V so far
     if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) {
@@ -548,7 +548,7 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a) {
       rv[j] = held_v.at(page, slot, j * kLoadRows);
     }
     if constexpr (KIND != kCacheSame)
-      rs = lane < 16 ? scale_k[page * a.ck.scale_page + slot + lane] * a.scale_log2 : scale_v[page * a.cv.scale_page + slot + (lane & 15)];
+      rs = lane < 16 ? scale_k[page * a.ck.scale_page + slot + lane] : scale_v[page * a.cv.scale_page + slot + (lane & 15)];
   };
   if (n_blocks > 0) request(0);
   const AttnRow mine = attn_row(a, it, kAttnTileRows, 32 * wave + col);
@@ -597,7 +597,7 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a) {
     const bool any = __any(strange);
     if (lane == 0) odd[at][wave] = any;
     if constexpr (KIND != kCacheSame) {
-      if (lane < 32) scales[at][lane / 16][16 * wave + (lane & 15)] = rs;
+      if (lane < 32) scales[at][lane / 16][16 * wave + (lane & 15)] = lane < 16 ? rs * a.scale_log2 : rs;
     }
   };
 

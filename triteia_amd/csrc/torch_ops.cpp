@@ -43,14 +43,14 @@ struct Args {
   bool nones[kMax] = {};
   double number = 0;        // a last argument that is neither a tensor nor None
   bool numeric = false;
-  Args(PyObject* const* values, Py_ssize_t count) : n(count <= kMax ? (int)count : 0) {
+  Args(PyObject* const* values, Py_ssize_t count, bool last = true) : n(count <= kMax ? (int)count : 0) {
     const bool traced = at::tracer::impl::is_dispatch_enabled();
     for (int i = 0; i < n; i++) {
       if (!traced && THPVariable_CheckExact(values[i]) && !at::isTensorSubclassLike(THPVariable_Unpack(values[i])))
         tensors[i] = &THPVariable_Unpack(values[i]);
       nones[i] = values[i] == Py_None;
     }
-    if (n == 0 || nones[n - 1] || THPVariable_Check(values[n - 1])) return;
+    if (!last || n == 0 || nones[n - 1] || THPVariable_Check(values[n - 1])) return;
     number = PyFloat_AsDouble(values[n - 1]);
     numeric = !PyErr_Occurred();
     PyErr_Clear();
@@ -441,17 +441,21 @@ struct MoreArgs : Args {
   bool given[kMax] = {};
   at::ScalarType types[kMax] = {};
   bool typed[kMax] = {};
-  MoreArgs(PyObject* const* values, Py_ssize_t count) : Args(values, count) {
+  MoreArgs(PyObject* const* values, Py_ssize_t count) : Args(values, count, false) {
     for (int i = 0; i < n; i++) {
-      if (nones[i] || THPVariable_Check(values[i])) continue;
-      if (THPDtype_Check(values[i])) {
-        types[i] = reinterpret_cast<THPDtype*>(values[i])->scalar_type, typed[i] = true;
-        continue;
+      if (nones[i] || tensors[i]) continue;
+      PyObject* v = values[i];
+      if (PyBool_Check(v)) {
+        numbers[i] = v == Py_True, given[i] = true;
+      } else if (PyFloat_CheckExact(v)) {
+        numbers[i] = PyFloat_AS_DOUBLE(v), given[i] = true;
+      } else if (PyLong_CheckExact(v)) {
+        numbers[i] = PyLong_AsDouble(v);
+        given[i] = !PyErr_Occurred();
+        PyErr_Clear();
+      } else if (THPDtype_Check(v)) {
+        types[i] = reinterpret_cast<THPDtype*>(v)->scalar_type, typed[i] = true;
       }
-      if (!PyLong_CheckExact(values[i]) && !PyFloat_CheckExact(values[i]) && !PyBool_Check(values[i])) continue;
-      numbers[i] = PyFloat_AsDouble(values[i]);
-      given[i] = !PyErr_Occurred();
-      PyErr_Clear();
     }
   }
   bool whole(int i, double most = 2147483647.0) const { return i < n && given[i] && numbers[i] >= 0 && numbers[i] <= most && numbers[i] == (double)(int64_t)numbers[i]; }
@@ -534,7 +538,7 @@ Outputs rotary_cache(const MoreArgs& a) {
     if (limit < 1 || rot < 16 || rot % 16 != 0 || rot > dim) return {};
   }
   for (int i : {11, 12})
-    if (a.tensor(i) && (a[i].dim() != 1 || a[i].size(0) != dim || a[i].scalar_type() != k.scalar_type() || !a[i].is_contiguous())) return {};
+    if (a.tensor(i) && (a[i].dim() != 1 || a[i].size(0) != dim || a[i].scalar_type() != k.scalar_type() || !a[i].is_contiguous() || !aligned(a[i]))) return {};
   const Cache c(a, 5);
   if (to_cache && (!c.ok || !c.takes(k.scalar_type()) || c.k->device() != k.device() || c.heads != kv_heads || c.dim != dim || a[2].size(1) != kv_heads || !index_vector(a[9], tokens))) return {};
   const Place at_(k);

@@ -8,6 +8,7 @@ from . import _ffi
 from ._native import native
 
 _DTYPES = (torch.float16, torch.bfloat16)
+_NONE = (None,) * 4
 CACHE_KINDS = {torch.float16: 0, torch.bfloat16: 0, torch.int8: 1, torch.float8_e4m3fn: 2}
 
 
@@ -104,7 +105,8 @@ class PagedCache:
 
 def rotary_cache(q, k, v, positions, table, cache, slots, interleaved=False, q_norm=None, k_norm=None, eps=1e-6):
     """The one launch behind ops.rotary, ops.rotary_cache_write and ops.cache_write: (q, k) of the outputs, None where there is none."""
-    out = native().rotary_cache(q, k, v, positions, table, *(cache._tensors if cache is not None else (None,) * 4), slots, interleaved, q_norm, k_norm, eps)
+    held = cache._tensors if cache is not None else _NONE
+    out = native().rotary_cache(q, k, v, positions, table, held[0], held[1], held[2], held[3], slots, interleaved, q_norm, k_norm, eps)
     if out is not None:
         return out
     device = _require(q=q, k=k, v=v, positions=positions, table=table, slots=slots, q_norm=q_norm, k_norm=k_norm)
@@ -138,7 +140,7 @@ def rotary_cache(q, k, v, positions, table, cache, slots, interleaved=False, q_n
     for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
         if t is not None and (t.shape != (dim,) or t.dtype != dtype):
             raise RuntimeError(f"{name} must be [{dim}] in {dtype}, got {tuple(t.shape)} in {t.dtype}")
-        norms.append(t.contiguous() if t is not None else None)
+        norms.append(t if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0) else t.clone(memory_format=torch.contiguous_format))
     q_out = torch.empty((tokens, q.shape[1], dim), dtype=dtype, device=device) if q is not None else None
     k_out = torch.empty((tokens, k.shape[1], dim), dtype=dtype, device=device) if cache is None else None
     strides = [s for t in (q, k, v) for s in (t.stride()[:2] if t is not None else (0, 0))]
