@@ -103,20 +103,21 @@ struct ReadLaunch {
 
 template <class T, int KIND, int D>
 void launch_attend(AttendArgs a, const AttnLayout& layout, float* scratch, long table_tokens, hipStream_t stream) {
+  int joins = 0;
   for (int which = 0; which < 2; which++) {
-    const AttnList& l = layout.list[which];
-    if (l.max_items == 0) continue;
-    a.list = l, a.which = which;
-    a.part_o = scratch;
-    a.part_ml = scratch + (long)l.max_parts * a.kv_heads * l.rows * D;
-    scratch = a.part_ml + 2L * l.max_parts * a.kv_heads * l.rows;
-    const dim3 grid((unsigned)((long)l.max_items * a.kv_heads));
-    if (which == 1) hipLaunchKernelGGL((attend_tile_kernel<T, KIND, D>), grid, dim3(256), 0, stream, a);
-    else if (l.rows == 16) hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 1>), grid, dim3(64 * kAttnWaves), 0, stream, a);
-    else hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 2>), grid, dim3(64 * kAttnWaves), 0, stream, a);
+    AttnList& l = a.list[which] = layout.list[which];
     // (no sequence is longer than its pages)
-    if (l.max_joins > 0 && table_tokens > (long)l.min_blocks * kAttnBlock) hipLaunchKernelGGL((attend_join_kernel<T, D>), dim3(l.max_joins * a.kv_heads, l.rows / 16), dim3(1024), 0, stream, a);
+    if (table_tokens <= (long)l.min_blocks * kAttnBlock) l.max_joins = 0;
+    joins += l.max_joins * a.kv_heads * (l.rows / 16);
+    a.part_o[which] = scratch;
+    a.part_ml[which] = scratch + (long)l.max_parts * a.kv_heads * l.rows * D;
+    scratch = a.part_ml[which] + 2L * l.max_parts * a.kv_heads * l.rows;
   }
+  const dim3 grid((unsigned)((long)(a.list[0].max_items + a.list[1].max_items) * a.kv_heads));
+  if (a.list[1].max_items > 0) hipLaunchKernelGGL((attend_mixed_kernel<T, KIND, D>), grid, dim3(256), 0, stream, a);
+  else if (a.list[0].rows == 16) hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 1>), grid, dim3(64 * kAttnWaves), 0, stream, a);
+  else hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 2>), grid, dim3(64 * kAttnWaves), 0, stream, a);
+  if (joins > 0) hipLaunchKernelGGL((attend_join_kernel<T, D>), dim3(joins), dim3(1024), 0, stream, a);
 }
 struct AttendLaunch {
   const AttendArgs& a;
@@ -141,7 +142,7 @@ int check_batch(const char* what, int n_seqs, int n_tokens, int heads, int kv_he
   if (window > 0 && !causal) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: a window needs causal", what);
   const AttnLayout l = attn_layout(n_seqs, n_tokens, heads, kv_heads, max_q, causal, window);
   for (const AttnList& x : l.list)
-    if ((long)x.max_items * kv_heads > 0x7fffffffL || x.max_items < 0)
+    if ((long)x.max_items * kv_heads > 0x3fffffffL || x.max_items < 0)
       return fail(TRITEIA_HIP_ERR_PROB_SHAPE, "%s: too many tiles", what);
   return TRITEIA_HIP_OK;
 }

@@ -11,8 +11,7 @@
 // device is clamped, so that no list passes its end.
 // A step's batch of 26 sequences 14.2 us with a workgroup of 1024 threads on one list after the other -> PLANUS.
 #pragma once
-#include <hip/hip_runtime.h>
-#include <stdint.h>
+#include "lora_routed.hip.h"
 
 namespace triteia_hip {
 
@@ -55,11 +54,11 @@ inline AttnLayout attn_layout(int n_seqs, int n_tokens, int heads, int kv_heads,
   const long live = n_seqs + 1 < n_tokens ? n_seqs + 1 : n_tokens;      // sequences with tokens, and the tokens behind them
   const bool only_short = most <= 32;
   AttnList &s = a.list[0], &l = a.list[1];
-  s.rows = only_short ? (most <= 16 ? 16 : 32) : a.group <= 16 ? 16 : 32;
-  a.short_rows = only_short ? 0x7fffffff : s.rows;
+  s.rows = only_short && most > 16 ? 32 : 16;
+  a.short_rows = only_short ? 0x7fffffff : a.group <= 16 ? 16 : 0;       // (one token's heads fill more than a tile of 16: a long sequence)
   s.slots = 256, s.min_blocks = 16, s.rounds = 4, l.slots = 512, l.min_blocks = 8, l.rounds = 2;
   l.rows = kAttnTileRows;
-  const long tiles[2] = {only_short ? live + rows / s.rows : live, only_short ? 0 : live + rows / l.rows};
+  const long tiles[2] = {only_short ? live + rows / s.rows : a.short_rows ? live : 0, only_short ? 0 : live + rows / l.rows};
   for (int which = 0; which < 2; which++) {
     AttnList& x = a.list[which];
     // (as the kernel cuts them: into the shares of whole rounds of workgroups; a cut tile has two at least)
@@ -80,14 +79,8 @@ inline AttnLayout attn_layout(int n_seqs, int n_tokens, int heads, int kv_heads,
 
 // Exclusive sums over a wavefront's lanes, and the total.
 __device__ __forceinline__ int attn_scan(int v, int* total) {
-  const int lane = threadIdx.x & 63;
-  int x = v;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
-  *total = __shfl(x, 63);
+  const int x = lane_sums(v);
+  *total = __builtin_amdgcn_readlane(x, 63);
   return x - v;
 }
 
@@ -128,7 +121,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const 
     int mine = 0;
     if (b <= a.n_seqs) {
       const long rows = (long)count[b] * a.group;
-      if ((rows <= a.short_rows) == (which == 0)) mine = (int)((rows + l.rows - 1) / l.rows);
+      if (rows > 0 && (rows <= a.short_rows) == (which == 0)) mine = (int)((rows + l.rows - 1) / l.rows);
     }
     int all;
     const int before = attn_scan(mine, &all);
@@ -154,36 +147,30 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const 
     t.blocks = (t.hi - t.lo + kAttnBlock - 1) / kAttnBlock;
     return t;
   };
+  int mine[kAttnSorted / 64];                                    // blocks of tiles `lane`, 64 + lane, ..
+#pragma unroll
+  for (int k = 0; k < kAttnSorted / 64; k++) mine[k] = 64 * k + lane < tiles ? at(64 * k + lane).blocks : -1;
   // Few tiles: the least share with which all shares still run in as many rounds as the tiles would.
   int share = 0x7fffffff;
   const long units = (long)tiles * a.kv_heads;
   if (units < (long)l.rounds * l.slots) {
     const int most = (int)((units + l.slots - 1) / l.slots * l.slots / a.kv_heads);        // shares of one head
-    long work = 0;
-    for (int i0 = 0; i0 < tiles; i0 += 64) work += i0 + lane < tiles ? at(i0 + lane).blocks : 0;
-    int total;
-    attn_scan((int)min(work, 0x7fffffffL / 64), &total);
-    total = __builtin_amdgcn_readfirstlane(total);
+    auto sum_of = [&](auto f) {                                  // f of every tile's blocks
+      long sum = 0;
+#pragma unroll
+      for (int k = 0; k < kAttnSorted / 64; k++) sum += mine[k] < 0 ? 0 : f(mine[k]);
+      for (int i0 = kAttnSorted; i0 < tiles; i0 += 64) sum += i0 + lane < tiles ? f(at(i0 + lane).blocks) : 0;
+      int total;
+      attn_scan((int)min(sum, 0x7fffffffL / 64), &total);
+      return total;
+    };
+    const int total = sum_of([](int blocks) { return blocks; });
     share = max(l.min_blocks, (total + most - 1) / max(most, 1));
-    while (true) {
-      int shares = 0;
-      for (int i0 = 0; i0 < tiles; i0 += 64) {
-        int sum;
-        attn_scan(i0 + lane < tiles ? max(1, (at(i0 + lane).blocks + share - 1) / share) : 0, &sum);
-        shares += sum;
-      }
-      if (__builtin_amdgcn_readfirstlane(shares) <= most || share > total) break;
-      share += (share + 7) / 8;
-    }
+    while (share <= total && sum_of([&](int blocks) { return max(1, (blocks + share - 1) / share); }) > most) share += (share + 7) / 8;
   }
   // longest first, so that the last workgroups to run are short ones
   if (tiles <= kAttnSorted) {
-    int mine[kAttnSorted / 64], place[kAttnSorted / 64];
-#pragma unroll
-    for (int k = 0; k < kAttnSorted / 64; k++) {
-      const int i = 64 * k + lane;
-      mine[k] = i < tiles ? at(i).blocks : -1, place[k] = 0;
-    }
+    int place[kAttnSorted / 64] = {};
 #pragma unroll
     for (int k = 0; k < kAttnSorted / 64; k++) {
       for (int i = 64 * k; i < min(tiles, 64 * k + 64); i++) {

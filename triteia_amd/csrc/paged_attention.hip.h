@@ -39,9 +39,8 @@ struct AttendArgs {
   int group, kv_heads, causal, window;
   float scale_log2;                     // scale * log2(e)
   const int* plan;
-  AttnList list;
-  int which;
-  float *part_o, *part_ml;              // [parts][kv_heads][rows][D], [parts][kv_heads][rows][2]
+  AttnList list[2];
+  float *part_o[2], *part_ml[2];        // of each list: [parts][kv_heads][rows][D], [parts][kv_heads][rows][2]
 };
 
 // The largest over lanes 32 apart, or 16 and 32 apart, in all of them: whole rows of lanes trade places on the vector ALU.
@@ -143,8 +142,8 @@ __device__ __forceinline__ kv8<T> attn_transposed(const uint8_t* lds, int first,
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-__device__ __forceinline__ AttnItem attn_item(const AttendArgs& a, int i) {
-  const int* p = a.plan + a.list.items + 8L * i;
+__device__ __forceinline__ AttnItem attn_item(const AttendArgs& a, int which, int i) {
+  const int* p = a.plan + a.list[which].items + 8L * i;
   return AttnItem{p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]};
 }
 
@@ -185,28 +184,35 @@ __device__ __forceinline__ AttnRow attn_row(const AttendArgs& a, const AttnItem&
 
 // ---------------------------------------------------------------------------------------------------------------------------------
 // Few rows: a decode step's heads, a handful of tokens.  Bound by the cache's bytes.  A workgroup takes a share of one tile's tokens; each of
-// its eight wavefronts walks sub-tiles of its own (8 KB of K and 8 KB of V: 32 tokens of 128 elements in 16 bits, 64 in 8) with the next one's whole rows
+// its wavefronts (eight, four beside a long list) walks sub-tiles of its own (8 KB of K and 8 KB of V: 32 tokens of 128 elements in 16 bits, 64 in 8) with the next one's whole rows
 // on their way in registers and this one's in LDS of its own, so that the loop has no barrier; maxima, sums and outputs are joined once at the end.
-// grid: list.max_items * kv_heads, block 64 kAttnWaves
-template <class T, int KIND, int D, int NQ>
-__global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendArgs a) {
+template <int KIND, int D, int NQ, int WAVES>
+struct AttnRowsLds {
+  static constexpr int kRowBytes = D * (KIND == kCacheSame ? 2 : 1);
+  static constexpr int kSub = KIND != kCacheSame && NQ == 2 ? 32 : 8192 / kRowBytes < 64 ? 8192 / kRowBytes : 64;   // (two tiles of rows fill the registers)
+  static constexpr int kTile = kSub * kRowBytes, kRows = 16 * NQ;
+  static constexpr int kStride = D + 4;                                      // floats of a row where the wavefronts meet
+  static constexpr int kMeet = WAVES / 2 * kRows * kStride * 4;
+  alignas(16) uint8_t tiles[WAVES * 2 * kTile > kMeet ? WAVES * 2 * kTile : kMeet];
+  float meet_m[WAVES][kRows], meet_l[WAVES][kRows];
+  alignas(16) float scales[KIND == kCacheSame ? 1 : WAVES][2][kSub];
+};
+
+template <class T, int KIND, int D, int NQ, int WAVES>
+__device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int head, AttnRowsLds<KIND, D, NQ, WAVES>& shared) {
   using M = AttnMma<T>;
   using v8 = typename M::v8;
-  constexpr int kRowBytes = D * (KIND == kCacheSame ? 2 : 1), kChunks = kRowBytes / 16;
-  constexpr int kSub = KIND != kCacheSame && NQ == 2 ? 32 : 8192 / kRowBytes < 64 ? 8192 / kRowBytes : 64;   // (two tiles of rows fill the registers)
+  using Lds = AttnRowsLds<KIND, D, NQ, WAVES>;
+  constexpr int kRowBytes = Lds::kRowBytes, kChunks = kRowBytes / 16, kSub = Lds::kSub, kTile = Lds::kTile, kRows = Lds::kRows, kStride = Lds::kStride;
   constexpr int kLoads = kSub * kChunks / 64, kLoadRows = 64 / kChunks;     // requests of a sub-tile, rows of each
   constexpr int kGroups = kSub / 16, kGroupLoads = kLoads / kGroups;
-  constexpr int kRows = 16 * NQ, kKeyRows = 256 / kRowBytes;
-  constexpr int kTile = kSub * kRowBytes;
-  constexpr int kStride = D + 4;                                             // floats of a row where the wavefronts meet
-  constexpr int kMeet = kAttnWaves / 2 * kRows * kStride * 4;
-  constexpr int kLds = kAttnWaves * 2 * kTile > kMeet ? kAttnWaves * 2 * kTile : kMeet;
-  __shared__ alignas(16) uint8_t lds[kLds];
-  __shared__ float meet_m[kAttnWaves][kRows], meet_l[kAttnWaves][kRows];
-  __shared__ alignas(16) float scales[KIND == kCacheSame ? 1 : kAttnWaves][2][kSub];
-  const int index = blockIdx.x / a.kv_heads, head = blockIdx.x - index * a.kv_heads;
-  const AttnItem it = attn_item(a, index);        // (requested together with the number of items)
-  if (index >= a.plan[2 * a.which]) return;
+  constexpr int kKeyRows = 256 / kRowBytes;
+  uint8_t* lds = shared.tiles;
+  auto& meet_m = shared.meet_m;
+  auto& meet_l = shared.meet_l;
+  auto& scales = shared.scales;
+  const AttnItem it = attn_item(a, 0, index);        // (requested together with the number of items)
+  if (index >= a.plan[0]) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, h = lane >> 4;
   uint8_t* lds_k = lds + wave * 2 * kTile;
@@ -222,15 +228,15 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendA
   // A lane fetches the page of one 16-token group of the wavefront's next sub-tiles: kIds sub-tiles' pages are one request, a request ahead.
   constexpr int kIds = 64 / kGroups;
   auto pages_from = [&](int i) {
-    const long token = it.kv_begin + (wave + (long)kAttnWaves * (i + lane / kGroups)) * kSub + 16 * (lane % kGroups);
+    const long token = it.kv_begin + (wave + (long)WAVES * (i + lane / kGroups)) * kSub + 16 * (lane % kGroups);
     return attn_page(a, it.seq, (int)min(token, (long)it.kv_end - 1));
   };
-  int ids = n_sub > wave ? pages_from(0) : 0, next_ids = n_sub > wave + kAttnWaves * kIds ? pages_from(kIds) : 0;
+  int ids = n_sub > wave ? pages_from(0) : 0, next_ids = n_sub > wave + WAVES * kIds ? pages_from(kIds) : 0;
   auto request = [&](int i) {                // the wavefront's i-th sub-tile
-    const int t0 = it.kv_begin + (wave + kAttnWaves * i) * kSub;
+    const int t0 = it.kv_begin + (wave + WAVES * i) * kSub;
     if (i > 0 && i % kIds == 0) {
       ids = next_ids;
-      if (wave + kAttnWaves * (i + kIds) < n_sub) next_ids = pages_from(i + kIds);
+      if (wave + WAVES * (i + kIds) < n_sub) next_ids = pages_from(i + kIds);
     }
 #pragma unroll
     for (int g = 0; g < kGroups; g++) {
@@ -281,7 +287,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendA
 #pragma unroll
     for (int d = 0; d < D / 16; d++) o[n][d] = attn_f4{0.f, 0.f, 0.f, 0.f};
   }
-  for (int sub = wave; sub < n_sub; sub += kAttnWaves) {
+  for (int sub = wave; sub < n_sub; sub += WAVES) {
     const int t0 = it.kv_begin + sub * kSub;
     if (t0 + kSub > it.kv_end) {             // tokens behind the last: whatever the page holds there must not meet a zero of P
 #pragma unroll
@@ -310,7 +316,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendA
       if (lane < kSub && t0 + lane < it.kv_end) norm_now = fmaxf(norm, vs);
       norm_now = attn_max16(across_row<16>(norm_now, [](float p, float q) { return fmaxf(p, q); }));
     }
-    if (sub + kAttnWaves < n_sub) request((sub - wave) / kAttnWaves + 1);
+    if (sub + WAVES < n_sub) request((sub - wave) / WAVES + 1);
 
     attn_f4 s[NQ][kGroups];
 #pragma unroll
@@ -442,7 +448,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendA
   for (int n = 0; n < NQ; n++) {
     float top = kAttnNone;
 #pragma unroll
-    for (int w = 0; w < kAttnWaves; w++) top = fmaxf(top, meet_m[w][16 * n + col]);
+    for (int w = 0; w < WAVES; w++) top = fmaxf(top, meet_m[w][16 * n + col]);
     float f = __builtin_amdgcn_exp2f(m[n] - top);
     if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) f *= norm;
 #pragma unroll
@@ -452,10 +458,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendA
   }
   // (rows that fill half a tile at most, as a decode step's of up to 8 heads do: all eight at once)
   const bool once = last_row < kRows / 2;
-  const int met = once ? kAttnWaves : kAttnWaves / 2, met_rows = once ? kRows / 2 : kRows;
+  const int met = once ? WAVES : WAVES / 2, met_rows = once ? kRows / 2 : kRows;
 #pragma unroll
   for (int upper = 1; upper >= 0; upper--) {
-    if (once ? upper == 1 : (wave >= kAttnWaves / 2) == (upper == 1)) {
+    if (once ? upper == 1 : (wave >= WAVES / 2) == (upper == 1)) {
 #pragma unroll
       for (int n = 0; n < NQ; n++)
 #pragma unroll
@@ -469,20 +475,20 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendA
     __syncthreads();
     if (once) break;
   }
-  for (int i = threadIdx.x; i < kRows * (D / 4); i += 64 * kAttnWaves) {
+  for (int i = threadIdx.x; i < kRows * (D / 4); i += 64 * WAVES) {
     const int r = i / (D / 4), d = 4 * (i % (D / 4));
     if (r > last_row) break;
     float top = kAttnNone, sum = 0.f;
     attn_f4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < kAttnWaves; w++) top = fmaxf(top, meet_m[w][r]);
+    for (int w = 0; w < WAVES; w++) top = fmaxf(top, meet_m[w][r]);
 #pragma unroll
-    for (int w = 0; w < kAttnWaves; w++) sum += meet_l[w][r] * __builtin_amdgcn_exp2f(meet_m[w][r] - top);
+    for (int w = 0; w < WAVES; w++) sum += meet_l[w][r] * __builtin_amdgcn_exp2f(meet_m[w][r] - top);
 #pragma unroll
-    for (int w = 0; w < kAttnWaves / 2; w++) x += *reinterpret_cast<const attn_f4*>(meet + (w * met_rows + r) * kStride + d);
+    for (int w = 0; w < WAVES / 2; w++) x += *reinterpret_cast<const attn_f4*>(meet + (w * met_rows + r) * kStride + d);
     if (once) {
 #pragma unroll
-      for (int w = kAttnWaves / 2; w < kAttnWaves; w++) x += *reinterpret_cast<const attn_f4*>(meet + (w * met_rows + r) * kStride + d);
+      for (int w = WAVES / 2; w < WAVES; w++) x += *reinterpret_cast<const attn_f4*>(meet + (w * met_rows + r) * kStride + d);
     }
     if (it.part < 0) {
       const AttnRow row = attn_row(a, it, kRows, r);
@@ -493,8 +499,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendA
       *reinterpret_cast<t4*>(static_cast<T*>(a.out) + ((long)(it.q_start + row.token) * (a.kv_heads * a.group) + head * a.group + row.head) * D + d) = y;
     } else {
       const long at = ((long)it.part * a.kv_heads + head) * kRows + r;
-      *reinterpret_cast<attn_f4*>(a.part_o + at * D + d) = x;
-      if (d == 0) a.part_ml[2 * at] = top, a.part_ml[2 * at + 1] = sum;
+      *reinterpret_cast<attn_f4*>(a.part_o[0] + at * D + d) = x;
+      if (d == 0) a.part_ml[0][2 * at] = top, a.part_ml[0][2 * at + 1] = sum;
     }
   }
 }
@@ -503,22 +509,28 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendA
 // Many rows: prompts.  Bound by the matrix cores and the exponentials.  A workgroup takes 128 rows, 32 a wavefront (as columns of 32 x 32 x 16
 // MFMAs), and walks the share's tokens in blocks of 64 that all of it reads from LDS: two places, the next block on its way in registers,
 // one barrier a block.  Codes of 8 bits become values on their way to LDS.
-// grid: list.max_items * kv_heads, block 256
+template <int D>
+struct AttnTileLds {
+  static constexpr int kTile = kAttnBlock * 2 * D;
+  alignas(16) uint8_t tiles[4 * kTile];                                                  // K, V, K, V
+  alignas(16) float scales[2][2][kAttnBlock];
+  int odd[2][4];                                                                         // infinities or NaNs among a wavefront's V
+};
+
 template <class T, int KIND, int D>
-__global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a) {
+__device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int head, AttnTileLds<D>& shared) {
   using M = AttnMma<T>;
   using v8 = typename M::v8;
   constexpr int kRowBytes = 2 * D, kChunks = kRowBytes / 16, kKeyRows = 256 / kRowBytes;
-  constexpr int kTile = kAttnBlock * kRowBytes;
+  constexpr int kTile = AttnTileLds<D>::kTile;
   constexpr int kHeld = D * (KIND == kCacheSame ? 2 : 1), kHeldChunks = kHeld / 16;      // a row in the cache
   constexpr int kLoads = 16 * kHeldChunks / 64, kLoadRows = 64 / kHeldChunks;            // of the wavefront's 16 tokens of a block
   static_assert(kLoads >= 1, "16 tokens are a request at least");
-  __shared__ alignas(16) uint8_t lds[4 * kTile];                                         // K, V, K, V
-  __shared__ alignas(16) float scales[2][2][kAttnBlock];
-  __shared__ int odd[2][4];                                                              // infinities or NaNs among a wavefront's V
-  const int index = blockIdx.x / a.kv_heads, head = blockIdx.x - index * a.kv_heads;
-  const AttnItem it = attn_item(a, index);
-  if (index >= a.plan[2 * a.which]) return;
+  uint8_t* lds = shared.tiles;
+  auto& scales = shared.scales;
+  auto& odd = shared.odd;
+  const AttnItem it = attn_item(a, 1, index);
+  if (index >= a.plan[2]) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, h = lane >> 5;
 
@@ -752,24 +764,48 @@ __global__ __launch_bounds__(256, 2) void attend_tile_kernel(AttendArgs a) {
         attn_f4 y;
 #pragma unroll
         for (int j = 0; j < 4; j++) y[j] = o[d][4 * i + j] * f;
-        *reinterpret_cast<attn_f4*>(a.part_o + at * D + 32 * d + 8 * i + 4 * h) = y;
+        *reinterpret_cast<attn_f4*>(a.part_o[1] + at * D + 32 * d + 8 * i + 4 * h) = y;
       }
-    if (h == 0) a.part_ml[2 * at] = m, a.part_ml[2 * at + 1] = l;
+    if (h == 0) a.part_ml[1][2 * at] = m, a.part_ml[1][2 * at + 1] = l;
   }
 }
 
+// A batch of short sequences: a workgroup for every item and head of the cache.  grid list[0].max_items * kv_heads, block 64 kAttnWaves
+template <class T, int KIND, int D, int NQ>
+__global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendArgs a) {
+  __shared__ AttnRowsLds<KIND, D, NQ, kAttnWaves> shared;
+  const int index = blockIdx.x / a.kv_heads;
+  attend_rows<T, KIND, D, NQ, kAttnWaves>(a, index, blockIdx.x - index * a.kv_heads, shared);
+}
+
+// Any batch: the long list's items first, then the short one's, in one launch, so that what waits for memory runs beside what computes.
+// grid (list[1].max_items + list[0].max_items) * kv_heads, block 256
+template <class T, int KIND, int D>
+__global__ __launch_bounds__(256, 2) void attend_mixed_kernel(AttendArgs a) {
+  __shared__ union {
+    AttnTileLds<D> tile;
+    AttnRowsLds<KIND, D, 1, 4> rows;
+  } shared;
+  const int index = blockIdx.x / a.kv_heads, head = blockIdx.x - index * a.kv_heads;
+  if (index < a.list[1].max_items) attend_tile<T, KIND, D>(a, index, head, shared.tile);
+  else attend_rows<T, KIND, D, 1, 4>(a, index - a.list[1].max_items, head, shared.rows);
+}
+
 // Shares of one tile.  D / 4 lanes hold a row; 16 rows at a time (or as many as there are, rounded up to a power of two) and, between them, the shares: a
-// group of lanes adds every n-th share, the groups' sums are added in their order.  grid (max_joins * kv_heads, rows / 16), block 1024
+// group of lanes adds every n-th share, the groups' sums are added in their order.  grid: of each list max_joins * kv_heads * rows / 16, the short one first; block 1024
 template <class T, int D>
 __global__ __launch_bounds__(1024) void attend_join_kernel(AttendArgs a) {
   constexpr int kLanes = D / 4, kGroups = 1024 / kLanes;
   __shared__ attn_f4 sums[1024];
   __shared__ float totals[kGroups];
-  const int index = blockIdx.x / a.kv_heads, head = blockIdx.x - index * a.kv_heads;
-  const int* j = a.plan + a.list.joins + 8L * index;
+  const int short_units = a.list[0].max_joins * a.kv_heads * (a.list[0].rows / 16);
+  const int which = (int)blockIdx.x < short_units ? 0 : 1, unit = blockIdx.x - (which ? short_units : 0);
+  const int rows = a.list[which].rows, pieces = rows / 16, piece = unit % pieces, index = unit / pieces / a.kv_heads, head = unit / pieces - index * a.kv_heads;
+  const int* j = a.plan + a.list[which].joins + 8L * index;
   const int q_start = j[0], n_tokens = j[1], tile = j[2], first = j[3], n_parts = j[4];
-  if (index >= a.plan[2 * a.which + 1]) return;
-  const int rows = a.list.rows, r0 = 16 * blockIdx.y;
+  if (index >= a.plan[2 * which + 1]) return;
+  const int r0 = 16 * piece;
+  const float *part_o = a.part_o[which], *part_ml = a.part_ml[which];
   const int live = (int)min(16L, (long)n_tokens * a.group - (long)tile * rows - r0);
   if (live <= 0) return;
   int wide = 1;                                  // rows side by side
@@ -778,13 +814,13 @@ __global__ __launch_bounds__(1024) void attend_join_kernel(AttendArgs a) {
   const long step = (long)a.kv_heads * rows, at = ((long)first * a.kv_heads + head) * rows + r0 + min(i, live - 1);
   float top = kAttnNone, sum = 0.f;
 #pragma unroll 4
-  for (int p = 0; p < n_parts; p++) top = fmaxf(top, a.part_ml[2 * (at + p * step)]);
+  for (int p = 0; p < n_parts; p++) top = fmaxf(top, part_ml[2 * (at + p * step)]);
   attn_f4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int p = group / wide; p < n_parts; p += n) {
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * (at + p * step)] - top);
-    sum += f * a.part_ml[2 * (at + p * step) + 1];
-    const attn_f4 y = *reinterpret_cast<const attn_f4*>(a.part_o + (at + p * step) * D + d);
+    const float f = __builtin_amdgcn_exp2f(part_ml[2 * (at + p * step)] - top);
+    sum += f * part_ml[2 * (at + p * step) + 1];
+    const attn_f4 y = *reinterpret_cast<const attn_f4*>(part_o + (at + p * step) * D + d);
 #pragma unroll
     for (int k = 0; k < 4; k++) x[k] = __builtin_fmaf(y[k], f, x[k]);
   }
