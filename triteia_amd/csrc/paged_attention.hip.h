@@ -633,11 +633,15 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
   __syncthreads();
   for (int block = 0; block < n_blocks; block++) {
     const int t0 = it.kv_begin + block * kAttnBlock, at = block & 1;
-    if (block + 1 < n_blocks) {
-      keep(t0 + kAttnBlock, at ^ 1);
-      if (block + 2 < n_blocks) request(block + 2);
-    }
-    if (wave_live && t0 < min(w1.hi, it.kv_end) && t0 + kAttnBlock > w0.lo) {
+    auto step = [&] {                        // the next block into LDS, the one behind it requested
+      if (block + 1 < n_blocks) {
+        keep(t0 + kAttnBlock, at ^ 1);
+        if (block + 2 < n_blocks) request(block + 2);
+      }
+    };
+    if (!wave_live || t0 >= min(w1.hi, it.kv_end) || t0 + kAttnBlock <= w0.lo) {
+      step();
+    } else {
       // (one lane constant each, kept from being spread over a register for every address)
       uint32_t at_k = at * 2 * kTile + lane_k, at_v = at * 2 * kTile + kTile + lane_v;
       asm volatile("" : "+v"(at_k), "+v"(at_v));
@@ -646,10 +650,13 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
       for (int g = 0; g < 2; g++)
 #pragma unroll
         for (int j = 0; j < 16; j++) s[g][j] = 0.f;
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int i = 0; i < D / 16; i++)
 #pragma unroll
         for (int g = 0; g < 2; g++) s[g] = M::m32(*reinterpret_cast<const v8*>(lds + (at_k ^ (32 * i)) + 32 * g * kRowBytes), qf[i], s[g]);
+      __builtin_amdgcn_s_setprio(0);
+      step();                                // (its writes under the softmax)
       const bool edge = t0 < w1.lo || t0 + kAttnBlock > min(w0.hi, it.kv_end);
       float grown = 1.f;
       if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) {
