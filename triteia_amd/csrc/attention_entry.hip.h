@@ -250,7 +250,7 @@ int triteia_hip_paged_attention(const void* q, long q_token, long q_head, void* 
   const long size = kind == kCacheSame ? 2 : 1;
   for (const CachePart* p : {&a.ck, &a.cv}) {
     if (!strides_ok({p->page, p->head, p->slot}, size, 16)) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: a cache's rows need 16-byte alignment", what);
-    if (p->slot * size > (1L << 26)) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: rows of a page %ld elements apart are too far", what, p->slot);
+    if (p->slot * size > (1L << 25)) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: rows of a page %ld elements apart are too far", what, p->slot);
     if (kind != kCacheSame && (!aligned16(p->scale) || p->scale_slot != 1 || !strides_ok({p->scale_page, p->scale_head}, 4, 16)))
       return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: a page's scales of one head have to be adjacent and 16-byte aligned", what);
   }

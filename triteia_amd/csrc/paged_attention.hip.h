@@ -153,15 +153,21 @@ __device__ __forceinline__ int attn_page(const AttendArgs& a, int seq, int token
   return (int)min((uint32_t)a.pages[seq * a.pages_seq + at], (uint32_t)(a.n_pages - 1));
 }
 
-// One head's keys or values: where the 16 tokens of a group start is the same for all lanes, a lane's own offset from there has 32 bits.
+// One head's keys or values.  Where the 16 tokens of a group start is the same for all lanes and the base of a buffer; a lane's own offset from there, and
+// the offset of the rows of each further request, have 32 bits.  (Added up as 64-bit addresses they were half of the loop's scalar instructions.)
+template <int ROWS>                // of a request
 struct AttnHeld {
   const uint8_t* head;
-  long page, slot;               // strides in bytes
-  uint32_t lane;
+  long page;                       // strides in bytes
+  uint32_t slot, step, lane;
   __device__ __forceinline__ AttnHeld(const CachePart& c, int h, int size, int row, int piece)
-      : head(static_cast<const uint8_t*>(c.data) + h * c.head * size), page(c.page * size), slot(c.slot * size), lane((uint32_t)(row * slot) + 16 * piece) {}
-  __device__ __forceinline__ kv_uint4 at(long p, int first, int row) const {
-    return *reinterpret_cast<const kv_uint4*>(head + p * page + (first + row) * slot + lane);
+      : head(static_cast<const uint8_t*>(c.data) + h * c.head * size), page(c.page * size), slot((uint32_t)(c.slot * size)), step(ROWS * slot),
+        lane(row * slot + 16 * piece) {}
+  template <int N>
+  __device__ __forceinline__ void read(kv_uint4* to, long p, int first) const {
+    const auto rows = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(head) + p * page + (long)first * slot, 0, 0xffffffffu, 0x00027000);
+#pragma unroll
+    for (int j = 0; j < N; j++) to[j] = __builtin_bit_cast(kv_uint4, __builtin_amdgcn_raw_buffer_load_b128(rows, lane, j * step, 0));
   }
 };
 
@@ -223,7 +229,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
   float ks = 0.f, vs = 0.f;                 // scales of token `lane` of the sub-tile
   const int load_row = lane / kChunks, load_chunk = lane % kChunks;
   const int page_mask = (1 << a.page_shift) - 1;
-  const AttnHeld held_k(a.ck, head, kRowBytes / D, load_row, load_chunk), held_v(a.cv, head, kRowBytes / D, load_row, load_chunk);
+  const AttnHeld<kLoadRows> held_k(a.ck, head, kRowBytes / D, load_row, load_chunk), held_v(a.cv, head, kRowBytes / D, load_row, load_chunk);
   const float *scale_k = a.ck.scale + head * a.ck.scale_head, *scale_v = a.cv.scale + head * a.cv.scale_head;
   // A lane fetches the page of one 16-token group of the wavefront's next sub-tiles: kIds sub-tiles' pages are one request, a request ahead.
   constexpr int kIds = 64 / kGroups;
@@ -242,11 +248,8 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
     for (int g = 0; g < kGroups; g++) {
       const long page = __builtin_amdgcn_readlane(ids, i % kIds * kGroups + g);
       const int slot = min(t0 + 16 * g, (it.kv_end - 1) & ~15) & page_mask;
-#pragma unroll
-      for (int j = 0; j < kGroupLoads; j++) {
-        rk[g * kGroupLoads + j] = held_k.at(page, slot, j * kLoadRows);
-        rv[g * kGroupLoads + j] = held_v.at(page, slot, j * kLoadRows);
-      }
+      held_k.template read<kGroupLoads>(rk + g * kGroupLoads, page, slot);
+      held_v.template read<kGroupLoads>(rv + g * kGroupLoads, page, slot);
     }
     if constexpr (KIND != kCacheSame) {
       const long page = __shfl(ids, i % kIds * kGroups + lane / 16);
@@ -539,7 +542,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
   float rs = 0.f;
   const int load_row = lane / kHeldChunks, load_chunk = lane % kHeldChunks;
   const int page_mask = (1 << a.page_shift) - 1;
-  const AttnHeld held_k(a.ck, head, kHeld / D, load_row, load_chunk), held_v(a.cv, head, kHeld / D, load_row, load_chunk);
+  const AttnHeld<kLoadRows> held_k(a.ck, head, kHeld / D, load_row, load_chunk), held_v(a.cv, head, kHeld / D, load_row, load_chunk);
   const float *scale_k = a.ck.scale + head * a.ck.scale_head, *scale_v = a.cv.scale + head * a.cv.scale_head;
   // a lane fetches the page of the wavefront's 16 tokens of one of the next 64 blocks
   auto pages_from = [&](int i) {
@@ -554,11 +557,8 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
     }
     const long page = __builtin_amdgcn_readlane(ids, i % 64);
     const int slot = min(it.kv_begin + i * kAttnBlock + 16 * wave, (it.kv_end - 1) & ~15) & page_mask;
-#pragma unroll
-    for (int j = 0; j < kLoads; j++) {
-      rk[j] = held_k.at(page, slot, j * kLoadRows);
-      rv[j] = held_v.at(page, slot, j * kLoadRows);
-    }
+    held_k.template read<kLoads>(rk, page, slot);
+    held_v.template read<kLoads>(rv, page, slot);
     if constexpr (KIND != kCacheSame)
       rs = lane < 16 ? scale_k[page * a.ck.scale_page + slot + lane] : scale_v[page * a.cv.scale_page + slot + (lane & 15)];
   };
@@ -699,14 +699,16 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
       }
       const float inv = KIND != kCacheSame && __is_same(T, _Float16) ? 1.f / fmaxf(norm, 1e-30f) : 1.f;
       v8 p[4];
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};   // (one running sum would be a chain of 32 additions)
 #pragma unroll
       for (int g = 0; g < 2; g++)
 #pragma unroll
         for (int j = 0; j < 16; j++) {
           const float e = __builtin_amdgcn_exp2f(KIND == kCacheSame ? __builtin_fmaf(s[g][j], a.scale_log2, -m) : s[g][j] - m);
-          l += e;
+          sum[j % 4] += e;
           s[g][j] = KIND == kCacheSame ? e : e * (scales[at][1][32 * g + 8 * (j / 4) + j % 4 + 4 * h] * inv);
         }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       if (KIND != kCacheSame && edge) {              // (a scale may be a NaN)
 #pragma unroll
         for (int g = 0; g < 2; g++)
