@@ -17,6 +17,7 @@ namespace triteia_hip {
 
 constexpr int kAttnBlock = 64;         // tokens of a block: shares begin and end on its multiples
 constexpr int kAttnTileRows = 128;     // rows of a tile of the long list
+constexpr int kAttnWaves = 8;          // at most, of a workgroup with few rows
 constexpr int kAttnSorted = 256;       // lists of up to this many tiles begin with the longest
 constexpr int kAttnMaxSeqs = 4096;
 constexpr int kAttnPlanThreads = 128;
@@ -35,6 +36,7 @@ struct AttnList {
   int max_items, max_joins;
   long items, joins;     // where they start in the plan, in ints
   int slots, min_blocks; // workgroups that run side by side, and the least length of a share
+  int waves;             // of a workgroup
   int rounds;            // lists of this many rounds of workgroups and more are not cut
   int max_parts;
 };
@@ -56,9 +58,14 @@ inline AttnLayout attn_layout(int n_seqs, int n_tokens, int heads, int kv_heads,
   AttnList &s = a.list[0], &l = a.list[1];
   s.rows = only_short && most > 16 ? 32 : 16;
   a.short_rows = only_short ? 0x7fffffff : a.group <= 16 ? 16 : 0;       // (one token's heads fill more than a tile of 16: a long sequence)
-  s.slots = 256, s.min_blocks = 16, s.rounds = 4, l.slots = 512, l.min_blocks = 8, l.rounds = 2;
+  s.min_blocks = 16, s.rounds = 4, l.slots = 512, l.min_blocks = 8, l.rounds = 2;
   l.rows = kAttnTileRows;
   const long tiles[2] = {only_short ? live + rows / s.rows : a.short_rows ? live : 0, only_short ? 0 : live + rows / l.rows};
+  // Up to 128 workgroups with short rows: eight wavefronts, one a CU, so that a context is walked fast.  More: four, two a CU, one beginning or
+  // ending while the other streams.  (us, eight / four: 32 of 500 tokens 8.0 / 8.7, 24 of 100000 cut into 256 / 512 215 / 220, 192 of up to 2000 in
+  // e4m3 22.9 / 21.0, 2048 of up to 1000 112 / 100 and 81 / 58, 1280 of 34 21.5 / 13.2, 2048 of up to 4096 395 / 390.)
+  s.waves = !only_short || tiles[0] * kv_heads > 128 ? 4 : kAttnWaves;
+  s.slots = only_short && s.waves == 4 ? 512 : 256, l.waves = 4;
   for (int which = 0; which < 2; which++) {
     AttnList& x = a.list[which];
     // (as the kernel cuts them: into the shares of whole rounds of workgroups; a cut tile has two at least)

@@ -24,7 +24,6 @@ typedef float attn_f16 __attribute__((ext_vector_type(16)));
 typedef short attn_s4 __attribute__((ext_vector_type(4)));
 typedef int attn_i2 __attribute__((ext_vector_type(2)));
 
-constexpr int kAttnWaves = 8;             // of a workgroup with few rows
 constexpr float kAttnNone = -1e30f;     // below every score: the maximum of nothing
 constexpr float kAttnSlack = 8.f;
 
@@ -190,7 +189,7 @@ __device__ __forceinline__ AttnRow attn_row(const AttendArgs& a, const AttnItem&
 
 // ---------------------------------------------------------------------------------------------------------------------------------
 // Few rows: a decode step's heads, a handful of tokens.  Bound by the cache's bytes.  A workgroup takes a share of one tile's tokens; each of
-// its wavefronts (eight, four beside a long list) walks sub-tiles of its own (8 KB of K and 8 KB of V: 32 tokens of 128 elements in 16 bits, 64 in 8) with the next one's whole rows
+// its four or eight wavefronts walks sub-tiles of its own (8 KB of K and 8 KB of V: 32 tokens of 128 elements in 16 bits, 64 in 8) with the next one's whole rows
 // on their way in registers and this one's in LDS of its own, so that the loop has no barrier; maxima, sums and outputs are joined once at the end.
 template <int KIND, int D, int NQ, int WAVES>
 struct AttnRowsLds {
@@ -459,7 +458,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
 #pragma unroll
       for (int j = 0; j < 4; j++) o[n][d][j] *= f;
   }
-  // (rows that fill half a tile at most, as a decode step's of up to 8 heads do: all eight at once)
+  // (rows that fill half a tile at most, as a decode step's of up to 8 heads do: all at once)
   const bool once = last_row < kRows / 2;
   const int met = once ? WAVES : WAVES / 2, met_rows = once ? kRows / 2 : kRows;
 #pragma unroll
@@ -779,12 +778,12 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
   }
 }
 
-// A batch of short sequences: a workgroup for every item and head of the cache.  grid list[0].max_items * kv_heads, block 64 kAttnWaves
-template <class T, int KIND, int D, int NQ>
-__global__ __launch_bounds__(64 * kAttnWaves, 2) void attend_rows_kernel(AttendArgs a) {
-  __shared__ AttnRowsLds<KIND, D, NQ, kAttnWaves> shared;
+// A batch of short sequences: a workgroup for every item and head of the cache.  grid list[0].max_items * kv_heads, block 64 WAVES
+template <class T, int KIND, int D, int NQ, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void attend_rows_kernel(AttendArgs a) {
+  __shared__ AttnRowsLds<KIND, D, NQ, WAVES> shared;
   const int index = blockIdx.x / a.kv_heads;
-  attend_rows<T, KIND, D, NQ, kAttnWaves>(a, index, blockIdx.x - index * a.kv_heads, shared);
+  attend_rows<T, KIND, D, NQ, WAVES>(a, index, blockIdx.x - index * a.kv_heads, shared);
 }
 
 // Any batch: the long list's items first, then the short one's, in one launch, so that what waits for memory runs beside what computes.
