@@ -119,7 +119,7 @@ void launch_attend(AttendArgs a, const AttnLayout& layout, float* scratch, long 
   else if (a.list[0].rows == 16) hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 1, 4>), grid, dim3(256), 0, stream, a);
   else if (a.list[0].waves == 8) hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 2, 8>), grid, dim3(512), 0, stream, a);
   else hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 2, 4>), grid, dim3(256), 0, stream, a);
-  if (joins > 0) hipLaunchKernelGGL((attend_join_kernel<T, D>), dim3(joins), dim3(1024), 0, stream, a);
+  if (joins > 0) hipLaunchKernelGGL((attend_join_kernel<T, D>), dim3(joins < kAttnJoiners ? joins : kAttnJoiners), dim3(1024), 0, stream, a);
 }
 struct AttendLaunch {
   const AttendArgs& a;

@@ -800,54 +800,58 @@ __global__ __launch_bounds__(256, 2) void attend_mixed_kernel(AttendArgs a) {
 }
 
 // Shares of one tile.  D / 4 lanes hold a row; 16 rows at a time (or as many as there are, rounded up to a power of two) and, between them, the shares: a
-// group of lanes adds every n-th share, the groups' sums are added in their order.  grid: of each list max_joins * kv_heads * rows / 16, the short one first; block 1024
+// group of lanes adds every n-th share, the groups' sums are added in their order.  The host knows bounds only, mostly far above what there is to join, so two
+// workgroups a CU walk what the plan says: one for every place of the bound took 10 to 15 us of a prompt's 180 to 370 to find that nothing was cut.
+// grid up to kAttnJoiners, block 1024
+constexpr int kAttnJoiners = 512;
 template <class T, int D>
 __global__ __launch_bounds__(1024) void attend_join_kernel(AttendArgs a) {
   constexpr int kLanes = D / 4, kGroups = 1024 / kLanes;
   __shared__ attn_f4 sums[1024];
   __shared__ float totals[kGroups];
-  const int short_units = a.list[0].max_joins * a.kv_heads * (a.list[0].rows / 16);
-  const int which = (int)blockIdx.x < short_units ? 0 : 1, unit = blockIdx.x - (which ? short_units : 0);
-  const int rows = a.list[which].rows, pieces = rows / 16, piece = unit % pieces, index = unit / pieces / a.kv_heads, head = unit / pieces - index * a.kv_heads;
-  const int* j = a.plan + a.list[which].joins + 8L * index;
-  const int q_start = j[0], n_tokens = j[1], tile = j[2], first = j[3], n_parts = j[4];
-  if (index >= a.plan[2 * which + 1]) return;
-  const int r0 = 16 * piece;
-  const float *part_o = a.part_o[which], *part_ml = a.part_ml[which];
-  const int live = (int)min(16L, (long)n_tokens * a.group - (long)tile * rows - r0);
-  if (live <= 0) return;
-  int wide = 1;                                  // rows side by side
-  while (wide < live) wide *= 2;
-  const int group = threadIdx.x / kLanes, d = 4 * (threadIdx.x % kLanes), i = group % wide, n = kGroups / wide;
-  const long step = (long)a.kv_heads * rows, at = ((long)first * a.kv_heads + head) * rows + r0 + min(i, live - 1);
-  float top = kAttnNone, sum = 0.f;
+  const int short_units = a.plan[1] * a.kv_heads * (a.list[0].rows / 16), units = short_units + a.plan[3] * a.kv_heads * (a.list[1].rows / 16);
+  const int group = threadIdx.x / kLanes, d = 4 * (threadIdx.x % kLanes);
+  for (int next = blockIdx.x; next < units; next += gridDim.x) {
+    const int which = next < short_units ? 0 : 1, unit = next - (which ? short_units : 0);
+    const int rows = a.list[which].rows, pieces = rows / 16, piece = unit % pieces, index = unit / pieces / a.kv_heads, head = unit / pieces - index * a.kv_heads;
+    const int* j = a.plan + a.list[which].joins + 8L * index;
+    const int q_start = j[0], n_tokens = j[1], tile = j[2], first = j[3], n_parts = j[4];
+    const int r0 = 16 * piece, live = min(16, n_tokens * a.group - tile * rows - r0);
+    if (live <= 0) continue;
+    const float *part_o = a.part_o[which], *part_ml = a.part_ml[which];
+    int wide = 1;                                  // rows side by side
+    while (wide < live) wide *= 2;
+    const int i = group % wide, n = kGroups / wide;
+    const long step = (long)a.kv_heads * rows, at = ((long)first * a.kv_heads + head) * rows + r0 + min(i, live - 1);
+    float top = kAttnNone, sum = 0.f;
 #pragma unroll 4
-  for (int p = 0; p < n_parts; p++) top = fmaxf(top, part_ml[2 * (at + p * step)]);
-  attn_f4 x = {0.f, 0.f, 0.f, 0.f};
+    for (int p = 0; p < n_parts; p++) top = fmaxf(top, part_ml[2 * (at + p * step)]);
+    attn_f4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int p = group / wide; p < n_parts; p += n) {
-    const float f = __builtin_amdgcn_exp2f(part_ml[2 * (at + p * step)] - top);
-    sum += f * part_ml[2 * (at + p * step) + 1];
-    const attn_f4 y = *reinterpret_cast<const attn_f4*>(part_o + (at + p * step) * D + d);
+    for (int p = group / wide; p < n_parts; p += n) {
+      const float f = __builtin_amdgcn_exp2f(part_ml[2 * (at + p * step)] - top);
+      sum += f * part_ml[2 * (at + p * step) + 1];
+      const attn_f4 y = *reinterpret_cast<const attn_f4*>(part_o + (at + p * step) * D + d);
 #pragma unroll
-    for (int k = 0; k < 4; k++) x[k] = __builtin_fmaf(y[k], f, x[k]);
-  }
-  sums[threadIdx.x] = x;
-  if (d == 0) totals[group] = sum;
-  __syncthreads();
-  if (group >= live) return;
-  x = sums[threadIdx.x], sum = totals[group];
-  for (int g = 1; g < n; g++) {
-    x += sums[threadIdx.x + g * wide * kLanes];
-    sum += totals[group + g * wide];
-  }
-  const long row = (long)tile * rows + r0 + group;
-  const int token = (int)(row / a.group), g = (int)(row - (long)token * a.group);
-  typedef T t4 __attribute__((ext_vector_type(4)));
-  t4 y;
+      for (int k = 0; k < 4; k++) x[k] = __builtin_fmaf(y[k], f, x[k]);
+    }
+    sums[threadIdx.x] = x;
+    if (d == 0) totals[group] = sum;
+    __syncthreads();
+    if (group < live) {
+      for (int g = 1; g < n; g++) {
+        x += sums[threadIdx.x + g * wide * kLanes];
+        sum += totals[group + g * wide];
+      }
+      const int row = tile * rows + r0 + group, token = row / a.group, g = row - token * a.group;
+      typedef T t4 __attribute__((ext_vector_type(4)));
+      t4 y;
 #pragma unroll
-  for (int k = 0; k < 4; k++) y[k] = sum == 0.f ? (T)0.f : (T)(x[k] / sum);
-  *reinterpret_cast<t4*>(static_cast<T*>(a.out) + ((long)(q_start + token) * (a.kv_heads * a.group) + head * a.group + g) * D + d) = y;
+      for (int k = 0; k < 4; k++) y[k] = sum == 0.f ? (T)0.f : (T)(x[k] / sum);
+      *reinterpret_cast<t4*>(static_cast<T*>(a.out) + ((long)(q_start + token) * (a.kv_heads * a.group) + head * a.group + g) * D + d) = y;
+    }
+    __syncthreads();
+  }
 }
 
 }  // namespace triteia_hip
