@@ -191,6 +191,9 @@ __device__ __forceinline__ AttnRow attn_row(const AttendArgs& a, const AttnItem&
 // Few rows: a decode step's heads, a handful of tokens.  Bound by the cache's bytes.  A workgroup takes a share of one tile's tokens; each of
 // its four or eight wavefronts walks sub-tiles of its own (8 KB of K and 8 KB of V: 32 tokens of 128 elements in 16 bits, 64 in 8) with the next one's whole rows
 // on their way in registers and this one's in LDS of its own, so that the loop has no barrier; maxima, sums and outputs are joined once at the end.
+// In 8 bits LDS holds the codes and each is converted once, behind its read (ds_read_b64_tr_b8 hands a lane eight tokens of a column).
+// Measured: 64 contexts of up to 4096 tokens, 32 heads, fp16 424 us (2.53 GB, 5.9 TB/s); 3 of up to 100000 over 8 heads in int8 77 + 8 us (402 MB, 5.2 TB/s in the
+// first launch); one of 500 8.2 us, of which about 1 are the plan's and 1 the pages' round trip, 1 the first rows', 2 two sub-tiles and 2 the joining.
 template <int KIND, int D, int NQ, int WAVES>
 struct AttnRowsLds {
   static constexpr int kRowBytes = D * (KIND == kCacheSame ? 2 : 1);
@@ -510,7 +513,13 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
 // ---------------------------------------------------------------------------------------------------------------------------------
 // Many rows: prompts.  Bound by the matrix cores and the exponentials.  A workgroup takes 128 rows, 32 a wavefront (as columns of 32 x 32 x 16
 // MFMAs), and walks the share's tokens in blocks of 64 that all of it reads from LDS: two places, the next block on its way in registers,
-// one barrier a block.  Codes of 8 bits become values on their way to LDS.
+// one barrier a block.  Codes of 8 bits become values on their way to LDS.  Two such workgroups a CU, so that one's exponentials run under the other's
+// MFMAs, which have priority; K rows, and V rows for the transposing reads, are XOR-swizzled by 16-byte pieces (no bank conflicts).
+// Measured: 4 x 500 new tokens behind contexts of up to 8200, 64 heads over 8, bf16 345 us = 808 TFLOP/s (equal contexts 890); 4000 from the first on, 32 heads,
+// fp16 173 us = 757.  Counters: matrix cores busy 45 % of the SIMDs' cycles, LDS 34 %, wavefronts waiting 28 % of theirs.  Loops of this MFMA reach
+// 1660 TFLOP/s alone and 1330 with the softmax's 4 vector instructions and 2 exponentials each between them.  In 8 bits 550: conversions and scales.
+// Measured and not kept: 256 rows on eight wavefronts and 128 tokens a barrier (equal contexts 1.02, e4m3 1.11, but 26 mixed sequences 0.87 and 3 x 100 new tokens
+// 0.81), V of the first columns read ahead of the softmax (1.00), priority around the second product as well (1.00).
 template <int D>
 struct AttnTileLds {
   static constexpr int kTile = kAttnBlock * 2 * D;
@@ -786,7 +795,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_rows_kernel(AttendArgs a
   attend_rows<T, KIND, D, NQ, WAVES>(a, index, blockIdx.x - index * a.kv_heads, shared);
 }
 
-// Any batch: the long list's items first, then the short one's, in one launch, so that what waits for memory runs beside what computes.
+// Any batch: the long list's items first, then the short one's, in one launch, so that what waits for memory runs beside what computes (a step of 26
+// sequences, two of them of 203 and 177 new tokens, in e4m3: 36.9 and 19.5 us one after the other, 39.2 together).
 // grid (list[1].max_items + list[0].max_items) * kv_heads, block 256
 template <class T, int KIND, int D>
 __global__ __launch_bounds__(256, 2) void attend_mixed_kernel(AttendArgs a) {
