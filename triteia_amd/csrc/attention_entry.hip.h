@@ -108,7 +108,7 @@ void launch_attend(AttendArgs a, const AttnLayout& layout, float* scratch, long 
     AttnList& l = a.list[which] = layout.list[which];
     // (no sequence is longer than its pages)
     if (table_tokens <= (long)l.min_blocks * kAttnBlock) l.max_joins = 0;
-    joins += l.max_joins * a.kv_heads * (l.rows / 16);
+    joins += l.max_joins * a.kv_heads * (l.rows / (1024 / D));
     a.part_o[which] = scratch;
     a.part_ml[which] = scratch + (long)l.max_parts * a.kv_heads * l.rows * D;
     scratch = a.part_ml[which] + 2L * l.max_parts * a.kv_heads * l.rows;
@@ -119,7 +119,7 @@ void launch_attend(AttendArgs a, const AttnLayout& layout, float* scratch, long 
   else if (a.list[0].rows == 16) hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 1, 4>), grid, dim3(256), 0, stream, a);
   else if (a.list[0].waves == 8) hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 2, 8>), grid, dim3(512), 0, stream, a);
   else hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 2, 4>), grid, dim3(256), 0, stream, a);
-  if (joins > 0) hipLaunchKernelGGL((attend_join_kernel<T, D>), dim3(joins < kAttnJoiners ? joins : kAttnJoiners), dim3(1024), 0, stream, a);
+  if (joins > 0) hipLaunchKernelGGL((attend_join_kernel<T, D>), dim3(joins < kAttnJoiners ? joins : kAttnJoiners), dim3(256), 0, stream, a);
 }
 struct AttendLaunch {
   const AttendArgs& a;

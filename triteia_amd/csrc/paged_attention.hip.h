@@ -809,24 +809,24 @@ __global__ __launch_bounds__(256, 2) void attend_mixed_kernel(AttendArgs a) {
   else attend_rows<T, KIND, D, 1, 4>(a, index - a.list[1].max_items, head, shared.rows);
 }
 
-// Shares of one tile.  D / 4 lanes hold a row; 16 rows at a time (or as many as there are, rounded up to a power of two) and, between them, the shares: a
-// group of lanes adds every n-th share, the groups' sums are added in their order.  The host knows bounds only, mostly far above what there is to join, so two
-// workgroups a CU walk what the plan says: one for every place of the bound took 10 to 15 us of a prompt's 180 to 370 to find that nothing was cut.
-// grid up to kAttnJoiners, block 1024
-constexpr int kAttnJoiners = 512;
+// Shares of one tile.  D / 4 lanes hold a row; a workgroup takes as many rows as it has such groups (or as many as there are, rounded up to a power of two) and,
+// between them, the shares: a group adds every n-th share, the groups' sums are added in their order.  The host knows bounds only, mostly far above
+// what there is to join, so a fixed number of workgroups walks what the plan says: one for every place of the bound took 10 to 15 us of a prompt's 180 to
+// 370 to find that nothing was cut.  grid up to kAttnJoiners, block 256
+constexpr int kAttnJoiners = 1024;
 template <class T, int D>
-__global__ __launch_bounds__(1024) void attend_join_kernel(AttendArgs a) {
-  constexpr int kLanes = D / 4, kGroups = 1024 / kLanes;
-  __shared__ attn_f4 sums[1024];
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
+  __shared__ attn_f4 sums[256];
   __shared__ float totals[kGroups];
-  const int short_units = a.plan[1] * a.kv_heads * (a.list[0].rows / 16), units = short_units + a.plan[3] * a.kv_heads * (a.list[1].rows / 16);
+  const int short_units = a.plan[1] * a.kv_heads * (a.list[0].rows / kGroups), units = short_units + a.plan[3] * a.kv_heads * (a.list[1].rows / kGroups);
   const int group = threadIdx.x / kLanes, d = 4 * (threadIdx.x % kLanes);
   for (int next = blockIdx.x; next < units; next += gridDim.x) {
     const int which = next < short_units ? 0 : 1, unit = next - (which ? short_units : 0);
-    const int rows = a.list[which].rows, pieces = rows / 16, piece = unit % pieces, index = unit / pieces / a.kv_heads, head = unit / pieces - index * a.kv_heads;
+    const int rows = a.list[which].rows, pieces = rows / kGroups, piece = unit % pieces, index = unit / pieces / a.kv_heads, head = unit / pieces - index * a.kv_heads;
     const int* j = a.plan + a.list[which].joins + 8L * index;
     const int q_start = j[0], n_tokens = j[1], tile = j[2], first = j[3], n_parts = j[4];
-    const int r0 = 16 * piece, live = min(16, n_tokens * a.group - tile * rows - r0);
+    const int r0 = kGroups * piece, live = min(kGroups, n_tokens * a.group - tile * rows - r0);
     if (live <= 0) continue;
     const float *part_o = a.part_o[which], *part_ml = a.part_ml[which];
     int wide = 1;                                  // rows side by side
