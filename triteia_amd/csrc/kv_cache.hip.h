@@ -13,7 +13,7 @@
 // two); a workgroup takes rows of one token, so cos, sin and the norms' weights are fetched once per lane and serve all its rows.
 // Measured: 8000 tokens of 40 + 40 heads of 128 in bf16 with norms 65.4 us (328 MB, 5.0 TB/s, what a copy reaches); 2000 tokens of 64 + 8 + 8 heads into an
 // int8 cache 23 us (78 MB: two rounds of workgroups, the second not full); 64 tokens of 32 + 32 + 32 heads 4.4 us; 20000 tokens of 32 heads
-// read back from e4m3 99 - 106 us (497 MB, 4.7 - 5.0 TB/s).
+// read back from e4m3 READUS.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -283,10 +283,11 @@ struct CacheReadArgs {
   const void* slots;
   int slots64, tokens, kv_heads, dim, page_shift;
   long n_slots;
+  int streamed;                  // stores that leave the caches to the rows that are read
 };
 
 // grid (tiles, 2: keys, values), block 256.  A tile is 4 heads of adjacent tokens, whose rows of a head lie side by side in a page (in the order of the
-// output, all heads of two tokens, 20000 tokens took 113 us instead of 105).  A slot outside the cache gives zeros.
+// output, all heads of two tokens, 20000 tokens of 32 heads took 113 us instead of 105).  A slot outside the cache gives zeros.
 template <class T, int KIND, int LPR, int U>
 __global__ __launch_bounds__(256) void cache_read_kernel(CacheReadArgs a) {
   constexpr int kRows = 256 / LPR, kTokens = kRows * U / 4;
@@ -327,7 +328,9 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheReadArgs a) {
       for (int j = 0; j < 8; j++) x[u][j] = (T)(y[j] * scale[u]);
     }
     if (!inside[u]) x[u] = kv8<T>{0, 0, 0, 0, 0, 0, 0, 0};
-    *reinterpret_cast<kv8<T>*>(out + (t * a.kv_heads + head) * a.dim + e) = x[u];
+    kv8<T>* dst = reinterpret_cast<kv8<T>*>(out + (t * a.kv_heads + head) * a.dim + e);
+    if (a.streamed) __builtin_nontemporal_store(x[u], dst);
+    else *dst = x[u];
   }
 }
 
