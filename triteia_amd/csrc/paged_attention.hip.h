@@ -154,7 +154,9 @@ __device__ __forceinline__ int attn_page(const AttendArgs& a, int seq, int token
 
 // One head's keys or values.  Where the 16 tokens of a group start is the same for all lanes and the base of a buffer; a lane's own offset from there, and
 // the offset of the rows of each further request, have 32 bits.  (Added up as 64-bit addresses they were half of the loop's scalar instructions.)
-template <int ROWS>                // of a request
+// ONCE: every row is read by one workgroup alone, as a decode step's are, and need not stay in the caches (64 contexts of up to 4096 tokens, 32 heads, 414 us
+// without that and 384, 3 of up to 100000 in int8 85.6 and 78; tiles of 128 rows, which share them, 335 and 349).
+template <int ROWS, bool ONCE>     // rows of a request
 struct AttnHeld {
   const uint8_t* head;
   long page;                       // strides in bytes
@@ -166,7 +168,7 @@ struct AttnHeld {
   __device__ __forceinline__ void read(kv_uint4* to, long p, int first) const {
     const auto rows = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(head) + p * page + (long)first * slot, 0, 0xffffffffu, 0x00027000);
 #pragma unroll
-    for (int j = 0; j < N; j++) to[j] = __builtin_bit_cast(kv_uint4, __builtin_amdgcn_raw_buffer_load_b128(rows, lane, j * step, 0));
+    for (int j = 0; j < N; j++) to[j] = __builtin_bit_cast(kv_uint4, __builtin_amdgcn_raw_buffer_load_b128(rows, lane, j * step, ONCE ? 2 : 0));
   }
 };
 
@@ -192,8 +194,8 @@ __device__ __forceinline__ AttnRow attn_row(const AttendArgs& a, const AttnItem&
 // its four or eight wavefronts walks sub-tiles of its own (8 KB of K and 8 KB of V: 32 tokens of 128 elements in 16 bits, 64 in 8) with the next one's whole rows
 // on their way in registers and this one's in LDS of its own, so that the loop has no barrier; maxima, sums and outputs are joined once at the end.
 // In 8 bits LDS holds the codes and each is converted once, behind its read (ds_read_b64_tr_b8 hands a lane eight tokens of a column).
-// Measured: 64 contexts of up to 4096 tokens, 32 heads, fp16 424 us (2.53 GB, 5.9 TB/s); 3 of up to 100000 over 8 heads in int8 77 + 8 us (402 MB, 5.2 TB/s in the
-// first launch); one of 500 8.2 us, of which about 1 are the plan's and 1 the pages' round trip, 1 the first rows', 2 two sub-tiles and 2 the joining.
+// Measured: 64 contexts of up to 4096 tokens, 32 heads, fp16 384 us a call (2.53 GB, 6.6 TB/s); 3 of up to 100000 over 8 heads in int8 78 us (402 MB), 8 of them
+// the joining launch's; one of 500 8.2 us, of which about 1 are the plan's and 1 the pages' round trip, 1 the first rows', 2 two sub-tiles and 2 the joining.
 template <int KIND, int D, int NQ, int WAVES>
 struct AttnRowsLds {
   static constexpr int kRowBytes = D * (KIND == kCacheSame ? 2 : 1);
@@ -231,7 +233,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
   float ks = 0.f, vs = 0.f;                 // scales of token `lane` of the sub-tile
   const int load_row = lane / kChunks, load_chunk = lane % kChunks;
   const int page_mask = (1 << a.page_shift) - 1;
-  const AttnHeld<kLoadRows> held_k(a.ck, head, kRowBytes / D, load_row, load_chunk), held_v(a.cv, head, kRowBytes / D, load_row, load_chunk);
+  const AttnHeld<kLoadRows, true> held_k(a.ck, head, kRowBytes / D, load_row, load_chunk), held_v(a.cv, head, kRowBytes / D, load_row, load_chunk);
   const float *scale_k = a.ck.scale + head * a.ck.scale_head, *scale_v = a.cv.scale + head * a.cv.scale_head;
   // A lane fetches the page of one 16-token group of the wavefront's next sub-tiles: kIds sub-tiles' pages are one request, a request ahead.
   constexpr int kIds = 64 / kGroups;
@@ -550,7 +552,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
   float rs = 0.f;
   const int load_row = lane / kHeldChunks, load_chunk = lane % kHeldChunks;
   const int page_mask = (1 << a.page_shift) - 1;
-  const AttnHeld<kLoadRows> held_k(a.ck, head, kHeld / D, load_row, load_chunk), held_v(a.cv, head, kHeld / D, load_row, load_chunk);
+  const AttnHeld<kLoadRows, false> held_k(a.ck, head, kHeld / D, load_row, load_chunk), held_v(a.cv, head, kHeld / D, load_row, load_chunk);
   const float *scale_k = a.ck.scale + head * a.ck.scale_head, *scale_v = a.cv.scale + head * a.cv.scale_head;
   // a lane fetches the page of the wavefront's 16 tokens of one of the next 64 blocks
   auto pages_from = [&](int i) {
