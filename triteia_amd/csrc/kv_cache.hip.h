@@ -11,9 +11,9 @@
 //
 // Bound by memory, and for a decode batch by the launch and one round trip.  LPR lanes of 16 bytes hold a row (D / 8 rounded up to a power of
 // two); a workgroup takes rows of one token, so cos, sin and the norms' weights are fetched once per lane and serve all its rows.
-// Measured: 8000 tokens of 40 + 40 heads of 128 in bf16 with norms 65.4 us (328 MB, 5.0 TB/s, what a copy reaches); 2000 tokens of 64 + 8 + 8 heads into an
-// int8 cache 23 us (78 MB: two rounds of workgroups, the second not full); 64 tokens of 32 + 32 + 32 heads 4.4 us; 20000 tokens of 32 heads
-// read back from e4m3 READUS.
+// Measured: 8000 tokens of 40 + 40 heads of 128 in bf16 with norms 63 - 66 us (328 MB, 5.0 - 5.2 TB/s, what a copy reaches); 2000 tokens of 64 + 8 + 8 heads
+// into an int8 cache 21 us (78 MB, 3.7 TB/s: position -> table row -> six passes, one after the other); 64 tokens of 32 + 32 + 32 heads 4.4 us; 20000
+// tokens of 32 heads read back from e4m3 98 - 103 us a call (497 MB, 4.8 - 5.1 TB/s).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -311,9 +311,11 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheReadArgs a) {
     const long page = inside[u] ? s >> a.page_shift : 0, slot = inside[u] ? s & ((1 << a.page_shift) - 1) : 0;
     const long at = page * c.page + head * c.head + slot * c.slot + e;
     if constexpr (KIND == kCacheSame) {
-      x[u] = *reinterpret_cast<const kv8<T>*>(static_cast<const T*>(c.data) + at);
+      const auto* src = reinterpret_cast<const kv8<T>*>(static_cast<const T*>(c.data) + at);
+      x[u] = a.streamed ? __builtin_nontemporal_load(src) : *src;
     } else {
-      code[u] = *reinterpret_cast<const kv_uint2*>(static_cast<const uint8_t*>(c.data) + at);
+      const auto* src = reinterpret_cast<const kv_uint2*>(static_cast<const uint8_t*>(c.data) + at);
+      code[u] = a.streamed ? __builtin_nontemporal_load(src) : *src;
       scale[u] = c.scale[page * c.scale_page + head * c.scale_head + slot * c.scale_slot];
     }
   }
