@@ -311,11 +311,9 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheReadArgs a) {
     const long page = inside[u] ? s >> a.page_shift : 0, slot = inside[u] ? s & ((1 << a.page_shift) - 1) : 0;
     const long at = page * c.page + head * c.head + slot * c.slot + e;
     if constexpr (KIND == kCacheSame) {
-      const auto* src = reinterpret_cast<const kv8<T>*>(static_cast<const T*>(c.data) + at);
-      x[u] = a.streamed ? __builtin_nontemporal_load(src) : *src;
+      x[u] = *reinterpret_cast<const kv8<T>*>(static_cast<const T*>(c.data) + at);
     } else {
-      const auto* src = reinterpret_cast<const kv_uint2*>(static_cast<const uint8_t*>(c.data) + at);
-      code[u] = a.streamed ? __builtin_nontemporal_load(src) : *src;
+      code[u] = *reinterpret_cast<const kv_uint2*>(static_cast<const uint8_t*>(c.data) + at);
       scale[u] = c.scale[page * c.scale_page + head * c.scale_head + slot * c.scale_slot];
     }
   }
