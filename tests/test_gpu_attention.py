@@ -321,6 +321,22 @@ def test_the_largest_number_of_new_tokens_is_a_hint(kind, most):
     batch.check(ops().paged_attention(*batch.inputs(), max_q=most))
 
 
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("most", [1, None])
+def test_the_scale_of_a_value_that_is_masked_changes_no_bit(kind, dtype, most):
+    for n, kv, heads, kv_heads, at in ((6, 40, 4, 2, 37), (20, 300, 8, 1, 290), (100, 150, 2, 2, 120), (1, 70, 2, 1, 10)):
+        window = 20 if n == 1 else 0
+        batch = Batch([(n, kv)], heads, kv_heads, 64, 16, kind, dtype)
+        clean = ops().paged_attention(*batch.inputs(), max_q=most, window=window)
+        page, slot = divmod(int(batch.slots(0, torch.tensor([at]))), 16)
+        batch.cache.v_scale[page, :, slot] *= 2.0 ** 14
+        got = ops().paged_attention(*batch.inputs(), max_q=most, window=window)
+        first = kv - n
+        sees = torch.tensor([first + t >= at and (not window or at > first + t - window) for t in range(n)])
+        assert torch.equal(got[~sees.cuda()], clean[~sees.cuda()])
+
+
 @pytest.mark.parametrize("kind", list(KINDS))
 @pytest.mark.parametrize("most", [1, None])
 def test_sequences_of_nothing(kind, most):

@@ -287,10 +287,10 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
   const int all_lo = last.lo, all_hi = first.hi;
 
   attn_f4 o[NQ][D / 16];
-  float m[NQ], l[NQ], norm = 0.f;           // norm: of the scales of V, so that P times a scale stays inside fp16
+  float m[NQ], l[NQ], norm[NQ];              // norm: the largest scale of V that the row has seen, so that P times a scale stays inside fp16
 #pragma unroll
   for (int n = 0; n < NQ; n++) {
-    m[n] = kAttnNone, l[n] = 0.f;
+    m[n] = kAttnNone, l[n] = 0.f, norm[n] = 0.f;
 #pragma unroll
     for (int d = 0; d < D / 16; d++) o[n][d] = attn_f4{0.f, 0.f, 0.f, 0.f};
   }
@@ -318,9 +318,9 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
     if constexpr (KIND != kCacheSame) {
       if (lane < kSub) scales[wave][0][lane] = ks * a.scale_log2, scales[wave][1][lane] = vs;
     }
-    float norm_now = norm;                   // the largest scale of V so far
+    float norm_now = 0.f;                    // the largest scale of V in this block
     if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) {
-      if (lane < kSub && t0 + lane < it.kv_end) norm_now = fmaxf(norm, vs);
+      if (lane < kSub && t0 + lane < it.kv_end) norm_now = fmaxf(0.f, vs);
       norm_now = attn_max16(across_row<16>(norm_now, [](float p, float q) { return fmaxf(p, q); }));
     }
     if (sub + WAVES < n_sub) request((sub - wave) / WAVES + 1);
@@ -348,10 +348,6 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
         }
       }
     }
-    float grown = 1.f;                       // what the outputs are multiplied by for a larger norm
-    if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) {
-      if (norm_now > norm) grown = norm / norm_now, norm = norm_now;
-    }
     v8 p[NQ][kSub / 32];
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
@@ -375,7 +371,20 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
           }
       }
       top = attn_max16(top);
-      float alpha = grown;
+      float alpha = 1.f;
+      if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) {
+        float most = norm_now;
+        if (edge) {                          // (of what the row sees alone)
+          most = 0.f;
+#pragma unroll
+          for (int g = 0; g < kGroups; g++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+              most = 16 * g + j < lo || 16 * g + j >= hi ? most : fmaxf(most, scales[wave][1][16 * g + 4 * h + j]);
+          most = attn_max16(most);
+        }
+        if (most > norm[n]) alpha = norm[n] / most, norm[n] = most;
+      }
       if (__any(top > m[n] + kAttnSlack)) {
         const float next = fmaxf(m[n], top);
         alpha *= __builtin_amdgcn_exp2f(m[n] - next);
@@ -388,7 +397,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
 #pragma unroll
           for (int j = 0; j < 4; j++) o[n][d][j] *= alpha;
       }
-      const float inv = KIND != kCacheSame && __is_same(T, _Float16) ? 1.f / fmaxf(norm, 1e-30f) : 1.f;
+      const float inv = KIND != kCacheSame && __is_same(T, _Float16) ? 1.f / fmaxf(norm[n], 1e-30f) : 1.f;
 #pragma unroll
       for (int g = 0; g < kGroups; g++)
 #pragma unroll
@@ -457,7 +466,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
 #pragma unroll
     for (int w = 0; w < WAVES; w++) top = fmaxf(top, meet_m[w][16 * n + col]);
     float f = __builtin_amdgcn_exp2f(m[n] - top);
-    if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) f *= norm;
+    if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) f *= norm[n];
 #pragma unroll
     for (int d = 0; d < D / 16; d++)
 #pragma unroll
@@ -519,7 +528,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
 // MFMAs, which have priority; K rows, and V rows for the transposing reads, are XOR-swizzled by 16-byte pieces (no bank conflicts).
 // Measured: 4 x 500 new tokens behind contexts of up to 8200, 64 heads over 8, bf16 345 us = 808 TFLOP/s (equal contexts 890); 4000 from the first on, 32 heads,
 // fp16 173 us = 757.  Counters: matrix cores busy 45 % of the SIMDs' cycles, LDS 34 %, wavefronts waiting 28 % of theirs.  Loops of this MFMA reach
-// 1660 TFLOP/s alone and 1330 with the softmax's 4 vector instructions and 2 exponentials each between them.  In 8 bits 550: conversions and scales.
+// 1660 TFLOP/s alone and 1330 with the softmax's 4 vector instructions and 2 exponentials each between them.  In 8 bits 630 (fp16, equal contexts): conversions and scales.
 // Measured and not kept: 256 rows on eight wavefronts and 128 tokens a barrier (equal contexts 1.02, e4m3 1.11, but 26 mixed sequences 0.87 and 3 x 100 new tokens
 // 0.81), V of the first columns read ahead of the softmax (1.00), priority around the second product as well (1.00).
 template <int D>
@@ -634,7 +643,9 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
   for (int d = 0; d < D / 32; d++)
 #pragma unroll
     for (int j = 0; j < 16; j++) o[d][j] = 0.f;
-  float m = kAttnNone, l = 0.f, norm = 0.f;
+  // (fp16 times a scale: P leaves the exponential over the largest scale of V that the row has seen so far, which the sums l and o then both are over as well)
+  constexpr bool kNormed = KIND != kCacheSame && __is_same(T, _Float16);
+  float m = kAttnNone, l = 0.f, norm = 1e-30f, log_norm = 0.f;
 
   if (n_blocks > 0) {
     keep(it.kv_begin, 0);
@@ -668,14 +679,26 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
       __builtin_amdgcn_s_setprio(0);
       step();                                // (its writes under the softmax)
       const bool edge = t0 < w1.lo || t0 + kAttnBlock > min(w0.hi, it.kv_end);
+      const int lo = mine.lo - t0 - 4 * h, hi = min(mine.hi, it.kv_end) - t0 - 4 * h;
       float grown = 1.f;
-      if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) {
-        float top = t0 + lane < it.kv_end ? fmaxf(norm, scales[at][1][lane]) : norm;
-        top = attn_max16(across_row<16>(top, [](float p, float q) { return fmaxf(p, q); }));
+      if constexpr (kNormed) {
+        float top = 0.f;
+        if (edge) {                          // (of what the row sees alone)
+#pragma unroll
+          for (int g = 0; g < 2; g++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+              const int token = 32 * g + 8 * (j / 4) + j % 4;
+              top = token < lo || token >= hi ? top : fmaxf(top, scales[at][1][token + 4 * h]);
+            }
+          top = attn_max32(top);
+        } else {
+          top = attn_max16(across_row<16>(scales[at][1][lane], [](float p, float q) { return fmaxf(p, q); }));
+        }
         if (top > norm) grown = norm / top, norm = top;
+        log_norm = __builtin_amdgcn_logf(norm);
       }
       float top = kAttnNone;
-      const int lo = mine.lo - t0 - 4 * h, hi = min(mine.hi, it.kv_end) - t0 - 4 * h;
 #pragma unroll
       for (int g = 0; g < 2; g++)
 #pragma unroll
@@ -697,6 +720,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
       if constexpr (KIND == kCacheSame) top = fmaxf(top * a.scale_log2, kAttnNone);
       top = attn_max32(top);
       float alpha = grown;
+      l *= grown;
       if (__any(top > m + kAttnSlack)) {
         const float next = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - next);
         alpha *= f, l *= f, m = next;
@@ -707,16 +731,16 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
 #pragma unroll
           for (int j = 0; j < 16; j++) o[d][j] *= alpha;
       }
-      const float inv = KIND != kCacheSame && __is_same(T, _Float16) ? 1.f / fmaxf(norm, 1e-30f) : 1.f;
+      const float under = kNormed ? m + log_norm : m;
       v8 p[4];
       float sum[4] = {0.f, 0.f, 0.f, 0.f};   // (one running sum would be a chain of 32 additions)
 #pragma unroll
       for (int g = 0; g < 2; g++)
 #pragma unroll
         for (int j = 0; j < 16; j++) {
-          const float e = __builtin_amdgcn_exp2f(KIND == kCacheSame ? __builtin_fmaf(s[g][j], a.scale_log2, -m) : s[g][j] - m);
+          const float e = __builtin_amdgcn_exp2f(KIND == kCacheSame ? __builtin_fmaf(s[g][j], a.scale_log2, -m) : s[g][j] - under);
           sum[j % 4] += e;
-          s[g][j] = KIND == kCacheSame ? e : e * (scales[at][1][32 * g + 8 * (j / 4) + j % 4 + 4 * h] * inv);
+          s[g][j] = KIND == kCacheSame ? e : e * scales[at][1][32 * g + 8 * (j / 4) + j % 4 + 4 * h];
         }
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       if (KIND != kCacheSame && edge) {              // (a scale may be a NaN)
@@ -759,11 +783,10 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
   }
   if (!mine.live || 32 * wave + col >= n_rows) return;
   l += __shfl_xor(l, 32);
-  float f = 1.f;
-  if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) f = norm;
+  float f = kNormed ? norm : 1.f;
   if (it.part < 0) {
     typedef T t4 __attribute__((ext_vector_type(4)));
-    f = l == 0.f ? 0.f : f / l;
+    f = l == 0.f ? 0.f : 1.f / l;
     T* out = static_cast<T*>(a.out) + ((long)(it.q_start + mine.token) * (a.kv_heads * a.group) + head * a.group + mine.head) * D + 4 * h;
 #pragma unroll
     for (int d = 0; d < D / 32; d++)
@@ -785,7 +808,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
         for (int j = 0; j < 4; j++) y[j] = o[d][4 * i + j] * f;
         *reinterpret_cast<attn_f4*>(a.part_o[1] + at * D + 32 * d + 8 * i + 4 * h) = y;
       }
-    if (h == 0) a.part_ml[1][2 * at] = m, a.part_ml[1][2 * at + 1] = l;
+    if (h == 0) a.part_ml[1][2 * at] = m, a.part_ml[1][2 * at + 1] = l * f;
   }
 }
 
