@@ -172,6 +172,18 @@ struct AttnHeld {
   }
 };
 
+// The tokens that a lane's row sees of a block, for the branches of blocks on an edge: a value of its own in each, or the compiler takes the comparisons of all
+// branches out of them and does them for every block (4 x 500 new tokens behind 8200 in e4m3 440 us that way, 373 this).
+struct AttnSpan {
+  int lo, hi;
+  __device__ __forceinline__ AttnSpan here() const {
+    AttnSpan x = *this;
+    asm volatile("" : "+v"(x.lo), "+v"(x.hi));
+    return x;
+  }
+  __device__ __forceinline__ bool hides(int token) const { return token < lo || token >= hi; }
+};
+
 // Which tokens row `r` of a tile sees: lo <= token < hi.  Rows behind the last see all that the tile sees and are not stored.
 struct AttnRow {
   int lo, hi, token, head;     // token of the sequence, head of the group
@@ -359,14 +371,15 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
           s[n][g][j] *= KIND == kCacheSame ? a.scale_log2 : scales[wave][0][16 * g + 4 * h + j];
           top = fmaxf(top, s[n][g][j]);
         }
-      const int lo = row_lo[n] - t0 - 4 * h, hi = min(row_hi[n], it.kv_end) - t0 - 4 * h;
+      const AttnSpan span = {row_lo[n] - t0 - 4 * h, min(row_hi[n], it.kv_end) - t0 - 4 * h};
       if (edge) {
+        const AttnSpan seen = span.here();
         top = kAttnNone;
 #pragma unroll
         for (int g = 0; g < kGroups; g++)
 #pragma unroll
           for (int j = 0; j < 4; j++) {
-            s[n][g][j] = 16 * g + j < lo || 16 * g + j >= hi ? -__builtin_inff() : s[n][g][j];
+            s[n][g][j] = seen.hides(16 * g + j) ? -__builtin_inff() : s[n][g][j];
             top = fmaxf(top, s[n][g][j]);
           }
       }
@@ -375,12 +388,13 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
       if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) {
         float most = norm_now;
         if (edge) {                          // (of what the row sees alone)
+          const AttnSpan seen = span.here();
           most = 0.f;
 #pragma unroll
           for (int g = 0; g < kGroups; g++)
 #pragma unroll
             for (int j = 0; j < 4; j++)
-              most = 16 * g + j < lo || 16 * g + j >= hi ? most : fmaxf(most, scales[wave][1][16 * g + 4 * h + j]);
+              most = seen.hides(16 * g + j) ? most : fmaxf(most, scales[wave][1][16 * g + 4 * h + j]);
           most = attn_max16(most);
         }
         if (most > norm[n]) alpha = norm[n] / most, norm[n] = most;
@@ -407,10 +421,11 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
           s[n][g][j] = KIND == kCacheSame ? e : e * (scales[wave][1][16 * g + 4 * h + j] * inv);
         }
       if (KIND != kCacheSame && edge) {              // (a scale may be a NaN)
+        const AttnSpan seen = span.here();
 #pragma unroll
         for (int g = 0; g < kGroups; g++)
 #pragma unroll
-          for (int j = 0; j < 4; j++) s[n][g][j] = 16 * g + j < lo || 16 * g + j >= hi ? 0.f : s[n][g][j];
+          for (int j = 0; j < 4; j++) s[n][g][j] = seen.hides(16 * g + j) ? 0.f : s[n][g][j];
       }
 #pragma unroll
       for (int g = 0; g < kGroups; g++)
@@ -528,7 +543,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
 // MFMAs, which have priority; K rows, and V rows for the transposing reads, are XOR-swizzled by 16-byte pieces (no bank conflicts).
 // Measured: 4 x 500 new tokens behind contexts of up to 8200, 64 heads over 8, bf16 345 us = 808 TFLOP/s (equal contexts 890); 4000 from the first on, 32 heads,
 // fp16 173 us = 757.  Counters: matrix cores busy 45 % of the SIMDs' cycles, LDS 34 %, wavefronts waiting 28 % of theirs.  Loops of this MFMA reach
-// 1660 TFLOP/s alone and 1330 with the softmax's 4 vector instructions and 2 exponentials each between them.  In 8 bits 630 (fp16, equal contexts): conversions and scales.
+// 1660 TFLOP/s alone and 1330 with the softmax's 4 vector instructions and 2 exponentials each between them.  In 8 bits 780 (e4m3, fp16, equal contexts): conversions and scales.
 // Measured and not kept: 256 rows on eight wavefronts and 128 tokens a barrier (equal contexts 1.02, e4m3 1.11, but 26 mixed sequences 0.87 and 3 x 100 new tokens
 // 0.81), V of the first columns read ahead of the softmax (1.00), priority around the second product as well (1.00).
 template <int D>
@@ -679,17 +694,18 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
       __builtin_amdgcn_s_setprio(0);
       step();                                // (its writes under the softmax)
       const bool edge = t0 < w1.lo || t0 + kAttnBlock > min(w0.hi, it.kv_end);
-      const int lo = mine.lo - t0 - 4 * h, hi = min(mine.hi, it.kv_end) - t0 - 4 * h;
+      const AttnSpan span = {mine.lo - t0 - 4 * h, min(mine.hi, it.kv_end) - t0 - 4 * h};
       float grown = 1.f;
       if constexpr (kNormed) {
         float top = 0.f;
         if (edge) {                          // (of what the row sees alone)
+          const AttnSpan seen = span.here();
 #pragma unroll
           for (int g = 0; g < 2; g++)
 #pragma unroll
             for (int j = 0; j < 16; j++) {
               const int token = 32 * g + 8 * (j / 4) + j % 4;
-              top = token < lo || token >= hi ? top : fmaxf(top, scales[at][1][token + 4 * h]);
+              top = seen.hides(token) ? top : fmaxf(top, scales[at][1][token + 4 * h]);
             }
           top = attn_max32(top);
         } else {
@@ -707,13 +723,14 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
           top = fmaxf(top, s[g][j]);
         }
       if (edge) {
+        const AttnSpan seen = span.here();
         top = kAttnNone;
 #pragma unroll
         for (int g = 0; g < 2; g++)
 #pragma unroll
           for (int j = 0; j < 16; j++) {
             const int token = 32 * g + 8 * (j / 4) + j % 4;
-            s[g][j] = token < lo || token >= hi ? -__builtin_inff() : s[g][j];
+            s[g][j] = seen.hides(token) ? -__builtin_inff() : s[g][j];
             top = fmaxf(top, s[g][j]);
           }
       }
@@ -744,12 +761,13 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
         }
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       if (KIND != kCacheSame && edge) {              // (a scale may be a NaN)
+        const AttnSpan seen = span.here();
 #pragma unroll
         for (int g = 0; g < 2; g++)
 #pragma unroll
           for (int j = 0; j < 16; j++) {
             const int token = 32 * g + 8 * (j / 4) + j % 4;
-            s[g][j] = token < lo || token >= hi ? 0.f : s[g][j];
+            s[g][j] = seen.hides(token) ? 0.f : s[g][j];
           }
       }
 #pragma unroll
