@@ -339,6 +339,14 @@ def test_the_scale_of_a_value_that_is_masked_changes_no_bit(kind, dtype, most):
 
 @pytest.mark.parametrize("kind", list(KINDS))
 @pytest.mark.parametrize("most", [1, None])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 40, 2 ** 30])
+def test_windows_longer_than_any_context(kind, most, window):
+    batch = Batch([(1, 300), (6, 2), (200, 30), (40, 0), (129, 263)], 6, 2, 64, 16, kind)
+    batch.check(ops().paged_attention(*batch.inputs(), max_q=most, window=window), window=window)
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("most", [1, None])
 def test_sequences_of_nothing(kind, most):
     """No new tokens, no context, new tokens that reach back ahead of the first token of the context, padding behind the last sequence."""
     batch = Batch([(0, 0), (1, 0), (0, 50), (1, 7), (6, 2), (40, 0), (200, 30), (0, 0)], 6, 2, 64, 16, kind, padding=21)

@@ -196,7 +196,7 @@ __device__ __forceinline__ AttnRow attn_row(const AttendArgs& a, const AttnItem&
   x.live = x.token < it.n_tokens;
   const int position = it.kv_len - it.n_tokens + x.token;
   x.hi = x.live && a.causal ? min(position + 1, it.kv_len) : it.kv_len;
-  x.lo = x.live && a.window > 0 ? position - a.window + 1 : 0;
+  x.lo = x.live && a.window > 0 ? max(0, max(position, 0) - a.window + 1) : 0;      // (a window may be as long as an int is large)
   if (!x.live) x.token = 0, x.head = 0;
   return x;
 }
