@@ -383,7 +383,8 @@ TRITEIA_HIP_API int triteia_hip_attention_plan(const void* q_starts, const void*
                              int window, void* plan, size_t plan_bytes, int dev, void* stream);
 /* out [n_tokens, heads, dim] = softmax(scale q k^T) v over the pages of each token's sequence, on a plan made with the same numbers.  causal: the
  * last new token sees the whole context, each one before it a token less; window > 0: the last `window` of those.  Head h reads head
- * h / (heads / kv_heads) of the cache.  pages int32 [n_seqs, table_width] with a row stride; a row without tokens to see gives zeros.  dim 64 or 128,
+ * h / (heads / kv_heads) of the cache.  pages int32 [n_seqs, table_width] with a row stride; tokens behind the table's last column are not
+ * seen; a row without tokens to see gives zeros.  dim 64 or 128,
  * scale positive; a page's scales of one head are adjacent and 16-byte aligned. */
 TRITEIA_HIP_API int triteia_hip_paged_attention(const void* q, long q_token, long q_head, void* out, const void* cache_k, const void* cache_v, const void* k_scale,
                              const void* v_scale, const long* strides, int n_pages, int page, int kind, const void* pages, long pages_seq, int table_width,

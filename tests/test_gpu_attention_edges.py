@@ -1,0 +1,79 @@
+"""The attention side where the range of a type, a table or a list ends, and the kernels' builds and the plan's branches that the ordinary batches do not reach.
+
+Bounds are those of test_gpu_attention.py unless a test derives its own."""
+import math
+
+import pytest
+import torch
+
+from tests.test_gpu_attention import HALF, KINDS, U, Batch, empty_cache, ops, randn, rows_of
+
+pytestmark = pytest.mark.gpu
+
+
+def attend_into_nan(batch, starts, lens, pages, most, causal=True, window=0):
+    """paged_attention by the C ABI with an output and a scratch full of NaN: what no kernel writes, or reads without having written it, shows."""
+    from triteia_amd.python.capi import _ffi
+    q, cache = batch.q.cuda(), batch.cache
+    plan = ops().attention_plan(cache, starts, lens, batch.heads, q.shape[0], most, causal, window)
+    out = torch.full_like(q, math.nan)
+    nbytes = _ffi.lib().triteia_hip_attention_scratch_bytes(plan.n_seqs, plan.n_tokens, plan.heads, plan.kv_heads, plan.max_q, cache.dim)
+    scratch = torch.full((nbytes,), 0xff, dtype=torch.uint8, device="cuda")
+    code = _ffi.lib().triteia_hip_paged_attention(
+        _ffi.ptr(q), q.stride(0), q.stride(1), _ffi.ptr(out), *cache._pointers(), cache._strides, cache.n_pages, cache.page, cache.kind, _ffi.ptr(pages),
+        pages.stride(0), pages.shape[1], _ffi.ptr(plan.buffer), plan.buffer.numel(), plan.n_seqs, plan.n_tokens, plan.heads, plan.kv_heads, cache.dim, plan.max_q,
+        int(causal), window, cache.dim ** -0.5, _ffi.ptr(scratch), nbytes, int(q.dtype == torch.bfloat16), _ffi.device_index(q), _ffi.stream_of(q))
+    assert code == 0, _ffi.last_error()
+    return out
+
+
+# --- lengths, offsets and tables that do not fit each other -----------------------------------------------------------------------
+
+def answer_within(batch, limit, lens, causal=True, window=0):
+    """Batch.answer with contexts of `lens` of which the table holds the first `limit` tokens."""
+    want = torch.zeros(batch.q.shape, dtype=torch.float64)
+    size, most = torch.zeros_like(want), torch.zeros(want.shape[:2] + (1,), dtype=torch.float64)
+    group = batch.heads // batch.kv_heads
+    for b, (n, _) in enumerate(batch.lengths):
+        rows = slice(batch.starts[b], batch.starts[b + 1])
+        k, v = (x[b][:limit].repeat_interleave(group, 1) for x in (batch.k, batch.v))
+        score = torch.einsum("thd,shd->hts", batch.q[rows].double(), k) * batch.dim ** -0.5
+        position, token = torch.arange(n)[:, None] + (lens[b] - n), torch.arange(k.shape[0])
+        seen = (token < lens[b]).expand(n, -1)
+        if causal:
+            seen = seen & (token <= position)
+        if window:
+            seen = seen & (token > position - window)
+        p = torch.nan_to_num(torch.softmax(score.masked_fill(~seen, -math.inf), -1))
+        want[rows], size[rows] = torch.einsum("hts,shd->thd", p, v), torch.einsum("hts,shd->thd", p, v.abs())
+        most[rows] = k.shape[0] * v.abs().max()
+    return want, size, most
+
+
+def close(batch, got, want, size, most):
+    bound = (2 * U[batch.dtype] + 2.0 ** -13) * size + 2.0 ** -24 * most + 1e-30
+    got = got.double().cpu()
+    assert bool(((got - want).abs() <= bound).all()), f"{float(((got - want).abs() / bound).nan_to_num(math.inf).max()):.3f} of the bound"
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("most", [1, None])
+@pytest.mark.parametrize("columns", [3, 10, 40])
+def test_tokens_that_the_table_does_not_hold_are_not_seen(kind, most, columns):
+    """The plan cuts by lengths, the attention joins by what the table can hold: every row is written all the same."""
+    batch = Batch([(1, 3000), (1, 40), (100, 2500), (6, 700), (1, 1030)], 4, 2, 64, 16, kind)
+    lens, pages = [kv for _, kv in batch.lengths], batch.pages[:, :columns].contiguous().cuda()
+    args = (torch.tensor(batch.starts, dtype=torch.int32).cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), pages)
+    for how in ({}, {"window": 50}, {"window": 2400}, {"causal": False}):
+        close(batch, attend_into_nan(batch, *args, most, **how), *answer_within(batch, 16 * columns, lens, **how))
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("most", [1, None])
+def test_the_largest_lengths_cost_what_the_table_holds(kind, most):
+    batch = Batch([(1, 300), (5, 300), (130, 300)], 4, 2, 64, 16, kind)
+    starts, pages = torch.tensor(batch.starts, dtype=torch.int32).cuda(), batch.pages[:, :18].contiguous().cuda()
+    for lens in ([2 ** 31 - 1] * 3, [2 ** 31 - 70, 300, 2 ** 30], [2 ** 31 - 1, 2 ** 31 - 129, 299]):
+        for how in ({}, {"window": 60}, {"causal": False}):
+            got = attend_into_nan(batch, starts, torch.tensor(lens, dtype=torch.int32).cuda(), pages, most, **how)
+            close(batch, got, *answer_within(batch, 288, lens, **how))

@@ -111,14 +111,14 @@ template <class T, int KIND, int D>
 void launch_attend(AttendArgs a, const AttnLayout& layout, float* scratch, long table_tokens, hipStream_t stream) {
   int joins = 0;
   for (int which = 0; which < 2; which++) {
-    AttnList& l = a.list[which] = layout.list[which];
-    // (no sequence is longer than its pages)
-    if (table_tokens <= (long)l.min_blocks * kAttnBlock) l.max_joins = 0;
-    joins += l.max_joins * a.kv_heads * (l.rows / (1024 / D));
+    const AttnList& l = a.list[which] = layout.list[which];
+    // (contexts that a table of so few tokens can hold are not cut)
+    if (table_tokens > (long)l.min_blocks * kAttnBlock) joins += l.max_joins * a.kv_heads * (l.rows / (1024 / D));
     a.part_o[which] = scratch;
     a.part_ml[which] = scratch + (long)l.max_parts * a.kv_heads * l.rows * D;
     scratch = a.part_ml[which] + 2L * l.max_parts * a.kv_heads * l.rows;
   }
+  a.joined = joins > 0;
   const dim3 grid((unsigned)((long)(a.list[0].max_items + a.list[1].max_items) * a.kv_heads));
   if (a.list[1].max_items > 0) hipLaunchKernelGGL((attend_mixed_kernel<T, KIND, D>), grid, dim3(256), 0, stream, a);
   else if (a.list[0].rows == 16 && a.list[0].waves == 8) hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 1, 8>), grid, dim3(512), 0, stream, a);
@@ -273,6 +273,7 @@ int triteia_hip_paged_attention(const void* q, long q_token, long q_head, void* 
     return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: plan or scratch too small", what);
   a.q = q, a.q_token = q_token, a.q_head = q_head, a.out = out;
   a.pages = static_cast<const int*>(pages), a.pages_seq = pages_seq, a.n_pages = n_pages, a.table_width = table_width, a.page_shift = page_shift_of(page);
+  a.held = (long)table_width * page < kAttnMaxTokens ? table_width * page : kAttnMaxTokens;
   a.group = heads / kv_heads, a.kv_heads = kv_heads, a.causal = causal, a.window = window, a.scale_log2 = scale * 1.44269504088896340736f;
   a.plan = static_cast<const int*>(plan);
   DeviceGuard g(dev);

@@ -21,6 +21,7 @@ constexpr int kAttnTileRows = 128;     // rows of a tile of the long list
 constexpr int kAttnWaves = 8;          // at most, of a workgroup with few rows
 constexpr int kAttnSorted = 256;       // lists of up to this many tiles begin with the longest
 constexpr int kAttnMaxSeqs = 4096;
+constexpr int kAttnMaxTokens = 0x7fffff80;   // a longer context is taken as this long, so that the end of its last block is still an int
 constexpr int kAttnPlanThreads = 128;
 
 // One share of one tile.
@@ -115,7 +116,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const 
   for (int b = threadIdx.x; b <= a.n_seqs; b += kAttnPlanThreads) {
     const bool rest = b == a.n_seqs;
     const int lo = max(0, min(q_starts[b], a.n_tokens)), hi = rest ? a.n_tokens : max(lo, min(q_starts[b + 1], a.n_tokens));
-    start[b] = lo, count[b] = hi - lo, context[b] = rest ? 0 : max(kv_lens[b], 0);
+    start[b] = lo, count[b] = hi - lo, context[b] = rest ? 0 : min(max(kv_lens[b], 0), kAttnMaxTokens);
   }
   __syncthreads();
   const int which = threadIdx.x >> 6, lane = threadIdx.x & 63;

@@ -35,6 +35,7 @@ struct AttendArgs {
   const int* pages;
   long pages_seq;                       // stride
   int n_pages, table_width, page_shift;
+  int held, joined;                     // tokens that a row of the table holds; whether a launch behind joins shares
   int group, kv_heads, causal, window;
   float scale_log2;                     // scale * log2(e)
   const int* plan;
@@ -201,6 +202,18 @@ __device__ __forceinline__ AttnRow attn_row(const AttendArgs& a, const AttnItem&
   return x;
 }
 
+// The plan knows lengths, not the table: an item is held to the tokens that the table has.  Where no context that the table can hold is worth cutting there
+// is no launch that joins, and a plan that has cut all the same (for lengths that the table cannot hold) leaves the tile to its first share, which takes
+// all of it.  False: nothing is left to do.
+__device__ __forceinline__ bool attn_within(const AttendArgs& a, int rows, AttnItem* it) {
+  if (it->part >= 0 && !a.joined) {
+    if (it->kv_begin != attn_row(a, *it, rows, 0).lo / kAttnBlock * kAttnBlock) return false;
+    it->part = -1, it->kv_end = it->kv_len;
+  }
+  it->kv_end = min(it->kv_end, a.held), it->kv_begin = min(it->kv_begin, it->kv_end);
+  return true;
+}
+
 // ---------------------------------------------------------------------------------------------------------------------------------
 // Few rows: a decode step's heads, a handful of tokens.  Bound by the cache's bytes.  A workgroup takes a share of one tile's tokens; each of
 // its four or eight wavefronts walks sub-tiles of its own (8 KB of K and 8 KB of V: 32 tokens of 128 elements in 16 bits, 64 in 8) with the next one's whole rows
@@ -233,8 +246,8 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
   auto& meet_m = shared.meet_m;
   auto& meet_l = shared.meet_l;
   auto& scales = shared.scales;
-  const AttnItem it = attn_item(a, 0, index);        // (requested together with the number of items)
-  if (index >= a.plan[0]) return;
+  AttnItem it = attn_item(a, 0, index);              // (requested together with the number of items)
+  if (index >= a.plan[0] || !attn_within(a, kRows, &it)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, h = lane >> 4;
   uint8_t* lds_k = lds + wave * 2 * kTile;
@@ -567,8 +580,8 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
   uint8_t* lds = shared.tiles;
   auto& scales = shared.scales;
   auto& odd = shared.odd;
-  const AttnItem it = attn_item(a, 1, index);
-  if (index >= a.plan[2]) return;
+  AttnItem it = attn_item(a, 1, index);
+  if (index >= a.plan[2] || !attn_within(a, kAttnTileRows, &it)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, h = lane >> 5;
 

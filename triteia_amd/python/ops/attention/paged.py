@@ -18,7 +18,7 @@ def paged_attention(q, cache, pages, q_starts, kv_lens, plan=None, max_q=None, c
     """softmax(scale * q k^T) v [tokens, heads, dim] of new tokens q [tokens, heads, dim] over their sequences' contexts, head h on head
     h // (heads / kv_heads) of the cache.
 
-    pages int32 [sequences, pages of one]: a sequence's pages in order (entries behind its last are not read).  causal: the last of a sequence's new tokens sees all of its context,
+    pages int32 [sequences, pages of one]: a sequence's pages in order (entries behind its last are not read; tokens behind the last column are not seen).  causal: the last of a sequence's new tokens sees all of its context,
     each one before it one token less; with `window` it sees the last `window` of those only.  causal=False: every token sees the whole context (cross attention
     to states of another length).  A token that sees nothing gets zeros.  `plan`: from `attention_plan` with the same
     lengths, causal and window (None: made here); scale: dim^-0.5 if None.  Serving only: no gradient is recorded."""
