@@ -77,3 +77,17 @@ def test_the_largest_lengths_cost_what_the_table_holds(kind, most):
         for how in ({}, {"window": 60}, {"causal": False}):
             got = attend_into_nan(batch, starts, torch.tensor(lens, dtype=torch.int32).cuda(), pages, most, **how)
             close(batch, got, *answer_within(batch, 288, lens, **how))
+
+
+@pytest.mark.parametrize("most", [1, None])
+@pytest.mark.parametrize("starts", [[0, 500, -3, 140], [0, 140, 0, 140], [-7, 1, 2, 10 ** 9], [3, 20, 50, 140], [140, 0, 0, 0], [50, 60, 10, 30], [9, 9, 9, 9]])
+def test_offsets_in_any_order_leave_no_row_out(most, starts):
+    """An offset is taken as the largest of those up to it, the first as 0: every token has one sequence, or none."""
+    batch = Batch([(1, 40), (9, 77), (130, 200)], 6, 3, 64, 16)
+    got = attend_into_nan(batch, torch.tensor(starts, dtype=torch.int32).cuda(), torch.tensor([kv for _, kv in batch.lengths], dtype=torch.int32).cuda(),
+                          batch.pages.cuda(), most)
+    taken = [0]
+    for s in starts[1:]:
+        taken.append(max(taken[-1], min(max(s, 0), 140)))
+    batch.starts, batch.lengths = taken, [(b - a, kv) for a, b, (_, kv) in zip(taken, taken[1:], batch.lengths)]
+    batch.check(got)

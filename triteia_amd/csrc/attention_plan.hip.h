@@ -8,7 +8,7 @@
 //
 // One workgroup of two wavefronts, a list each, so that nothing but the sequences' lengths in LDS is waited for: sums over the lanes, a lane finds the
 // sequence of a tile by a binary search.  Tokens behind the last sequence get tiles without keys, whose rows are zeros.  Every number read from the
-// device is clamped, so that no list passes its end.
+// device is clamped and offsets that do not ascend are made to, so that every row has one tile and no list passes its end.
 // Bound by latency: 6.5 us for one sequence, 8.3 for a step's 26 of which two are long (14.2 with 1024 threads on one list after the other, whose barriers
 // and shuffles were the time), 11.6 for 64, which are also put in order.
 #pragma once
@@ -113,12 +113,30 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const 
   __shared__ int start[kAttnMaxSeqs + 1], count[kAttnMaxSeqs + 1], context[kAttnMaxSeqs + 1];
   __shared__ int tiles_ahead[2][kAttnMaxSeqs + 1];       // of each sequence, in each list
   __shared__ int order[2][kAttnSorted];
+  __shared__ int crossed[kAttnPlanThreads / 64];
+  bool back = false;                                     // an offset below the one ahead of it
   for (int b = threadIdx.x; b <= a.n_seqs; b += kAttnPlanThreads) {
     const bool rest = b == a.n_seqs;
-    const int lo = max(0, min(q_starts[b], a.n_tokens)), hi = rest ? a.n_tokens : max(lo, min(q_starts[b + 1], a.n_tokens));
+    const int lo = b == 0 ? 0 : max(0, min(q_starts[b], a.n_tokens)), hi = rest ? a.n_tokens : max(0, min(q_starts[b + 1], a.n_tokens));
+    back |= hi < lo;
     start[b] = lo, count[b] = hi - lo, context[b] = rest ? 0 : min(max(kv_lens[b], 0), kAttnMaxTokens);
   }
+  const bool any_back = __any(back);
+  if ((threadIdx.x & 63) == 0) crossed[threadIdx.x >> 6] = any_back;
   __syncthreads();
+  bool mend = false;
+#pragma unroll
+  for (int w = 0; w < kAttnPlanThreads / 64; w++) mend |= crossed[w] != 0;
+  if (mend) {                                            // offsets in no order: each as the largest up to it, so that every token has one place
+    if (threadIdx.x == 0) {
+      for (int b = 1; b <= a.n_seqs; b++) {
+        start[b] = max(start[b], start[b - 1]);
+        count[b - 1] = start[b] - start[b - 1];
+      }
+      count[a.n_seqs] = a.n_tokens - start[a.n_seqs];
+    }
+    __syncthreads();
+  }
   const int which = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const AttnList& l = a.list[which];
   if (l.max_items == 0) {
@@ -198,7 +216,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const 
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
   }
   int n_items = 0, n_joins = 0, n_parts = 0;
-  int end_items = l.max_items, end_joins = l.max_joins;          // (all have a place, but for offsets that do not ascend)
+  int end_items = l.max_items, end_joins = l.max_joins;          // (all have a place: the cut leaves no more shares than the host has counted)
   for (int i0 = 0; i0 < tiles; i0 += 64) {
     // (of long lists a sequence's last tile, its longest, first)
     const int i = i0 + lane >= tiles ? -1 : tiles <= kAttnSorted ? order[which][i0 + lane] : tiles - 1 - (i0 + lane);
