@@ -91,3 +91,37 @@ def test_offsets_in_any_order_leave_no_row_out(most, starts):
         taken.append(max(taken[-1], min(max(s, 0), 140)))
     batch.starts, batch.lengths = taken, [(b - a, kv) for a, b, (_, kv) in zip(taken, taken[1:], batch.lengths)]
     batch.check(got)
+
+
+# --- weights, scores and scales far apart -----------------------------------------------------------------------------------------
+
+def put(batch, b, k, v):
+    """Other keys and values [tokens, heads of the cache, dim] for sequence b."""
+    place = batch.slots(b, torch.arange(batch.lengths[b][1]))
+    ops().cache_write(batch.cache, k.to(batch.dtype).cuda(), v.to(batch.dtype).cuda(), place)
+    for keep, raw, scale in ((batch.k, batch.cache.k, batch.cache.k_scale), (batch.v, batch.cache.v, batch.cache.v_scale)):
+        x = rows_of(raw, batch.page)[place.cpu()].double()
+        keep[b] = x if scale is None else x * rows_of(scale, batch.page)[place.cpu()].double()[..., None]
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("seqs,n", [(64, 1), (32, 128)])
+def test_many_small_weights_count(kind, seqs, n):
+    """Ten thousand weights of 2^-26 of the largest, whose value is zero: below what fp16 holds beside 1, and all of the answer.  As many sequences as leave the
+    context whole, on the same pages.
+
+    A row's largest weight stands at 2^7 or more in fp16, so that a smaller one is off by 2^-32 of it at most."""
+    kv, heads, dim = 10000, 32, 64
+    batch = Batch([(1, kv)], heads, heads, dim, 64, kind)
+    k, v = torch.zeros(kv, heads, dim), torch.ones(kv, heads, dim)
+    k[0, :, 0], v[0] = 26 * math.log(2.0), 0.0
+    put(batch, 0, k, v)
+    batch.q[:] = 0
+    batch.q[..., 0] = 1
+    want, size, _ = batch.answer(scale=1.0)
+    starts, lens = torch.arange(seqs + 1, dtype=torch.int32).cuda() * n, torch.full((seqs,), kv, dtype=torch.int32, device="cuda")
+    got = ops().paged_attention(batch.q.repeat(seqs * n, 1, 1).cuda(), batch.cache, batch.pages.repeat(seqs, 1).cuda(), starts, lens, causal=False, scale=1.0,
+                                max_q=n).double().cpu()
+    assert want.min() > 1e-4
+    bound = (2 * U[batch.dtype] + 2.0 ** -13) * size + kv * 2.0 ** -32
+    assert bool(((got - want).abs() <= bound).all()), float(((got - want).abs() / bound).max())

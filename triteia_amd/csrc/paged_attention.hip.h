@@ -9,7 +9,9 @@
 //                      MFMA's K is free as long as V has the same, and ds_read_b64_tr_b16 (_b8) takes four (eight) rows of any addresses and
 //                      hands a lane one column of them.  P never leaves the registers.
 // Scores, running maxima and sums and the output's sums are 32 bits; P is rounded once to the activations' type for the MFMA.  The maximum is
-// a reference that is only moved (and the sums rescaled) when a score passes it by 2^kAttnSlack: P <= 2^8 is far from the types' ends.
+// a reference that is only moved (and the sums rescaled) when a weight would pass 2^kHigh; it is put where the largest weight is 2^kLow.  fp16 ends at 2^16 and
+// loses what is below 2^-25, so its largest weight stands at 2^7 to 2^15 and one of 2^-24 of it keeps 8 bits; beside a largest of 1, ten thousand of 2^-26
+// counted in the sum and not in the output.  bf16 has the exponents of 32 bits.
 // Masked scores are -infinity ahead of the maximum; a row that sees nothing has a sum of zero and gives zeros.  What is masked for some rows of
 // a tile and holds an infinity or a NaN in V must not reach those rows by 0 * inf: blocks on such an edge enter LDS without them (attn_clean),
 // and the rows that see them get them added one by one (attn_strange).
@@ -25,7 +27,6 @@ typedef short attn_s4 __attribute__((ext_vector_type(4)));
 typedef int attn_i2 __attribute__((ext_vector_type(2)));
 
 constexpr float kAttnNone = -1e30f;     // below every score: the maximum of nothing
-constexpr float kAttnSlack = 8.f;
 
 struct AttendArgs {
   const void* q;
@@ -61,6 +62,7 @@ template <>
 struct AttnMma<_Float16> {
   typedef _Float16 v8 __attribute__((ext_vector_type(8)));
   static constexpr uint32_t kInf = 0x7c00;
+  static constexpr float kLow = 7.f, kHigh = 15.f;
   static __device__ __forceinline__ attn_f4 m16(v8 a, v8 b, attn_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ attn_f16 m32(v8 a, v8 b, attn_f16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
@@ -68,6 +70,7 @@ template <>
 struct AttnMma<__bf16> {
   typedef __bf16 v8 __attribute__((ext_vector_type(8)));
   static constexpr uint32_t kInf = 0x7f80;
+  static constexpr float kLow = 0.f, kHigh = 8.f;
   static __device__ __forceinline__ attn_f4 m16(v8 a, v8 b, attn_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ attn_f16 m32(v8 a, v8 b, attn_f16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
@@ -412,8 +415,8 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
         }
         if (most > norm[n]) alpha = norm[n] / most, norm[n] = most;
       }
-      if (__any(top > m[n] + kAttnSlack)) {
-        const float next = fmaxf(m[n], top);
+      if (__any(top > m[n] + M::kHigh)) {
+        const float next = fmaxf(m[n], top - M::kLow);
         alpha *= __builtin_amdgcn_exp2f(m[n] - next);
         l[n] *= __builtin_amdgcn_exp2f(m[n] - next);
         m[n] = next;
@@ -752,8 +755,8 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
       top = attn_max32(top);
       float alpha = grown;
       l *= grown;
-      if (__any(top > m + kAttnSlack)) {
-        const float next = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - next);
+      if (__any(top > m + M::kHigh)) {
+        const float next = fmaxf(m, top - M::kLow), f = __builtin_amdgcn_exp2f(m - next);
         alpha *= f, l *= f, m = next;
       }
       if (__any(alpha != 1.f)) {
