@@ -125,3 +125,53 @@ def test_many_small_weights_count(kind, seqs, n):
     assert want.min() > 1e-4
     bound = (2 * U[batch.dtype] + 2.0 ** -13) * size + kv * 2.0 ** -32
     assert bool(((got - want).abs() <= bound).all()), float(((got - want).abs() / bound).max())
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("n", [1, 5, 90])
+def test_large_values_of_no_weight_do_not_hide_small_ones(kind, dtype, n):
+    """Visible tokens whose values are 10^7 times the others' and whose weight is next to nothing: from the first on, later on, and with all of the weight until other
+    tokens come.  Weights times scales are kept in fp16's range by the largest such product of the row, which stands at 1 or more there: an error of
+    2^-25 of it for a token."""
+    kv, dim, most_code = 700, 64, 127 if kind == "int8" else 448
+    for case in ("first", "apart", "last", "until"):
+        batch = Batch([(n, kv)], 4, 2, dim, 16, kind, dtype)
+        big = {"first": [0], "apart": list(range(3, 600, 50)), "last": [kv - n - 1], "until": [0, 1, 17]}[case]
+        k, v = randn(kv, 2, dim, seed=1) * 0.1, randn(kv, 2, dim, seed=2) * 2e-3
+        v[big] = randn(len(big), 2, dim, seed=3) * 10000
+        k[..., 0] = 0
+        k[big, :, 0] = -40.0
+        if case == "until":
+            k[100:, :, 0] = 40.0
+            k[big, :, 0] = 0.0
+            k[2:17, :, 0], k[18:100, :, 0] = -40.0, -40.0
+        put(batch, 0, k, v)
+        batch.q[..., 0] = 1
+        want, size, _ = batch.answer(scale=1.0)
+        got = ops().paged_attention(*batch.inputs(), scale=1.0, max_q=n).double().cpu()
+        # the largest weight times scale of every row
+        top = torch.zeros(want.shape[:2] + (1,), dtype=torch.float64)
+        v_scale = (batch.v[0].abs().amax(-1) / most_code).repeat_interleave(2, 1)                # [kv, heads]
+        score = torch.einsum("thd,shd->hts", batch.q.double(), batch.k[0].repeat_interleave(2, 1))
+        p = torch.softmax(score.masked_fill(torch.arange(kv) > torch.arange(kv - n, kv)[:, None], -math.inf), -1)
+        top[..., 0] = (p * v_scale.t()[:, None]).amax(-1).t()
+        bound = (2 * U[dtype] + 2.0 ** -13) * size + kv * 2.0 ** -25 * most_code * top + (2.0 ** -25 if dtype == torch.float16 else 0)
+        assert bool(((got - want).abs() <= bound).all()), (case, float(((got - want).abs() / bound).max()))
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("n", [1, 90])
+def test_scales_of_either_sign(kind, dtype, n):
+    """A cache that a program has filled itself may hold negative scales, large ones among them."""
+    batch = Batch([(n, 300)], 4, 2, 64, 16, kind, dtype)
+    flip = torch.where(torch.arange(16) % 3 == 0, -3e4, 1.0).cuda()
+    batch.cache.v_scale.mul_(flip)
+    place = batch.slots(0, torch.arange(300)).cpu()
+    batch.v[0] = rows_of(batch.cache.v, 16)[place].double() * rows_of(batch.cache.v_scale, 16)[place].double()[..., None]
+    want, size, most = batch.answer()
+    got = ops().paged_attention(*batch.inputs(), max_q=n).double().cpu()
+    bound = (2 * U[dtype] + 2.0 ** -13) * size + 2.0 ** -24 * most
+    finite = want.abs() < (60000 if dtype == torch.float16 else 1e30)
+    assert bool(((got - want).abs() <= bound)[finite].all())

@@ -11,7 +11,9 @@
 // Scores, running maxima and sums and the output's sums are 32 bits; P is rounded once to the activations' type for the MFMA.  The maximum is
 // a reference that is only moved (and the sums rescaled) when a weight would pass 2^kHigh; it is put where the largest weight is 2^kLow.  fp16 ends at 2^16 and
 // loses what is below 2^-25, so its largest weight stands at 2^7 to 2^15 and one of 2^-24 of it keeps 8 bits; beside a largest of 1, ten thousand of 2^-26
-// counted in the sum and not in the output.  bf16 has the exponents of 32 bits.
+// counted in the sum and not in the output.  bf16 has the exponents of 32 bits.  Over 8-bit caches P takes V's scales in (kept out of V, whose rounding would
+// grow), and fp16's range is kept by the row's largest weight times scale, `peak`, in the same way (attn_shift): by the largest scale, a value far above the others
+// with a weight of next to nothing took their bits.
 // Masked scores are -infinity ahead of the maximum; a row that sees nothing has a sum of zero and gives zeros.  What is masked for some rows of
 // a tile and holds an infinity or a NaN in V must not reach those rows by 0 * inf: blocks on such an edge enter LDS without them (attn_clean),
 // and the rows that see them get them added one by one (attn_strange).
@@ -188,6 +190,11 @@ struct AttnSpan {
   __device__ __forceinline__ bool hides(int token) const { return token < lo || token >= hi; }
 };
 
+// The power of two by which a row's sums and weights move so that its largest weight times scale, which has left 1 .. 2^15, is 2^7 to 2^8 again.  (Exact; the
+// reference of scores is a whole number where this is in use, so that less the shift it is exact too.)  Beyond 2^+-64 fp16's outputs have ended.
+__device__ __forceinline__ bool attn_off(float peak) { return peak > 32768.f || (peak < 1.f && peak > 0.f); }
+__device__ __forceinline__ int attn_shift(float peak, int now) { return attn_off(peak) ? max(-64, min(64, now + 8 - __builtin_amdgcn_frexp_expf(peak))) - now : 0; }
+
 // Which tokens row `r` of a tile sees: lo <= token < hi.  Rows behind the last see all that the tile sees and are not stored.
 struct AttnRow {
   int lo, hi, token, head;     // token of the sequence, head of the group
@@ -315,10 +322,12 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
   const int all_lo = last.lo, all_hi = first.hi;
 
   attn_f4 o[NQ][D / 16];
-  float m[NQ], l[NQ], norm[NQ];              // norm: the largest scale of V that the row has seen, so that P times a scale stays inside fp16
+  constexpr bool kNormed = KIND != kCacheSame && __is_same(T, _Float16);
+  float m[NQ], l[NQ], peak[NQ];              // l, o and peak are times 2^shift
+  int shift[NQ];
 #pragma unroll
   for (int n = 0; n < NQ; n++) {
-    m[n] = kAttnNone, l[n] = 0.f, norm[n] = 0.f;
+    m[n] = kAttnNone, l[n] = 0.f, peak[n] = 0.f, shift[n] = 0;
 #pragma unroll
     for (int d = 0; d < D / 16; d++) o[n][d] = attn_f4{0.f, 0.f, 0.f, 0.f};
   }
@@ -345,11 +354,6 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
     }
     if constexpr (KIND != kCacheSame) {
       if (lane < kSub) scales[wave][0][lane] = ks * a.scale_log2, scales[wave][1][lane] = vs;
-    }
-    float norm_now = 0.f;                    // the largest scale of V in this block
-    if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) {
-      if (lane < kSub && t0 + lane < it.kv_end) norm_now = fmaxf(0.f, vs);
-      norm_now = attn_max16(across_row<16>(norm_now, [](float p, float q) { return fmaxf(p, q); }));
     }
     if (sub + WAVES < n_sub) request((sub - wave) / WAVES + 1);
 
@@ -400,41 +404,22 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
           }
       }
       top = attn_max16(top);
-      float alpha = 1.f;
-      if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) {
-        float most = norm_now;
-        if (edge) {                          // (of what the row sees alone)
-          const AttnSpan seen = span.here();
-          most = 0.f;
-#pragma unroll
-          for (int g = 0; g < kGroups; g++)
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-              most = seen.hides(16 * g + j) ? most : fmaxf(most, scales[wave][1][16 * g + 4 * h + j]);
-          most = attn_max16(most);
-        }
-        if (most > norm[n]) alpha = norm[n] / most, norm[n] = most;
-      }
       if (__any(top > m[n] + M::kHigh)) {
-        const float next = fmaxf(m[n], top - M::kLow);
-        alpha *= __builtin_amdgcn_exp2f(m[n] - next);
-        l[n] *= __builtin_amdgcn_exp2f(m[n] - next);
-        m[n] = next;
-      }
-      if (__any(alpha != 1.f)) {
+        const float low = top - M::kLow, next = fmaxf(m[n], kNormed ? __builtin_floorf(low) : low), f = __builtin_amdgcn_exp2f(m[n] - next);
+        l[n] *= f, peak[n] *= f, m[n] = next;
 #pragma unroll
         for (int d = 0; d < D / 16; d++)
 #pragma unroll
-          for (int j = 0; j < 4; j++) o[n][d][j] *= alpha;
+          for (int j = 0; j < 4; j++) o[n][d][j] *= f;
       }
-      const float inv = KIND != kCacheSame && __is_same(T, _Float16) ? 1.f / fmaxf(norm[n], 1e-30f) : 1.f;
+      const float under = kNormed ? m[n] - (float)shift[n] : m[n];
 #pragma unroll
       for (int g = 0; g < kGroups; g++)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          const float e = __builtin_amdgcn_exp2f(s[n][g][j] - m[n]);
+          const float e = __builtin_amdgcn_exp2f(s[n][g][j] - under);
           l[n] += e;
-          s[n][g][j] = KIND == kCacheSame ? e : e * (scales[wave][1][16 * g + 4 * h + j] * inv);
+          s[n][g][j] = KIND == kCacheSame ? e : e * scales[wave][1][16 * g + 4 * h + j];
         }
       if (KIND != kCacheSame && edge) {              // (a scale may be a NaN)
         const AttnSpan seen = span.here();
@@ -442,6 +427,26 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
         for (int g = 0; g < kGroups; g++)
 #pragma unroll
           for (int j = 0; j < 4; j++) s[n][g][j] = seen.hides(16 * g + j) ? 0.f : s[n][g][j];
+      }
+      if constexpr (kNormed) {
+        float most = 0.f;
+#pragma unroll
+        for (int g = 0; g < kGroups; g++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) most = fmaxf(most, __builtin_fabsf(s[n][g][j]));
+        peak[n] = fmaxf(peak[n], attn_max16(most));
+        if (__any(attn_off(peak[n]))) {
+          const int by = attn_shift(peak[n], shift[n]);
+          shift[n] += by, peak[n] = __builtin_ldexpf(peak[n], by), l[n] = __builtin_ldexpf(l[n], by);
+#pragma unroll
+          for (int g = 0; g < kGroups; g++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) s[n][g][j] = __builtin_ldexpf(s[n][g][j], by);
+#pragma unroll
+          for (int d = 0; d < D / 16; d++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[n][d][j] = __builtin_ldexpf(o[n][d][j], by);
+        }
       }
 #pragma unroll
       for (int g = 0; g < kGroups; g++)
@@ -485,6 +490,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
   // the wavefronts' results: through LDS, the upper half's taken in by the lower half
 #pragma unroll
   for (int n = 0; n < NQ; n++) {
+    if constexpr (kNormed) l[n] = __builtin_ldexpf(l[n], -shift[n]);
     l[n] += __shfl_xor(l[n], 16);
     l[n] += __shfl_xor(l[n], 32);
     if (h == 0) meet_m[wave][16 * n + col] = m[n], meet_l[wave][16 * n + col] = l[n];
@@ -497,7 +503,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
 #pragma unroll
     for (int w = 0; w < WAVES; w++) top = fmaxf(top, meet_m[w][16 * n + col]);
     float f = __builtin_amdgcn_exp2f(m[n] - top);
-    if constexpr (KIND != kCacheSame && __is_same(T, _Float16)) f *= norm[n];
+    if constexpr (kNormed) f = __builtin_ldexpf(f, -shift[n]);
 #pragma unroll
     for (int d = 0; d < D / 16; d++)
 #pragma unroll
@@ -675,9 +681,9 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
   for (int d = 0; d < D / 32; d++)
 #pragma unroll
     for (int j = 0; j < 16; j++) o[d][j] = 0.f;
-  // (fp16 times a scale: P leaves the exponential over the largest scale of V that the row has seen so far, which the sums l and o then both are over as well)
   constexpr bool kNormed = KIND != kCacheSame && __is_same(T, _Float16);
-  float m = kAttnNone, l = 0.f, norm = 1e-30f, log_norm = 0.f;
+  float m = kAttnNone, l = 0.f, peak = 0.f;  // l, o and peak are times 2^shift
+  int shift = 0;
 
   if (n_blocks > 0) {
     keep(it.kv_begin, 0);
@@ -712,25 +718,6 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
       step();                                // (its writes under the softmax)
       const bool edge = t0 < w1.lo || t0 + kAttnBlock > min(w0.hi, it.kv_end);
       const AttnSpan span = {mine.lo - t0 - 4 * h, min(mine.hi, it.kv_end) - t0 - 4 * h};
-      float grown = 1.f;
-      if constexpr (kNormed) {
-        float top = 0.f;
-        if (edge) {                          // (of what the row sees alone)
-          const AttnSpan seen = span.here();
-#pragma unroll
-          for (int g = 0; g < 2; g++)
-#pragma unroll
-            for (int j = 0; j < 16; j++) {
-              const int token = 32 * g + 8 * (j / 4) + j % 4;
-              top = seen.hides(token) ? top : fmaxf(top, scales[at][1][token + 4 * h]);
-            }
-          top = attn_max32(top);
-        } else {
-          top = attn_max16(across_row<16>(scales[at][1][lane], [](float p, float q) { return fmaxf(p, q); }));
-        }
-        if (top > norm) grown = norm / top, norm = top;
-        log_norm = __builtin_amdgcn_logf(norm);
-      }
       float top = kAttnNone;
 #pragma unroll
       for (int g = 0; g < 2; g++)
@@ -753,19 +740,15 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
       }
       if constexpr (KIND == kCacheSame) top = fmaxf(top * a.scale_log2, kAttnNone);
       top = attn_max32(top);
-      float alpha = grown;
-      l *= grown;
       if (__any(top > m + M::kHigh)) {
-        const float next = fmaxf(m, top - M::kLow), f = __builtin_amdgcn_exp2f(m - next);
-        alpha *= f, l *= f, m = next;
-      }
-      if (__any(alpha != 1.f)) {
+        const float low = top - M::kLow, next = fmaxf(m, kNormed ? __builtin_floorf(low) : low), f = __builtin_amdgcn_exp2f(m - next);
+        l *= f, peak *= f, m = next;
 #pragma unroll
         for (int d = 0; d < D / 32; d++)
 #pragma unroll
-          for (int j = 0; j < 16; j++) o[d][j] *= alpha;
+          for (int j = 0; j < 16; j++) o[d][j] *= f;
       }
-      const float under = kNormed ? m + log_norm : m;
+      const float under = kNormed ? m - (float)shift : m;
       v8 p[4];
       float sum[4] = {0.f, 0.f, 0.f, 0.f};   // (one running sum would be a chain of 32 additions)
 #pragma unroll
@@ -786,6 +769,26 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
             const int token = 32 * g + 8 * (j / 4) + j % 4;
             s[g][j] = seen.hides(token) ? 0.f : s[g][j];
           }
+      }
+      if constexpr (kNormed) {
+        float most = 0.f;
+#pragma unroll
+        for (int g = 0; g < 2; g++)
+#pragma unroll
+          for (int j = 0; j < 16; j++) most = fmaxf(most, __builtin_fabsf(s[g][j]));
+        peak = fmaxf(peak, attn_max32(most));
+        if (__any(attn_off(peak))) {
+          const int by = attn_shift(peak, shift);
+          shift += by, peak = __builtin_ldexpf(peak, by), l = __builtin_ldexpf(l, by);
+#pragma unroll
+          for (int g = 0; g < 2; g++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) s[g][j] = __builtin_ldexpf(s[g][j], by);
+#pragma unroll
+          for (int d = 0; d < D / 32; d++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) o[d][j] = __builtin_ldexpf(o[d][j], by);
+        }
       }
 #pragma unroll
       for (int g = 0; g < 2; g++)
@@ -818,7 +821,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
   }
   if (!mine.live || 32 * wave + col >= n_rows) return;
   l += __shfl_xor(l, 32);
-  float f = kNormed ? norm : 1.f;
+  float f = kNormed ? __builtin_ldexpf(1.f, -shift) : 1.f;
   if (it.part < 0) {
     typedef T t4 __attribute__((ext_vector_type(4)));
     f = l == 0.f ? 0.f : 1.f / l;
