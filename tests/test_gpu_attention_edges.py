@@ -175,3 +175,20 @@ def test_scales_of_either_sign(kind, dtype, n):
     bound = (2 * U[dtype] + 2.0 ** -13) * size + 2.0 ** -24 * most
     finite = want.abs() < (60000 if dtype == torch.float16 else 1e30)
     assert bool(((got - want).abs() <= bound)[finite].all())
+
+
+@pytest.mark.parametrize("kind", ["same", "int8"])
+@pytest.mark.parametrize("dtype,size", [(torch.float16, 3e4), (torch.bfloat16, 1e5), (torch.bfloat16, 1e16), (torch.bfloat16, 1e18)])
+@pytest.mark.parametrize("n", [1, 5, 90])
+def test_scores_near_the_end_of_32_bits(kind, dtype, size, n):
+    """Scores of 10^10 to 3 * 10^38 of either sign, further apart than any exponential reaches: the largest takes all of the weight."""
+    kv, dim = 200, 64
+    for most, others in ((-0.5, -1.0), (1.0, 0.5), (1.0, -1.0)):
+        batch = Batch([(n, kv)], 2, 1, dim, 16, kind, dtype)
+        k, v = torch.full((kv, 1, dim), others * size), randn(kv, 1, dim, seed=2)
+        k[37] = most * size
+        put(batch, 0, k, v)
+        batch.q[:] = size / 8
+        got = ops().paged_attention(*batch.inputs(), max_q=n).double().cpu()
+        want = batch.v[0][37, 0].expand_as(got)
+        assert bool(((got - want).abs() <= 2 * U[dtype] * want.abs() + 2.0 ** -25).all())

@@ -28,7 +28,7 @@ typedef float attn_f16 __attribute__((ext_vector_type(16)));
 typedef short attn_s4 __attribute__((ext_vector_type(4)));
 typedef int attn_i2 __attribute__((ext_vector_type(2)));
 
-constexpr float kAttnNone = -1e30f;     // below every score: the maximum of nothing
+constexpr float kAttnNone = -3e38f;     // the maximum of nothing: below every score that is a number, but for the last eighth of their range
 
 struct AttendArgs {
   const void* q;
@@ -718,7 +718,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
       step();                                // (its writes under the softmax)
       const bool edge = t0 < w1.lo || t0 + kAttnBlock > min(w0.hi, it.kv_end);
       const AttnSpan span = {mine.lo - t0 - 4 * h, min(mine.hi, it.kv_end) - t0 - 4 * h};
-      float top = kAttnNone;
+      float top = -__builtin_inff();
 #pragma unroll
       for (int g = 0; g < 2; g++)
 #pragma unroll
@@ -728,7 +728,7 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
         }
       if (edge) {
         const AttnSpan seen = span.here();
-        top = kAttnNone;
+        top = -__builtin_inff();
 #pragma unroll
         for (int g = 0; g < 2; g++)
 #pragma unroll
@@ -738,7 +738,8 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
             top = fmaxf(top, s[g][j]);
           }
       }
-      if constexpr (KIND == kCacheSame) top = fmaxf(top * a.scale_log2, kAttnNone);
+      if constexpr (KIND == kCacheSame) top *= a.scale_log2;
+      top = fmaxf(top, kAttnNone);
       top = attn_max32(top);
       if (__any(top > m + M::kHigh)) {
         const float low = top - M::kLow, next = fmaxf(m, kNormed ? __builtin_floorf(low) : low), f = __builtin_amdgcn_exp2f(m - next);
@@ -749,13 +750,25 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
           for (int j = 0; j < 16; j++) o[d][j] *= f;
       }
       const float under = kNormed ? m - (float)shift : m;
+      float to_log2 = KIND == kCacheSame ? a.scale_log2 : 1.f;
+      if constexpr (KIND == kCacheSame) {
+        // (a far reference's rounding, which a product inside the fma does not share, would pass an exponential's end)
+        const bool far = __builtin_fabsf(m) > 1048576.f && m > kAttnNone;
+        if (__any(far)) {
+#pragma unroll
+          for (int g = 0; g < 2; g++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) s[g][j] *= far ? to_log2 : 1.f;
+          to_log2 = far ? 1.f : to_log2;
+        }
+      }
       v8 p[4];
       float sum[4] = {0.f, 0.f, 0.f, 0.f};   // (one running sum would be a chain of 32 additions)
 #pragma unroll
       for (int g = 0; g < 2; g++)
 #pragma unroll
         for (int j = 0; j < 16; j++) {
-          const float e = __builtin_amdgcn_exp2f(KIND == kCacheSame ? __builtin_fmaf(s[g][j], a.scale_log2, -m) : s[g][j] - under);
+          const float e = __builtin_amdgcn_exp2f(KIND == kCacheSame ? __builtin_fmaf(s[g][j], to_log2, -m) : s[g][j] - under);
           sum[j % 4] += e;
           s[g][j] = KIND == kCacheSame ? e : e * scales[at][1][32 * g + 8 * (j / 4) + j % 4 + 4 * h];
         }
