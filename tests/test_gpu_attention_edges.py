@@ -192,3 +192,25 @@ def test_scores_near_the_end_of_32_bits(kind, dtype, size, n):
         got = ops().paged_attention(*batch.inputs(), max_q=n).double().cpu()
         want = batch.v[0][37, 0].expand_as(got)
         assert bool(((got - want).abs() <= 2 * U[dtype] * want.abs() + 2.0 ** -25).all())
+
+
+# --- the cache ----------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", HALF)
+def test_codes_are_the_nearest_to_the_quotient(kind, dtype):
+    """code = x / scale, as 32 bits round it, to the nearest code, on rows that hold quotients near the middle of two (a product with 1 / scale takes the other one of
+    some of them)."""
+    dim, tokens, held = 256, 4000, KINDS[kind]
+    x = torch.rand(tokens, 1, dim, generator=torch.Generator().manual_seed(1))
+    top = torch.rand(tokens, 1, 1, generator=torch.Generator().manual_seed(2)) * 4 + 0.1
+    middle = torch.randint(0, 127, x.shape, generator=torch.Generator().manual_seed(3)).float() + 0.5
+    x = torch.where(x < 0.9, middle / 127 * top, x * top).to(dtype)
+    x[..., :1] = top.to(dtype)
+    x = torch.minimum(x, x[..., :1])
+    cache = ops().paged_cache(tokens // 16, 1, dim, 16, held)
+    ops().cache_write(cache, x.cuda(), -x.cuda(), torch.arange(tokens).cuda())
+    for y, raw, scale in ((x, cache.k, cache.k_scale), (-x, cache.v, cache.v_scale)):
+        quotient = y.float() / rows_of(scale, 16)[..., None]
+        want = quotient.round() if kind == "int8" else quotient.clamp(-448, 448).to(held).float()
+        assert torch.equal(rows_of(raw, 16), want)

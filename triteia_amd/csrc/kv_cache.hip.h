@@ -63,14 +63,21 @@ __device__ __forceinline__ long shared_index_at(const void* p, int wide, long i)
   return wide ? reinterpret_cast<Wide>(reinterpret_cast<uintptr_t>(p))[i] : (long)reinterpret_cast<Narrow>(reinterpret_cast<uintptr_t>(p))[i];
 }
 
-// 8 values as codes of the row's scale; inv = 1 / scale
+// 8 values as codes of the row's scale; inv = 1 / scale.  The quotient is x / scale as 32 bits round it, by one correction of x * inv: without it one value in
+// 20000 takes the code on the other side of the middle.
 template <int KIND>
-__device__ __forceinline__ kv_uint2 codes_of(const float (&x)[8], float inv) {
+__device__ __forceinline__ kv_uint2 codes_of(const float (&x)[8], float scale, float inv) {
   kv_uint2 c = {0, 0};
+  float quotient[8];
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const float y = x[j] * inv;
+    quotient[j] = __builtin_fmaf(__builtin_fmaf(-y, scale, x[j]), inv, y);
+  }
   if constexpr (KIND == kCacheInt8) {
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-      const int v = (int)__builtin_amdgcn_fmed3f(__builtin_rintf(x[j] * inv), -127.f, 127.f);
+      const int v = (int)__builtin_amdgcn_fmed3f(__builtin_rintf(quotient[j]), -127.f, 127.f);
       c[j / 4] |= (uint32_t)(v & 255) << (8 * (j % 4));
     }
   } else {
@@ -79,7 +86,7 @@ __device__ __forceinline__ kv_uint2 codes_of(const float (&x)[8], float inv) {
       int w = 0;
       float y[4];
 #pragma unroll
-      for (int j = 0; j < 4; j++) y[j] = __builtin_amdgcn_fmed3f(x[4 * i + j] * inv, -448.f, 448.f);
+      for (int j = 0; j < 4; j++) y[j] = __builtin_amdgcn_fmed3f(quotient[4 * i + j], -448.f, 448.f);
       w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], w, false);
       w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
       c[i] = (uint32_t)w;
@@ -136,7 +143,7 @@ __device__ __forceinline__ void cache_row(const CachePart& c, long page, long he
     const float most = __builtin_bit_cast(float, top);
     float scale = most / (KIND == kCacheInt8 ? 127.f : 448.f), inv = 1.f / scale;
     if (most < 1e-30f) scale = 0.f, inv = 0.f;
-    kv_uint2 code = codes_of<KIND>(x, inv);
+    kv_uint2 code = codes_of<KIND>(x, scale, inv);
     if (top >= 0x7f800000u) scale = __builtin_nanf(""), code = kv_uint2{0, 0};
     if (live) *reinterpret_cast<kv_uint2*>(static_cast<uint8_t*>(c.data) + at) = code;
     if (e == 0) c.scale[page * c.scale_page + head * c.scale_head + slot * c.scale_slot] = scale;
