@@ -214,3 +214,19 @@ def test_codes_are_the_nearest_to_the_quotient(kind, dtype):
         quotient = y.float() / rows_of(scale, 16)[..., None]
         want = quotient.round() if kind == "int8" else quotient.clamp(-448, 448).to(held).float()
         assert torch.equal(rows_of(raw, 16), want)
+
+
+# --- the layer ------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("seqs", [0, 2])
+@pytest.mark.parametrize("planned", [False, True])
+def test_a_layer_of_no_tokens(seqs, planned):
+    from triteia_amd.python.capi import route_plan
+    from triteia_amd.python.nn import multi_delta_attention
+    layer = multi_delta_attention(512, 4, 2, 64, 3).cuda()
+    cache, table = ops().paged_cache(4, 2, 64, 16), ops().rotary_table(100, 64)
+    int32 = dict(dtype=torch.int32, device="cuda")
+    indices, starts, lens = torch.zeros(0, **int32), torch.zeros(seqs + 1, **int32), torch.full((seqs,), 9, **int32)
+    extra = dict(plan=layer.plan(cache, starts, lens, 0), route=route_plan(indices, 3)) if planned else {}
+    out = layer(torch.zeros(0, 512, dtype=torch.float16, device="cuda"), indices, indices, table, cache, indices, torch.zeros(seqs, 1, **int32), starts, lens, **extra)
+    assert out.shape == (0, 512) and out.dtype == torch.float16

@@ -33,8 +33,8 @@ class multi_delta_attention(nn.Module):
         `cache` (a PagedCache, this layer's); table: from ops.rotary_table; pages, q_starts, kv_lens, plan, max_q: as for ops.paged_attention."""
         from triteia_amd.python.ops import paged_attention, rotary_cache_write
         tokens = x.shape[0]
-        qkv = self.qkv_proj(x, indices, route).view(tokens, -1, self.head_dim)
+        qkv = self.qkv_proj(x, indices, route).view(tokens, self.n_heads + 2 * self.n_kv_heads, self.head_dim)
         q, k, v = qkv.split([self.n_heads, self.n_kv_heads, self.n_kv_heads], 1)
         q = rotary_cache_write(q, k, v, positions, table, cache, slots, self.interleaved, self.q_norm, self.k_norm, self.eps)
         out = paged_attention(q, cache, pages, q_starts, kv_lens, plan=plan, max_q=max_q)
-        return self.o_proj(out.view(tokens, -1), indices, route)
+        return self.o_proj(out.view(tokens, self.n_heads * self.head_dim), indices, route)
