@@ -15,6 +15,7 @@ class multi_delta_attention(nn.Module):
     def __init__(self, hidden, n_heads, n_kv_heads, head_dim, n_deltas, with_base=True, qk_norm=False, interleaved=False, eps=1e-6):
         super().__init__()
         assert n_heads % n_kv_heads == 0, f"{n_heads} heads over {n_kv_heads} heads of the cache"
+        assert head_dim in (64, 128), f"attention takes heads of 64 or 128 elements, got {head_dim}"
         self.n_heads, self.n_kv_heads, self.head_dim, self.interleaved, self.eps = n_heads, n_kv_heads, head_dim, interleaved, eps
         self.qkv_proj = multi_delta_linear(hidden, (n_heads + 2 * n_kv_heads) * head_dim, n_deltas, with_base)
         self.o_proj = multi_delta_linear(n_heads * head_dim, hidden, n_deltas, with_base)
