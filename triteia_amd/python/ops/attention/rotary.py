@@ -6,12 +6,13 @@ import torch
 from triteia_amd.python import capi
 
 __all__ = ["rotary_table", "rotary", "rotary_cache_write"]
+_NEEDED = {"linear": ("factor",), "ntk": ("factor",), "bands": ("factor", "low", "high", "original"), "yarn": ("factor", "original")}
 
 
 def rotary_table(limit, rotary_dim, base=10000.0, scaling=None, device="cuda"):
     """cos and sin of positions 0 .. limit - 1: float32 [limit, rotary_dim / 2, 2], worked out in 64 bits.  Pair i turns by position * base^(-2 i / rotary_dim).
 
-    `scaling` for contexts longer than those of training, a dict with `type`:
+    `scaling` for contexts longer than those of training, a dict with `type` and `factor` and what else is named here:
       "linear": positions divided by `factor`;
       "ntk":    the base multiplied by factor^(d / (d - 2)), so that the slowest pair is stretched by `factor` and the fastest is not;
       "bands":  pairs that turn fewer than `low` times over `original` positions slowed by `factor`, more than `high` times not, between the two linear
@@ -23,10 +24,18 @@ def rotary_table(limit, rotary_dim, base=10000.0, scaling=None, device="cuda"):
     if limit < 1:
         raise RuntimeError(f"a table of {limit} positions")
     pair = torch.arange(0, rotary_dim, 2, device=device, dtype=torch.float64)
-    how = dict(scaling or {"type": None})
-    kind, factor, magnitude = how.pop("type", None), float(how.pop("factor", 1.0)), 1.0
-    if kind not in (None, "linear", "ntk", "bands", "yarn") or not factor >= 1.0:
-        raise RuntimeError(f"unknown scaling of positions: {scaling}")
+    kind, how, factor, magnitude = None, {}, 1.0, 1.0
+    if scaling is not None:
+        how = dict(scaling)
+        kind = how.pop("type", None)
+        if kind not in ("linear", "ntk", "bands", "yarn"):
+            raise RuntimeError(f"unknown scaling of positions: {scaling}")
+        missing = [name for name in _NEEDED[kind] if name not in how]
+        if missing:
+            raise RuntimeError(f"{kind} scaling needs {', '.join(missing)}: {scaling}")
+        factor = float(how.pop("factor"))
+        if not 1.0 <= factor < math.inf:
+            raise RuntimeError(f"a factor of {factor}: 1 at least")
     if kind == "ntk":
         base = base * factor ** (rotary_dim / (rotary_dim - 2))
     rate = float(base) ** (-pair / rotary_dim)
@@ -34,6 +43,8 @@ def rotary_table(limit, rotary_dim, base=10000.0, scaling=None, device="cuda"):
         rate = rate / factor
     elif kind == "bands":
         low, high, original = float(how.pop("low")), float(how.pop("high")), float(how.pop("original"))
+        if not low < high:
+            raise RuntimeError(f"bands from {low} to {high} turns")
         keep = ((original * rate / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
         rate = rate * keep + rate / factor * (1 - keep)
     elif kind == "yarn":
