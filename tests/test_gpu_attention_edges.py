@@ -230,3 +230,21 @@ def test_a_layer_of_no_tokens(seqs, planned):
     extra = dict(plan=layer.plan(cache, starts, lens, 0), route=route_plan(indices, 3)) if planned else {}
     out = layer(torch.zeros(0, 512, dtype=torch.float16, device="cuda"), indices, indices, table, cache, indices, torch.zeros(seqs, 1, **int32), starts, lens, **extra)
     assert out.shape == (0, 512) and out.dtype == torch.float16
+
+
+# --- refusals -----------------------------------------------------------------------------------------------------------------------
+
+def test_tangents_are_refused():
+    """Forward mode: a tangent that the kernels would drop."""
+    import torch.autograd.forward_ad as fwd
+    x, table, positions = randn(3, 2, 64, dtype=torch.float16).cuda(), ops().rotary_table(10, 64), torch.zeros(3, dtype=torch.int32, device="cuda")
+    cache = ops().paged_cache(4, 2, 64, page=16)
+    pages, starts, lens = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([[0]], [0, 3], [3]))
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for call in (lambda: ops().rotary(dual, x, positions, table), lambda: ops().rotary(x, dual, positions, table),
+                     lambda: ops().cache_write(cache, x, dual, positions), lambda: ops().paged_attention(dual, cache, pages, starts, lens),
+                     lambda: ops().rotary(x, x, positions, table, q_norm=fwd.make_dual(x[0, 0].clone(), x[0, 0].clone()))):
+            with pytest.raises(RuntimeError, match="tangent"):
+                call()
+        assert ops().rotary(x, x, positions, table)[0].shape == x.shape

@@ -3,6 +3,7 @@ has no counterpart."""
 import ctypes
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _ffi
 from ._native import native
@@ -20,7 +21,7 @@ def _check(err):
 
 
 def _require(like=None, **tensors):
-    """Plain GPU tensors of one device, in any layout, that record no gradient."""
+    """GPU tensors of one device, in any layout, that record no gradient in either direction."""
     for name, t in tensors.items():
         if t is None:
             continue
@@ -33,6 +34,8 @@ def _require(like=None, **tensors):
         like = t.device
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{name} requires a gradient, which this op does not record")
+        if unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has a tangent, which this op does not carry on")
     return like
 
 
