@@ -248,3 +248,20 @@ def test_tangents_are_refused():
             with pytest.raises(RuntimeError, match="tangent"):
                 call()
         assert ops().rotary(x, x, positions, table)[0].shape == x.shape
+
+
+def test_arguments_that_belong_together():
+    x, table, positions = randn(3, 2, 64, dtype=torch.float16).cuda(), ops().rotary_table(10, 64), torch.arange(3).cuda()
+    cache = ops().paged_cache(4, 2, 64, page=16)
+    for call in (lambda: ops().rotary(x, x, positions, None), lambda: ops().rotary(x, x, None, table),
+                 lambda: ops().rotary_cache_write(x, x, x, positions, None, cache, positions)):
+        with pytest.raises(RuntimeError, match="positions and table"):
+            call()
+    for call in (lambda: ops().rotary(x, None, positions, table), lambda: ops().rotary_cache_write(x, x, None, positions, table, cache, positions),
+                 lambda: ops().cache_write(cache, x, x, None), lambda: ops().cache_write(cache, None, x, positions), lambda: ops().cache_read(cache, None)):
+        with pytest.raises(TypeError, match="must be a torch.Tensor"):
+            call()
+    # (norms alone, without a rotation, are a pass of their own)
+    w = torch.full((64,), 2.0, dtype=torch.float16, device="cuda")
+    y = ops().rotary(x, x, None, None, q_norm=w)
+    assert torch.equal(y[1], x) and torch.allclose(y[0].float().pow(2).mean(-1), torch.tensor(4.0, device="cuda"), rtol=2e-3)

@@ -20,10 +20,10 @@ def _check(err):
         raise RuntimeError(_ffi.last_error())
 
 
-def _require(like=None, **tensors):
-    """GPU tensors of one device, in any layout, that record no gradient in either direction."""
+def _require(like=None, optional=(), **tensors):
+    """GPU tensors of one device, in any layout, that record no gradient in either direction; those named in `optional` may be None."""
     for name, t in tensors.items():
-        if t is None:
+        if t is None and name in optional:
             continue
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch.Tensor")
@@ -66,7 +66,7 @@ class PagedCache:
     Slot `page * (tokens of a page) + offset` names a token's place."""
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
-        device = _require(k=k, v=v, k_scale=k_scale, v_scale=v_scale)
+        device = _require(optional=("k_scale", "v_scale"), k=k, v=v, k_scale=k_scale, v_scale=v_scale)
         if k.dtype not in CACHE_KINDS or v.dtype != k.dtype:
             raise RuntimeError(f"a cache holds fp16, bf16, int8 or float8_e4m3fn, the same for k and v, got {k.dtype} and {v.dtype}")
         if k.dim() != 4 or v.shape != k.shape:
@@ -112,9 +112,11 @@ def rotary_cache(q, k, v, positions, table, cache, slots, interleaved=False, q_n
     out = native().rotary_cache(q, k, v, positions, table, held[0], held[1], held[2], held[3], slots, interleaved, q_norm, k_norm, eps)
     if out is not None:
         return out
-    device = _require(q=q, k=k, v=v, positions=positions, table=table, slots=slots, q_norm=q_norm, k_norm=k_norm)
-    like = k if k is not None else q
-    tokens, dim, dtype = like.shape[0], like.shape[-1], like.dtype
+    if (positions is None) != (table is None):
+        raise RuntimeError("positions and table go together")
+    optional = ("q", "positions", "table", "q_norm", "k_norm") + (("v", "slots") if cache is None else ())
+    device = _require(optional=optional, q=q, k=k, v=v, positions=positions, table=table, slots=slots, q_norm=q_norm, k_norm=k_norm)
+    tokens, dim, dtype = k.shape[0], k.shape[-1], k.dtype
     if cache is not None:
         if cache.device != device:
             raise RuntimeError(f"the cache is on {cache.device}, expected {device}")
@@ -153,7 +155,7 @@ def rotary_cache(q, k, v, positions, table, cache, slots, interleaved=False, q_n
         tokens, q.shape[1] if q is not None else 0, k.shape[1], dim, rot, _ffi.ptr(positions),
         int(positions is not None and positions.dtype == torch.int64), _ffi.ptr(table) if positions is not None else None, limit, int(bool(interleaved)),
         _ffi.ptr(norms[0]), _ffi.ptr(norms[1]), float(eps), _ffi.ptr(slots), int(slots is not None and slots.dtype == torch.int64), *place,
-        int(dtype == torch.bfloat16), _ffi.device_index(like), _ffi.stream_of(like)))
+        int(dtype == torch.bfloat16), _ffi.device_index(k), _ffi.stream_of(k)))
     return q_out, k_out
 
 
