@@ -265,3 +265,13 @@ def test_arguments_that_belong_together():
     w = torch.full((64,), 2.0, dtype=torch.float16, device="cuda")
     y = ops().rotary(x, x, None, None, q_norm=w)
     assert torch.equal(y[1], x) and torch.allclose(y[0].float().pow(2).mean(-1), torch.tensor(4.0, device="cuda"), rtol=2e-3)
+
+
+def test_no_heads_of_queries():
+    x, table, positions = randn(3, 2, 64, dtype=torch.float16).cuda(), ops().rotary_table(10, 64), torch.arange(3).cuda()
+    q, k = ops().rotary(x[:, :0], x, positions, table)
+    assert q.shape == (3, 0, 64) and torch.equal(k, ops().rotary(x, x, positions, table)[1])
+    q, k = ops().rotary(x, x[:, :0], positions, table)
+    assert k.shape == (3, 0, 64) and torch.equal(q, ops().rotary(x, x, positions, table)[0])
+    cache = ops().paged_cache(4, 2, 64, page=16)
+    assert ops().rotary_cache_write(x[:, :0], x, x, positions, table, cache, positions).shape == (3, 0, 64)

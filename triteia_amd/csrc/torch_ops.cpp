@@ -543,7 +543,7 @@ Outputs rotary_cache(const MoreArgs& a) {
   if (to_cache && (!c.ok || !c.takes(k.scalar_type()) || c.k->device() != k.device() || c.heads != kv_heads || c.dim != dim || a[2].size(1) != kv_heads || !index_vector(a[9], tokens))) return {};
   const Place at_(k);
   Outputs out;
-  if (heads) out.first = at::empty({tokens, heads, dim}, k.options());
+  if (!a.none(0)) out.first = at::empty({tokens, heads, dim}, k.options());
   if (!to_cache) out.second = at::empty({tokens, kv_heads, dim}, k.options());
   const Tensor *q = a.get(0), *v = a.get(2), *slots = a.get(9);
   auto stride = [](const Tensor* t, int i) -> long { return t ? t->stride(i) : 0; };
