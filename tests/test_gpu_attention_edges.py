@@ -275,3 +275,21 @@ def test_no_heads_of_queries():
     assert k.shape == (3, 0, 64) and torch.equal(q, ops().rotary(x, x, positions, table)[0])
     cache = ops().paged_cache(4, 2, 64, page=16)
     assert ops().rotary_cache_write(x[:, :0], x, x, positions, table, cache, positions).shape == (3, 0, 64)
+
+
+def test_lazily_negated_tensors():
+    """(torch gives such a view for the imaginary part of a conjugate: its memory holds the other sign.)"""
+    x, table, positions = randn(3, 2, 64, dtype=torch.float16).cuda(), ops().rotary_table(10, 64), torch.arange(3).cuda()
+    w = randn(64, seed=1, dtype=torch.float16).cuda()
+    cache = ops().paged_cache(4, 2, 64, page=16)
+    lazy = torch._neg_view
+    for args in ((lazy(x), x, positions, table, False, w), (x, lazy(x), positions, table, False, w), (x, x, positions, lazy(table), False, w),
+                 (x, x, positions, table, False, lazy(w), lazy(w))):
+        plain = [a.resolve_neg().clone() if isinstance(a, torch.Tensor) else a for a in args]
+        assert all(torch.equal(a, b) for a, b in zip(ops().rotary(*args), ops().rotary(*plain)))
+    ops().cache_write(cache, lazy(x), x, positions)
+    assert torch.equal(ops().cache_read(cache, positions)[0], -x)
+    pages, starts, lens = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([[0]], [0, 3], [3]))
+    assert torch.equal(ops().paged_attention(lazy(x), cache, pages, starts, lens), ops().paged_attention(-x, cache, pages, starts, lens))
+    with pytest.raises(RuntimeError, match="negated"):
+        ops().PagedCache(lazy(cache.k), cache.v)

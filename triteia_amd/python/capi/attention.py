@@ -76,6 +76,8 @@ class PagedCache:
             raise RuntimeError(f"a cache needs pages of 16, 32, .. 1024 tokens, one page and one head at least, got {tuple(k.shape)}")
         if n_pages * page > 2 ** 31 - 1:
             raise RuntimeError(f"a cache of {n_pages} pages of {page} tokens has more than 2^31 slots")
+        if any(t is not None and t.is_neg() for t in (k, v, k_scale, v_scale)):
+            raise RuntimeError("a cache of lazily negated tensors: its memory holds the other sign")
         kind = CACHE_KINDS[k.dtype]
         align = 16 // k.element_size() if kind == 0 or dim % 16 == 0 else 8
         for name, t in (("k", k), ("v", v)):
@@ -138,6 +140,7 @@ def rotary_cache(q, k, v, positions, table, cache, slots, interleaved=False, q_n
         positions = _integers("positions", positions, tokens)
         if table.dtype != torch.float32 or table.dim() != 3 or table.shape[2] != 2 or not table.is_contiguous():
             raise RuntimeError(f"table must be contiguous float32 [positions, pairs, 2], got {table.dtype} {tuple(table.shape)}")
+        table = table.resolve_neg()
         limit, rot = table.shape[0], 2 * table.shape[1]
         if rot % 16 or not 16 <= rot <= dim or limit < 1:
             raise RuntimeError(f"a table of {limit} positions that rotates {rot} of {dim} elements: a position at least, a multiple of 16 elements")
@@ -145,7 +148,7 @@ def rotary_cache(q, k, v, positions, table, cache, slots, interleaved=False, q_n
     for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
         if t is not None and (t.shape != (dim,) or t.dtype != dtype):
             raise RuntimeError(f"{name} must be [{dim}] in {dtype}, got {tuple(t.shape)} in {t.dtype}")
-        norms.append(t if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0) else t.clone(memory_format=torch.contiguous_format))
+        norms.append(t if t is None or (t.is_contiguous() and not t.is_neg() and t.data_ptr() % 16 == 0) else t.resolve_neg().clone(memory_format=torch.contiguous_format))
     q_out = torch.empty((tokens, q.shape[1], dim), dtype=dtype, device=device) if q is not None else None
     k_out = torch.empty((tokens, k.shape[1], dim), dtype=dtype, device=device) if cache is None else None
     strides = [s for t in (q, k, v) for s in (t.stride()[:2] if t is not None else (0, 0))]
