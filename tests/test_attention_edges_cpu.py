@@ -21,3 +21,15 @@ def test_a_scaling_of_positions_that_is_not_whole_is_refused(scaling, match):
     """(A missing type or factor gave the table without any scaling.)"""
     with pytest.raises(RuntimeError, match=match):
         ops.rotary_table(10, 64, scaling=scaling, device="cpu")
+
+
+def test_scratch_does_not_shrink_with_the_batch():
+    """More tokens of as many sequences, or more sequences of as many tokens, never need less."""
+    from triteia_amd.python.capi import _ffi
+    bytes_of = _ffi.lib().triteia_hip_attention_scratch_bytes
+    for heads, kv_heads in ((32, 32), (64, 8), (20, 1), (3, 3)):
+        for max_q in (1, 2, 16, 1000):
+            sizes = [bytes_of(8, tokens, heads, kv_heads, max_q, 128) for tokens in range(1, 600)]
+            assert all(0 < a <= b for a, b in zip(sizes, sizes[1:]))
+            sizes = [bytes_of(seqs, 4000, heads, kv_heads, max_q, 128) for seqs in range(1, 600, 7)]
+            assert all(0 < a <= b for a, b in zip(sizes, sizes[1:]))

@@ -232,6 +232,127 @@ def test_a_layer_of_no_tokens(seqs, planned):
     assert out.shape == (0, 512) and out.dtype == torch.float16
 
 
+# --- the plan's branches and the builds that other batches do not reach -------------------------------------------------------------
+
+def many(n, new, kv, seed=0):
+    """n lengths of up to `new` new tokens (none among them) on contexts of up to `kv`."""
+    g = torch.Generator().manual_seed(seed)
+    out = []
+    for i in range(n):
+        tokens = int(torch.randint(0 if i % 5 == 0 else 1, new + 1, (), generator=g))
+        out.append((tokens, max(tokens, int(torch.randint(1, kv + 1, (), generator=g)))))
+    return out
+
+
+@pytest.mark.parametrize("n", [63, 64, 65, 130, 300])
+@pytest.mark.parametrize("kind", ["same", "fp8"])
+@pytest.mark.parametrize("new,most", [(1, 1), (1, None), (5, 5), (40, None)])
+def test_many_sequences(n, kind, new, most):
+    """The plan's sums over the sequences in rounds of 64, its order of tiles up to 256 of them and beyond."""
+    batch = Batch(many(n, new, 90, n), 4, 2, 64, 16, kind, padding=5)
+    batch.check(ops().paged_attention(*batch.inputs(), max_q=most))
+    batch.check(ops().paged_attention(*batch.inputs(), max_q=most, window=20), window=20)
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("most", [1, None])
+def test_lists_of_many_tiles_are_cut(kind, most):
+    """300 single tokens over one head of the cache, two on long contexts: their tiles are cut in a list that is not sorted."""
+    lengths = many(300, 1, 60, 3)
+    lengths[7], lengths[290] = (1, 9000), (1, 5001)
+    batch = Batch(lengths, 2, 1, 64, 16, kind, torch.bfloat16)
+    got = ops().paged_attention(*batch.inputs(), max_q=most)
+    batch.check(got)
+    long = torch.tensor([batch.starts[7], batch.starts[290]])
+    near(got[long.cuda()], batch.answer()[0][long], batch.dtype)
+
+
+@pytest.mark.parametrize("kind", ["same", "int8"])
+def test_lists_of_many_long_tiles_are_cut(kind):
+    lengths = [(17 + i % 9, 30 + i % 70) for i in range(262)]
+    lengths[100], lengths[3] = (300, 6000), (1, 4000)
+    batch = Batch(lengths, 1, 1, 64, 16, kind)
+    got = ops().paged_attention(*batch.inputs())
+    batch.check(got)
+    rows = slice(batch.starts[100], batch.starts[101])
+    near(got[rows], batch.answer()[0][rows], batch.dtype)
+
+
+def near(got, want, dtype):
+    """Beside the bound on each element, the norm of the error.  Weights are off by u (their rounding) and 2^-13 (scores), the output by u.  Random values of either sign
+    add up like their squares, weights' errors with them: 2 u + 2^-13 of the norm.  (A block of 64 tokens that is lost or counted twice among 9000 is 8 %.)"""
+    error = (got.double().cpu() - want).norm() / want.norm()
+    assert error <= 2 * U[dtype] + 2.0 ** -13, float(error)
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("lengths", [[(1, 9000)], [(4, 9001), (1, 5000)], [(150, 9001), (1, 12345), (20, 4100)]])
+def test_cut_contexts_by_their_norm(kind, dtype, lengths):
+    batch = Batch(lengths, 4, 1, 128, 64, kind, dtype)
+    most = max(n for n, _ in lengths)
+    for how in ({}, {"window": 4000}, {"causal": False}):
+        got = ops().paged_attention(*batch.inputs(), max_q=most, **how)
+        batch.check(got, **how)
+        want = batch.answer(**how)[0]
+        for b in range(len(lengths)):
+            rows = slice(batch.starts[b], batch.starts[b + 1])
+            near(got[rows], want[rows], dtype)
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("seqs,most", [(60, 1), (3, 1), (40, 4), (5, 4)], ids=["16 rows, 4 wavefronts", "16 rows, 8", "32 rows, 4", "32 rows, 8"])
+def test_each_build_for_few_rows(kind, dtype, dim, seqs, most):
+    """Tiles of 16 or 32 rows (8 heads of a group, 1 or 4 tokens) on four wavefronts (more than 128 workgroups by the plan's bounds) or eight."""
+    group, kv_heads = 8, 4
+    batch = Batch(many(seqs, most, 200, seqs + most), group * kv_heads, kv_heads, dim, 32, kind, dtype)
+    tokens = batch.starts[-1]
+    bound = min(seqs + 1, tokens) + tokens * group // (32 if most * group > 16 else 16)
+    assert most * group <= 32 and (bound * kv_heads > 128) == (seqs >= 40)
+    for how in ({}, {"window": 33}, {"causal": False}):
+        got = ops().paged_attention(*batch.inputs(), max_q=most, **how)
+        batch.check(got, **how)
+        near(got, batch.answer(**how)[0], dtype)
+
+
+@pytest.mark.parametrize("kind", ["same", "fp8"])
+def test_a_mixed_step_in_a_graph(kind):
+    """The launch of long and short tiles, a plan whose cuts and joins change, recorded once and replayed on other offsets, lengths, pages and tokens with work between."""
+    heads, kv_heads, dim, page, tokens = 8, 2, 64, 16, 230
+    batch = Batch([(1, 9000), (130, 9000), (99, 9000)], heads, kv_heads, dim, page, kind)
+    q, cache, pages, starts, lens = batch.inputs()
+
+    def step():
+        return ops().paged_attention(q, cache, pages, starts, lens)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    batches = [([0, 1, 131, 230], [9000, 9000, 9000]), ([0, 1, 131, 230], [40, 130, 99]), ([0, 200, 200, 201], [8000, 0, 5000]), ([0, 3, 20, 228], [9000, 20, 208]),
+               ([0, 1, 131, 230], [9000, 9000, 9000]), ([0, 0, 0, 0], [1, 2, 3])]
+    for i, (s, n) in enumerate(batches):
+        new = randn(tokens, heads, dim, seed=i).to(q.dtype)
+        q.copy_(new)
+        starts.copy_(torch.tensor(s, dtype=torch.int32))
+        lens.copy_(torch.tensor(n, dtype=torch.int32))
+        graph.replay()
+        got = out.clone()
+        assert torch.equal(got, step())
+        torch.cuda.synchronize()
+        # (the cache stays; sequences see the first tokens of their contexts)
+        now = Batch.__new__(Batch)
+        now.__dict__.update(batch.__dict__)
+        now.q, now.starts, now.lengths = new, s, [(b - a, kv) for a, b, kv in zip(s, s[1:], n)]
+        now.k, now.v = ([x[b][:n[b]] for b in range(3)] for x in (batch.k, batch.v))
+        now.check(got)
+
+
 # --- refusals -----------------------------------------------------------------------------------------------------------------------
 
 def test_tangents_are_refused():
