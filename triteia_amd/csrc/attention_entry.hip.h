@@ -6,9 +6,6 @@ namespace {
 // Workgroups that walk a large batch's tokens: the five that a CU's registers hold.  (One for every token left the last round half empty: 2000 tokens of 64 + 8 + 8
 // heads into an int8 cache 22.9 us, 20.9 with 1280, 21.9 with 1536, 23.5 with 768; 8000 of 40 + 40 63.7, 62.8, 70.7, 69.5.)
 constexpr int kRotaryWalks = 1280;
-// Bytes of a read-back from which its stores pass the caches by: a result that fills a quarter of the Infinity Cache drives out what is still to be read (20000
-// tokens of 32 heads from e4m3, 328 MB, 104 us and 68); a smaller one is there for its reader.
-constexpr long kStreamedBytes = 64L << 20;
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
@@ -208,7 +205,6 @@ int triteia_hip_cache_read(const void* cache_k, const void* cache_v, const void*
   if (!aligned16(k_out) || !aligned16(v_out)) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: outputs need 16-byte alignment", what);
   a.k_out = k_out, a.v_out = v_out, a.slots = slots, a.slots64 = slots64, a.tokens = tokens, a.kv_heads = kv_heads, a.dim = dim;
   a.page_shift = page_shift_of(page), a.n_slots = (long)n_pages * page;
-  a.streamed = 4L * tokens * kv_heads * dim >= kStreamedBytes;
   DeviceGuard g(dev);
   if (!g.ok) return fail(TRITEIA_HIP_ERR_RUNTIME, "cannot select device %d", dev);
   by_types(bf16, kind, ReadLaunch{a, static_cast<hipStream_t>(stream)});

@@ -290,11 +290,11 @@ struct CacheReadArgs {
   const void* slots;
   int slots64, tokens, kv_heads, dim, page_shift;
   long n_slots;
-  int streamed;                  // stores that leave the caches to the rows that are read
 };
 
 // grid (tiles, 2: keys, values), block 256.  A tile is 4 heads of adjacent tokens, whose rows of a head lie side by side in a page (in the order of the
-// output, all heads of two tokens, 20000 tokens of 32 heads took 113 us instead of 105).  A slot outside the cache gives zeros.
+// output, all heads of two tokens, 20000 tokens of 32 heads took 113 us instead of 105; stores past the caches made no difference at any size, 102.3 and
+// 102.0).  A slot outside the cache gives zeros.
 template <class T, int KIND, int LPR, int U>
 __global__ __launch_bounds__(256) void cache_read_kernel(CacheReadArgs a) {
   constexpr int kRows = 256 / LPR, kTokens = kRows * U / 4;
@@ -335,9 +335,7 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheReadArgs a) {
       for (int j = 0; j < 8; j++) x[u][j] = (T)(y[j] * scale[u]);
     }
     if (!inside[u]) x[u] = kv8<T>{0, 0, 0, 0, 0, 0, 0, 0};
-    kv8<T>* dst = reinterpret_cast<kv8<T>*>(out + (t * a.kv_heads + head) * a.dim + e);
-    if (a.streamed) __builtin_nontemporal_store(x[u], dst);
-    else *dst = x[u];
+    *reinterpret_cast<kv8<T>*>(out + (t * a.kv_heads + head) * a.dim + e) = x[u];
   }
 }
 
