@@ -359,7 +359,7 @@ TRITEIA_HIP_API int triteia_hip_pack_2_4(const void* weight, const void* scales,
  *
  * Queries and keys [tokens, heads, dim] with token and head strides: normalised per head (x * rsqrt(mean(x^2) + eps) * norm, where the norm
  * is not null), their first `rot` elements rotated by row positions[t] of table [limit, rot / 2, 2] (float: cos, sin; positions null: not
- * rotated; outside the table: NaN), pairs (i, i + rot / 2) or, interleaved, (2 i, 2 i + 1).  Queries go to q_out [tokens, heads, dim]; keys
+ * rotated; outside the table: NaN in the rotated elements), pairs (i, i + rot / 2) or, interleaved, (2 i, 2 i + 1).  Queries go to q_out [tokens, heads, dim]; keys
  * to k_out likewise (strides and v null), or, with k_out null, keys and values into the cache at slots[t] (outside it: not written).  8-bit rows get the
  * scale max|x| / 127 or max|x| / 448.  positions and slots are int32, or int64 with positions64, slots64.  dim a multiple of 8 up to 256, rot of 16;
  * rows of q, k, v start on 16 bytes. */
@@ -374,8 +374,8 @@ TRITEIA_HIP_API int triteia_hip_cache_read(const void* cache_k, const void* cach
                              int dev, void* stream);
 
 /* The work list of a batch, once for a forward pass: int32 q_starts [n_seqs + 1] (where each sequence's new tokens begin) and kv_lens [n_seqs]
- * (tokens of its context, the new ones last) on the device; max_q: no sequence brings more new tokens (it chooses kernels, results do not
- * depend on it).  Tokens behind q_starts[n_seqs] get zeros.  Up to 4096 sequences.  Sizes of the plan and of an attention call's scratch, both 16-byte
+ * (tokens of its context, the new ones last) on the device; max_q: no sequence brings more new tokens (it chooses kernels, grids and scratch; any
+ * number is right, which one may change the order of sums).  Tokens behind q_starts[n_seqs] get zeros.  Up to 4096 sequences.  Sizes of the plan and of an attention call's scratch, both 16-byte
  * aligned, contents irrelevant on entry; 0: sizes that are refused. */
 TRITEIA_HIP_API size_t triteia_hip_attention_plan_bytes(int n_seqs, int n_tokens, int heads, int kv_heads, int max_q);
 TRITEIA_HIP_API size_t triteia_hip_attention_scratch_bytes(int n_seqs, int n_tokens, int heads, int kv_heads, int max_q, int dim);

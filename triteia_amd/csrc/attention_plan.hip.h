@@ -9,8 +9,8 @@
 // One workgroup of two wavefronts, a list each, so that nothing but the sequences' lengths in LDS is waited for: sums over the lanes, a lane finds the
 // sequence of a tile by a binary search.  Tokens behind the last sequence get tiles without keys, whose rows are zeros.  Every number read from the
 // device is clamped and offsets that do not ascend are made to, so that every row has one tile and no list passes its end.
-// Bound by latency: 6.5 us for one sequence, 8.3 for a step's 26 of which two are long (14.2 with 1024 threads on one list after the other, whose barriers
-// and shuffles were the time), 11.6 for 64, which are also put in order.
+// Bound by latency: 6.4 us for one sequence, 8.2 for a step's 26 of which two are long (14.2 with 1024 threads on one list after the other, whose barriers
+// and shuffles were the time), 10.9 for 64, 15.7 for four prompts of 500 tokens and 64 heads over 8 (108 tiles), all of which are also put in order.
 #pragma once
 #include "lora_routed.hip.h"
 

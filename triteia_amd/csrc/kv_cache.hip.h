@@ -4,7 +4,7 @@
 //   norm (where there is a weight)   x <- x * rsqrt(sum(x^2) / D + eps) * w
 //   rotation of the first R elements (a, b) <- (a cos - b sin, b cos + a sin) with the pair (i, i + R / 2) or, interleaved,
 //                                    (2 i, 2 i + 1), cos and sin of pair i from row `position` of a table [P, R / 2, 2]
-// and one rounding to the type of the output.  A position outside the table gives a row of NaN (loud, and no access out of bounds).
+// and one rounding to the type of the output.  A position outside the table gives NaN in the elements that are rotated (loud, and no access out of bounds).
 // In a cache of 8 bits a row is codes and one scale: scale = max|x| / 127, code = x / scale to the nearest whole number (int8), or
 // scale = max|x| / 448, code = x / scale to the nearest e4m3 (fp8).  Ties go to even.  A row of magnitudes below 1e-30 is zeros with scale 0; one that
 // holds a NaN or an infinity gets the scale NaN, so that all of it reads back as NaN.
@@ -12,7 +12,7 @@
 // Bound by memory, and for a decode batch by the launch and one round trip.  LPR lanes of 16 bytes hold a row (D / 8 rounded up to a power of
 // two); a workgroup takes rows of one token, so cos, sin and the norms' weights are fetched once per lane and serve all its rows.
 // Measured: 8000 tokens of 40 + 40 heads of 128 in bf16 with norms 63 - 66 us (328 MB, 5.0 - 5.2 TB/s, what a copy reaches); 2000 tokens of 64 + 8 + 8 heads
-// into an int8 cache 21 us (78 MB, 3.7 TB/s: position -> table row -> six passes, one after the other); 64 tokens of 32 + 32 + 32 heads 4.4 us; 20000
+// into an int8 cache 21 us (78 MB, 3.7 TB/s: position -> table row -> six passes, one after the other), 18 into a bf16 one; 64 tokens of 32 + 32 + 32 heads 4.4 us; 20000
 // tokens of 32 heads read back from e4m3 98 - 103 us a call (497 MB, 4.8 - 5.1 TB/s).
 #pragma once
 #include <hip/hip_runtime.h>

@@ -160,8 +160,8 @@ __device__ __forceinline__ int attn_page(const AttendArgs& a, int seq, int token
 
 // One head's keys or values.  Where the 16 tokens of a group start is the same for all lanes and the base of a buffer; a lane's own offset from there, and
 // the offset of the rows of each further request, have 32 bits.  (Added up as 64-bit addresses they were half of the loop's scalar instructions.)
-// ONCE: every row is read by one workgroup alone, as a decode step's are, and need not stay in the caches (64 contexts of up to 4096 tokens, 32 heads, 414 us
-// without that and 384, 3 of up to 100000 in int8 85.6 and 78 when both were measured; tiles of 128 rows, which share them, 335 and 349).
+// ONCE: every row is read by one workgroup alone, as a decode step's are, and need not stay in the caches (64 contexts of up to 4096 tokens, 32 heads, 430 us
+// without that and 386, 3 of up to 100000 in int8 85.0 and 76.4; tiles of 128 rows, which share them, 335 and 349).
 template <int ROWS, bool ONCE>     // rows of a request
 struct AttnHeld {
   const uint8_t* head;
@@ -179,7 +179,7 @@ struct AttnHeld {
 };
 
 // The tokens that a lane's row sees of a block, for the branches of blocks on an edge: a value of its own in each, or the compiler takes the comparisons of all
-// branches out of them and does them for every block (4 x 500 new tokens behind 8200 in e4m3 440 us that way, 373 this).
+// branches out of them and does them for every block (4 x 500 new tokens behind up to 8200 in e4m3 were 440 us that way, 373 this).
 struct AttnSpan {
   int lo, hi;
   __device__ __forceinline__ AttnSpan here() const {
@@ -229,8 +229,8 @@ __device__ __forceinline__ bool attn_within(const AttendArgs& a, int rows, AttnI
 // its four or eight wavefronts walks sub-tiles of its own (8 KB of K and 8 KB of V: 32 tokens of 128 elements in 16 bits, 64 in 8) with the next one's whole rows
 // on their way in registers and this one's in LDS of its own, so that the loop has no barrier; maxima, sums and outputs are joined once at the end.
 // In 8 bits LDS holds the codes and each is converted once, behind its read (ds_read_b64_tr_b8 hands a lane eight tokens of a column).
-// Measured: 64 contexts of up to 4096 tokens, 32 heads, fp16 384 us a call (2.53 GB, 6.6 TB/s); 3 of up to 100000 over 8 heads in int8 76 us (402 MB), 7 of them
-// the joining launch's; one of 500 8.2 us, of which about 1 are the plan's and 1 the pages' round trip, 1 the first rows', 2 two sub-tiles and 2 the joining.
+// Measured: 64 contexts of up to 4096 tokens, 32 heads, fp16 386 us a call (2.53 GB, 6.6 TB/s); 3 of up to 100000 over 8 heads in int8 76 us (402 MB), 7 of them
+// the joining launch's; one of 500 8.0 us, of which about 1 are the plan's and 1 the pages' round trip, 1 the first rows', 2 two sub-tiles and 2 the joining.
 template <int KIND, int D, int NQ, int WAVES>
 struct AttnRowsLds {
   static constexpr int kRowBytes = D * (KIND == kCacheSame ? 2 : 1);
@@ -563,9 +563,10 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
 // MFMAs), and walks the share's tokens in blocks of 64 that all of it reads from LDS: two places, the next block on its way in registers,
 // one barrier a block.  Codes of 8 bits become values on their way to LDS.  Two such workgroups a CU, so that one's exponentials run under the other's
 // MFMAs, which have priority; K rows, and V rows for the transposing reads, are XOR-swizzled by 16-byte pieces (no bank conflicts).
-// Measured: 4 x 500 new tokens behind contexts of up to 8200, 64 heads over 8, bf16 345 us = 808 TFLOP/s (equal contexts 890); 4000 from the first on, 32 heads,
-// fp16 173 us = 757.  Counters: matrix cores busy 45 % of the SIMDs' cycles, LDS 34 %, wavefronts waiting 28 % of theirs.  Loops of this MFMA reach
-// 1660 TFLOP/s alone and 1330 with the softmax's 4 vector instructions and 2 exponentials each between them.  In 8 bits 780 (e4m3, fp16, equal contexts): conversions and scales.
+// Measured: 4 x 500 new tokens in contexts of up to 8200, 64 heads over 8, bf16 338 us = 826 TFLOP/s (all four of 8200 940, in fp16 890); 4000 from the first on, 32
+// heads, fp16 170 us = 771.  Counters of the first: matrix cores busy 41 % of the SIMDs' cycles, LDS 32 %, wavefronts waiting 29 % of theirs.  Loops of this MFMA reach
+// 1660 TFLOP/s alone and 1330 with the softmax's 4 vector instructions and 2 exponentials each between them.  In e4m3, contexts of 8200, 805 in fp16 and 855 in bf16:
+// conversions and scales.
 // Measured and not kept: 256 rows on eight wavefronts and 128 tokens a barrier (equal contexts 1.02, e4m3 1.11, but 26 mixed sequences 0.87 and 3 x 100 new tokens
 // 0.81), V of the first columns read ahead of the softmax (1.00), priority around the second product as well (1.00),
 // the sums of P as one more product, of ones (0.99), three workgroups a CU for heads of 64 (16 bits 0.85; e4m3 1.06 on long batches, 0.8 to 0.9 on others).

@@ -9,14 +9,15 @@ def attention_plan(cache, q_starts, kv_lens, n_heads, n_tokens, max_q=None, caus
     heads as `cache`.
 
     q_starts int32 [sequences + 1]: where each sequence's new tokens begin, from 0 on; kv_lens int32 [sequences]: tokens of its context, the
-    new ones among them; n_tokens: rows of the queries (behind q_starts[-1]: padding, whose outputs are zeros); max_q: no sequence brings more new tokens than this (it
-    chooses kernels; the result does not depend on it)."""
+    new ones among them; n_tokens: rows of the queries (behind q_starts[-1]: padding, whose outputs are zeros); max_q: no sequence brings more new tokens than this.  It
+    chooses kernels, grids and scratch: a batch of single tokens should say 1 (None: n_tokens, which runs it as prompts).  Any number is right; which one may change the
+    order of sums."""
     return capi.attention_plan(q_starts, kv_lens, n_tokens, n_heads, cache.kv_heads, max_q, causal, window)
 
 
 def paged_attention(q, cache, pages, q_starts, kv_lens, plan=None, max_q=None, causal=True, window=0, scale=None):
     """softmax(scale * q k^T) v [tokens, heads, dim] of new tokens q [tokens, heads, dim] over their sequences' contexts, head h on head
-    h // (heads / kv_heads) of the cache.
+    h // (heads / kv_heads) of the cache.  Heads of 64 or 128 elements.
 
     pages int32 [sequences, pages of one]: a sequence's pages in order (entries behind its last are not read; tokens behind the last column are not seen).  causal: the last of a sequence's new tokens sees all of its context,
     each one before it one token less; with `window` it sees the last `window` of those only.  causal=False: every token sees the whole context (cross attention

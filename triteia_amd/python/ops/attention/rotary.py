@@ -64,7 +64,7 @@ def rotary(q, k, positions, table, interleaved=False, q_norm=None, k_norm=None, 
     """(q, k) [tokens, heads, dim] with each head normalised (x * rsqrt(mean(x^2) + eps) * norm, where there is one) and its first
     2 * table.shape[1] elements rotated: pairs (i, i + half), or (2 i, 2 i + 1) if `interleaved`.  Inputs may be views, e.g. of the fused projection's output.
 
-    positions int32 / int64 [tokens]; one outside the table gives NaN.  Serving only: no gradient is recorded."""
+    positions int32 / int64 [tokens]; one outside the table gives NaN in the rotated elements.  Serving only: no gradient is recorded."""
     return capi.rotary_cache(q, k, None, positions, table, None, None, interleaved, q_norm, k_norm, eps)
 
 
