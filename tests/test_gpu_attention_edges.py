@@ -194,6 +194,19 @@ def test_scores_near_the_end_of_32_bits(kind, dtype, size, n):
         assert bool(((got - want).abs() <= 2 * U[dtype] * want.abs() + 2.0 ** -25).all())
 
 
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("n", [1, 5, 90])
+def test_equal_scores_of_any_size(kind, dtype, n):
+    """Keys that are all the same: the mean of what a row sees, at scores of 0 to 10^10 of either sign, with values small enough to move fp16's range."""
+    kv, dim = 700, 64
+    for size, sign in ((0.0, 1), (30.0, 1), (3e3, -1), (3e4, 1), (3e4, -1)):
+        batch = Batch([(n, kv)], 2, 1, dim, 16, kind, dtype)
+        put(batch, 0, torch.full((kv, 1, dim), sign * size), randn(kv, 1, dim, seed=2) * 1e-2)
+        batch.q[:] = size
+        batch.check(ops().paged_attention(*batch.inputs(), max_q=n))
+
+
 # --- the cache ----------------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("kind", ["int8", "fp8"])

@@ -191,9 +191,12 @@ struct AttnSpan {
 };
 
 // The power of two by which a row's sums and weights move so that its largest weight times scale, which has left 1 .. 2^15, is 2^7 to 2^8 again.  (Exact; the
-// reference of scores is a whole number where this is in use, so that less the shift it is exact too.)  Beyond 2^+-64 fp16's outputs have ended.
+// reference of scores is a whole number where this is in use, so that less the shift it is exact too, up to attn_far.)  Beyond 2^+-64 fp16's outputs have ended.
 __device__ __forceinline__ bool attn_off(float peak) { return peak > 32768.f || (peak < 1.f && peak > 0.f); }
 __device__ __forceinline__ int attn_shift(float peak, int now) { return attn_off(peak) ? max(-64, min(64, now + 8 - __builtin_amdgcn_frexp_expf(peak))) - now : 0; }
+
+// A reference so large that its rounding, which a product inside an fma does not share, would pass an exponential's end, or that takes the shift up.
+__device__ __forceinline__ bool attn_far(float m) { return __builtin_fabsf(m) > 1048576.f && m > kAttnNone; }
 
 // Which tokens row `r` of a tile sees: lo <= token < hi.  Rows behind the last see all that the tile sees and are not stored.
 struct AttnRow {
@@ -412,7 +415,17 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
 #pragma unroll
           for (int j = 0; j < 4; j++) o[n][d][j] *= f;
       }
-      const float under = kNormed ? m[n] - (float)shift[n] : m[n];
+      float under = kNormed ? m[n] - (float)shift[n] : m[n];
+      if constexpr (kNormed) {
+        const bool far = attn_far(m[n]);
+        if (__any(far)) {
+#pragma unroll
+          for (int g = 0; g < kGroups; g++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) s[n][g][j] -= far ? m[n] : 0.f;
+          under = far ? -(float)shift[n] : under;
+        }
+      }
 #pragma unroll
       for (int g = 0; g < kGroups; g++)
 #pragma unroll
@@ -750,17 +763,16 @@ __device__ __forceinline__ void attend_tile(const AttendArgs& a, int index, int 
 #pragma unroll
           for (int j = 0; j < 16; j++) o[d][j] *= f;
       }
-      const float under = kNormed ? m - (float)shift : m;
-      float to_log2 = KIND == kCacheSame ? a.scale_log2 : 1.f;
-      if constexpr (KIND == kCacheSame) {
-        // (a far reference's rounding, which a product inside the fma does not share, would pass an exponential's end)
-        const bool far = __builtin_fabsf(m) > 1048576.f && m > kAttnNone;
+      float under = kNormed ? m - (float)shift : m, to_log2 = KIND == kCacheSame ? a.scale_log2 : 1.f;
+      if constexpr (KIND == kCacheSame || kNormed) {
+        const bool far = attn_far(m);
         if (__any(far)) {
 #pragma unroll
           for (int g = 0; g < 2; g++)
 #pragma unroll
-            for (int j = 0; j < 16; j++) s[g][j] *= far ? to_log2 : 1.f;
-          to_log2 = far ? 1.f : to_log2;
+            for (int j = 0; j < 16; j++) s[g][j] = KIND == kCacheSame ? s[g][j] * (far ? to_log2 : 1.f) : s[g][j] - (far ? m : 0.f);
+          if (KIND == kCacheSame) to_log2 = far ? 1.f : to_log2;
+          else under = far ? -(float)shift : under;
         }
       }
       v8 p[4];
