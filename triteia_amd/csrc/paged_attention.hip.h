@@ -576,9 +576,9 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
 // MFMAs), and walks the share's tokens in blocks of 64 that all of it reads from LDS: two places, the next block on its way in registers,
 // one barrier a block.  Codes of 8 bits become values on their way to LDS.  Two such workgroups a CU, so that one's exponentials run under the other's
 // MFMAs, which have priority; K rows, and V rows for the transposing reads, are XOR-swizzled by 16-byte pieces (no bank conflicts).
-// Measured: 4 x 500 new tokens in contexts of up to 8200, 64 heads over 8, bf16 338 us = 826 TFLOP/s (all four of 8200 940, in fp16 890); 4000 from the first on, 32
+// Measured: 4 x 500 new tokens in contexts of up to 8200, 64 heads over 8, bf16 338 us = 826 TFLOP/s (all four of 8200 910 - 940, in fp16 870 - 900); 4000 from the first on, 32
 // heads, fp16 170 us = 771.  Counters of the first: matrix cores busy 41 % of the SIMDs' cycles, LDS 32 %, wavefronts waiting 29 % of theirs.  Loops of this MFMA reach
-// 1660 TFLOP/s alone and 1330 with the softmax's 4 vector instructions and 2 exponentials each between them.  In e4m3, contexts of 8200, 805 in fp16 and 855 in bf16:
+// 1660 TFLOP/s alone and 1330 with the softmax's 4 vector instructions and 2 exponentials each between them.  In e4m3, contexts of 8200, 780 - 810 in fp16 and 830 - 860 in bf16:
 // conversions and scales.
 // Measured and not kept: 256 rows on eight wavefronts and 128 tokens a barrier (equal contexts 1.02, e4m3 1.11, but 26 mixed sequences 0.87 and 3 x 100 new tokens
 // 0.81), V of the first columns read ahead of the softmax (1.00), priority around the second product as well (1.00),
