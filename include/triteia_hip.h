@@ -391,6 +391,25 @@ TRITEIA_HIP_API int triteia_hip_paged_attention(const void* q, long q_token, lon
                              const void* plan, size_t plan_bytes, int n_seqs, int n_tokens, int heads, int kv_heads, int dim, int max_q, int causal,
                              int window, float scale, void* scratch, size_t scratch_bytes, int bf16, int dev, void* stream);
 
+/* ---- The base weight in 8 bits (no counterpart that runs in the reference: triteia/python/nn/linear.py:144-175 calls torch's product). ----
+ *
+ * Values in e4m3 with a 32-bit scale for every block of 128 elements of a row (activations) or of 128 rows (weights), the last blocks smaller: value =
+ * code * scale, scale = max|x| / 448, code = x / scale to the nearest, both rounded as 32-bit divisions are.  Magnitudes below 1e-30: zeros with scale 0; a
+ * block with an infinity or a NaN: scale NaN.  scales[row / rows][block] by strides in floats.  Rows start on 16 bytes, k is a multiple of 16.
+ * x [n, k] in fp16 or bf16 -> codes [n, k], scales [ceil(n / rows), ceil(k / 128)], rows 1 or 128. */
+TRITEIA_HIP_API int triteia_hip_fp8_quantize(const void* x, long x_stride, int n, int k, int rows, void* codes, long codes_stride, void* scales, long scale_row,
+                             long scale_block, int bf16, int dev, void* stream);
+/* The values: out [n, k] contiguous, in fp16 (type 0), bf16 (1) or fp32 (2). */
+TRITEIA_HIP_API int triteia_hip_fp8_values(const void* codes, long codes_stride, const void* scales, long scale_row, long scale_block, int rows, int n, int k,
+                             void* out, int type, int dev, void* stream);
+/* out [tokens, m] = x [tokens, k] @ weight [m, k]^T, weight in codes with w_scale [ceil(m / 128), ceil(k / 128)]; x in codes (x_type 2) with x_scale
+ * [tokens, ceil(k / 128)], or in fp16 (0) or bf16 (1), quantised first as above with a scale for every token.  Sums in 32 bits, rounded once to
+ * out_type (0, 1, 2 as above); out is contiguous.  Scratch: contents irrelevant on entry, 16-byte aligned; 0 bytes: none, or sizes that are refused. */
+TRITEIA_HIP_API size_t triteia_hip_fp8_scratch_bytes(int tokens, int m, int k, int x_type);
+TRITEIA_HIP_API int triteia_hip_fp8_matmul(const void* x, long x_stride, int x_type, const void* x_scale, long xs_token, long xs_block, const void* weight,
+                             long w_stride, const void* w_scale, long ws_row, long ws_block, void* out, int out_type, int tokens, int m, int k, void* scratch,
+                             size_t scratch_bytes, int dev, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,158 @@
+// C entry points of the product in 8 bits and its quantiser (fp8_quant.hip.h, fp8_gemm.hip.h); part of triteia_hip.hip.
+#pragma once
+
+namespace {
+
+constexpr int kFp8Most = 1 << 24;        // rows, columns and features of one call
+
+int check_fp8(const char* what, int n, int k) {
+  if (n < 0 || k < 0 || n > kFp8Most || k > kFp8Most || k % 16 != 0)
+    return fail(TRITEIA_HIP_ERR_PROB_SHAPE, "%s: %d rows of %d elements: a multiple of 16, up to 2^24", what, n, k);
+  return TRITEIA_HIP_OK;
+}
+int fp8_blocks(int k) { return (k + kFp8Block - 1) / kFp8Block; }
+
+// 16 rows x U blocks a workgroup
+long fp8_groups(int n, int k, int u) { return (n + 15L) / 16 * ((fp8_blocks(k) + u - 1) / u); }
+constexpr int kFp8Wide = 4;
+int fp8_width(int n, int k) { return fp8_groups(n, k, 1) > 1024 ? kFp8Wide : 1; }
+
+template <class T>
+int launch_fp8_quant(const Fp8QuantArgs& a, int rows, hipStream_t st) {
+  if (rows != 1) {
+    hipLaunchKernelGGL(fp8_quant_tiles_kernel<T>, dim3((unsigned)((a.n + 127L) / 128 * fp8_blocks(a.k))), dim3(256), 0, st, a);
+    return check_launch("fp8_quant_tiles_kernel");
+  }
+  const int u = fp8_width(a.n, a.k);
+  const dim3 grid((unsigned)fp8_groups(a.n, a.k, u));
+  if (u == 1) hipLaunchKernelGGL((fp8_quant_rows_kernel<T, 1>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((fp8_quant_rows_kernel<T, kFp8Wide>), grid, dim3(256), 0, st, a);
+  return check_launch("fp8_quant_rows_kernel");
+}
+template <class T>
+void launch_fp8_values(const Fp8ValuesArgs& a, hipStream_t st) {
+  const int u = fp8_width(a.n, a.k);
+  const dim3 grid((unsigned)fp8_groups(a.n, a.k, u));
+  if (u == 1) hipLaunchKernelGGL((fp8_values_kernel<T, 1>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((fp8_values_kernel<T, kFp8Wide>), grid, dim3(256), 0, st, a);
+}
+
+struct Fp8Pick {
+  int tokens, features, splits;
+};
+Fp8Pick pick_fp8(int tokens, int m, int k) {
+  (void)tokens, (void)m, (void)k;
+  return {64, 64, 1};
+}
+
+template <int NT, int TW, int F, int FW, int STAGES>
+int launch_fp8_tile(const Fp8Args& a, hipStream_t st) {
+  using Tile = Fp8Tile<NT, TW, F, FW, STAGES>;
+  if (int e = grant_lds<fp8_tile_kernel<NT, TW, F, FW, STAGES>>(Tile::kLdsBytes, "fp8_tile_kernel")) return e;
+  const long units = (long)((a.m + Tile::kFeatures - 1) / Tile::kFeatures) * ((a.tokens + Tile::kTokens - 1) / Tile::kTokens) * a.splits;
+  if (units > 0x7ffffff0L) return fail(TRITEIA_HIP_ERR_PROB_SHAPE, "fp8_matmul: too many work units (%ld)", units);
+  hipLaunchKernelGGL((fp8_tile_kernel<NT, TW, F, FW, STAGES>), dim3((unsigned)((units + 7) / 8 * 8)), dim3(Tile::kThreads), Tile::kLdsBytes, st, a);
+  return check_launch("fp8_tile_kernel");
+}
+
+template <class T>
+void launch_fp8_reduce(const Fp8Args& a, hipStream_t st) {
+  const long results = (long)a.tokens * a.m;
+  if (results % 4 == 0) hipLaunchKernelGGL((fp8_reduce_kernel<T, 4>), dim3((unsigned)((results / 4 + 255) / 256)), dim3(256), 0, st, a.partial, a.splits, results, static_cast<T*>(a.out));
+  else hipLaunchKernelGGL((fp8_reduce_kernel<T, 1>), dim3((unsigned)((results + 255) / 256)), dim3(256), 0, st, a.partial, a.splits, results, static_cast<T*>(a.out));
+}
+
+size_t round16(size_t bytes) { return (bytes + 15) / 16 * 16; }
+// activations in 16 bits: their codes and scales, a block's of all tokens adjacent
+size_t fp8_codes_bytes(int tokens, int k) { return (size_t)tokens * k; }
+size_t fp8_scales_bytes(int tokens, int k) { return round16(sizeof(float) * (size_t)tokens * fp8_blocks(k)); }
+
+}  // namespace
+
+extern "C" {
+
+int triteia_hip_fp8_quantize(const void* x, long x_stride, int n, int k, int rows, void* codes, long codes_stride, void* scales, long scale_row, long scale_block,
+                             int bf16, int dev, void* stream) {
+  const char* what = "fp8_quantize";
+  if (int e = check_fp8(what, n, k)) return e;
+  if (rows != 1 && rows != 128) return fail(TRITEIA_HIP_ERR_KERN_SHAPE, "%s: %d rows a scale: 1 or 128", what, rows);
+  if (n == 0 || k == 0) return TRITEIA_HIP_OK;
+  if (!x || !codes || !scales) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: null tensor pointer", what);
+  if (!aligned16(x) || !aligned16(codes) || reinterpret_cast<uintptr_t>(scales) % 4 != 0 || !strides_ok({x_stride}, 2, 16) || !strides_ok({codes_stride}, 1, 8) ||
+      codes_stride < k || scale_row < 0 || scale_block < 0)
+    return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: rows of whole 16 bytes", what);
+  if (fp8_groups(n, k, 1) > 0x7fffffffL) return fail(TRITEIA_HIP_ERR_PROB_SHAPE, "%s: too many work units", what);
+  DeviceGuard g(dev);
+  if (!g.ok) return fail(TRITEIA_HIP_ERR_RUNTIME, "cannot select device %d", dev);
+  const Fp8QuantArgs a = {x, x_stride, static_cast<uint8_t*>(codes), codes_stride, static_cast<float*>(scales), scale_row, scale_block, n, k};
+  return bf16 ? launch_fp8_quant<__bf16>(a, rows, static_cast<hipStream_t>(stream)) : launch_fp8_quant<_Float16>(a, rows, static_cast<hipStream_t>(stream));
+}
+
+int triteia_hip_fp8_values(const void* codes, long codes_stride, const void* scales, long scale_row, long scale_block, int rows, int n, int k, void* out, int type,
+                           int dev, void* stream) {
+  const char* what = "fp8_values";
+  if (int e = check_fp8(what, n, k)) return e;
+  if ((rows != 1 && rows != 128) || type < 0 || type > 2) return fail(TRITEIA_HIP_ERR_KERN_SHAPE, "%s: %d rows a scale, type %d: 1 or 128, 0 to 2", what, rows, type);
+  if (n == 0 || k == 0) return TRITEIA_HIP_OK;
+  if (!codes || !scales || !out) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: null tensor pointer", what);
+  if (!aligned16(codes) || !aligned16(out) || reinterpret_cast<uintptr_t>(scales) % 4 != 0 || !strides_ok({codes_stride}, 1, 8) || scale_row < 0 || scale_block < 0)
+    return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: rows of whole 16 bytes", what);
+  if (fp8_groups(n, k, 1) > 0x7fffffffL) return fail(TRITEIA_HIP_ERR_PROB_SHAPE, "%s: too many work units", what);
+  DeviceGuard g(dev);
+  if (!g.ok) return fail(TRITEIA_HIP_ERR_RUNTIME, "cannot select device %d", dev);
+  const Fp8ValuesArgs a = {static_cast<const uint8_t*>(codes), codes_stride, static_cast<const float*>(scales), scale_row, scale_block, rows == 1 ? 0 : 7, out, n, k};
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (type == 0) launch_fp8_values<_Float16>(a, st);
+  else if (type == 1) launch_fp8_values<__bf16>(a, st);
+  else launch_fp8_values<float>(a, st);
+  return check_launch("fp8_values_kernel");
+}
+
+size_t triteia_hip_fp8_scratch_bytes(int tokens, int m, int k, int x_type) {
+  if (tokens <= 0 || m <= 0 || k <= 0 || check_fp8("fp8_matmul", tokens, k) || m > kFp8Most) return 0;
+  const int splits = pick_fp8(tokens, m, k).splits;
+  return (x_type == 2 ? 0 : fp8_codes_bytes(tokens, k) + fp8_scales_bytes(tokens, k)) + (splits > 1 ? sizeof(float) * (size_t)splits * tokens * m : 0);
+}
+
+int triteia_hip_fp8_matmul(const void* x, long x_stride, int x_type, const void* x_scale, long xs_token, long xs_block, const void* weight, long w_stride,
+                           const void* w_scale, long ws_row, long ws_block, void* out, int out_type, int tokens, int m, int k, void* scratch, size_t scratch_bytes,
+                           int dev, void* stream) {
+  const char* what = "fp8_matmul";
+  if (int e = check_fp8(what, tokens, k)) return e;
+  if (m < 0 || m > kFp8Most) return fail(TRITEIA_HIP_ERR_PROB_SHAPE, "%s: %d features: up to 2^24", what, m);
+  if (x_type < 0 || x_type > 2 || out_type < 0 || out_type > 2) return fail(TRITEIA_HIP_ERR_KERN_SHAPE, "%s: types %d and %d: 0 to 2", what, x_type, out_type);
+  if (tokens == 0 || m == 0) return TRITEIA_HIP_OK;
+  if (k == 0) return fail(TRITEIA_HIP_ERR_PROB_SHAPE, "%s: rows without elements", what);
+  if (!x || !weight || !w_scale || !out || (x_type == 2 && !x_scale)) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: null tensor pointer", what);
+  if (!aligned16(x) || !aligned16(weight) || !aligned16(out) || !strides_ok({x_stride}, x_type == 2 ? 1 : 2, 16) || !strides_ok({w_stride}, 1, 16) ||
+      ws_row < 0 || ws_block < 0 || (x_type == 2 && (xs_token < 0 || xs_block < 0)))
+    return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: rows of x and of the weight start on 16 bytes", what);
+  const size_t need = triteia_hip_fp8_scratch_bytes(tokens, m, k, x_type);
+  if (need && (!scratch || scratch_bytes < need || !aligned16(scratch)))
+    return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: scratch must hold %zu bytes (got %zu), aligned to 16", what, need, scratch_bytes);
+  DeviceGuard g(dev);
+  if (!g.ok) return fail(TRITEIA_HIP_ERR_RUNTIME, "cannot select device %d", dev);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  Fp8Args a = {};
+  uint8_t* at = static_cast<uint8_t*>(scratch);
+  if (x_type == 2) {
+    a.x = static_cast<const uint8_t*>(x), a.x_stride = x_stride, a.xs = static_cast<const float*>(x_scale), a.xs_token = xs_token, a.xs_block = xs_block;
+  } else {
+    float* scales = reinterpret_cast<float*>(at + fp8_codes_bytes(tokens, k));
+    const Fp8QuantArgs quant = {x, x_stride, at, k, scales, 1, tokens, tokens, k};
+    if (int e = x_type == 1 ? launch_fp8_quant<__bf16>(quant, 1, st) : launch_fp8_quant<_Float16>(quant, 1, st)) return e;
+    a.x = at, a.x_stride = k, a.xs = scales, a.xs_token = 1, a.xs_block = tokens;
+    at += fp8_codes_bytes(tokens, k) + fp8_scales_bytes(tokens, k);
+  }
+  const Fp8Pick t = pick_fp8(tokens, m, k);
+  a.w = static_cast<const uint8_t*>(weight), a.w_stride = w_stride, a.ws = static_cast<const float*>(w_scale), a.ws_row = ws_row, a.ws_block = ws_block;
+  a.out = out, a.type = out_type, a.tokens = tokens, a.m = m, a.k = k, a.splits = t.splits, a.partial = reinterpret_cast<float*>(at);
+  if (int e = launch_fp8_tile<2, 2, 2, 2, 3>(a, st)) return e;
+  if (t.splits == 1) return TRITEIA_HIP_OK;
+  if (out_type == 0) launch_fp8_reduce<_Float16>(a, st);
+  else if (out_type == 1) launch_fp8_reduce<__bf16>(a, st);
+  else launch_fp8_reduce<float>(a, st);
+  return check_launch("fp8_reduce_kernel");
+}
+
+}  // extern "C"

@@ -1,0 +1,214 @@
+// y[t, j] = sum over blocks b of 128 k of  x_scale[t, b] w_scale[j / 128, b] sum_{i in b} x[t, i] w[j, i]
+//
+// x [tokens, k] and w [m, k] in e4m3, rows of adjacent codes.  A block is one 16 x 16 x 128 MFMA: its sums start at zero and go into the running 32-bit sums by one
+// fma with the product of both scales, which a lane has to know for its token only (weights are the MFMA's rows, tokens its columns; a wavefront's features lie
+// in one block of 128).
+//
+// What the instruction does inside a block, measured: it adds the products of eight adjacent codes in fixed point, down to 2^-13 of the largest of the eight,
+// and these sums in 32 bits.  Random codes come out 1.3e-5 off in norm; the codes themselves are 2e-2 off what they stand for.  Sums that are exact to 32 bits would take the
+// instruction of 16 bits on widened codes, at half the rate.
+#pragma once
+#include "sparse24_gemm.hip.h"
+
+namespace triteia_hip {
+
+struct Fp8Args {
+  const uint8_t* x;       // [tokens, k]
+  long x_stride;
+  const float* xs;        // [tokens, blocks] by strides
+  long xs_token, xs_block;
+  const uint8_t* w;       // [m, k]
+  long w_stride;
+  const float* ws;        // [m / 128, blocks]
+  long ws_row, ws_block;
+  void* out;              // [tokens, m]
+  int type;               // of out: 0 fp16, 1 bf16, 2 fp32
+  int tokens, m, k;       // k a multiple of 16
+  int splits;             // shares of K over workgroups; 1: the result goes to `out`
+  float* partial;         // [splits][tokens][m] (splits > 1)
+};
+
+typedef int fp8_v8 __attribute__((ext_vector_type(8)));
+
+__device__ const uint4_t fp8_zeros = {0, 0, 0, 0};     // what lies behind the last code of a row
+
+// 4 bytes a lane to `lds` (uniform) + 4 lane; the caller waits (see direct_load)
+__device__ __forceinline__ void direct_load4(const void* src, uint32_t lds) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(src), "{m0}"(lds) : "memory");
+}
+
+__device__ __forceinline__ float4_t fp8_mma(const fp8_v8& a, const fp8_v8& b) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, float4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ fp8_v8 fp8_operand(const unsigned char* row, int piece) {      // pieces of 16 codes, and the one 64 further on
+  union { fp8_v8 v; uint4_t h[2]; } u;
+  u.h[0] = *reinterpret_cast<const uint4_t*>(row + piece);
+  u.h[1] = *reinterpret_cast<const uint4_t*>(row + (piece ^ 64));
+  return u.v;
+}
+
+// four results of a row of m, from the j0-th on
+template <class T>
+__device__ __forceinline__ void fp8_store(T* to, const float4_t& v, int m, int j0) {
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  if (m % 4 == 0) {
+    *reinterpret_cast<t4*>(to) = t4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+  } else {
+    for (int j = 0; j < 4; j++)
+      if (j0 + j < m) to[j] = (T)v[j];
+  }
+}
+
+// NT x F: 16-token by 16-feature tiles of a wavefront; TW x FW wavefronts side by side.
+template <int NT, int TW, int F, int FW, int STAGES>
+struct Fp8Tile {
+  static constexpr int kTokens = 16 * NT * TW, kFeatures = 16 * F * FW;
+  static constexpr int kWaves = TW * FW, kThreads = 64 * kWaves;
+  static constexpr int kCodes = 128 * (kTokens + kFeatures), kScales = 256 * kWaves;
+  static constexpr int kStageBytes = kCodes + kScales;
+  static constexpr int kWeightScales = (kFeatures + 127) / 128;
+  static constexpr int kLdsBytes = STAGES * kStageBytes;
+  static_assert(16 * F <= 128 && 128 % (16 * F) == 0 && kTokens + kWeightScales <= 64 * kWaves && kFeatures % 8 == 0, "");
+};
+
+template <int NT, int TW, int F, int FW, int STAGES>
+__global__ __launch_bounds__(64 * TW * FW) void fp8_tile_kernel(const Fp8Args p) {
+  using Tile = Fp8Tile<NT, TW, F, FW, STAGES>;
+  constexpr int TT = Tile::kTokens, FF = Tile::kFeatures, WAVES = Tile::kWaves;
+  constexpr int kXLoads = (TT / 8 + WAVES - 1) / WAVES, kWLoads = (FF / 8 + WAVES - 1) / WAVES;
+  constexpr int kLoads = kXLoads + kWLoads + 1;      // a wavefront's requests per block: the same in all of them (a few are made twice)
+  constexpr int AHEAD = STAGES - 1;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, q = lane >> 4;
+  const int tw = wave / FW, fw = wave % FW;
+
+  // Units in the order (feature group, share of K, token tile), token tiles fastest; an XCD (workgroup u runs on XCD u % 8) takes a run of them.
+  const int ttiles = (p.tokens + TT - 1) / TT, groups = (p.m + FF - 1) / FF;
+  const int units = ttiles * groups * p.splits;
+  const int per_xcd = (units + 7) >> 3;
+  const int u = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per_xcd || u >= units) return;
+  const int tt = u % ttiles, z = (u / ttiles) % p.splits, fg = u / (ttiles * p.splits);
+  const int t0 = tt * TT, f0 = fg * FF;
+  const int blocks = (p.k + 127) >> 7;
+  const int c0 = (int)((long)z * blocks / p.splits), n = (int)((long)(z + 1) * blocks / p.splits) - c0;
+
+  // A request: 8 rows x 128 bytes; lane l takes 16 bytes of row l / 8, the piece (l % 8) ^ (l / 8) to position l % 8.
+  // (rows past the end repeat the last one: their sums are not stored)
+  const uint8_t* src[kLoads - 1];
+  uint32_t dst[kLoads - 1];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
+  const int lane_piece = (lane & 7) ^ (lane >> 3);
+#pragma unroll
+  for (int i = 0; i < kLoads - 1; i++) {
+    const bool is_x = i < kXLoads;
+    const int g = min(wave + WAVES * (is_x ? i : i - kXLoads), (is_x ? TT : FF) / 8 - 1), row = 8 * g + (lane >> 3);
+    const uint8_t* base = is_x ? p.x + (long)min(t0 + row, p.tokens - 1) * p.x_stride : p.w + (long)min(f0 + row, p.m - 1) * p.w_stride;
+    src[i] = base + 16 * lane_piece + 128L * c0;
+    dst[i] = lds0 + (is_x ? 0 : 128 * TT) + 1024 * g;
+  }
+  // scales of a block: those of the tile's tokens, then those of its weights' blocks, 64 a wavefront
+  const int which = 64 * wave + lane;
+  const float* scale_src = which < TT ? p.xs + (long)min(t0 + which, p.tokens - 1) * p.xs_token + c0 * p.xs_block
+                                      : p.ws + (long)min((f0 >> 7) + min(which - TT, Tile::kWeightScales - 1), (p.m - 1) >> 7) * p.ws_row + c0 * p.ws_block;
+  const long scale_step = which < TT ? p.xs_block : p.ws_block;
+  const bool short_piece = 128 * (blocks - 1) + 16 * lane_piece >= p.k;      // of the last block
+  auto issue = [&](int i, int c, int stage) {
+    if (i == kLoads - 1) {
+      direct_load4(scale_src + c * scale_step, __builtin_amdgcn_readfirstlane(lds0 + stage * Tile::kStageBytes + Tile::kCodes + 256 * wave));
+    } else {
+      const uint8_t* s = src[i] + 128L * c;
+      if (c0 + c == blocks - 1 && short_piece) s = reinterpret_cast<const uint8_t*>(&fp8_zeros);
+      direct_load(s, __builtin_amdgcn_readfirstlane(dst[i] + stage * Tile::kStageBytes));
+    }
+  };
+
+  float4_t acc[F][NT];
+#pragma unroll
+  for (int f = 0; f < F; f++)
+#pragma unroll
+    for (int t = 0; t < NT; t++) acc[f][t] = float4_t{0.f, 0.f, 0.f, 0.f};
+  const int piece = (q ^ (r & 7)) * 16;
+  const uint32_t xrow = (16 * NT * tw + r) * 128;
+  const uint32_t wrow = 128 * TT + (16 * F * fw + r) * 128;
+  auto compute = [&](int stage, auto&& request) {
+    const unsigned char* s = smem + stage * Tile::kStageBytes;
+    const float* scales = reinterpret_cast<const float*>(s + Tile::kCodes);
+    const float sw = scales[TT + 16 * F * fw / 128];
+    fp8_v8 w[F];
+#pragma unroll
+    for (int f = 0; f < F; f++) w[f] = fp8_operand(s + wrow + 2048 * f, piece);
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const fp8_v8 x = fp8_operand(s + xrow + 2048 * t, piece);
+      const float scale = scales[16 * (NT * tw + t) + r] * sw;
+#pragma unroll
+      for (int f = 0; f < F; f++) {
+        const float4_t d = fp8_mma(w[f], x);
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[f][t][j] = __builtin_fmaf(d[j], scale, acc[f][t][j]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kLoads; i++) request(i);
+  };
+
+  for (int c = 0; c < AHEAD && c < n; c++)
+#pragma unroll
+    for (int i = 0; i < kLoads; i++) issue(i, c, c);
+  int stage = 0, c = 0;
+  // AHEAD blocks are in flight at the top, kLoads requests each, and complete in order (as in dense_base_kernel)
+  for (; c + AHEAD <= n; c++) {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"((AHEAD - 1) * kLoads) : "memory");
+    lds_barrier();
+    const int free_stage = stage == 0 ? STAGES - 1 : stage - 1;
+    if (c + AHEAD < n) compute(stage, [&](int i) { issue(i, c + AHEAD, free_stage); });
+    else compute(stage, [](int) {});
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+  }
+  for (; c < n; c++) {
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+    lds_barrier();
+    compute(stage, [](int) {});
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+  }
+
+  // D: lane (token r, q) holds features 4q .. 4q + 3 of a tile
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    const int token = t0 + 16 * (NT * tw + t) + r;
+#pragma unroll
+    for (int f = 0; f < F; f++) {
+      const int j0 = f0 + 16 * (F * fw + f) + 4 * q;
+      if (token >= p.tokens || j0 >= p.m) continue;
+      const long at = (long)token * p.m + j0;
+      if (p.splits > 1) fp8_store<float>(p.partial + (long)z * p.tokens * p.m + at, acc[f][t], p.m, j0);
+      else if (p.type == 0) fp8_store<_Float16>(static_cast<_Float16*>(p.out) + at, acc[f][t], p.m, j0);
+      else if (p.type == 1) fp8_store<__bf16>(static_cast<__bf16*>(p.out) + at, acc[f][t], p.m, j0);
+      else fp8_store<float>(static_cast<float*>(p.out) + at, acc[f][t], p.m, j0);
+    }
+  }
+}
+
+// The shares of K, added in order and rounded once; 4 results a thread (or one, where rows do not divide by 4).
+template <class T, int N>
+__global__ __launch_bounds__(256) void fp8_reduce_kernel(const float* __restrict__ partial, int splits, long results, T* __restrict__ out) {
+  typedef float vN __attribute__((ext_vector_type(N)));
+  const long e = ((long)blockIdx.x * 256 + threadIdx.x) * N;
+  if (e >= results) return;
+  float sum[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) sum[i] = 0.f;
+#pragma unroll 4
+  for (int z = 0; z < splits; z++) {
+    const vN v = *reinterpret_cast<const vN*>(partial + z * results + e);
+#pragma unroll
+    for (int i = 0; i < N; i++) sum[i] += v[i];
+  }
+#pragma unroll
+  for (int i = 0; i < N; i++) out[e + i] = (T)sum[i];
+}
+
+}  // namespace triteia_hip

@@ -617,6 +617,78 @@ Outputs paged_attention(const MoreArgs& a) {
   return out;
 }
 
+// --- the base weight in 8 bits ---
+
+int fp8_type(at::ScalarType t) { return t == at::kHalf ? 0 : t == at::kBFloat16 ? 1 : t == at::kFloat ? 2 : -1; }
+// [rows, elements] of adjacent elements whose rows start on 16 bytes
+bool fp8_rows_ok(const Tensor& t, int64_t rows, int64_t k) {
+  return t.dim() == 2 && t.size(0) == rows && t.size(1) == k && t.stride(1) == 1 && t.stride(0) >= 0 && t.stride(0) * t.element_size() % 16 == 0 && aligned(t);
+}
+bool fp8_scales_ok(const Tensor& t, int64_t rows, int64_t k) {
+  return t.scalar_type() == at::kFloat && t.dim() == 2 && t.size(0) == rows && t.size(1) == (k + 127) / 128 && t.stride(0) >= 0 && t.stride(1) >= 0;
+}
+
+// quantize_fp8(x, rows of a scale)
+Outputs quantize_fp8(const MoreArgs& a) {
+  if (a.n != 2 || !a.tensor(0) || !a.whole(1)) return {};
+  const Tensor& x = a[0];
+  if (!x.is_cuda() || x.dim() != 2 || !half_type(x.scalar_type()) || !a.plain(0, x) || !sizes_ok({x.size(0), x.size(1)}) || !fp8_rows_ok(x, x.size(0), x.size(1))) return {};
+  const int64_t n = x.size(0), k = x.size(1), blocks = (k + 127) / 128;
+  const int rows = a.integer(1);
+  if ((rows != 1 && rows != 128) || k % 16 != 0) return {};
+  const Place at_(x);
+  Outputs out;
+  out.first = at::empty({n, k}, x.options().dtype(at::kFloat8_e4m3fn));
+  // (a row's scales apart, a block's of all rows adjacent, as the product reads them)
+  out.second = rows == 1 ? at::empty({blocks, n}, x.options().dtype(at::kFloat)).t() : at::empty({(n + 127) / 128, blocks}, x.options().dtype(at::kFloat));
+  out.done = launched(triteia_hip_fp8_quantize(x.data_ptr(), x.stride(0), n, k, rows, out.first.data_ptr(), k, out.second.data_ptr(), out.second.stride(0),
+                                               out.second.stride(1), x.scalar_type() == at::kBFloat16, at_.dev, at_.handle()));
+  return out;
+}
+
+// dequantize_fp8(codes, scales, dtype)
+Outputs dequantize_fp8(const MoreArgs& a) {
+  if (a.n != 3 || !a.tensor(0) || !a.tensor(1) || !a.typed[2] || fp8_type(a.types[2]) < 0) return {};
+  const Tensor &codes = a[0], &scales = a[1];
+  if (!codes.is_cuda() || codes.dim() != 2 || codes.scalar_type() != at::kFloat8_e4m3fn || scales.dim() != 2 || !a.plain(0, codes) || !a.plain(1, codes)) return {};
+  const int64_t n = codes.size(0), k = codes.size(1);
+  const int rows = scales.size(0) == n ? 1 : 128;
+  if (!sizes_ok({n, k}) || !fp8_rows_ok(codes, n, k) || !fp8_scales_ok(scales, rows == 1 ? n : (n + 127) / 128, k)) return {};
+  const Place at_(codes);
+  Outputs out;
+  out.first = at::empty({n, k}, codes.options().dtype(a.types[2]));
+  out.done = launched(triteia_hip_fp8_values(codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(0), scales.stride(1), rows, n, k, out.first.data_ptr(),
+                                             fp8_type(a.types[2]), at_.dev, at_.handle()));
+  return out;
+}
+
+// matmul_fp8(x, weight, its scales, x's scales or None, dtype or None)
+Outputs matmul_fp8(const MoreArgs& a) {
+  if (a.n != 5 || !a.tensor(0) || !a.tensor(1) || !a.tensor(2) || !a.maybe(3) || !(a.none(4) || a.typed[4])) return {};
+  const Tensor &x = a[0], &w = a[1], &ws = a[2];
+  for (int i = 0; i < 4; i++)
+    if (a.tensor(i) && !a.plain(i, x)) return {};
+  const bool codes = x.scalar_type() == at::kFloat8_e4m3fn;
+  if (!x.is_cuda() || x.dim() < 1 || (!codes && !half_type(x.scalar_type())) || codes == a.none(3) || w.dim() != 2 || w.scalar_type() != at::kFloat8_e4m3fn) return {};
+  const int64_t k = x.size(-1), m = w.size(0), tokens = k > 0 ? x.numel() / k : 0;
+  const at::ScalarType type = a.typed[4] ? a.types[4] : codes ? at::kHalf : x.scalar_type();
+  if (fp8_type(type) < 0 || !sizes_ok({tokens, k, m}) || !fp8_rows_ok(w, m, k) || !fp8_scales_ok(ws, (m + 127) / 128, k)) return {};
+  if (codes ? x.dim() != 2 || !fp8_scales_ok(a[3], tokens, k) : x.dim() != 2 && !x.is_contiguous()) return {};
+  if (x.dim() == 2 ? !fp8_rows_ok(x, tokens, k) : !aligned(x) || k % 8 != 0) return {};
+  const Place at_(x);
+  c10::SmallVector<int64_t, 5> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = m;
+  Outputs out;
+  out.first = at::empty(shape, x.options().dtype(type));
+  const int x_type = codes ? 2 : fp8_type(x.scalar_type());
+  const size_t bytes = triteia_hip_fp8_scratch_bytes(tokens, m, k, x_type);
+  const Tensor scratch = bytes ? scratch_bytes(bytes, x) : Tensor();
+  out.done = launched(triteia_hip_fp8_matmul(x.data_ptr(), x.dim() == 2 ? x.stride(0) : k, x_type, codes ? a[3].data_ptr() : nullptr, codes ? a[3].stride(0) : 0,
+                                             codes ? a[3].stride(1) : 0, w.data_ptr(), w.stride(0), ws.data_ptr(), ws.stride(0), ws.stride(1), out.first.data_ptr(),
+                                             fp8_type(type), tokens, m, k, bytes ? scratch.data_ptr() : nullptr, bytes, at_.dev, at_.handle()));
+  return out;
+}
+
 // One output as a tensor, two (and a missing first) as a tuple.
 template <Outputs (*F)(const MoreArgs&), bool PAIR>
 PyObject* call_more(PyObject*, PyObject* const* v, Py_ssize_t n) {
@@ -642,7 +714,9 @@ PyObject* call_more(PyObject*, PyObject* const* v, Py_ssize_t n) {
 PyMethodDef methods[] = {METHOD("matmul", (call<matmul>)), METHOD("bmm", (call<bmm>)), METHOD("sbmm", (call<sbmm>)), METHOD("lora", (call<lora>)), METHOD("ldmm", (call<ldmm>)),
                          METHOD("pack", pack), METHOD("sparse", sparse), METHOD("rotary_cache", (call_more<rotary_cache, true>)),
                          METHOD("cache_read", (call_more<cache_read, true>)), METHOD("attention_plan", (call_more<attention_plan, false>)),
-                         METHOD("paged_attention", (call_more<paged_attention, false>)), {nullptr, nullptr, 0, nullptr}};
+                         METHOD("paged_attention", (call_more<paged_attention, false>)),
+                         METHOD("quantize_fp8", (call_more<quantize_fp8, true>)), METHOD("dequantize_fp8", (call_more<dequantize_fp8, false>)),
+                         METHOD("matmul_fp8", (call_more<matmul_fp8, false>)), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "triteia_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -12,6 +12,8 @@
 #include <mutex>
 
 #include "dense_base.hip.h"
+#include "fp8_gemm.hip.h"
+#include "fp8_quant.hip.h"
 #include "lora.hip.h"
 #include "lora_fused.hip.h"
 #include "lora_mfma.hip.h"
@@ -2133,3 +2135,4 @@ int triteia_hip_pack_2_4(const void* weight, const void* scales, void* qweight, 
 }  // extern "C"
 
 #include "attention_entry.hip.h"
+#include "fp8_entry.hip.h"

@@ -77,6 +77,11 @@ SIGNATURES = {
     "triteia_hip_attention_plan": (_c_int, [_c_vp] * 2 + [_c_int] * 7 + [_c_vp, _c_sz, _c_int, _c_vp]),
     "triteia_hip_paged_attention": (_c_int, [_c_vp, _c_long, _c_long] + [_c_vp] * 6 + [_c_int] * 3 + [_c_vp, _c_long, _c_int, _c_vp, _c_sz]
                                     + [_c_int] * 8 + [_c_float, _c_vp, _c_sz] + [_c_int] * 2 + [_c_vp]),
+    "triteia_hip_fp8_quantize": (_c_int, [_c_vp, _c_long] + [_c_int] * 3 + [_c_vp, _c_long, _c_vp, _c_long, _c_long] + [_c_int] * 2 + [_c_vp]),
+    "triteia_hip_fp8_values": (_c_int, [_c_vp, _c_long, _c_vp, _c_long, _c_long] + [_c_int] * 3 + [_c_vp] + [_c_int] * 2 + [_c_vp]),
+    "triteia_hip_fp8_scratch_bytes": (_c_sz, [_c_int] * 4),
+    "triteia_hip_fp8_matmul": (_c_int, [_c_vp, _c_long, _c_int, _c_vp, _c_long, _c_long, _c_vp, _c_long, _c_vp, _c_long, _c_long, _c_vp] + [_c_int] * 4
+                               + [_c_vp, _c_sz, _c_int, _c_vp]),
     "triteia_hip_pack_2_4": (_c_int, [_c_vp] * 5 + [_c_int] * 3 + [_c_vp]),
 }
 

@@ -3,6 +3,7 @@ from .matmul.bmm import *
 from .matmul.sbmm import *
 from .matmul.lora import *
 from .matmul.ldmm import ldmm, baseline_ldmm
+from .matmul.fp8 import *
 from .attention.rotary import *
 from .attention.cache import *
 from .attention.paged import *
