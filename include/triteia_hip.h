@@ -391,6 +391,19 @@ TRITEIA_HIP_API int triteia_hip_paged_attention(const void* q, long q_token, lon
                              const void* plan, size_t plan_bytes, int n_seqs, int n_tokens, int heads, int kv_heads, int dim, int max_q, int causal,
                              int window, float scale, void* scratch, size_t scratch_bytes, int bf16, int dev, void* stream);
 
+/* The same for sequences in groups that share their first tokens: group g is sequences group_starts[g] .. group_starts[g + 1] - 1 (int32 [n_groups + 1], ascending;
+ * sequences ahead of the first and behind the last are in none), whose rows of `pages` name the same pages for the first prefix_lens[g] tokens (int32 [n_groups]).  Of
+ * those, the tokens that all rows of a group see are read and multiplied once for all of the group.  Any prefix_lens are right as long as the pages are the same;
+ * with a window nothing is shared.  Up to 1024 groups, n_seqs + n_groups up to 4096.  A plan, and the call on it, with the same n_groups. */
+TRITEIA_HIP_API size_t triteia_hip_shared_plan_bytes(int n_seqs, int n_groups, int n_tokens, int heads, int kv_heads, int max_q);
+TRITEIA_HIP_API size_t triteia_hip_shared_scratch_bytes(int n_seqs, int n_groups, int n_tokens, int heads, int kv_heads, int max_q, int dim);
+TRITEIA_HIP_API int triteia_hip_shared_plan(const void* q_starts, const void* kv_lens, const void* group_starts, const void* prefix_lens, int n_seqs, int n_groups,
+                             int n_tokens, int heads, int kv_heads, int max_q, int causal, int window, void* plan, size_t plan_bytes, int dev, void* stream);
+TRITEIA_HIP_API int triteia_hip_shared_attention(const void* q, long q_token, long q_head, void* out, const void* cache_k, const void* cache_v, const void* k_scale,
+                             const void* v_scale, const long* strides, int n_pages, int page, int kind, const void* pages, long pages_seq, int table_width,
+                             const void* plan, size_t plan_bytes, int n_seqs, int n_groups, int n_tokens, int heads, int kv_heads, int dim, int max_q, int causal,
+                             int window, float scale, void* scratch, size_t scratch_bytes, int bf16, int dev, void* stream);
+
 /* ---- The base weight in 8 bits (no counterpart that runs in the reference: triteia/python/nn/linear.py:144-175 calls torch's product). ----
  *
  * Values in e4m3 with a 32-bit scale for every block of 128 elements of a row (activations) or of 128 rows (weights), the last blocks smaller: value =

@@ -1,0 +1,271 @@
+"""Attention of sequences in groups that share a prefix: the answer of every sequence by itself.
+
+Bounds are those of test_gpu_attention.py: which tokens go into which partial sum changes no rounding but those of sums in 32 bits."""
+import math
+
+import pytest
+import torch
+
+from tests.test_gpu_attention import HALF, KINDS, Batch, empty_cache, ops, rows_of
+
+pytestmark = pytest.mark.gpu
+
+
+class Shared(Batch):
+    """Groups (tokens of the prefix, [(new tokens, tokens of its own), ..]); a group with prefix None: sequences that belong to none.  Whole pages of a prefix are the same
+    ones for all of its sequences, a page that it ends in is copied."""
+
+    def __init__(self, groups, heads=4, kv_heads=2, dim=128, page=16, kind="same", dtype=torch.float16, padding=0, seed=0, big=1.0):
+        g = torch.Generator().manual_seed(seed)
+        self.heads, self.kv_heads, self.dim, self.page, self.kind, self.dtype = heads, kv_heads, dim, page, kind, dtype
+        self.lengths = [(n, (prefix or 0) + own) for prefix, seqs in groups for n, own in seqs]
+        need = sum((prefix or 0) // page for prefix, _ in groups) + sum(-(-kv // page) for _, kv in self.lengths)
+        n_pages = need + 2
+        self.cache = empty_cache(kind, dtype, n_pages, kv_heads, page, dim)
+        order = torch.randperm(n_pages, generator=g).to(torch.int32)
+        self.width = max((-(-kv // page) for _, kv in self.lengths), default=0) + 1
+        self.pages = torch.full((len(self.lengths), self.width), 2 ** 31 - 1, dtype=torch.int32)
+        self.group_starts, self.prefix_lens, self.k, self.v = [], [], [], []
+        at = b = 0
+        for prefix, seqs in groups:
+            if prefix is not None:
+                assert not self.group_starts or self.group_starts[-1] == b
+                self.group_starts += [b, b + len(seqs)] if not self.group_starts else [b + len(seqs)]
+                self.prefix_lens.append(prefix)
+            whole = (prefix or 0) // page
+            shared = order[at:at + whole]
+            at += whole
+            first = [torch.randn(((prefix or 0), kv_heads, dim), generator=g) * big for _ in range(2)]
+            for n, own in seqs:
+                kv = (prefix or 0) + own
+                mine = -(-kv // page) - whole
+                self.pages[b, :whole], self.pages[b, whole:whole + mine] = shared, order[at:at + mine]
+                at += mine
+                k, v = (torch.cat([x, torch.randn((own, kv_heads, dim), generator=g) * big]) for x in first)
+                place = self.slots(b, torch.arange(kv))
+                ops().cache_write(self.cache, k.to(dtype).cuda(), v.to(dtype).cuda(), place)
+                for keep, raw, scale in ((self.k, self.cache.k, self.cache.k_scale), (self.v, self.cache.v, self.cache.v_scale)):
+                    x = rows_of(raw, page)[place.cpu()].double()
+                    keep.append(x if scale is None else x * rows_of(scale, page)[place.cpu()].double()[..., None])
+                b += 1
+        self.starts = [0]
+        for n, _ in self.lengths:
+            self.starts.append(self.starts[-1] + n)
+        self.q = (torch.randn((self.starts[-1] + padding, heads, dim), generator=g) * 2).to(dtype)
+
+    def groups(self):
+        return dict(group_starts=torch.tensor(self.group_starts or [0], dtype=torch.int32).cuda(), prefix_lens=torch.tensor(self.prefix_lens, dtype=torch.int32).cuda())
+
+    def attend(self, max_q=None, causal=True, window=0, scale=None, **groups):
+        q, cache, pages, starts, lens = self.inputs()
+        plan = ops().attention_plan(cache, starts, lens, self.heads, q.shape[0], max_q, causal, window, **(groups or self.groups()))
+        return ops().paged_attention(q, cache, pages, starts, lens, plan=plan, causal=causal, window=window, scale=scale)
+
+
+DECODES = [(300, [(1, 1), (1, 15), (1, 70)]), (0, [(1, 40), (1, 3)]), (64, [(1, 1), (1, 64)]), (1100, [(1, 5), (1, 130), (1, 1), (1, 200), (1, 64), (1, 63), (1, 65)]),
+           (500, [(1, 20)]), (None, [(1, 90), (1, 1)])]
+CHUNKS = [(None, [(3, 100)]), (190, [(5, 5), (1, 40), (70, 70)]), (400, [(64, 128), (33, 33)]), (1000, [(200, 263), (129, 129), (1, 1), (40, 41)])]
+MANY = [(700, [(1, 1 + 7 * i % 90) for i in range(40)]), (65, [(1, 3)] * 30), (None, [(1, 100)] * 5)]
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,kv_heads,page", [(4, 4, 16), (8, 2, 32), (20, 1, 64), (3, 1, 128)])
+@pytest.mark.parametrize("groups", [DECODES, CHUNKS, MANY], ids=["decodes", "chunks", "many"])
+def test_shared_prefix(kind, dtype, dim, heads, kv_heads, page, groups):
+    batch = Shared(groups, heads, kv_heads, dim, page, kind, dtype)
+    most = max(n for n, _ in batch.lengths)
+    batch.check(batch.attend(most))
+    batch.check(batch.attend(most, causal=False, scale=0.2), causal=False, scale=0.2)
+    batch.check(batch.attend(most, window=50), window=50)
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("most", [None, 1, 2, 7, 100000])
+@pytest.mark.parametrize("groups", [DECODES, CHUNKS], ids=["decodes", "chunks"])
+def test_the_largest_number_of_new_tokens_is_a_hint(kind, most, groups):
+    batch = Shared(groups, 8, 2, 128, 16, kind)
+    batch.check(batch.attend(most))
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("most", [1, None])
+def test_groups_of_nothing(kind, most):
+    """Sequences without new tokens, groups without sequences, new tokens that reach back into the prefix or ahead of the context, no tokens of their own, padding."""
+    batch = Shared([(200, [(0, 0), (1, 30), (0, 10), (1, 7)]), (300, []), (128, [(6, 2), (40, 3)]), (100, [(150, 30), (1, 1)]), (256, [(0, 9), (0, 1)]), (64, []),
+                    (None, [(2, 50)])], 6, 2, 64, 16, kind, padding=21)
+    batch.check(batch.attend(most))
+    batch.check(batch.attend(most, causal=False), causal=False)
+    cross = Shared([(320, [(3, 0), (1, 0), (20, 0)]), (70, [(1, 0), (2, 0)])], 6, 2, 64, 16, kind)
+    cross.check(cross.attend(most, causal=False), causal=False)                 # states that all rows see all of, and nothing else
+    none = Shared([(None, [])], padding=3)
+    assert not none.attend(most).any()
+    assert Shared([(100, [(0, 5), (0, 1)])]).attend(most).shape == (0, 4, 128)
+    no_groups = Shared([(None, [(1, 100), (3, 70)])], 4, 2, 128, 16, kind)
+    no_groups.check(no_groups.attend(most))
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+def test_prefixes_that_are_cut_into_shares(kind):
+    for groups in ([(9000, [(1, 30), (1, 700), (2, 5)])], [(20000, [(3, 40), (40, 5000)]), (5000, [(1, 1), (1, 1)])], [(12000, [(150, 151), (1, 12), (90, 3000)])]):
+        batch = Shared(groups, 4, 1, 128, 64, kind, torch.bfloat16)
+        most = max(n for n, _ in batch.lengths)
+        for how in ({}, {"causal": False}):
+            batch.check(batch.attend(most, **how), **how)
+
+
+@pytest.mark.parametrize("most", [1, None])
+def test_more_groups_and_tiles_than_a_wavefront_has_lanes(most):
+    groups = [(64 * (i % 3) + 5, [(1, 1 + i % 5)] * (1 + i % 4)) for i in range(150)]
+    batch = Shared(groups, 8, 1, 64, 16)
+    batch.check(batch.attend(most))
+    batch = Shared([(130, [(20, 20)] * 6)] * 70, 8, 1, 64, 16)                  # more than 256 tiles
+    batch.check(batch.attend(most))
+
+
+def test_a_prefix_is_what_the_pages_say():
+    """Prefix lengths shorter than what is shared are as right as the whole; longer ones end where some row's own context begins."""
+    batch = Shared([(1024, [(1, 30), (1, 90), (4, 200)])], 8, 2, 128, 16)
+    starts = torch.tensor([0, 3], dtype=torch.int32).cuda()
+    for prefix in (-5, 0, 1, 63, 64, 500, 1024):
+        batch.check(batch.attend(4, group_starts=starts, prefix_lens=torch.tensor([prefix], dtype=torch.int32).cuda()))
+    twins = Shared([(1024, [(3, 0), (3, 0)])], 8, 2, 128, 16)                   # the same context twice
+    for prefix in (1024, 2000, 2 ** 31 - 1):
+        twins.check(twins.attend(3, group_starts=torch.tensor([0, 2], dtype=torch.int32).cuda(), prefix_lens=torch.tensor([prefix], dtype=torch.int32).cuda()))
+
+
+@pytest.mark.parametrize("starts", [[0, 3, 2, 7], [5, 0, 3, 9], [-4, 2, 100, 50], [7, 7, 7, 7], [2 ** 31 - 1, 0, 0, -2 ** 31]])
+def test_group_offsets_in_no_order(starts):
+    """Each is taken as the largest ahead of it, inside the batch: any sequence is in one group at most, and every row is written.  (All share all of the prefix here, so that
+    any grouping is right.)"""
+    batch = Shared([(300, [(1, 5), (2, 40), (1, 1), (3, 9), (1, 30), (1, 2), (1, 70)])], 4, 2, 64, 16)
+    for prefixes in ([300, 300, 300], [64, 0, 200]):
+        batch.check(batch.attend(3, group_starts=torch.tensor(starts, dtype=torch.int32).cuda(), prefix_lens=torch.tensor(prefixes, dtype=torch.int32).cuda()))
+
+
+def test_a_table_shorter_than_the_prefix():
+    """Tokens behind the table's last column are not seen, of a prefix as of any context."""
+    batch = Shared([(640, [(1, 40), (2, 10)]), (320, [(1, 1), (1, 1)])], 4, 2, 64, 16)
+    q, cache, pages, starts, lens = batch.inputs()
+    for columns in (1, 3, 20, 30):
+        plan = ops().attention_plan(cache, starts, lens, 4, q.shape[0], 2, causal=False, **batch.groups())
+        got = ops().paged_attention(q, cache, pages[:, :columns], starts, lens, plan=plan, causal=False)
+        held = Batch.__new__(Batch)
+        held.__dict__.update(batch.__dict__)
+        held.lengths = [(n, min(kv, 16 * columns)) for n, kv in batch.lengths]
+        held.k, held.v = ([x[:16 * columns] for x in held] for held in (batch.k, batch.v))
+        held.check(got, causal=False)
+
+
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_what_is_no_number_reaches_the_rows_that_see_it(bad):
+    """In the shared part all of the group, in a sequence's own part its own rows, behind the last token of a page none."""
+    for most in (1, None):
+        batch = Shared([(256, [(1, 20), (2, 30), (1, 90)]), (128, [(1, 3), (1, 4)])], 4, 2, 64, 16)
+        clean = batch.attend(most)
+        batch.check(clean)
+        page, slot = divmod(int(batch.slots(1, torch.tensor([256 + 29]))), 16)      # the second sequence's newest token
+        batch.cache.v[page, :, slot, 5] = bad
+        got = batch.attend(most)
+        assert not got[2, :, 5].isfinite().any() and torch.equal(got[[0, 1, 3, 4, 5]], clean[[0, 1, 3, 4, 5]])
+        page, slot = divmod(int(batch.slots(0, torch.tensor([70]))), 16)
+        batch.cache.v[page, :, slot, 9] = bad
+        got = batch.attend(most)
+        assert not got[:4, :, 9].isfinite().any() and torch.equal(got[4:], clean[4:])
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("groups,most", [(DECODES, 1), (CHUNKS, None), (MANY, 1)])
+def test_scratch_and_output_of_nan(kind, groups, most):
+    """What no kernel writes, or reads without having written it, shows; twice, with the same bits."""
+    from triteia_amd.python.capi import _ffi
+    batch = Shared(groups, 8, 2, 128, 16, kind, padding=9)
+    q, cache, pages, starts, lens = batch.inputs()
+    plan = ops().attention_plan(cache, starts, lens, batch.heads, q.shape[0], most, **batch.groups())
+    sizes = (plan.n_seqs, plan.n_groups, plan.n_tokens, plan.heads, plan.kv_heads)
+    nbytes = _ffi.lib().triteia_hip_shared_scratch_bytes(*sizes, plan.max_q, cache.dim)
+    outs = []
+    for _ in range(2):
+        out, scratch = torch.full_like(q, math.nan), torch.full((nbytes,), 0xff, dtype=torch.uint8, device="cuda")
+        code = _ffi.lib().triteia_hip_shared_attention(
+            _ffi.ptr(q), q.stride(0), q.stride(1), _ffi.ptr(out), *cache._pointers(), cache._strides, cache.n_pages, cache.page, cache.kind, _ffi.ptr(pages),
+            pages.stride(0), pages.shape[1], _ffi.ptr(plan.buffer), plan.buffer.numel(), *sizes, cache.dim, plan.max_q, 1, 0, cache.dim ** -0.5, _ffi.ptr(scratch), nbytes,
+            0, _ffi.device_index(q), _ffi.stream_of(q))
+        assert code == 0, _ffi.last_error()
+        outs.append(out)
+    batch.check(outs[0])
+    assert torch.equal(*outs)
+
+
+def test_large_scores():
+    """Sums of both parts meet under one maximum, however far apart their own are."""
+    for big in (0.01, 30.0, 300.0):
+        for kind in KINDS:
+            batch = Shared([(500, [(1, 60), (1, 3), (5, 90)])], 4, 2, 64, 16, kind, torch.bfloat16, big=big)
+            batch.q = (batch.q.float() * 0.2).to(batch.dtype)
+            got = batch.attend(None)
+            want, size, _ = batch.answer()
+            exact = torch.stack([torch.ones(())])                               # (a score of 32 bits is off by 2^-24 of its terms' sum, and a weight by as much)
+            terms = (batch.q.double().abs().amax() * max(k.abs().max() for k in batch.k) * 64 * 64 ** -0.5 * 1.45) * 2.0 ** -23 * 64 * exact
+            bound = (2 * 2.0 ** -8 + 2.0 ** -13 + 2 * terms) * size + 1e-30
+            assert bool(((got.double().cpu() - want).abs() <= bound).all())
+
+
+def test_replays_and_streams():
+    """A plan and a call recorded into a graph, its lengths, groups and cache changed between replays; two graphs, and eager calls on another stream, side by side."""
+    batch = Shared(DECODES, 8, 2, 128, 16)
+    q, cache, pages, starts, lens = batch.inputs()
+    groups = batch.groups()
+
+    def call():
+        plan = ops().attention_plan(cache, starts, lens, batch.heads, q.shape[0], 1, **groups)
+        return ops().paged_attention(q, cache, pages, starts, lens, plan=plan)
+
+    want = call()
+    batch.check(want)
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    outs = []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            outs.append(call())
+    side = torch.cuda.Stream()
+    for turn, prefixes in enumerate((batch.prefix_lens, [0] * len(batch.prefix_lens), [64] * len(batch.prefix_lens), batch.prefix_lens)):
+        groups["prefix_lens"].copy_(torch.tensor([min(p, most) for p, most in zip(prefixes, batch.prefix_lens)], dtype=torch.int32))
+        q.copy_(batch.q * (turn + 1) / 4)
+        torch.cuda.synchronize()
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+            beside = call()
+        alone = call()
+        torch.cuda.synchronize()
+        assert all(torch.equal(alone, x) for x in (*outs, beside))
+        held, batch.q = batch.q, q.cpu()
+        batch.check(alone)
+        batch.q = held
+
+
+def test_refusals_and_the_python_path(monkeypatch):
+    from triteia_amd.python.capi import attention
+    batch = Shared(DECODES, 8, 2, 128, 16)
+    q, cache, pages, starts, lens = batch.inputs()
+    groups = batch.groups()
+    plan = lambda **how: ops().attention_plan(cache, starts, lens, 8, q.shape[0], 1, **{**groups, **how})  # noqa: E731
+    for how, text in ((dict(group_starts=None), "together"), (dict(prefix_lens=None), "together"), (dict(prefix_lens=groups["prefix_lens"][:-1].contiguous()), "group_starts must have"),
+                      (dict(prefix_lens=groups["prefix_lens"].long()), "int32"), (dict(group_starts=groups["group_starts"].float()), "int32"),
+                      (dict(prefix_lens=groups["prefix_lens"].cpu()), "GPU tensor"), (dict(prefix_lens=groups["prefix_lens"].repeat(2)[::2]), "contiguous"),
+                      (dict(group_starts=torch.zeros(1026, dtype=torch.int32).cuda(), prefix_lens=torch.zeros(1025, dtype=torch.int32).cuda()), "groups")):
+        with pytest.raises(RuntimeError, match=text):
+            plan(**how)
+    with pytest.raises(RuntimeError, match="causal"):
+        ops().paged_attention(q, cache, pages, starts, lens, plan=plan(), causal=False)
+    want = batch.attend(1)
+
+    class Nothing:
+        def __getattr__(self, name):
+            return lambda *args: None
+
+    assert attention.native().shared_plan(starts, lens, groups["group_starts"], groups["prefix_lens"], q.shape[0], 8, 2, 1, True, 0) is not None
+    monkeypatch.setattr(attention, "native", lambda: Nothing())
+    assert torch.equal(batch.attend(1), want)

@@ -115,6 +115,7 @@ void launch_attend(AttendArgs a, const AttnLayout& layout, float* scratch, long 
     a.part_ml[which] = scratch + (long)l.max_parts * a.kv_heads * l.rows * D;
     scratch = a.part_ml[which] + 2L * l.max_parts * a.kv_heads * l.rows;
   }
+  if (layout.n_groups > 0) joins = (int)std::min<long>(kAttnJoiners, ((long)a.list[0].max_joins * a.list[0].rows + (long)a.list[1].max_joins * a.list[1].rows) / (1024 / D) * a.kv_heads);
   a.joined = joins > 0;
   const dim3 grid((unsigned)((long)(a.list[0].max_items + a.list[1].max_items) * a.kv_heads));
   if (a.list[1].max_items > 0) hipLaunchKernelGGL((attend_mixed_kernel<T, KIND, D>), grid, dim3(256), 0, stream, a);
@@ -122,7 +123,9 @@ void launch_attend(AttendArgs a, const AttnLayout& layout, float* scratch, long 
   else if (a.list[0].rows == 16) hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 1, 4>), grid, dim3(256), 0, stream, a);
   else if (a.list[0].waves == 8) hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 2, 8>), grid, dim3(512), 0, stream, a);
   else hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 2, 4>), grid, dim3(256), 0, stream, a);
-  if (joins > 0) hipLaunchKernelGGL((attend_join_kernel<T, D>), dim3(joins < kAttnJoiners ? joins : kAttnJoiners), dim3(256), 0, stream, a);
+  const dim3 joiners(joins < kAttnJoiners ? joins : kAttnJoiners);
+  if (layout.n_groups > 0) hipLaunchKernelGGL((attend_join_kernel<T, D, true>), joiners, dim3(256), 0, stream, a);
+  else if (joins > 0) hipLaunchKernelGGL((attend_join_kernel<T, D, false>), joiners, dim3(256), 0, stream, a);
 }
 struct AttendLaunch {
   const AttendArgs& a;
@@ -137,19 +140,89 @@ struct AttendLaunch {
   }
 };
 
-int check_batch(const char* what, int n_seqs, int n_tokens, int heads, int kv_heads, int max_q, int causal, int window) {
+int check_batch(const char* what, int n_seqs, int n_tokens, int heads, int kv_heads, int max_q, int causal, int window, int n_groups = 0) {
   if (n_seqs < 0 || n_seqs > kAttnMaxSeqs || n_tokens < 0 || n_tokens > (1 << 24) || max_q < 0 || window < 0)
     return fail(TRITEIA_HIP_ERR_PROB_SHAPE, "%s: %d sequences, %d tokens, at most %d of one, window %d: up to %d sequences and 2^24 tokens", what, n_seqs, n_tokens, max_q,
                 window, kAttnMaxSeqs);
+  if (n_groups < 0 || n_groups > kAttnMaxGroups || n_seqs > kAttnMaxSeqs - n_groups)
+    return fail(TRITEIA_HIP_ERR_PROB_SHAPE, "%s: %d sequences in %d groups: up to %d groups, and %d sequences and groups together", what, n_seqs, n_groups, kAttnMaxGroups,
+                kAttnMaxSeqs);
   if (heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || heads > 1024)
     return fail(TRITEIA_HIP_ERR_PROB_SHAPE, "%s: %d heads over %d heads of the cache: a multiple, up to 1024", what, heads, kv_heads);
   if ((long)n_tokens * (heads / kv_heads) > (1L << 30)) return fail(TRITEIA_HIP_ERR_PROB_SHAPE, "%s: %d tokens of %d heads are too many", what, n_tokens, heads);
   if (window > 0 && !causal) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: a window needs causal", what);
-  const AttnLayout l = attn_layout(n_seqs, n_tokens, heads, kv_heads, max_q, causal, window);
+  const AttnLayout l = attn_layout(n_seqs, n_tokens, heads, kv_heads, max_q, causal, window, n_groups);
   for (const AttnList& x : l.list)
     if ((long)x.max_items * kv_heads > 0x3fffffffL || x.max_items < 0)
       return fail(TRITEIA_HIP_ERR_PROB_SHAPE, "%s: too many tiles", what);
   return TRITEIA_HIP_OK;
+}
+
+size_t attention_plan_bytes(int n_seqs, int n_groups, int n_tokens, int heads, int kv_heads, int max_q) {
+  if (check_batch("attention_plan", n_seqs, n_tokens, heads, kv_heads, max_q, 1, 0, n_groups)) return 0;
+  return 4 * (size_t)attn_layout(n_seqs, n_tokens, heads, kv_heads, max_q, 1, 0, n_groups).ints;
+}
+
+size_t attention_scratch_bytes(int n_seqs, int n_groups, int n_tokens, int heads, int kv_heads, int max_q, int dim) {
+  if (check_batch("paged_attention", n_seqs, n_tokens, heads, kv_heads, max_q, 1, 0, n_groups)) return 0;
+  const AttnLayout l = attn_layout(n_seqs, n_tokens, heads, kv_heads, max_q, 1, 0, n_groups);
+  size_t bytes = 0;
+  for (const AttnList& x : l.list) bytes += 4 * (size_t)x.max_parts * kv_heads * x.rows * (dim + 2);
+  return bytes;
+}
+
+int attention_plan(const void* q_starts, const void* kv_lens, const void* group_starts, const void* prefix_lens, int n_seqs, int n_groups, int n_tokens, int heads,
+                   int kv_heads, int max_q, int causal, int window, void* plan, size_t plan_bytes, int dev, void* stream) {
+  if (const int e = check_batch("attention_plan", n_seqs, n_tokens, heads, kv_heads, max_q, causal, window, n_groups)) return e;
+  if (n_tokens == 0) return TRITEIA_HIP_OK;
+  const AttnLayout l = attn_layout(n_seqs, n_tokens, heads, kv_heads, max_q, causal, window, n_groups);
+  if (!q_starts || (n_seqs && !kv_lens) || !plan || (n_groups && (!group_starts || !prefix_lens))) return fail(TRITEIA_HIP_ERR_ARGUMENT, "attention_plan: null tensor pointer");
+  if (plan_bytes < 4 * (size_t)l.ints || !aligned16(plan))
+    return fail(TRITEIA_HIP_ERR_ARGUMENT, "attention_plan: a plan of %zu bytes, 16-byte aligned, is needed, got %zu", 4 * (size_t)l.ints, plan_bytes);
+  DeviceGuard g(dev);
+  if (!g.ok) return fail(TRITEIA_HIP_ERR_RUNTIME, "cannot select device %d", dev);
+  const auto kernel = n_groups > 0 ? attention_plan_kernel<true> : attention_plan_kernel<false>;
+  hipLaunchKernelGGL(kernel, dim3(1), dim3(kAttnPlanThreads), 0, static_cast<hipStream_t>(stream), static_cast<const int*>(q_starts), static_cast<const int*>(kv_lens),
+                     static_cast<const int*>(group_starts), static_cast<const int*>(prefix_lens), l, static_cast<int*>(plan));
+  return check_launch("attention_plan_kernel");
+}
+
+int paged_attention(const void* q, long q_token, long q_head, void* out, const void* cache_k, const void* cache_v, const void* k_scale, const void* v_scale, const long* strides, int n_pages, int page, int kind, const void* pages, long pages_seq, int table_width, const void* plan,
+                    size_t plan_bytes, int n_seqs, int n_groups, int n_tokens, int heads, int kv_heads, int dim, int max_q, int causal, int window, float scale,
+                    void* scratch, size_t scratch_bytes, int bf16, int dev, void* stream) {
+  const char* what = "paged_attention";
+  if (const int e = check_batch(what, n_seqs, n_tokens, heads, kv_heads, max_q, causal, window, n_groups)) return e;
+  if (dim != 64 && dim != 128) return fail(TRITEIA_HIP_ERR_KERN_SHAPE, "%s: heads of %d elements: 64 or 128", what, dim);
+  if (!(scale > 0.f) || !(scale < 1e30f)) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: a scale of %g: a positive number", what, (double)scale);
+  if (!strides) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: null strides", what);
+  AttendArgs a = {};
+  a.ck = cache_part(cache_k, k_scale, strides, strides + 6);
+  a.cv = cache_part(cache_v, v_scale, strides + 3, strides + 9);
+  if (const int e = check_cache(what, a.ck, a.cv, n_pages, kv_heads, page, dim, kind)) return e;
+  const long size = kind == kCacheSame ? 2 : 1;
+  for (const CachePart* p : {&a.ck, &a.cv}) {
+    if (!strides_ok({p->page, p->head, p->slot}, size, 16)) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: a cache's rows need 16-byte alignment", what);
+    if (p->slot * size > (1L << 25)) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: rows of a page %ld elements apart are too far", what, p->slot);
+    if (kind != kCacheSame && (!aligned16(p->scale) || p->scale_slot != 1 || !strides_ok({p->scale_page, p->scale_head}, 4, 16)))
+      return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: a page's scales of one head have to be adjacent and 16-byte aligned", what);
+  }
+  if (n_tokens == 0) return TRITEIA_HIP_OK;
+  const AttnLayout l = attn_layout(n_seqs, n_tokens, heads, kv_heads, max_q, causal, window, n_groups);
+  if (n_seqs > 0 && (table_width < 1 || !pages)) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: a table of pages with a column at least", what);
+  if (!q || !out || !plan || !scratch) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: null tensor pointer", what);
+  if (!aligned16(q) || !aligned16(out) || !aligned16(plan) || !aligned16(scratch) || !strides_ok({q_token, q_head}, 2, 16))
+    return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: queries, output, plan and scratch need 16-byte alignment", what);
+  if (plan_bytes < 4 * (size_t)l.ints || scratch_bytes < attention_scratch_bytes(n_seqs, n_groups, n_tokens, heads, kv_heads, max_q, dim))
+    return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: plan or scratch too small", what);
+  a.q = q, a.q_token = q_token, a.q_head = q_head, a.out = out;
+  a.pages = static_cast<const int*>(pages), a.pages_seq = pages_seq, a.n_pages = n_pages, a.table_width = table_width, a.page_shift = page_shift_of(page);
+  a.held = (long)table_width * page < kAttnMaxTokens ? table_width * page : kAttnMaxTokens;
+  a.group = heads / kv_heads, a.kv_heads = kv_heads, a.causal = causal, a.window = window, a.scale_log2 = scale * 1.44269504088896340736f;
+  a.plan = static_cast<const int*>(plan);
+  DeviceGuard g(dev);
+  if (!g.ok) return fail(TRITEIA_HIP_ERR_RUNTIME, "cannot select device %d", dev);
+  by_types(bf16, kind, AttendLaunch{a, l, static_cast<float*>(scratch), (long)table_width * page, dim, static_cast<hipStream_t>(stream)});
+  return check_launch("paged attention");
 }
 
 }  // namespace
@@ -212,70 +285,45 @@ int triteia_hip_cache_read(const void* cache_k, const void* cache_v, const void*
 }
 
 size_t triteia_hip_attention_plan_bytes(int n_seqs, int n_tokens, int heads, int kv_heads, int max_q) {
-  if (check_batch("attention_plan", n_seqs, n_tokens, heads, kv_heads, max_q, 1, 0)) return 0;
-  return 4 * (size_t)attn_layout(n_seqs, n_tokens, heads, kv_heads, max_q, 1, 0).ints;
+  return attention_plan_bytes(n_seqs, 0, n_tokens, heads, kv_heads, max_q);
 }
 
 size_t triteia_hip_attention_scratch_bytes(int n_seqs, int n_tokens, int heads, int kv_heads, int max_q, int dim) {
-  if (check_batch("paged_attention", n_seqs, n_tokens, heads, kv_heads, max_q, 1, 0)) return 0;
-  const AttnLayout l = attn_layout(n_seqs, n_tokens, heads, kv_heads, max_q, 1, 0);
-  size_t bytes = 0;
-  for (const AttnList& x : l.list) bytes += 4 * (size_t)x.max_parts * kv_heads * x.rows * (dim + 2);
-  return bytes;
+  return attention_scratch_bytes(n_seqs, 0, n_tokens, heads, kv_heads, max_q, dim);
 }
 
 int triteia_hip_attention_plan(const void* q_starts, const void* kv_lens, int n_seqs, int n_tokens, int heads, int kv_heads, int max_q, int causal, int window,
                                void* plan, size_t plan_bytes, int dev, void* stream) {
-  if (const int e = check_batch("attention_plan", n_seqs, n_tokens, heads, kv_heads, max_q, causal, window)) return e;
-  if (n_tokens == 0) return TRITEIA_HIP_OK;
-  const AttnLayout l = attn_layout(n_seqs, n_tokens, heads, kv_heads, max_q, causal, window);
-  if (!q_starts || (n_seqs && !kv_lens) || !plan) return fail(TRITEIA_HIP_ERR_ARGUMENT, "attention_plan: null tensor pointer");
-  if (plan_bytes < 4 * (size_t)l.ints || !aligned16(plan))
-    return fail(TRITEIA_HIP_ERR_ARGUMENT, "attention_plan: a plan of %zu bytes, 16-byte aligned, is needed, got %zu", 4 * (size_t)l.ints, plan_bytes);
-  DeviceGuard g(dev);
-  if (!g.ok) return fail(TRITEIA_HIP_ERR_RUNTIME, "cannot select device %d", dev);
-  hipLaunchKernelGGL(attention_plan_kernel, dim3(1), dim3(kAttnPlanThreads), 0, static_cast<hipStream_t>(stream), static_cast<const int*>(q_starts),
-                     static_cast<const int*>(kv_lens), l, static_cast<int*>(plan));
-  return check_launch("attention_plan_kernel");
+  return attention_plan(q_starts, kv_lens, nullptr, nullptr, n_seqs, 0, n_tokens, heads, kv_heads, max_q, causal, window, plan, plan_bytes, dev, stream);
 }
 
 int triteia_hip_paged_attention(const void* q, long q_token, long q_head, void* out, const void* cache_k, const void* cache_v, const void* k_scale, const void* v_scale,
                                 const long* strides, int n_pages, int page, int kind, const void* pages, long pages_seq, int table_width, const void* plan,
                                 size_t plan_bytes, int n_seqs, int n_tokens, int heads, int kv_heads, int dim, int max_q, int causal, int window, float scale,
                                 void* scratch, size_t scratch_bytes, int bf16, int dev, void* stream) {
-  const char* what = "paged_attention";
-  if (const int e = check_batch(what, n_seqs, n_tokens, heads, kv_heads, max_q, causal, window)) return e;
-  if (dim != 64 && dim != 128) return fail(TRITEIA_HIP_ERR_KERN_SHAPE, "%s: heads of %d elements: 64 or 128", what, dim);
-  if (!(scale > 0.f) || !(scale < 1e30f)) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: a scale of %g: a positive number", what, (double)scale);
-  if (!strides) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: null strides", what);
-  AttendArgs a = {};
-  a.ck = cache_part(cache_k, k_scale, strides, strides + 6);
-  a.cv = cache_part(cache_v, v_scale, strides + 3, strides + 9);
-  if (const int e = check_cache(what, a.ck, a.cv, n_pages, kv_heads, page, dim, kind)) return e;
-  const long size = kind == kCacheSame ? 2 : 1;
-  for (const CachePart* p : {&a.ck, &a.cv}) {
-    if (!strides_ok({p->page, p->head, p->slot}, size, 16)) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: a cache's rows need 16-byte alignment", what);
-    if (p->slot * size > (1L << 25)) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: rows of a page %ld elements apart are too far", what, p->slot);
-    if (kind != kCacheSame && (!aligned16(p->scale) || p->scale_slot != 1 || !strides_ok({p->scale_page, p->scale_head}, 4, 16)))
-      return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: a page's scales of one head have to be adjacent and 16-byte aligned", what);
-  }
-  if (n_tokens == 0) return TRITEIA_HIP_OK;
-  const AttnLayout l = attn_layout(n_seqs, n_tokens, heads, kv_heads, max_q, causal, window);
-  if (n_seqs > 0 && (table_width < 1 || !pages)) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: a table of pages with a column at least", what);
-  if (!q || !out || !plan || !scratch) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: null tensor pointer", what);
-  if (!aligned16(q) || !aligned16(out) || !aligned16(plan) || !aligned16(scratch) || !strides_ok({q_token, q_head}, 2, 16))
-    return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: queries, output, plan and scratch need 16-byte alignment", what);
-  if (plan_bytes < 4 * (size_t)l.ints || scratch_bytes < triteia_hip_attention_scratch_bytes(n_seqs, n_tokens, heads, kv_heads, max_q, dim))
-    return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: plan or scratch too small", what);
-  a.q = q, a.q_token = q_token, a.q_head = q_head, a.out = out;
-  a.pages = static_cast<const int*>(pages), a.pages_seq = pages_seq, a.n_pages = n_pages, a.table_width = table_width, a.page_shift = page_shift_of(page);
-  a.held = (long)table_width * page < kAttnMaxTokens ? table_width * page : kAttnMaxTokens;
-  a.group = heads / kv_heads, a.kv_heads = kv_heads, a.causal = causal, a.window = window, a.scale_log2 = scale * 1.44269504088896340736f;
-  a.plan = static_cast<const int*>(plan);
-  DeviceGuard g(dev);
-  if (!g.ok) return fail(TRITEIA_HIP_ERR_RUNTIME, "cannot select device %d", dev);
-  by_types(bf16, kind, AttendLaunch{a, l, static_cast<float*>(scratch), (long)table_width * page, dim, static_cast<hipStream_t>(stream)});
-  return check_launch("paged attention");
+  return paged_attention(q, q_token, q_head, out, cache_k, cache_v, k_scale, v_scale, strides, n_pages, page, kind, pages, pages_seq, table_width, plan, plan_bytes,
+                         n_seqs, 0, n_tokens, heads, kv_heads, dim, max_q, causal, window, scale, scratch, scratch_bytes, bf16, dev, stream);
+}
+
+size_t triteia_hip_shared_plan_bytes(int n_seqs, int n_groups, int n_tokens, int heads, int kv_heads, int max_q) {
+  return attention_plan_bytes(n_seqs, n_groups, n_tokens, heads, kv_heads, max_q);
+}
+
+size_t triteia_hip_shared_scratch_bytes(int n_seqs, int n_groups, int n_tokens, int heads, int kv_heads, int max_q, int dim) {
+  return attention_scratch_bytes(n_seqs, n_groups, n_tokens, heads, kv_heads, max_q, dim);
+}
+
+int triteia_hip_shared_plan(const void* q_starts, const void* kv_lens, const void* group_starts, const void* prefix_lens, int n_seqs, int n_groups, int n_tokens,
+                            int heads, int kv_heads, int max_q, int causal, int window, void* plan, size_t plan_bytes, int dev, void* stream) {
+  return attention_plan(q_starts, kv_lens, group_starts, prefix_lens, n_seqs, n_groups, n_tokens, heads, kv_heads, max_q, causal, window, plan, plan_bytes, dev, stream);
+}
+
+int triteia_hip_shared_attention(const void* q, long q_token, long q_head, void* out, const void* cache_k, const void* cache_v, const void* k_scale, const void* v_scale,
+                                 const long* strides, int n_pages, int page, int kind, const void* pages, long pages_seq, int table_width, const void* plan,
+                                 size_t plan_bytes, int n_seqs, int n_groups, int n_tokens, int heads, int kv_heads, int dim, int max_q, int causal, int window,
+                                 float scale, void* scratch, size_t scratch_bytes, int bf16, int dev, void* stream) {
+  return paged_attention(q, q_token, q_head, out, cache_k, cache_v, k_scale, v_scale, strides, n_pages, page, kind, pages, pages_seq, table_width, plan, plan_bytes,
+                         n_seqs, n_groups, n_tokens, heads, kv_heads, dim, max_q, causal, window, scale, scratch, scratch_bytes, bf16, dev, stream);
 }
 
 }  // extern "C"

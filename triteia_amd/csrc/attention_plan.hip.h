@@ -9,6 +9,11 @@
 // One workgroup of two wavefronts, a list each, so that nothing but the sequences' lengths in LDS is waited for: sums over the lanes, a lane finds the
 // sequence of a tile by a binary search.  Tokens behind the last sequence get tiles without keys, whose rows are zeros.  Every number read from the
 // device is clamped and offsets that do not ascend are made to, so that every row has one tile and no list passes its end.
+//
+// Sequences in groups that share their first tokens (SHARED): group g is sequences group_starts[g] .. group_starts[g + 1] - 1, whose tables begin with the
+// same pages.  Of prefix_lens[g] tokens, those that every row of the group sees, in whole blocks, are attended to once: by one more sequence, whose rows are the
+// new tokens of all of the group and whose context is the prefix, without a mask.  The group's own sequences begin behind it.  Each of their tiles is joined
+// from its own shares and the shares of the prefix's tiles that hold its rows.
 // Bound by latency: 6.4 us for one sequence, 8.2 for a step's 26 of which two are long (14.2 with 1024 threads on one list after the other, whose barriers
 // and shuffles were the time), 10.9 for 64, 15.7 for four prompts of 500 tokens and 64 heads over 8 (108 tiles), all of which are also put in order.
 #pragma once
@@ -21,6 +26,7 @@ constexpr int kAttnTileRows = 128;     // rows of a tile of the long list
 constexpr int kAttnWaves = 8;          // at most, of a workgroup with few rows
 constexpr int kAttnSorted = 256;       // lists of up to this many tiles begin with the longest
 constexpr int kAttnMaxSeqs = 4096;
+constexpr int kAttnMaxGroups = 1024;
 constexpr int kAttnMaxTokens = 0x7fffff80;   // a longer context is taken as this long, so that the end of its last block is still an int
 constexpr int kAttnPlanThreads = 128;
 
@@ -28,9 +34,9 @@ constexpr int kAttnPlanThreads = 128;
 struct AttnItem {
   int seq, q_start, n_tokens, kv_len, tile, kv_begin, kv_end, part;   // part: of the scratch, -1: the whole tile
 };
-// A tile of several shares.
+// A tile of several shares, or of a group: the list of the group's prefix (-1: none), the prefix's first tile there and its row of the tile's sequence's first.
 struct AttnJoin {
-  int q_start, n_tokens, tile, first, n_parts, unused[3];
+  int q_start, n_tokens, tile, first, n_parts, prefix_list, prefix_tile, prefix_row;
 };
 
 struct AttnList {
@@ -41,22 +47,25 @@ struct AttnList {
   int waves;             // of a workgroup
   int rounds;            // lists of this many rounds of workgroups and more are not cut
   int max_parts;
+  long prefixes;         // of each tile, its first share and their number (groups only)
 };
 
 struct AttnLayout {
-  int n_seqs, n_tokens, group, kv_heads, causal, window;
+  int n_seqs, n_tokens, group, kv_heads, causal, window, n_groups;
   int short_rows;        // sequences of more rows go to the long list; 0x7fffffff: there is none
   AttnList list[2];      // short, long
   long ints;
 };
 
 // Everything that the host knows of a plan.
-inline AttnLayout attn_layout(int n_seqs, int n_tokens, int heads, int kv_heads, int max_q, int causal, int window) {
+inline AttnLayout attn_layout(int n_seqs, int n_tokens, int heads, int kv_heads, int max_q, int causal, int window, int n_groups = 0) {
   AttnLayout a = {};
-  a.n_seqs = n_seqs, a.n_tokens = n_tokens, a.group = heads / kv_heads, a.kv_heads = kv_heads, a.causal = causal, a.window = window;
+  a.n_seqs = n_seqs, a.n_tokens = n_tokens, a.group = heads / kv_heads, a.kv_heads = kv_heads, a.causal = causal, a.window = window, a.n_groups = n_groups;
   const long rows = (long)n_tokens * a.group, most = (long)(max_q < n_tokens ? max_q : n_tokens) * a.group;
   const long live = n_seqs + 1 < n_tokens ? n_seqs + 1 : n_tokens;      // sequences with tokens, and the tokens behind them
-  const bool only_short = most <= 32;
+  // (a group that shares has two sequences with tokens at least; its prefix has the rows of all of them)
+  const long pairs = (n_seqs < n_tokens ? n_seqs : n_tokens) / 2, sharing = n_groups < pairs ? n_groups : pairs;
+  const bool only_short = most <= 32 && (sharing == 0 || rows <= 32);
   AttnList &s = a.list[0], &l = a.list[1];
   s.rows = only_short && most > 16 ? 32 : 16;
   a.short_rows = only_short ? 0x7fffffff : a.group <= 16 ? 16 : 0;       // (one token's heads fill more than a tile of 16: a long sequence)
@@ -64,7 +73,14 @@ inline AttnLayout attn_layout(int n_seqs, int n_tokens, int heads, int kv_heads,
   // tokens on up to 2000, in e4m3, 59.5 / 49.2 / 62.7 us with 256 / 512 / 768; 3 of 100 on 3000 58.1 / 58.3 / 63.3, 8 of 300 on 300 36.1 / 21.4 / 21.5).
   s.min_blocks = 16, s.rounds = 4, l.slots = 512, l.min_blocks = 8, l.rounds = 2;
   l.rows = kAttnTileRows;
-  const long tiles[2] = {only_short ? live + rows / s.rows : a.short_rows ? live : 0, only_short ? 0 : live + rows / l.rows};
+  long tiles[2] = {only_short ? live + rows / s.rows : a.short_rows ? live : 0, only_short ? 0 : live + rows / l.rows};
+  if (sharing > 0) {
+    if (only_short || a.short_rows) tiles[0] += sharing + (only_short ? rows / s.rows : 0);
+    if (!only_short) {
+      const long most_long = rows / (a.short_rows + 1);  // sequences of the long list
+      tiles[1] = (live < most_long ? live : most_long) + rows / l.rows + sharing + rows / l.rows;
+    }
+  }
   // Up to 128 workgroups with short rows: eight wavefronts, one a CU, so that a context is walked fast.  More: four, two a CU, one beginning or
   // ending while the other streams.  (us, eight / four: 32 of 500 tokens 8.0 / 8.7, 24 of 100000 cut into 256 / 512 215 / 220, 192 of up to 2000 in
   // e4m3 22.9 / 21.0, 2048 of up to 1000 112 / 100 and 81 / 58, 1280 of 34 21.5 / 13.2, 2048 of up to 4096 395 / 390.)
@@ -78,11 +94,13 @@ inline AttnLayout attn_layout(int n_seqs, int n_tokens, int heads, int kv_heads,
     x.max_joins = (int)(tiles[which] < shares / 2 ? tiles[which] : shares / 2);
     x.max_parts = (int)(tiles[which] > 0 ? shares : 0);
     x.max_items = (int)(tiles[which] > shares ? tiles[which] : shares);
+    if (n_groups > 0) x.max_joins = (int)tiles[which], x.max_parts = x.max_items;      // (a group's tiles are shares, cut or not)
   }
   long at = 8;
   for (AttnList& x : a.list) {
     x.items = at, at += 8L * x.max_items;
     x.joins = at, at += 8L * x.max_joins;
+    if (n_groups > 0) x.prefixes = at, at += 2L * x.max_joins;
   }
   a.ints = at;
   return a;
@@ -96,7 +114,7 @@ __device__ __forceinline__ int attn_scan(int v, int* total) {
 }
 
 struct AttnSeq {
-  int start, n, kv;
+  int start, n, kv, from;                                // from: where its own part of the context begins, a whole number of blocks
 };
 // the tokens of the cache that some row of a tile sees, its beginning on a whole block
 __device__ __forceinline__ void attn_range(const AttnSeq& s, int tile, int rows, const AttnLayout& a, int* lo, int* hi) {
@@ -104,16 +122,27 @@ __device__ __forceinline__ void attn_range(const AttnSeq& s, int tile, int rows,
   const int t0 = (int)(row / (uint32_t)a.group), t1 = min(s.n - 1, (int)((row + rows - 1) / (uint32_t)a.group));
   const long before = (long)s.kv - s.n;
   *hi = a.causal ? (int)max(0L, before + t1 + 1) : s.kv;
-  *lo = a.window > 0 ? (int)max(0L, before + t0 - a.window + 1) / kAttnBlock * kAttnBlock : 0;
+  *lo = a.window > 0 ? (int)max(0L, before + t0 - a.window + 1) / kAttnBlock * kAttnBlock : s.from;
   *lo = min(*lo, *hi / kAttnBlock * kAttnBlock);
 }
 
+// What is known of groups, in LDS.  Of the sequences behind n_seqs, n_seqs + 1 + g is the prefix of group g.
+template <bool SHARED>
+struct AttnGroups {
+  static constexpr int kSize = SHARED ? kAttnMaxGroups + 1 : 1;
+  int start[kSize], first[kSize], least[kSize], live[kSize];
+  int home[SHARED ? kAttnMaxSeqs : 1];                   // a sequence's group, -1: none
+};
+
 // grid 1, block kAttnPlanThreads
-__global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const int* q_starts, const int* kv_lens, AttnLayout a, int* plan) {
+template <bool SHARED>
+__global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const int* q_starts, const int* kv_lens, const int* group_starts, const int* prefix_lens,
+                                                                          AttnLayout a, int* plan) {
   __shared__ int start[kAttnMaxSeqs + 1], count[kAttnMaxSeqs + 1], context[kAttnMaxSeqs + 1];
   __shared__ int tiles_ahead[2][kAttnMaxSeqs + 1];       // of each sequence, in each list
   __shared__ int order[2][kAttnSorted];
   __shared__ int crossed[kAttnPlanThreads / 64];
+  __shared__ AttnGroups<SHARED> groups;
   bool back = false;                                     // an offset below the one ahead of it
   for (int b = threadIdx.x; b <= a.n_seqs; b += kAttnPlanThreads) {
     const bool rest = b == a.n_seqs;
@@ -137,42 +166,95 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const 
     }
     __syncthreads();
   }
+  const int last = SHARED ? a.n_seqs + a.n_groups : a.n_seqs;      // of the sequences, the tokens behind them and the prefixes among them
+  if constexpr (SHARED) {
+    bool unordered = false;
+    for (int g = threadIdx.x; g <= a.n_groups; g += kAttnPlanThreads) {
+      const int at = max(0, min(group_starts[g], a.n_seqs));
+      groups.start[g] = at, groups.least[g] = 0x7e000000, groups.live[g] = 0, groups.first[g] = 0x7fffffff;
+      if (g > 0) unordered |= at < max(0, min(group_starts[g - 1], a.n_seqs));
+    }
+    const bool any_unordered = __any(unordered);
+    __syncthreads();                                     // (`crossed` has been read)
+    if ((threadIdx.x & 63) == 0) crossed[threadIdx.x >> 6] = any_unordered;
+    __syncthreads();
+    if ((crossed[0] | crossed[kAttnPlanThreads / 64 - 1]) != 0) {
+      if (threadIdx.x == 0)
+        for (int g = 1; g <= a.n_groups; g++) groups.start[g] = max(groups.start[g], groups.start[g - 1]);
+      __syncthreads();
+    }
+    for (int b = threadIdx.x; b < a.n_seqs; b += kAttnPlanThreads) {
+      int lo = -1, hi = a.n_groups;                      // the last group that starts at or ahead of sequence b
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (groups.start[mid] <= b) lo = mid; else hi = mid - 1;
+      }
+      if (lo == a.n_groups) lo = -1;                     // behind the last
+      groups.home[b] = lo;
+      if (lo >= 0 && count[b] > 0) {
+        atomicMin(&groups.least[lo], a.causal ? context[b] - count[b] : context[b]);
+        atomicMin(&groups.first[lo], b);
+        atomicAdd(&groups.live[lo], 1);
+      }
+    }
+    __syncthreads();
+    for (int g = threadIdx.x; g < a.n_groups; g += kAttnPlanThreads) {
+      // (a window hides of the prefix from each row what it hides; nothing is shared then)
+      int prefix = groups.live[g] < 2 || a.window > 0 ? 0 : min(prefix_lens[g], groups.least[g]);
+      prefix = max(prefix, 0) / kAttnBlock * kAttnBlock;
+      const int b = a.n_seqs + 1 + g, from = start[groups.start[g]];
+      start[b] = from, count[b] = prefix > 0 ? start[groups.start[g + 1]] - from : 0, context[b] = prefix;
+    }
+    __syncthreads();
+  }
   const int which = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const AttnList& l = a.list[which];
   if (l.max_items == 0) {
     if (lane < 2) plan[2 * which + lane] = 0;
+    if constexpr (SHARED) __syncthreads();
     return;
   }
   int* ahead = tiles_ahead[which];
   int tiles = 0;
-  for (int b0 = 0; b0 <= a.n_seqs; b0 += 64) {
+  for (int b0 = 0; b0 <= last; b0 += 64) {
     const int b = b0 + lane;
     int mine = 0;
-    if (b <= a.n_seqs) {
+    if (b <= last) {
       const long rows = (long)count[b] * a.group;
       if (rows > 0 && (rows <= a.short_rows) == (which == 0)) mine = (int)((rows + l.rows - 1) / l.rows);
     }
     int all;
     const int before = attn_scan(mine, &all);
-    if (b <= a.n_seqs) ahead[b] = tiles + before;
+    if (b <= last) ahead[b] = tiles + before;
     tiles += all;
   }
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");        // (the wavefront's own list: its lanes run together)
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+  if constexpr (SHARED) __syncthreads();                         // (a tile's prefix may be in the other list)
   struct Tile {
-    int seq, tile, lo, hi, blocks;
+    int seq, tile, lo, hi, blocks, home;                         // home: the sequence that is its prefix, -1: none, -2: a prefix itself
     AttnSeq s;
   };
   auto at = [&](int i) {
-    int lo = 0, hi = a.n_seqs;                                   // the last sequence that starts at or ahead of tile i
+    int lo = 0, hi = last;                                       // the last sequence that starts at or ahead of tile i
     while (lo < hi) {
       const int mid = (lo + hi + 1) / 2;
       if (ahead[mid] <= i) lo = mid; else hi = mid - 1;
     }
     Tile t;
-    t.seq = lo, t.tile = i - ahead[lo], t.s = {start[lo], count[lo], context[lo]};
-    attn_range(t.s, t.tile, l.rows, a, &t.lo, &t.hi);
+    t.seq = lo, t.tile = i - ahead[lo], t.s = {start[lo], count[lo], context[lo], 0};
+    if (SHARED && lo > a.n_seqs) {
+      t.seq = groups.first[lo - a.n_seqs - 1], t.s.kv += t.s.n;  // (as if the new tokens came behind it: all of them see all of it)
+      t.lo = 0, t.hi = context[lo], t.home = -2;
+    } else {
+      t.home = -1;
+      if (SHARED && lo < a.n_seqs && groups.home[lo] >= 0 && context[a.n_seqs + 1 + groups.home[lo]] > 0) {
+        t.home = a.n_seqs + 1 + groups.home[lo];
+        t.s.from = context[t.home];
+      }
+      attn_range(t.s, t.tile, l.rows, a, &t.lo, &t.hi);
+    }
     t.blocks = (t.hi - t.lo + kAttnBlock - 1) / kAttnBlock;
     return t;
   };
@@ -222,6 +304,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const 
     const int i = i0 + lane >= tiles ? -1 : tiles <= kAttnSorted ? order[which][i0 + lane] : tiles - 1 - (i0 + lane);
     int splits = 0, per = 0;
     Tile t = {};
+    t.home = -1;
     if (i >= 0) {
       t = at(i);
       splits = max(1, (int)(((long)t.blocks + share - 1) / share));
@@ -230,16 +313,24 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const 
     }
     int all_items, all_joins, all_parts;
     const int item = n_items + attn_scan(splits, &all_items);
-    const int join = n_joins + attn_scan(splits > 1, &all_joins);
-    const int part = n_parts + attn_scan(splits > 1 ? splits : 0, &all_parts);
-    if (i >= 0 && (item + splits > l.max_items || (splits > 1 && join >= l.max_joins))) {
+    const bool cut = splits > 1 || (SHARED && i >= 0 && t.home != -1), joins = cut && t.home != -2;
+    const int join = n_joins + attn_scan(joins, &all_joins);
+    const int part = n_parts + attn_scan(cut ? splits : 0, &all_parts);
+    if (i >= 0 && (item + splits > l.max_items || (joins && join >= l.max_joins))) {
       end_items = min(end_items, item), end_joins = min(end_joins, join);
     } else if (i >= 0) {
       AttnItem* out = reinterpret_cast<AttnItem*>(plan + l.items) + item;
       for (int p = 0; p < splits; p++)
         out[p] = AttnItem{t.seq, t.s.start, t.s.n, t.s.kv, t.tile, t.lo + p * per * kAttnBlock, splits == 1 ? t.hi : min(t.hi, t.lo + (p + 1) * per * kAttnBlock),
-                          splits == 1 ? -1 : part + p};
-      if (splits > 1) reinterpret_cast<AttnJoin*>(plan + l.joins)[join] = AttnJoin{t.s.start, t.s.n, t.tile, part, splits, {0, 0, 0}};
+                          cut ? part + p : -1};
+      AttnJoin j = {t.s.start, t.s.n, t.tile, part, splits, -1, 0, 0};
+      if (SHARED && t.home > 0) {
+        const long rows = (long)count[t.home] * a.group;
+        j.prefix_list = rows <= a.short_rows ? 0 : 1;
+        j.prefix_tile = tiles_ahead[j.prefix_list][t.home], j.prefix_row = (t.s.start - start[t.home]) * a.group;
+      }
+      if (joins) reinterpret_cast<AttnJoin*>(plan + l.joins)[join] = j;
+      if (SHARED && t.home == -2) plan[l.prefixes + 2L * i] = part, plan[l.prefixes + 2L * i + 1] = splits;
     }
     n_items += all_items, n_joins += all_joins, n_parts += all_parts;
   }

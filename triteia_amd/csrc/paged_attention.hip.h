@@ -902,8 +902,9 @@ __global__ __launch_bounds__(256, 2) void attend_mixed_kernel(AttendArgs a) {
 // between them, the shares: a group adds every n-th share, the groups' sums are added in their order.  The host knows bounds only, mostly far above
 // what there is to join, so a fixed number of workgroups walks what the plan says: one for every place of the bound took 10 to 15 us of a prompt's 180 to
 // 370 to find that nothing was cut.  grid up to kAttnJoiners, block 256
+// SHARED: a tile of a group has the shares of its group's prefix behind its own, in the place of the prefix's tiles that its rows have there.
 constexpr int kAttnJoiners = 1024;
-template <class T, int D>
+template <class T, int D, bool SHARED>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
   __shared__ attn_f4 sums[256];
@@ -914,7 +915,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
     const int which = next < short_units ? 0 : 1, unit = next - (which ? short_units : 0);
     const int rows = a.list[which].rows, pieces = rows / kGroups, piece = unit % pieces, index = unit / pieces / a.kv_heads, head = unit / pieces - index * a.kv_heads;
     const int* j = a.plan + a.list[which].joins + 8L * index;
-    const int q_start = j[0], n_tokens = j[1], tile = j[2], first = j[3], n_parts = j[4];
+    const int q_start = j[0], n_tokens = j[1], tile = j[2], first = j[3], n_own = j[4];
     const int r0 = kGroups * piece, live = min(kGroups, n_tokens * a.group - tile * rows - r0);
     if (live <= 0) continue;
     const float *part_o = a.part_o[which], *part_ml = a.part_ml[which];
@@ -922,15 +923,27 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
     while (wide < live) wide *= 2;
     const int i = group % wide, n = kGroups / wide;
     const long step = (long)a.kv_heads * rows, at = ((long)first * a.kv_heads + head) * rows + r0 + min(i, live - 1);
+    int n_parts = n_own;
+    const float *prefix_o = nullptr, *prefix_ml = nullptr;
+    long prefix_step = 0, prefix_at = 0;
+    if (SHARED && j[5] >= 0) {
+      const int prefix_rows = a.list[j[5]].rows, row = j[7] + tile * rows + r0 + min(i, live - 1);
+      const int* p = a.plan + a.list[j[5]].prefixes + 2L * (j[6] + row / prefix_rows);
+      prefix_o = a.part_o[j[5]], prefix_ml = a.part_ml[j[5]], prefix_step = (long)a.kv_heads * prefix_rows;
+      prefix_at = ((long)p[0] * a.kv_heads + head) * prefix_rows + row % prefix_rows, n_parts += p[1];
+    }
+    auto place = [&](int p) { return !SHARED || p < n_own ? at + p * step : prefix_at + (p - n_own) * prefix_step; };
+    auto ml = [&](int p) { return !SHARED || p < n_own ? part_ml : prefix_ml; };
+    auto o = [&](int p) { return !SHARED || p < n_own ? part_o : prefix_o; };
     float top = kAttnNone, sum = 0.f;
 #pragma unroll 4
-    for (int p = 0; p < n_parts; p++) top = fmaxf(top, part_ml[2 * (at + p * step)]);
+    for (int p = 0; p < n_parts; p++) top = fmaxf(top, ml(p)[2 * place(p)]);
     attn_f4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int p = group / wide; p < n_parts; p += n) {
-      const float f = __builtin_amdgcn_exp2f(part_ml[2 * (at + p * step)] - top);
-      sum += f * part_ml[2 * (at + p * step) + 1];
-      const attn_f4 y = *reinterpret_cast<const attn_f4*>(part_o + (at + p * step) * D + d);
+      const float f = __builtin_amdgcn_exp2f(ml(p)[2 * place(p)] - top);
+      sum += f * ml(p)[2 * place(p) + 1];
+      const attn_f4 y = *reinterpret_cast<const attn_f4*>(o(p) + place(p) * D + d);
 #pragma unroll
       for (int k = 0; k < 4; k++) x[k] = __builtin_fmaf(y[k], f, x[k]);
     }

@@ -572,29 +572,42 @@ Outputs cache_read(const MoreArgs& a) {
   return out;
 }
 
-// attention_plan(q_starts, kv_lens, tokens, heads, heads of the cache, max_q, causal, window)
-Outputs attention_plan(const MoreArgs& a) {
-  if (a.n != 8 || !a.tensor(0) || !a.tensor(1) || !a.whole(6, 1)) return {};
-  for (int i : {2, 3, 4, 5, 7})
-    if (!a.whole(i)) return {};
+// The plan of a batch whose lengths are arguments 0 and 1 and whose numbers begin at `at`; `groups`: of starts and prefixes, at 2 and 3
+Outputs plan_of(const MoreArgs& a, int at, bool groups) {
+  if (a.n != at + 6 || !a.tensor(0) || !a.tensor(1) || !a.whole(at + 4, 1)) return {};
+  for (int i : {0, 1, 2, 3, 5})
+    if (!a.whole(at + i)) return {};
   const Tensor &starts = a[0], &lens = a[1];
   if (!starts.is_cuda() || !a.plain(0, starts) || !a.plain(1, starts) || !dense_on(starts, starts, at::kInt, 1) || !dense_on(lens, starts, at::kInt, 1) ||
       starts.size(0) != lens.size(0) + 1 || starts.size(0) > 0x7fffffff)
     return {};
-  const int seqs = (int)lens.size(0), tokens = a.integer(2), heads = a.integer(3), kv_heads = a.integer(4), most = a.integer(5);
-  const size_t bytes = triteia_hip_attention_plan_bytes(seqs, tokens, heads, kv_heads, most);
+  const int seqs = (int)lens.size(0), tokens = a.integer(at), heads = a.integer(at + 1), kv_heads = a.integer(at + 2), most = a.integer(at + 3);
+  int n_groups = 0;
+  if (groups) {
+    if (!a.plain(2, starts) || !a.plain(3, starts) || !dense_on(a[2], starts, at::kInt, 1) || !dense_on(a[3], starts, at::kInt, 1) || a[2].size(0) != a[3].size(0) + 1 ||
+        a[2].size(0) > 0x7fffffff)
+      return {};
+    n_groups = (int)a[3].size(0);
+  }
+  const size_t bytes = triteia_hip_shared_plan_bytes(seqs, n_groups, tokens, heads, kv_heads, most);
   if (bytes == 0) return {};
   const Place at_(starts);
   Outputs out;
   out.first = at::empty({(int64_t)bytes}, starts.options().dtype(at::kByte));
-  out.done = launched(triteia_hip_attention_plan(starts.data_ptr(), lens.data_ptr(), seqs, tokens, heads, kv_heads, most, a.integer(6), a.integer(7),
-                                                 out.first.data_ptr(), bytes, at_.dev, at_.handle()));
+  out.done = launched(groups ? triteia_hip_shared_plan(starts.data_ptr(), lens.data_ptr(), a[2].data_ptr(), a[3].data_ptr(), seqs, n_groups, tokens, heads, kv_heads, most,
+                                                       a.integer(at + 4), a.integer(at + 5), out.first.data_ptr(), bytes, at_.dev, at_.handle())
+                             : triteia_hip_attention_plan(starts.data_ptr(), lens.data_ptr(), seqs, tokens, heads, kv_heads, most, a.integer(at + 4), a.integer(at + 5),
+                                                          out.first.data_ptr(), bytes, at_.dev, at_.handle()));
   return out;
 }
+// attention_plan(q_starts, kv_lens, tokens, heads, heads of the cache, max_q, causal, window)
+Outputs attention_plan(const MoreArgs& a) { return plan_of(a, 2, false); }
+// shared_plan(q_starts, kv_lens, group_starts, prefix_lens, tokens, heads, heads of the cache, max_q, causal, window)
+Outputs shared_plan(const MoreArgs& a) { return plan_of(a, 4, true); }
 
-// paged_attention(q, cache k, v, scales, pages, plan, sequences, heads of the plan, its max_q, causal, window, scale)
-Outputs paged_attention(const MoreArgs& a) {
-  if (a.n != 13 || !a.tensor(0) || !a.tensor(5) || !a.tensor(6) || !a.given[12] || !a.whole(10, 1)) return {};
+// (q, cache k, v, scales, pages, plan, sequences, heads of the plan, its max_q, causal, window, scale) and, behind them, the plan's groups
+Outputs attention_of(const MoreArgs& a, int n_groups) {
+  if (!a.tensor(0) || !a.tensor(5) || !a.tensor(6) || !a.given[12] || !a.whole(10, 1)) return {};
   for (int i : {7, 8, 9, 11})
     if (!a.whole(i)) return {};
   const Tensor &q = a[0], &pages = a[5], &plan = a[6];
@@ -604,18 +617,20 @@ Outputs paged_attention(const MoreArgs& a) {
   if (!sizes_ok({tokens, heads, seqs}) || !rows_ok(q, q.scalar_type(), tokens, c.dim) || q.size(1) != heads || pages.scalar_type() != at::kInt || pages.dim() != 2 ||
       pages.size(0) != seqs || !sizes_ok({pages.size(1)}) || pages.stride(1) != 1 || pages.stride(0) < 0 || !dense_on(plan, q, at::kByte, 1))
     return {};
-  const size_t bytes = triteia_hip_attention_scratch_bytes(seqs, tokens, heads, c.heads, a.integer(9), c.dim);
+  const size_t bytes = triteia_hip_shared_scratch_bytes(seqs, n_groups, tokens, heads, c.heads, a.integer(9), c.dim);
   if (bytes == 0) return {};
   const Place at_(q);
   Outputs out;
   out.first = at::empty({tokens, heads, c.dim}, q.options());
   const Tensor scratch = scratch_bytes(bytes, q);
-  out.done = launched(triteia_hip_paged_attention(
+  out.done = launched(triteia_hip_shared_attention(
       q.data_ptr(), q.stride(0), q.stride(1), out.first.data_ptr(), data(c.k), data(c.v), data(c.ks), data(c.vs), c.strides, c.n_pages, c.page, c.kind,
-      pages.data_ptr(), pages.stride(0), pages.size(1), plan.data_ptr(), plan.numel(), seqs, tokens, heads, c.heads, c.dim, a.integer(9), a.integer(10),
+      pages.data_ptr(), pages.stride(0), pages.size(1), plan.data_ptr(), plan.numel(), seqs, n_groups, tokens, heads, c.heads, c.dim, a.integer(9), a.integer(10),
       a.integer(11), (float)a.numbers[12], scratch.data_ptr(), bytes, q.scalar_type() == at::kBFloat16, at_.dev, at_.handle()));
   return out;
 }
+Outputs paged_attention(const MoreArgs& a) { return a.n == 13 ? attention_of(a, 0) : Outputs{}; }
+Outputs shared_attention(const MoreArgs& a) { return a.n == 14 && a.whole(13) ? attention_of(a, a.integer(13)) : Outputs{}; }
 
 // --- the base weight in 8 bits ---
 
@@ -715,6 +730,7 @@ PyMethodDef methods[] = {METHOD("matmul", (call<matmul>)), METHOD("bmm", (call<b
                          METHOD("pack", pack), METHOD("sparse", sparse), METHOD("rotary_cache", (call_more<rotary_cache, true>)),
                          METHOD("cache_read", (call_more<cache_read, true>)), METHOD("attention_plan", (call_more<attention_plan, false>)),
                          METHOD("paged_attention", (call_more<paged_attention, false>)),
+                         METHOD("shared_plan", (call_more<shared_plan, false>)), METHOD("shared_attention", (call_more<shared_attention, false>)),
                          METHOD("quantize_fp8", (call_more<quantize_fp8, true>)), METHOD("dequantize_fp8", (call_more<dequantize_fp8, false>)),
                          METHOD("matmul_fp8", (call_more<matmul_fp8, false>)), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "triteia_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

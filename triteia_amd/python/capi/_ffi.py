@@ -77,6 +77,11 @@ SIGNATURES = {
     "triteia_hip_attention_plan": (_c_int, [_c_vp] * 2 + [_c_int] * 7 + [_c_vp, _c_sz, _c_int, _c_vp]),
     "triteia_hip_paged_attention": (_c_int, [_c_vp, _c_long, _c_long] + [_c_vp] * 6 + [_c_int] * 3 + [_c_vp, _c_long, _c_int, _c_vp, _c_sz]
                                     + [_c_int] * 8 + [_c_float, _c_vp, _c_sz] + [_c_int] * 2 + [_c_vp]),
+    "triteia_hip_shared_plan_bytes": (_c_sz, [_c_int] * 6),
+    "triteia_hip_shared_scratch_bytes": (_c_sz, [_c_int] * 7),
+    "triteia_hip_shared_plan": (_c_int, [_c_vp] * 4 + [_c_int] * 8 + [_c_vp, _c_sz, _c_int, _c_vp]),
+    "triteia_hip_shared_attention": (_c_int, [_c_vp, _c_long, _c_long] + [_c_vp] * 6 + [_c_int] * 3 + [_c_vp, _c_long, _c_int, _c_vp, _c_sz]
+                                     + [_c_int] * 9 + [_c_float, _c_vp, _c_sz] + [_c_int] * 2 + [_c_vp]),
     "triteia_hip_fp8_quantize": (_c_int, [_c_vp, _c_long] + [_c_int] * 3 + [_c_vp, _c_long, _c_vp, _c_long, _c_long] + [_c_int] * 2 + [_c_vp]),
     "triteia_hip_fp8_values": (_c_int, [_c_vp, _c_long, _c_vp, _c_long, _c_long] + [_c_int] * 3 + [_c_vp] + [_c_int] * 2 + [_c_vp]),
     "triteia_hip_fp8_scratch_bytes": (_c_sz, [_c_int] * 4),

@@ -180,36 +180,48 @@ def cache_read(cache, slots, dtype):
 class AttentionPlan:
     """The work list of a batch (from `attention_plan`), for every layer of a forward pass whose heads are as many."""
 
-    def __init__(self, buffer, n_seqs, n_tokens, heads, kv_heads, max_q, causal, window):
-        self.buffer = buffer
+    def __init__(self, buffer, n_seqs, n_tokens, heads, kv_heads, max_q, causal, window, n_groups=0):
+        self.buffer, self.n_groups = buffer, n_groups
         self.n_seqs, self.n_tokens, self.heads, self.kv_heads, self.max_q, self.causal, self.window = n_seqs, n_tokens, heads, kv_heads, max_q, causal, window
 
 
-def attention_plan(q_starts, kv_lens, n_tokens, heads, kv_heads, max_q=None, causal=True, window=0):
+def attention_plan(q_starts, kv_lens, n_tokens, heads, kv_heads, max_q=None, causal=True, window=0, group_starts=None, prefix_lens=None):
     max_q = n_tokens if max_q is None else max_q
-    buffer = native().attention_plan(q_starts, kv_lens, n_tokens, heads, kv_heads, max_q, causal, window)
-    if buffer is not None:
-        return AttentionPlan(buffer, kv_lens.shape[0], n_tokens, heads, kv_heads, max_q, bool(causal), window)
-    device = _require(q_starts=q_starts, kv_lens=kv_lens)
-    for name, t in (("q_starts", q_starts), ("kv_lens", kv_lens)):
-        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+    if group_starts is None and prefix_lens is None:
+        buffer = native().attention_plan(q_starts, kv_lens, n_tokens, heads, kv_heads, max_q, causal, window)
+        if buffer is not None:
+            return AttentionPlan(buffer, kv_lens.shape[0], n_tokens, heads, kv_heads, max_q, bool(causal), window)
+    else:
+        buffer = native().shared_plan(q_starts, kv_lens, group_starts, prefix_lens, n_tokens, heads, kv_heads, max_q, causal, window)
+        if buffer is not None:
+            return AttentionPlan(buffer, kv_lens.shape[0], n_tokens, heads, kv_heads, max_q, bool(causal), window, prefix_lens.shape[0])
+        if group_starts is None or prefix_lens is None:
+            raise RuntimeError("group_starts and prefix_lens go together")
+    device = _require(optional=("group_starts", "prefix_lens"), q_starts=q_starts, kv_lens=kv_lens, group_starts=group_starts, prefix_lens=prefix_lens)
+    for name, t in (("q_starts", q_starts), ("kv_lens", kv_lens), ("group_starts", group_starts), ("prefix_lens", prefix_lens)):
+        if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous()):
             raise RuntimeError(f"{name} must be a contiguous vector of torch.int32, got {tuple(t.shape)} of {t.dtype}")
-    n_seqs = kv_lens.shape[0]
+    n_seqs, n_groups = kv_lens.shape[0], 0 if prefix_lens is None else prefix_lens.shape[0]
     if q_starts.shape[0] != n_seqs + 1:
         raise RuntimeError(f"q_starts must have {n_seqs + 1} entries for {n_seqs} sequences, got {q_starts.shape[0]}")
-    sizes = (n_seqs, int(n_tokens), int(heads), int(kv_heads), int(max_q))
-    nbytes = _ffi.lib().triteia_hip_attention_plan_bytes(*sizes)
+    if group_starts is not None and group_starts.shape[0] != n_groups + 1:
+        raise RuntimeError(f"group_starts must have {n_groups + 1} entries for {n_groups} groups, got {group_starts.shape[0]}")
+    sizes = (n_seqs, n_groups, int(n_tokens), int(heads), int(kv_heads), int(max_q))
+    nbytes = _ffi.lib().triteia_hip_shared_plan_bytes(*sizes)
     if nbytes == 0:
         raise RuntimeError(_ffi.last_error())
     buffer = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    _check(_ffi.lib().triteia_hip_attention_plan(_ffi.ptr(q_starts), _ffi.ptr(kv_lens), *sizes, int(bool(causal)), int(window), _ffi.ptr(buffer), nbytes,
-                                                 _ffi.device_index(q_starts), _ffi.stream_of(q_starts)))
-    return AttentionPlan(buffer, *sizes, bool(causal), int(window))
+    _check(_ffi.lib().triteia_hip_shared_plan(_ffi.ptr(q_starts), _ffi.ptr(kv_lens), _ffi.ptr(group_starts), _ffi.ptr(prefix_lens), *sizes, int(bool(causal)), int(window),
+                                              _ffi.ptr(buffer), nbytes, _ffi.device_index(q_starts), _ffi.stream_of(q_starts)))
+    return AttentionPlan(buffer, n_seqs, *sizes[2:], bool(causal), int(window), n_groups)
 
 
 def paged_attention(q, cache, pages, plan, scale):
     if isinstance(q, torch.Tensor) and q.dim() == 3 and q.shape[0] == plan.n_tokens and cache.kv_heads == plan.kv_heads:
-        out = native().paged_attention(q, *cache._tensors, pages, plan.buffer, plan.n_seqs, plan.heads, plan.max_q, plan.causal, plan.window, scale)
+        if plan.n_groups:
+            out = native().shared_attention(q, *cache._tensors, pages, plan.buffer, plan.n_seqs, plan.heads, plan.max_q, plan.causal, plan.window, scale, plan.n_groups)
+        else:
+            out = native().paged_attention(q, *cache._tensors, pages, plan.buffer, plan.n_seqs, plan.heads, plan.max_q, plan.causal, plan.window, scale)
         if out is not None:
             return out
     device = _require(cache.device, q=q, pages=pages, plan=plan.buffer)
@@ -220,11 +232,11 @@ def paged_attention(q, cache, pages, plan, scale):
     if pages.dtype != torch.int32 or pages.dim() != 2 or pages.shape[0] != plan.n_seqs or (pages.numel() and pages.stride(1) != 1) or (pages.numel() and pages.stride(0) < 0):
         raise RuntimeError(f"pages must be torch.int32 [{plan.n_seqs}, pages of a sequence], its rows adjacent, got {pages.dtype} {tuple(pages.shape)}")
     out = torch.empty((plan.n_tokens, plan.heads, cache.dim), dtype=q.dtype, device=device)
-    sizes = (plan.n_seqs, plan.n_tokens, plan.heads, plan.kv_heads, plan.max_q)
-    nbytes = _ffi.lib().triteia_hip_attention_scratch_bytes(*sizes, cache.dim)
+    sizes = (plan.n_seqs, plan.n_groups, plan.n_tokens, plan.heads, plan.kv_heads)
+    nbytes = _ffi.lib().triteia_hip_shared_scratch_bytes(*sizes, plan.max_q, cache.dim)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    _check(_ffi.lib().triteia_hip_paged_attention(
+    _check(_ffi.lib().triteia_hip_shared_attention(
         _ffi.ptr(q), q.stride(0), q.stride(1), _ffi.ptr(out), *cache._pointers(), cache._strides, cache.n_pages, cache.page, cache.kind, _ffi.ptr(pages),
-        pages.stride(0), pages.shape[1], _ffi.ptr(plan.buffer), plan.buffer.numel(), plan.n_seqs, plan.n_tokens, plan.heads, plan.kv_heads, cache.dim, plan.max_q,
+        pages.stride(0), pages.shape[1], _ffi.ptr(plan.buffer), plan.buffer.numel(), *sizes, cache.dim, plan.max_q,
         int(plan.causal), plan.window, float(scale), _ffi.ptr(scratch), nbytes, int(q.dtype == torch.bfloat16), _ffi.device_index(q), _ffi.stream_of(q)))
     return out

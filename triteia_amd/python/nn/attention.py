@@ -22,10 +22,11 @@ class multi_delta_attention(nn.Module):
         for name in ("q_norm", "k_norm"):
             self.register_buffer(name, torch.ones(head_dim, dtype=torch.float16) if qk_norm else None)
 
-    def plan(self, cache, q_starts, kv_lens, n_tokens, max_q=None):
-        """The attention's work list for a batch: one serves every layer of a forward pass."""
+    def plan(self, cache, q_starts, kv_lens, n_tokens, max_q=None, group_starts=None, prefix_lens=None):
+        """The attention's work list for a batch: one serves every layer of a forward pass.  group_starts, prefix_lens: sequences that share a prefix, as
+        for ops.attention_plan; keys and values are a variant's own, so those of a group take the same one."""
         from triteia_amd.python.ops import attention_plan
-        return attention_plan(cache, q_starts, kv_lens, self.n_heads, n_tokens, max_q)
+        return attention_plan(cache, q_starts, kv_lens, self.n_heads, n_tokens, max_q, group_starts=group_starts, prefix_lens=prefix_lens)
 
     def forward(self, x, indices, positions, table, cache, slots, pages, q_starts, kv_lens, plan=None, route=None, max_q=None):
         """x [tokens, hidden] fp16, the new tokens of all sequences one after the other -> [tokens, hidden].
