@@ -417,7 +417,9 @@ TRITEIA_HIP_API int triteia_hip_fp8_values(const void* codes, long codes_stride,
                              void* out, int type, int dev, void* stream);
 /* out [tokens, m] = x [tokens, k] @ weight [m, k]^T, weight in codes with w_scale [ceil(m / 128), ceil(k / 128)]; x in codes (x_type 2) with x_scale
  * [tokens, ceil(k / 128)], or in fp16 (0) or bf16 (1), quantised first as above with a scale for every token.  Sums in 32 bits, rounded once to
- * out_type (0, 1, 2 as above); out is contiguous.  Scratch: contents irrelevant on entry, 16-byte aligned; 0 bytes: none, or sizes that are refused. */
+ * out_type (0, 1, 2 as above); out is contiguous.  Rows of codes are up to 2^24 apart.  Scratch: contents irrelevant on entry, 16-byte aligned; 0 bytes: none, or sizes that are refused.
+ * triteia_hip_fp8_tile: the tile of a product, its tokens + 1000 x its features + 10^6 x shares of K; 0 for sizes that are refused.  For tests and measurements. */
+TRITEIA_HIP_API int triteia_hip_fp8_tile(int tokens, int m, int k);
 TRITEIA_HIP_API size_t triteia_hip_fp8_scratch_bytes(int tokens, int m, int k, int x_type);
 TRITEIA_HIP_API int triteia_hip_fp8_matmul(const void* x, long x_stride, int x_type, const void* x_scale, long xs_token, long xs_block, const void* weight,
                              long w_stride, const void* w_scale, long ws_row, long ws_block, void* out, int out_type, int tokens, int m, int k, void* scratch,

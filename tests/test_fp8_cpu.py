@@ -61,7 +61,7 @@ def test_read_back_refusals(what, code):
 @pytest.mark.parametrize("what,code", [
     (dict(tokens=0), 0), (dict(m=0), 0), (dict(k=0), SHAPE), (dict(k=24), SHAPE), (dict(tokens=-1), SHAPE), (dict(m=-1), SHAPE), (dict(m=(1 << 24) + 1), SHAPE),
     (dict(x_type=3), KERNEL), (dict(kind=3), KERNEL), (dict(x=NULL), ARGUMENT), (dict(w=NULL), ARGUMENT), (dict(ws=NULL), ARGUMENT), (dict(out=NULL), ARGUMENT),
-    (dict(x_type=2), ARGUMENT), (dict(x_type=2, xs=ONE, xs_token=-1), ARGUMENT), (dict(stride=12), ARGUMENT), (dict(w_stride=24), ARGUMENT), (dict(w=ODD), ARGUMENT),
+    (dict(x_type=2), ARGUMENT), (dict(x_type=2, xs=ONE, xs_token=-1), ARGUMENT), (dict(stride=12), ARGUMENT), (dict(w_stride=24), ARGUMENT), (dict(w_stride=(1 << 24) + 16), ARGUMENT), (dict(w=ODD), ARGUMENT),
     (dict(ws_row=-2), ARGUMENT), (dict(scratch=NULL), ARGUMENT), (dict(scratch=ODD), ARGUMENT), (dict(scratch_bytes=64), ARGUMENT)])
 def test_product_refusals(what, code):
     assert matmul(**what) == code
@@ -75,6 +75,36 @@ def test_sizes_of_scratch():
         for m, k in ((1, 16), (1001, 2000), (4096, 4096), (28672, 8192)):
             codes = tokens * (k + 4 * -(-k // 128))
             assert codes <= need(tokens, m, k, 0) == need(tokens, m, k, 1) and need(tokens, m, k, 2) <= need(tokens, m, k, 0) - codes
+
+
+def test_tiles():
+    """Every tile has sizes that it is taken for; tests of the product run on all of them."""
+    tile = _ffi.lib().triteia_hip_fp8_tile
+    assert tile(0, 8, 256) == tile(1, 0, 256) == tile(1, 8, 24) == 0
+    found = {tile(t, m, k) % 10 ** 6 for t in (1, 16, 17, 33, 48, 64, 100, 200, 300, 700, 1000, 2000, 8000) for m in (16, 640, 1001, 2050, 4096, 11008, 28672)
+             for k in (128, 1040, 2000, 4096, 8192, 11008)}
+    assert found >= {16016, 32016, 32032, 128016, 128032, 64064, 128064, 128128, 256128, 256256}, found
+    assert tile(1, 4096, 4096) == 1016016 and tile(8000, 28672, 8192) == 1256256 and tile(64, 28672, 8192) == 1128064
+    assert tile(128, 4096, 11008) // 10 ** 6 > 1                                # a long K over few tiles: in shares
+
+
+def test_wait_states_ahead_of_direct_loads(tmp_path):
+    """As of the other kernels: a scalar write of M0 is never right ahead of the load that uses it, of 16 bytes or 4, and a scalar base written by the vector unit five."""
+    import re
+
+    from tests.test_direct_loads_cpu import _kernels
+    seen = set()
+    for kernel, code in _kernels(tmp_path).items():
+        for i, instruction in enumerate(code):
+            if "fp8_" not in kernel or not instruction.startswith("global_load_lds"):
+                continue
+            seen.add((re.search(r"fp8_(tile|stream)", kernel).group(1), instruction.split()[0]))
+            before = code[max(0, i - 5):i]
+            assert not re.match(r"\S+ m0\b", before[-1]), (kernel, before[-1], instruction)
+            scalars = re.search(r"s\[(\d+):(\d+)\]", instruction)
+            if scalars:
+                assert not [b for b in before if re.match(rf"v_\S+ s(\[?)({scalars.group(1)}|{scalars.group(2)})\b", b)], (kernel, before, instruction)
+    assert seen == {(kind, "global_load_lds_" + size) for kind in ("tile", "stream") for size in ("dwordx4", "dword")}
 
 
 class Subclass(torch.Tensor):

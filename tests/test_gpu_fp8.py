@@ -168,6 +168,39 @@ def test_product_of_real_sizes(tokens, k, m):
     assert torch.equal(ops().matmul_fp8(x8, w, ws, x_scale=xs, dtype=torch.bfloat16), ops().matmul_fp8(x, w, ws))      # the same codes, the same sums
 
 
+def sizes_of_every_tile():
+    """For each tile, whole and in shares of K, the smallest of a grid of ragged sizes that are multiplied on it."""
+    from triteia_amd.python.capi import _ffi
+    found = {}
+    for tokens in (1, 15, 17, 31, 33, 47, 61, 67, 97, 131, 193, 259, 389, 515, 771, 1027, 2051):
+        for k in (272, 1040, 2000, 4112, 8208, 11024):
+            for m in (131, 515, 1001, 2050, 4097, 8199, 11012, 20004):
+                tile = _ffi.lib().triteia_hip_fp8_tile(tokens, m, k)
+                key = (tile % 10 ** 6, tile >= 2 * 10 ** 6)
+                if key not in found or tokens * k * m < found[key][0]:
+                    found[key] = (tokens * k * m, (tokens, k, m))
+    return {key: size for key, (_, size) in sorted(found.items())}
+
+
+@pytest.mark.parametrize("tile", [16016, 32016, 32032, 128016, 128032, 64064, 128064, 128128, 256128, 256256])
+def test_every_tile(tile):
+    sizes = [size for key, size in sizes_of_every_tile().items() if key[0] == tile]
+    assert sizes
+    for tokens, k, m in sizes:
+        x = (randn(tokens, k, seed=1) * torch.exp(randn(tokens, 1, seed=2))).half().cuda()
+        w, ws = (t.cuda() for t in weight(m, k, seed=3))
+        x8, xs = ops().quantize_fp8(x)
+        xv, wv = values(x8, xs, 1), values(w, ws, 128)
+        for dtype in (torch.float16, torch.bfloat16, torch.float32):
+            close(ops().matmul_fp8(x, w, ws, dtype=dtype), xv, wv, dtype)
+        twice = [ops().matmul_fp8(x8, w, ws, x_scale=by, dtype=torch.float32) for by in (xs, xs.contiguous())]
+        assert torch.equal(*twice)
+
+
+def test_shares_of_k_are_tested():
+    assert sum(split for _, split in sizes_of_every_tile()) >= 3
+
+
 def test_product_layouts():
     tokens, k, m = 37, 400, 260
     w, ws = (t.cuda() for t in weight(m, k, seed=8))

@@ -37,22 +37,87 @@ void launch_fp8_values(const Fp8ValuesArgs& a, hipStream_t st) {
   else hipLaunchKernelGGL((fp8_values_kernel<T, kFp8Wide>), grid, dim3(256), 0, st, a);
 }
 
+// A kernel's tile, and what a call on it takes: `start` us for the first workgroups of a CU and 1.5 for each further round of them; for every block of K that a workgroup
+// (of the streaming kernels: a wavefront) walks, `alone` us or, where more workgroups share the CU, `shared` for each.
+struct Fp8Kernel {
+  int tokens, features, beside, walkers;      // beside: workgroups that a CU holds; walkers: wavefronts that share the blocks
+  float start, alone, shared;
+};
+// Fitted to 8000 timings of 20 tiles in graphs, on 8 layers from 1024 x 1024 to 8192 x 28672 with 1 to 2048 tokens, whole and with K in 2 to 16 shares, weights not in the caches.  On
+// these the rule's pick is 1.9 % behind the best of all that were timed on average, 19 % at most.
+constexpr Fp8Kernel kFp8Kernels[] = {
+    {16, 16, 2, 8, 3.644f, 0.306f, 0.369f},  {16, 32, 1, 8, 3.357f, 0.140f, 0.639f},  {32, 32, 1, 8, 3.500f, 0.885f, 0.414f},   {16, 128, 2, 1, 4.175f, 0.311f, 0.260f},
+    {32, 128, 1, 1, 4.640f, 0.379f, 0.286f}, {64, 64, 2, 1, 4.963f, 0.354f, 0.255f},  {64, 128, 2, 1, 5.695f, 0.421f, 0.377f},  {64, 128, 1, 1, 5.446f, 0.516f, 0.418f},
+    {128, 128, 1, 1, 5.864f, 0.626f, 0.091f}, {128, 256, 1, 1, 7.185f, 0.942f, 0.152f}, {256, 256, 1, 1, 7.492f, 1.662f, 0.189f}};
+constexpr int kFp8KernelCount = sizeof(kFp8Kernels) / sizeof(kFp8Kernels[0]);
+constexpr int kFp8MaxSplits = 8;
+
 struct Fp8Pick {
-  int tokens, features, splits;
+  int kernel, splits;
 };
 Fp8Pick pick_fp8(int tokens, int m, int k) {
-  (void)tokens, (void)m, (void)k;
-  return {64, 64, 1};
+  Fp8Pick best = {0, 1};
+  float least = 3e38f;
+  const int blocks = fp8_blocks(k);
+  for (int i = 0; i < kFp8KernelCount; i++) {
+    const Fp8Kernel& c = kFp8Kernels[i];
+    if (c.walkers > 1 && c.features > 16 && tokens <= 16) continue;      // (4096 x 11008 on 16 features a workgroup 10.9 us, on 32 12.1)
+    const long tiles = ((tokens + c.tokens - 1L) / c.tokens) * ((m + c.features - 1L) / c.features);
+    for (int splits = 1; splits <= kFp8MaxSplits; splits *= 2) {
+      if (splits > 1 && (tiles * splits > 512 || blocks / splits < 8 || (c.walkers > 1 && (splits > 2 || tiles > 96)))) break;
+      const int share = (blocks + splits - 1) / splits, walk = (share + c.walkers - 1) / c.walkers;
+      const long deep = (tiles * splits + 255) / 256, rounds = deep / c.beside, rest = deep % c.beside;
+      const float full = std::max(c.alone, c.shared * c.beside), part = rest ? std::max(c.alone, c.shared * rest) : 0.f;
+      float us = c.start + 1.5f * (rounds + (rest > 0) - 1) + walk * (rounds * full + part);
+      // the weights at 6.2 TB/s, and a part of what all tiles read from L2
+      us = std::max(us, 3.f + ((float)m * k + (float)tokens * k) / 6.2e6f + 0.015e-6f * tiles * (c.tokens + c.features) * k);
+      if (splits > 1) us += 2.f + 1e-6f * tokens * m * (splits + 1);
+      if (us < least) least = us, best = {i, splits};
+    }
+  }
+  return best;
 }
+// Rows of W lie a power of two apart, and walks in lockstep read the same few channels: 64 tokens on 8192 x 28672 53 us, spread 43.  From 512 tokens on, and on small layers,
+// there is nothing to spread (2048 tokens on 4096 x 4096 39.0 and 39.4).
+bool fp8_rotates(int tokens, int m, int k) { return tokens <= 512 && (long)m * k >= (1L << 25); }
+
+long fp8_units(const Fp8Args& a, int tokens, int features) { return ((a.m + features - 1L) / features) * ((a.tokens + tokens - 1L) / tokens) * a.splits; }
 
 template <int NT, int TW, int F, int FW, int STAGES>
 int launch_fp8_tile(const Fp8Args& a, hipStream_t st) {
   using Tile = Fp8Tile<NT, TW, F, FW, STAGES>;
+  static_assert(Tile::kLdsBytes <= 163840, "");
   if (int e = grant_lds<fp8_tile_kernel<NT, TW, F, FW, STAGES>>(Tile::kLdsBytes, "fp8_tile_kernel")) return e;
-  const long units = (long)((a.m + Tile::kFeatures - 1) / Tile::kFeatures) * ((a.tokens + Tile::kTokens - 1) / Tile::kTokens) * a.splits;
+  const long units = fp8_units(a, Tile::kTokens, Tile::kFeatures);
   if (units > 0x7ffffff0L) return fail(TRITEIA_HIP_ERR_PROB_SHAPE, "fp8_matmul: too many work units (%ld)", units);
   hipLaunchKernelGGL((fp8_tile_kernel<NT, TW, F, FW, STAGES>), dim3((unsigned)((units + 7) / 8 * 8)), dim3(Tile::kThreads), Tile::kLdsBytes, st, a);
   return check_launch("fp8_tile_kernel");
+}
+template <int NT, int F, int WAVES, int STAGES>
+int launch_fp8_stream(const Fp8Args& a, hipStream_t st) {
+  using Tile = Fp8Stream<NT, F, WAVES, STAGES>;
+  static_assert(Tile::kLdsBytes <= 163840, "");
+  if (int e = grant_lds<fp8_stream_kernel<NT, F, WAVES, STAGES>>(Tile::kLdsBytes, "fp8_stream_kernel")) return e;
+  const long units = fp8_units(a, Tile::kTokens, Tile::kFeatures);
+  if (units > 0x7ffffff0L) return fail(TRITEIA_HIP_ERR_PROB_SHAPE, "fp8_matmul: too many work units (%ld)", units);
+  hipLaunchKernelGGL((fp8_stream_kernel<NT, F, WAVES, STAGES>), dim3((unsigned)((units + 7) / 8 * 8)), dim3(Tile::kThreads), Tile::kLdsBytes, st, a);
+  return check_launch("fp8_stream_kernel");
+}
+// in the order of kFp8Kernels
+int launch_fp8(const Fp8Args& a, int kernel, hipStream_t st) {
+  switch (kernel) {
+    case 0: return launch_fp8_stream<1, 1, 8, 2>(a, st);
+    case 1: return launch_fp8_stream<1, 2, 8, 2>(a, st);
+    case 2: return launch_fp8_stream<2, 2, 8, 2>(a, st);
+    case 3: return launch_fp8_tile<1, 1, 2, 4, 4>(a, st);
+    case 4: return launch_fp8_tile<2, 1, 2, 4, 4>(a, st);
+    case 5: return launch_fp8_tile<2, 2, 2, 2, 4>(a, st);
+    case 6: return launch_fp8_tile<2, 2, 2, 4, 3>(a, st);
+    case 7: return launch_fp8_tile<4, 1, 2, 4, 6>(a, st);
+    case 8: return launch_fp8_tile<4, 2, 2, 4, 3>(a, st);
+    case 9: return launch_fp8_tile<4, 2, 4, 4, 3>(a, st);
+    default: return launch_fp8_tile<8, 2, 4, 4, 2>(a, st);
+  }
 }
 
 template <class T>
@@ -108,6 +173,12 @@ int triteia_hip_fp8_values(const void* codes, long codes_stride, const void* sca
   return check_launch("fp8_values_kernel");
 }
 
+int triteia_hip_fp8_tile(int tokens, int m, int k) {
+  if (tokens <= 0 || m <= 0 || k <= 0 || check_fp8("fp8_matmul", tokens, k) || m > kFp8Most) return 0;
+  const Fp8Pick t = pick_fp8(tokens, m, k);
+  return (t.splits * 1000 + kFp8Kernels[t.kernel].features) * 1000 + kFp8Kernels[t.kernel].tokens;
+}
+
 size_t triteia_hip_fp8_scratch_bytes(int tokens, int m, int k, int x_type) {
   if (tokens <= 0 || m <= 0 || k <= 0 || check_fp8("fp8_matmul", tokens, k) || m > kFp8Most) return 0;
   const int splits = pick_fp8(tokens, m, k).splits;
@@ -125,8 +196,8 @@ int triteia_hip_fp8_matmul(const void* x, long x_stride, int x_type, const void*
   if (k == 0) return fail(TRITEIA_HIP_ERR_PROB_SHAPE, "%s: rows without elements", what);
   if (!x || !weight || !w_scale || !out || (x_type == 2 && !x_scale)) return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: null tensor pointer", what);
   if (!aligned16(x) || !aligned16(weight) || !aligned16(out) || !strides_ok({x_stride}, x_type == 2 ? 1 : 2, 16) || !strides_ok({w_stride}, 1, 16) ||
-      ws_row < 0 || ws_block < 0 || (x_type == 2 && (xs_token < 0 || xs_block < 0)))
-    return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: rows of x and of the weight start on 16 bytes", what);
+      ws_row < 0 || ws_block < 0 || (x_type == 2 && (xs_token < 0 || xs_block < 0)) || w_stride > kFp8Most || (x_type == 2 && x_stride > kFp8Most))
+    return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: rows of x and of the weight start on 16 bytes, those of codes up to 2^24 apart", what);
   const size_t need = triteia_hip_fp8_scratch_bytes(tokens, m, k, x_type);
   if (need && (!scratch || scratch_bytes < need || !aligned16(scratch)))
     return fail(TRITEIA_HIP_ERR_ARGUMENT, "%s: scratch must hold %zu bytes (got %zu), aligned to 16", what, need, scratch_bytes);
@@ -146,8 +217,9 @@ int triteia_hip_fp8_matmul(const void* x, long x_stride, int x_type, const void*
   }
   const Fp8Pick t = pick_fp8(tokens, m, k);
   a.w = static_cast<const uint8_t*>(weight), a.w_stride = w_stride, a.ws = static_cast<const float*>(w_scale), a.ws_row = ws_row, a.ws_block = ws_block;
-  a.out = out, a.type = out_type, a.tokens = tokens, a.m = m, a.k = k, a.splits = t.splits, a.partial = reinterpret_cast<float*>(at);
-  if (int e = launch_fp8_tile<2, 2, 2, 2, 3>(a, st)) return e;
+  a.out = out, a.type = out_type, a.tokens = tokens, a.m = m, a.k = k, a.splits = t.splits, a.rotate = fp8_rotates(tokens, m, k);
+  a.partial = reinterpret_cast<float*>(at);
+  if (int e = launch_fp8(a, t.kernel, st)) return e;
   if (t.splits == 1) return TRITEIA_HIP_OK;
   if (out_type == 0) launch_fp8_reduce<_Float16>(a, st);
   else if (out_type == 1) launch_fp8_reduce<__bf16>(a, st);

@@ -14,7 +14,7 @@ namespace triteia_hip {
 
 struct Fp8Args {
   const uint8_t* x;       // [tokens, k]
-  long x_stride;
+  long x_stride;          // up to 2^24, as w_stride: a tile's rows are 32-bit offsets apart
   const float* xs;        // [tokens, blocks] by strides
   long xs_token, xs_block;
   const uint8_t* w;       // [m, k]
@@ -25,12 +25,13 @@ struct Fp8Args {
   int type;               // of out: 0 fp16, 1 bf16, 2 fp32
   int tokens, m, k;       // k a multiple of 16
   int splits;             // shares of K over workgroups; 1: the result goes to `out`
+  int rotate;             // 1: feature groups start their walks over K spread around its blocks, 0: at the first
   float* partial;         // [splits][tokens][m] (splits > 1)
 };
 
-typedef int fp8_v8 __attribute__((ext_vector_type(8)));
+constexpr int kFp8Band = 4;
 
-__device__ const uint4_t fp8_zeros = {0, 0, 0, 0};     // what lies behind the last code of a row
+typedef int fp8_v8 __attribute__((ext_vector_type(8)));
 
 // 4 bytes a lane to `lds` (uniform) + 4 lane; the caller waits (see direct_load)
 __device__ __forceinline__ void direct_load4(const void* src, uint32_t lds) {
@@ -59,6 +60,14 @@ __device__ __forceinline__ void fp8_store(T* to, const float4_t& v, int m, int j
   }
 }
 
+__device__ __forceinline__ void fp8_result(const Fp8Args& p, int share, int token, int j0, const float4_t& v) {
+  const long at = (long)token * p.m + j0;
+  if (p.splits > 1) fp8_store<float>(p.partial + (long)share * p.tokens * p.m + at, v, p.m, j0);
+  else if (p.type == 0) fp8_store<_Float16>(static_cast<_Float16*>(p.out) + at, v, p.m, j0);
+  else if (p.type == 1) fp8_store<__bf16>(static_cast<__bf16*>(p.out) + at, v, p.m, j0);
+  else fp8_store<float>(static_cast<float*>(p.out) + at, v, p.m, j0);
+}
+
 // NT x F: 16-token by 16-feature tiles of a wavefront; TW x FW wavefronts side by side.
 template <int NT, int TW, int F, int FW, int STAGES>
 struct Fp8Tile {
@@ -70,6 +79,15 @@ struct Fp8Tile {
   static constexpr int kLdsBytes = STAGES * kStageBytes;
   static_assert(16 * F <= 128 && 128 % (16 * F) == 0 && kTokens + kWeightScales <= 64 * kWaves && kFeatures % 8 == 0, "");
 };
+
+// all but the newest MOST sets of requests, or as many as there are behind the block
+template <int MOST, int LOADS>
+__device__ __forceinline__ void fp8_wait(int behind) {
+  if constexpr (MOST > 0) {
+    if (behind < MOST) return fp8_wait<MOST - 1, LOADS>(behind);
+  }
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(MOST * LOADS) : "memory");
+}
 
 template <int NT, int TW, int F, int FW, int STAGES>
 __global__ __launch_bounds__(64 * TW * FW) void fp8_tile_kernel(const Fp8Args p) {
@@ -84,29 +102,31 @@ __global__ __launch_bounds__(64 * TW * FW) void fp8_tile_kernel(const Fp8Args p)
   const int r = lane & 15, q = lane >> 4;
   const int tw = wave / FW, fw = wave % FW;
 
-  // Units in the order (feature group, share of K, token tile), token tiles fastest; an XCD (workgroup u runs on XCD u % 8) takes a run of them.
+  // Units: token tiles in bands of kBand, in a band (feature group, share of K, token tile), token tiles fastest.  An XCD (workgroup u runs on XCD u % 8) takes a run of
+  // them, so that what runs there at once is a band's token tiles on a few feature groups and its L2 serves both.
   const int ttiles = (p.tokens + TT - 1) / TT, groups = (p.m + FF - 1) / FF;
   const int units = ttiles * groups * p.splits;
   const int per_xcd = (units + 7) >> 3;
   const int u = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
   if ((int)(blockIdx.x >> 3) >= per_xcd || u >= units) return;
-  const int tt = u % ttiles, z = (u / ttiles) % p.splits, fg = u / (ttiles * p.splits);
+  const int band = u / (kFp8Band * groups * p.splits), in_band = u - band * (kFp8Band * groups * p.splits), deep = min(kFp8Band, ttiles - kFp8Band * band);
+  const int tt = kFp8Band * band + in_band % deep, z = (in_band / deep) % p.splits, fg = in_band / (deep * p.splits);
   const int t0 = tt * TT, f0 = fg * FF;
   const int blocks = (p.k + 127) >> 7;
   const int c0 = (int)((long)z * blocks / p.splits), n = (int)((long)(z + 1) * blocks / p.splits) - c0;
+  const int rot = p.rotate ? (int)((long)fg * n / groups) : 0;
 
   // A request: 8 rows x 128 bytes; lane l takes 16 bytes of row l / 8, the piece (l % 8) ^ (l / 8) to position l % 8.
-  // (rows past the end repeat the last one: their sums are not stored)
-  const uint8_t* src[kLoads - 1];
-  uint32_t dst[kLoads - 1];
+  // (rows past the end repeat the last one: their sums are not stored; a tile's rows lie within 2^32 bytes)
+  const uint8_t *x0 = p.x + (long)t0 * p.x_stride + 128L * c0, *w0 = p.w + (long)f0 * p.w_stride + 128L * c0;
+  uint32_t src[kLoads - 1], dst[kLoads - 1];
   const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
   const int lane_piece = (lane & 7) ^ (lane >> 3);
 #pragma unroll
   for (int i = 0; i < kLoads - 1; i++) {
     const bool is_x = i < kXLoads;
     const int g = min(wave + WAVES * (is_x ? i : i - kXLoads), (is_x ? TT : FF) / 8 - 1), row = 8 * g + (lane >> 3);
-    const uint8_t* base = is_x ? p.x + (long)min(t0 + row, p.tokens - 1) * p.x_stride : p.w + (long)min(f0 + row, p.m - 1) * p.w_stride;
-    src[i] = base + 16 * lane_piece + 128L * c0;
+    src[i] = (is_x ? (uint32_t)min(row, p.tokens - 1 - t0) * (uint32_t)p.x_stride : (uint32_t)min(row, p.m - 1 - f0) * (uint32_t)p.w_stride) + 16 * lane_piece;
     dst[i] = lds0 + (is_x ? 0 : 128 * TT) + 1024 * g;
   }
   // scales of a block: those of the tile's tokens, then those of its weights' blocks, 64 a wavefront
@@ -114,66 +134,92 @@ __global__ __launch_bounds__(64 * TW * FW) void fp8_tile_kernel(const Fp8Args p)
   const float* scale_src = which < TT ? p.xs + (long)min(t0 + which, p.tokens - 1) * p.xs_token + c0 * p.xs_block
                                       : p.ws + (long)min((f0 >> 7) + min(which - TT, Tile::kWeightScales - 1), (p.m - 1) >> 7) * p.ws_row + c0 * p.ws_block;
   const long scale_step = which < TT ? p.xs_block : p.ws_block;
-  const bool short_piece = 128 * (blocks - 1) + 16 * lane_piece >= p.k;      // of the last block
+  // The last block of a K that ends inside it: lanes whose piece lies behind the end read the block's first piece instead, and put zeros in its place in LDS.
+  const int odd_block = p.k % 128 ? blocks - 1 - c0 : -1;
+  const uint32_t back = 128 * (blocks - 1) + 16 * lane_piece >= p.k ? 16 * lane_piece : 0;
+  auto block_of = [&](int c) { return c + rot < n ? c + rot : c + rot - n; };      // the c-th of the walk
   auto issue = [&](int i, int c, int stage) {
     if (i == kLoads - 1) {
       direct_load4(scale_src + c * scale_step, __builtin_amdgcn_readfirstlane(lds0 + stage * Tile::kStageBytes + Tile::kCodes + 256 * wave));
     } else {
-      const uint8_t* s = src[i] + 128L * c;
-      if (c0 + c == blocks - 1 && short_piece) s = reinterpret_cast<const uint8_t*>(&fp8_zeros);
-      direct_load(s, __builtin_amdgcn_readfirstlane(dst[i] + stage * Tile::kStageBytes));
+      const uint8_t* base = (i < kXLoads ? x0 : w0) + 128L * c;
+      direct_load(src[i] - (c == odd_block ? back : 0), base, __builtin_amdgcn_readfirstlane(dst[i] + stage * Tile::kStageBytes));
     }
   };
-
-  float4_t acc[F][NT];
+  auto clear = [&](int stage) {
+    if (back == 0) return;
 #pragma unroll
-  for (int f = 0; f < F; f++)
+    for (int i = 0; i < kLoads - 1; i++) *reinterpret_cast<uint4_t*>(smem + (dst[i] - lds0) + stage * Tile::kStageBytes + 16 * lane) = uint4_t{0, 0, 0, 0};
+  };
+
+  float4_t acc[F][NT], d[F];
+#pragma unroll
+  for (int f = 0; f < F; f++) {
+    d[f] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int t = 0; t < NT; t++) acc[f][t] = float4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  float scale = 0.f;                                       // of the sums in d
   const int piece = (q ^ (r & 7)) * 16;
   const uint32_t xrow = (16 * NT * tw + r) * 128;
   const uint32_t wrow = 128 * TT + (16 * F * fw + r) * 128;
+  // A block: between the MFMAs of one token tile the sums of the tile before it are added, so that neither waits for the other; the last tile's are added
+  // in the next block.
+  auto add = [&](int f, int t) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) acc[f][t][j] = __builtin_fmaf(d[f][j], scale, acc[f][t][j]);
+  };
   auto compute = [&](int stage, auto&& request) {
     const unsigned char* s = smem + stage * Tile::kStageBytes;
     const float* scales = reinterpret_cast<const float*>(s + Tile::kCodes);
     const float sw = scales[TT + 16 * F * fw / 128];
-    fp8_v8 w[F];
+    fp8_v8 w[F], x = fp8_operand(s + xrow, piece);
+    float next = scales[16 * NT * tw + r];
 #pragma unroll
     for (int f = 0; f < F; f++) w[f] = fp8_operand(s + wrow + 2048 * f, piece);
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      const fp8_v8 x = fp8_operand(s + xrow + 2048 * t, piece);
-      const float scale = scales[16 * (NT * tw + t) + r] * sw;
+      const fp8_v8 now = x;
+      const float mine = next * sw;
+      if (t + 1 < NT) x = fp8_operand(s + xrow + 2048 * (t + 1), piece), next = scales[16 * (NT * tw + t + 1) + r];
 #pragma unroll
       for (int f = 0; f < F; f++) {
-        const float4_t d = fp8_mma(w[f], x);
-#pragma unroll
-        for (int j = 0; j < 4; j++) acc[f][t][j] = __builtin_fmaf(d[j], scale, acc[f][t][j]);
+        add(f, t == 0 ? NT - 1 : t - 1);
+        d[f] = fp8_mma(w[f], now);
+        __builtin_amdgcn_sched_barrier(0);
       }
-    }
+      scale = mine;
+      constexpr int kEach = 4 * NT < kLoads ? (kLoads + NT - 1) / NT : 4;      // (early: the last of them have the rest of the block to arrive)
 #pragma unroll
-    for (int i = 0; i < kLoads; i++) request(i);
+      for (int i = t * kEach; i < (t + 1) * kEach && i < kLoads; i++) request(i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
 
   for (int c = 0; c < AHEAD && c < n; c++)
 #pragma unroll
-    for (int i = 0; i < kLoads; i++) issue(i, c, c);
-  int stage = 0, c = 0;
-  // AHEAD blocks are in flight at the top, kLoads requests each, and complete in order (as in dense_base_kernel)
-  for (; c + AHEAD <= n; c++) {
+    for (int i = 0; i < kLoads; i++) issue(i, block_of(c), c);
+  // AHEAD blocks are in flight at the top, kLoads requests each, and complete in order: all but the newest AHEAD - 1 sets done means that this wavefront's part
+  // of block c has landed.  The barrier makes all parts visible and says that every wavefront has read the block before, whose stage takes block c + AHEAD.
+  // (One loop with a branch around the requests would hold the sums twice.)
+  int c = 0, stage = 0;
+  for (; c + AHEAD < n; c++) {
     asm volatile("s_waitcnt vmcnt(%0)" : : "n"((AHEAD - 1) * kLoads) : "memory");
+    if (block_of(c) == odd_block) clear(stage);
     lds_barrier();
-    const int free_stage = stage == 0 ? STAGES - 1 : stage - 1;
-    if (c + AHEAD < n) compute(stage, [&](int i) { issue(i, c + AHEAD, free_stage); });
-    else compute(stage, [](int) {});
+    const int free_stage = stage == 0 ? STAGES - 1 : stage - 1, ahead = block_of(c + AHEAD);
+    compute(stage, [&](int i) { issue(i, ahead, free_stage); });
     stage = stage + 1 == STAGES ? 0 : stage + 1;
   }
   for (; c < n; c++) {
-    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+    fp8_wait<AHEAD - 1, kLoads>(n - 1 - c);
+    if (block_of(c) == odd_block) clear(stage);
     lds_barrier();
     compute(stage, [](int) {});
     stage = stage + 1 == STAGES ? 0 : stage + 1;
   }
+#pragma unroll
+  for (int f = 0; f < F; f++) add(f, NT - 1);
 
   // D: lane (token r, q) holds features 4q .. 4q + 3 of a tile
 #pragma unroll
@@ -182,13 +228,132 @@ __global__ __launch_bounds__(64 * TW * FW) void fp8_tile_kernel(const Fp8Args p)
 #pragma unroll
     for (int f = 0; f < F; f++) {
       const int j0 = f0 + 16 * (F * fw + f) + 4 * q;
-      if (token >= p.tokens || j0 >= p.m) continue;
-      const long at = (long)token * p.m + j0;
-      if (p.splits > 1) fp8_store<float>(p.partial + (long)z * p.tokens * p.m + at, acc[f][t], p.m, j0);
-      else if (p.type == 0) fp8_store<_Float16>(static_cast<_Float16*>(p.out) + at, acc[f][t], p.m, j0);
-      else if (p.type == 1) fp8_store<__bf16>(static_cast<__bf16*>(p.out) + at, acc[f][t], p.m, j0);
-      else fp8_store<float>(static_cast<float*>(p.out) + at, acc[f][t], p.m, j0);
+      if (token < p.tokens && j0 < p.m) fp8_result(p, z, token, j0, acc[f][t]);
     }
+  }
+}
+
+// Few tokens: bound by the weights' way from HBM, on small layers by a launch and its round trips.  A workgroup takes 16 F features and 16 NT tokens at most; its
+// wavefronts take turns at the blocks of K, each with a ring of its own in LDS, so that nothing is waited for but a wavefront's own requests; their sums
+// meet once at the end.
+template <int NT, int F, int WAVES, int STAGES>
+struct Fp8Stream {
+  static constexpr int kTokens = 16 * NT, kFeatures = 16 * F, kThreads = 64 * WAVES;
+  static constexpr int kScaleLoads = (kTokens + 1 + 63) / 64;
+  static constexpr int kCodes = 128 * (kTokens + kFeatures), kStageBytes = kCodes + 256 * kScaleLoads;
+  static constexpr int kMeet = WAVES * kTokens * (kFeatures + 4) * 4;
+  static constexpr int kLdsBytes = WAVES * STAGES * kStageBytes > kMeet ? WAVES * STAGES * kStageBytes : kMeet;
+};
+
+template <int NT, int F, int WAVES, int STAGES>
+__global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const Fp8Args p) {
+  using Tile = Fp8Stream<NT, F, WAVES, STAGES>;
+  constexpr int TT = Tile::kTokens, FF = Tile::kFeatures, kXLoads = TT / 8, kWLoads = FF / 8, kLoads = kXLoads + kWLoads + Tile::kScaleLoads, AHEAD = STAGES - 1;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, q = lane >> 4;
+  const int ttiles = (p.tokens + TT - 1) / TT, groups = (p.m + FF - 1) / FF, units = ttiles * groups * p.splits, per_xcd = (units + 7) >> 3;
+  const int u = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per_xcd || u >= units) return;
+  const int tt = u % ttiles, z = (u / ttiles) % p.splits, fg = u / (ttiles * p.splits);
+  const int t0 = tt * TT, f0 = fg * FF;
+  const int blocks = (p.k + 127) >> 7;
+  const int c0 = (int)((long)z * blocks / p.splits), all = (int)((long)(z + 1) * blocks / p.splits) - c0;
+  const int rot = p.rotate ? (int)((long)fg * all / groups) : 0;
+  const int n = wave < all ? (all - wave + WAVES - 1) / WAVES : 0;      // of the wavefront
+
+  const uint8_t *x0 = p.x + (long)t0 * p.x_stride + 128L * c0, *w0 = p.w + (long)f0 * p.w_stride + 128L * c0;
+  uint32_t src[kXLoads + kWLoads];
+  const int lane_piece = (lane & 7) ^ (lane >> 3);
+#pragma unroll
+  for (int i = 0; i < kXLoads + kWLoads; i++) {
+    const bool is_x = i < kXLoads;
+    const int row = 8 * (is_x ? i : i - kXLoads) + (lane >> 3);
+    src[i] = (is_x ? (uint32_t)min(row, p.tokens - 1 - t0) * (uint32_t)p.x_stride : (uint32_t)min(row, p.m - 1 - f0) * (uint32_t)p.w_stride) + 16 * lane_piece;
+  }
+  const float* scale_src[Tile::kScaleLoads];
+  long scale_step[Tile::kScaleLoads];
+#pragma unroll
+  for (int i = 0; i < Tile::kScaleLoads; i++) {
+    const int e = 64 * i + lane;
+    scale_src[i] = e < TT ? p.xs + (long)min(t0 + e, p.tokens - 1) * p.xs_token + c0 * p.xs_block : p.ws + (long)(f0 >> 7) * p.ws_row + c0 * p.ws_block;
+    scale_step[i] = e < TT ? p.xs_block : p.ws_block;
+  }
+  const int odd_block = p.k % 128 ? blocks - 1 - c0 : -1;
+  const uint32_t back = 128 * (blocks - 1) + 16 * lane_piece >= p.k ? 16 * lane_piece : 0;
+  const uint32_t ring = wave * STAGES * Tile::kStageBytes, lds0 = (uint32_t)(uintptr_t)smem + ring;
+  auto block_of = [&](int c) {
+    const int b = wave + WAVES * c + rot;
+    return b < all ? b : b - all;
+  };
+  auto issue = [&](int c, int stage) {
+    const int b = block_of(c);
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + stage * Tile::kStageBytes), less = b == odd_block ? back : 0;
+#pragma unroll
+    for (int i = 0; i < kXLoads + kWLoads; i++) direct_load(src[i] - less, (i < kXLoads ? x0 : w0) + 128L * b, to + 1024 * i);
+#pragma unroll
+    for (int i = 0; i < Tile::kScaleLoads; i++) direct_load4(scale_src[i] + b * scale_step[i], to + Tile::kCodes + 256 * i);
+  };
+
+  float4_t acc[F][NT];
+#pragma unroll
+  for (int f = 0; f < F; f++)
+#pragma unroll
+    for (int t = 0; t < NT; t++) acc[f][t] = float4_t{0.f, 0.f, 0.f, 0.f};
+  const int piece = (q ^ (r & 7)) * 16;
+  auto compute = [&](int c, int stage) {
+    unsigned char* s = smem + ring + stage * Tile::kStageBytes;
+    if (block_of(c) == odd_block && back != 0) {
+#pragma unroll
+      for (int i = 0; i < kXLoads + kWLoads; i++) *reinterpret_cast<uint4_t*>(s + 1024 * i + 16 * lane) = uint4_t{0, 0, 0, 0};
+    }
+    const float* scales = reinterpret_cast<const float*>(s + Tile::kCodes);
+    const float sw = scales[TT];
+    fp8_v8 w[F], x[NT];
+    float scale[NT];
+#pragma unroll
+    for (int f = 0; f < F; f++) w[f] = fp8_operand(s + 128 * TT + 2048 * f + 128 * r, piece);
+#pragma unroll
+    for (int t = 0; t < NT; t++) x[t] = fp8_operand(s + 2048 * t + 128 * r, piece), scale[t] = scales[16 * t + r] * sw;
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int f = 0; f < F; f++) {
+        const float4_t d = fp8_mma(w[f], x[t]);
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[f][t][j] = __builtin_fmaf(d[j], scale[t], acc[f][t][j]);
+      }
+  };
+
+#pragma unroll
+  for (int c = 0; c < AHEAD; c++)
+    if (c < n) issue(c, c);
+  int stage = 0;
+  for (int c = 0; c < n; c++) {
+    // (the place that block c + AHEAD takes was read in the turn before)
+    if (c + AHEAD < n) issue(c + AHEAD, stage == 0 ? STAGES - 1 : stage - 1);
+    fp8_wait<AHEAD, kLoads>(n - 1 - c);
+    compute(c, stage);
+    __builtin_amdgcn_sched_barrier(0);
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+  }
+
+  // the wavefronts' sums, in their order
+  __syncthreads();
+  float* meet = reinterpret_cast<float*>(smem);
+  constexpr int kStride = FF + 4;
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int f = 0; f < F; f++) *reinterpret_cast<float4_t*>(meet + (wave * TT + 16 * t + r) * kStride + 16 * f + 4 * q) = acc[f][t];
+  __syncthreads();
+  for (int e = threadIdx.x; e < TT * FF / 4; e += Tile::kThreads) {
+    const int token = e / (FF / 4), j = 4 * (e % (FF / 4));
+    if (t0 + token >= p.tokens || f0 + j >= p.m) continue;
+    float4_t sum = *reinterpret_cast<const float4_t*>(meet + token * kStride + j);
+#pragma unroll
+    for (int w = 1; w < WAVES; w++) sum += *reinterpret_cast<const float4_t*>(meet + (w * TT + token) * kStride + j);
+    fp8_result(p, z, t0 + token, f0 + j, sum);
   }
 }
 

@@ -84,6 +84,7 @@ SIGNATURES = {
                                      + [_c_int] * 9 + [_c_float, _c_vp, _c_sz] + [_c_int] * 2 + [_c_vp]),
     "triteia_hip_fp8_quantize": (_c_int, [_c_vp, _c_long] + [_c_int] * 3 + [_c_vp, _c_long, _c_vp, _c_long, _c_long] + [_c_int] * 2 + [_c_vp]),
     "triteia_hip_fp8_values": (_c_int, [_c_vp, _c_long, _c_vp, _c_long, _c_long] + [_c_int] * 3 + [_c_vp] + [_c_int] * 2 + [_c_vp]),
+    "triteia_hip_fp8_tile": (_c_int, [_c_int] * 3),
     "triteia_hip_fp8_scratch_bytes": (_c_sz, [_c_int] * 4),
     "triteia_hip_fp8_matmul": (_c_int, [_c_vp, _c_long, _c_int, _c_vp, _c_long, _c_long, _c_vp, _c_long, _c_vp, _c_long, _c_long, _c_vp] + [_c_int] * 4
                                + [_c_vp, _c_sz, _c_int, _c_vp]),

@@ -17,7 +17,7 @@ def _blocks(n):
 def _adjacent(t, rows):
     """Rows of adjacent elements that start on 16 bytes: `t` [rows, k] itself, or a copy."""
     t = t.reshape(rows, t.shape[-1])
-    if t.is_neg() or (t.numel() and (t.stride(1) != 1 or t.stride(0) < 0 or t.stride(0) * t.element_size() % 16 or t.data_ptr() % 16)):
+    if t.is_neg() or (t.numel() and (t.stride(1) != 1 or not 0 <= t.stride(0) <= 1 << 24 or t.stride(0) * t.element_size() % 16 or t.data_ptr() % 16)):
         return t.resolve_neg().clone(memory_format=torch.contiguous_format)
     return t
 
@@ -80,8 +80,8 @@ def matmul_fp8(x, weight, weight_scale, x_scale, dtype):
         raise RuntimeError(f"weight must be [features, elements] in torch.float8_e4m3fn, got {tuple(weight.shape)} in {weight.dtype}")
     m, k = weight.shape
     _width("weight", k)
-    if m and (weight.stride(1) != 1 or weight.stride(0) < 0 or weight.stride(0) % 16 or weight.data_ptr() % 16):
-        raise RuntimeError(f"weight's rows must be of adjacent elements and start on 16 bytes, got strides {weight.stride()}")
+    if m and (weight.stride(1) != 1 or not 0 <= weight.stride(0) <= 1 << 24 or weight.stride(0) % 16 or weight.data_ptr() % 16 or weight.is_neg()):
+        raise RuntimeError(f"weight's rows must be of adjacent elements, start on 16 bytes and lie up to 2^24 elements apart, got strides {weight.stride()}")
     weight_scale = _scales("weight_scale", weight_scale, _blocks(m), k)
     codes = x.dtype == torch.float8_e4m3fn
     if not codes and x.dtype not in (torch.float16, torch.bfloat16):
