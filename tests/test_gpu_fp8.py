@@ -197,6 +197,29 @@ def test_every_tile(tile):
         assert torch.equal(*twice)
 
 
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("tokens", [1, 3, 4, 5, 8])
+def test_few_tokens_quantised_on_the_way(tokens, dtype):
+    """The bits of the quantiser and the product apart, for any K, values that are no numbers and views among the inputs."""
+    from triteia_amd.python.capi import _ffi
+    for k, m in ((16, 16), (48, 40), (128, 1000), (144, 129), (1040, 3001), (2000, 515), (4096, 4096), (11024, 1027)):
+        x = (randn(tokens, k, seed=k) * torch.exp(2 * randn(k, seed=1))).to(dtype).cuda()
+        w, ws = (t.cuda() for t in weight(m, k, seed=4))
+        if tokens <= 4 and _ffi.lib().triteia_hip_fp8_tile(tokens, m, k) == 1016016:
+            assert _ffi.lib().triteia_hip_fp8_scratch_bytes(tokens, m, k, 0) == 0
+        for bad in (None, math.inf, math.nan):
+            if bad is not None:
+                x[tokens // 2, k - 1] = bad
+                x[0, :min(k, 128)] = 0
+            x8, xs = ops().quantize_fp8(x)
+            want = ops().matmul_fp8(x8, w, ws, x_scale=xs, dtype=torch.float32)
+            wide = torch.full((tokens + 1, k + 200), math.nan, dtype=dtype, device="cuda")
+            wide[:tokens, 72:72 + k] = x
+            for view in (x, wide[:tokens, 72:72 + k], x.clone()):
+                got = ops().matmul_fp8(view, w, ws, dtype=torch.float32)
+                assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
+
+
 def test_shares_of_k_are_tested():
     assert sum(split for _, split in sizes_of_every_tile()) >= 3
 

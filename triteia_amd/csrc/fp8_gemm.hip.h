@@ -8,12 +8,13 @@
 // and these sums in 32 bits.  Random codes come out 1.3e-5 off in norm; the codes themselves are 2e-2 off what they stand for.  Sums that are exact to 32 bits would take the
 // instruction of 16 bits on widened codes, at half the rate.
 #pragma once
+#include "fp8_quant.hip.h"
 #include "sparse24_gemm.hip.h"
 
 namespace triteia_hip {
 
 struct Fp8Args {
-  const uint8_t* x;       // [tokens, k]
+  const uint8_t* x;       // [tokens, k] (fp8_stream_kernel on 16 bits: of those)
   long x_stride;          // up to 2^24, as w_stride: a tile's rows are 32-bit offsets apart
   const float* xs;        // [tokens, blocks] by strides
   long xs_token, xs_block;
@@ -236,19 +237,26 @@ __global__ __launch_bounds__(64 * TW * FW) void fp8_tile_kernel(const Fp8Args p)
 // Few tokens: bound by the weights' way from HBM, on small layers by a launch and its round trips.  A workgroup takes 16 F features and 16 NT tokens at most; its
 // wavefronts take turns at the blocks of K, each with a ring of its own in LDS, so that nothing is waited for but a wavefront's own requests; their sums
 // meet once at the end.
-template <int NT, int F, int WAVES, int STAGES>
+// T: what x holds, codes (uint8_t) or, for up to 4 tokens, values of 16 bits that the wavefront quantises block by block (as fp8_quant_rows_kernel does, 16 lanes a
+// row), every workgroup for itself: a launch less, and no scratch.
+template <class T, int NT, int F, int WAVES, int STAGES>
 struct Fp8Stream {
+  static constexpr bool kQuant = !__is_same(T, uint8_t);
   static constexpr int kTokens = 16 * NT, kFeatures = 16 * F, kThreads = 64 * WAVES;
-  static constexpr int kScaleLoads = (kTokens + 1 + 63) / 64;
-  static constexpr int kCodes = 128 * (kTokens + kFeatures), kStageBytes = kCodes + 256 * kScaleLoads;
+  static constexpr int kXLoads = kQuant ? 1 : kTokens / 8, kWLoads = kFeatures / 8;
+  static constexpr int kScaleLoads = kQuant ? 1 : (kTokens + 1 + 63) / 64;
+  static constexpr int kCodes = 1024 * (kXLoads + kWLoads), kStageBytes = kCodes + 256 * kScaleLoads;
+  static constexpr int kOwnBytes = kQuant ? 128 * kTokens + 4 * kTokens : 0;       // a wavefront's codes and scales of the block that it multiplies
+  static constexpr int kWaveBytes = STAGES * kStageBytes + kOwnBytes;
   static constexpr int kMeet = WAVES * kTokens * (kFeatures + 4) * 4;
-  static constexpr int kLdsBytes = WAVES * STAGES * kStageBytes > kMeet ? WAVES * STAGES * kStageBytes : kMeet;
+  static constexpr int kLdsBytes = WAVES * kWaveBytes > kMeet ? WAVES * kWaveBytes : kMeet;
+  static_assert(!kQuant || (NT == 1 && kOwnBytes % 16 == 0), "");
 };
 
-template <int NT, int F, int WAVES, int STAGES>
+template <class T, int NT, int F, int WAVES, int STAGES>
 __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const Fp8Args p) {
-  using Tile = Fp8Stream<NT, F, WAVES, STAGES>;
-  constexpr int TT = Tile::kTokens, FF = Tile::kFeatures, kXLoads = TT / 8, kWLoads = FF / 8, kLoads = kXLoads + kWLoads + Tile::kScaleLoads, AHEAD = STAGES - 1;
+  using Tile = Fp8Stream<T, NT, F, WAVES, STAGES>;
+  constexpr int TT = Tile::kTokens, FF = Tile::kFeatures, kXLoads = Tile::kXLoads, kWLoads = Tile::kWLoads, kLoads = kXLoads + kWLoads + Tile::kScaleLoads, AHEAD = STAGES - 1;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
@@ -262,7 +270,8 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const Fp8Args p)
   const int rot = p.rotate ? (int)((long)fg * all / groups) : 0;
   const int n = wave < all ? (all - wave + WAVES - 1) / WAVES : 0;      // of the wavefront
 
-  const uint8_t *x0 = p.x + (long)t0 * p.x_stride + 128L * c0, *w0 = p.w + (long)f0 * p.w_stride + 128L * c0;
+  constexpr int kXBlock = Tile::kQuant ? 256 : 128;                     // bytes of a row
+  const uint8_t *x0 = p.x + (long)t0 * p.x_stride * (kXBlock / 128) + (long)kXBlock * c0, *w0 = p.w + (long)f0 * p.w_stride + 128L * c0;
   uint32_t src[kXLoads + kWLoads];
   const int lane_piece = (lane & 7) ^ (lane >> 3);
 #pragma unroll
@@ -270,27 +279,33 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const Fp8Args p)
     const bool is_x = i < kXLoads;
     const int row = 8 * (is_x ? i : i - kXLoads) + (lane >> 3);
     src[i] = (is_x ? (uint32_t)min(row, p.tokens - 1 - t0) * (uint32_t)p.x_stride : (uint32_t)min(row, p.m - 1 - f0) * (uint32_t)p.w_stride) + 16 * lane_piece;
+    if (Tile::kQuant && is_x) src[i] = (uint32_t)min(q, p.tokens - 1) * (uint32_t)p.x_stride * 2 + 16 * r;      // 4 rows in a request
   }
   const float* scale_src[Tile::kScaleLoads];
   long scale_step[Tile::kScaleLoads];
 #pragma unroll
   for (int i = 0; i < Tile::kScaleLoads; i++) {
     const int e = 64 * i + lane;
-    scale_src[i] = e < TT ? p.xs + (long)min(t0 + e, p.tokens - 1) * p.xs_token + c0 * p.xs_block : p.ws + (long)(f0 >> 7) * p.ws_row + c0 * p.ws_block;
-    scale_step[i] = e < TT ? p.xs_block : p.ws_block;
+    const bool is_x = !Tile::kQuant && e < TT;
+    scale_src[i] = is_x ? p.xs + (long)min(t0 + e, p.tokens - 1) * p.xs_token + c0 * p.xs_block : p.ws + (long)(f0 >> 7) * p.ws_row + c0 * p.ws_block;
+    scale_step[i] = is_x ? p.xs_block : p.ws_block;
   }
+  // (a last block that is not whole: as in fp8_tile_kernel)
   const int odd_block = p.k % 128 ? blocks - 1 - c0 : -1;
-  const uint32_t back = 128 * (blocks - 1) + 16 * lane_piece >= p.k ? 16 * lane_piece : 0;
-  const uint32_t ring = wave * STAGES * Tile::kStageBytes, lds0 = (uint32_t)(uintptr_t)smem + ring;
+  const uint32_t back = 128 * (blocks - 1) + 16 * lane_piece >= p.k ? 16 * lane_piece : 0, back_x = 128 * (blocks - 1) + 8 * r >= p.k ? 16 * r : 0;
+  const uint32_t ring = wave * Tile::kWaveBytes, lds0 = (uint32_t)(uintptr_t)smem + ring;
   auto block_of = [&](int c) {
     const int b = wave + WAVES * c + rot;
     return b < all ? b : b - all;
   };
   auto issue = [&](int c, int stage) {
     const int b = block_of(c);
-    const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + stage * Tile::kStageBytes), less = b == odd_block ? back : 0;
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + stage * Tile::kStageBytes), less = b == odd_block ? back : 0, less_x = b != odd_block ? 0 : Tile::kQuant ? back_x : back;
 #pragma unroll
-    for (int i = 0; i < kXLoads + kWLoads; i++) direct_load(src[i] - less, (i < kXLoads ? x0 : w0) + 128L * b, to + 1024 * i);
+    for (int i = 0; i < kXLoads + kWLoads; i++) {
+      if (i < kXLoads) direct_load(src[i] - less_x, x0 + (long)kXBlock * b, to + 1024 * i);
+      else direct_load(src[i] - less, w0 + 128L * b, to + 1024 * i);
+    }
 #pragma unroll
     for (int i = 0; i < Tile::kScaleLoads; i++) direct_load4(scale_src[i] + b * scale_step[i], to + Tile::kCodes + 256 * i);
   };
@@ -303,18 +318,32 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const Fp8Args p)
   const int piece = (q ^ (r & 7)) * 16;
   auto compute = [&](int c, int stage) {
     unsigned char* s = smem + ring + stage * Tile::kStageBytes;
-    if (block_of(c) == odd_block && back != 0) {
+    const bool odd = block_of(c) == odd_block;
+    if (odd && back != 0) {
 #pragma unroll
-      for (int i = 0; i < kXLoads + kWLoads; i++) *reinterpret_cast<uint4_t*>(s + 1024 * i + 16 * lane) = uint4_t{0, 0, 0, 0};
+      for (int i = Tile::kQuant ? kXLoads : 0; i < kXLoads + kWLoads; i++) *reinterpret_cast<uint4_t*>(s + 1024 * i + 16 * lane) = uint4_t{0, 0, 0, 0};
     }
     const float* scales = reinterpret_cast<const float*>(s + Tile::kCodes);
-    const float sw = scales[TT];
+    const float sw = scales[Tile::kQuant ? 0 : TT];
+    unsigned char* own = Tile::kQuant ? smem + ring + STAGES * Tile::kStageBytes : s;
+    float* own_scales = reinterpret_cast<float*>(Tile::kQuant ? own + 128 * TT : s + Tile::kCodes);
+    if constexpr (Tile::kQuant) {
+      kv8<T> v = *reinterpret_cast<const kv8<T>*>(s + 16 * lane);
+      if (odd && back_x != 0) v = kv8<T>{0, 0, 0, 0, 0, 0, 0, 0};
+      float scale;
+      const kv_uint2 code = fp8_quantised<T>(v, &scale);
+      *reinterpret_cast<kv_uint2*>(own + 128 * q + ((r / 2) ^ q) * 16 + 8 * (r & 1)) = code;
+      if (r == 0) own_scales[q] = scale;
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");      // (the wavefront's own: its lanes run together)
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    }
     fp8_v8 w[F], x[NT];
     float scale[NT];
 #pragma unroll
-    for (int f = 0; f < F; f++) w[f] = fp8_operand(s + 128 * TT + 2048 * f + 128 * r, piece);
+    for (int f = 0; f < F; f++) w[f] = fp8_operand(s + 1024 * kXLoads + 2048 * f + 128 * r, piece);
 #pragma unroll
-    for (int t = 0; t < NT; t++) x[t] = fp8_operand(s + 2048 * t + 128 * r, piece), scale[t] = scales[16 * t + r] * sw;
+    for (int t = 0; t < NT; t++) x[t] = fp8_operand(own + 2048 * t + 128 * r, piece), scale[t] = own_scales[16 * t + r] * sw;
 #pragma unroll
     for (int t = 0; t < NT; t++)
 #pragma unroll

@@ -39,6 +39,16 @@ __device__ __forceinline__ uint32_t fp8_top(const kv8<T>& v, float (&x)[8]) {
   return top;
 }
 
+// 8 values of a row of a block, which 16 lanes hold: their codes and the block's scale
+template <class T>
+__device__ __forceinline__ kv_uint2 fp8_quantised(const kv8<T>& v, float* scale) {
+  float x[8], inv;
+  const uint32_t top = across_row<16>(fp8_top<T>(v, x), [](uint32_t p, uint32_t q) { return max(p, q); });
+  fp8_scale(top, scale, &inv);
+  const kv_uint2 code = codes_of<kCacheFp8>(x, *scale, inv);
+  return top >= 0x7f800000u ? kv_uint2{0, 0} : code;
+}
+
 // Rows by themselves.  A workgroup takes 16 rows x U blocks.  1-D grid (row groups x block groups, block groups fastest), block 256
 template <class T, int U>
 __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(Fp8QuantArgs a) {
@@ -55,11 +65,8 @@ __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(Fp8QuantArgs a) {
   }
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    float x[8], scale, inv;
-    const uint32_t top = across_row<16>(fp8_top<T>(v[u], x), [](uint32_t p, uint32_t q) { return max(p, q); });
-    fp8_scale(top, &scale, &inv);
-    kv_uint2 code = codes_of<kCacheFp8>(x, scale, inv);
-    if (top >= 0x7f800000u) code = kv_uint2{0, 0};
+    float scale;
+    const kv_uint2 code = fp8_quantised<T>(v[u], &scale);
     const int e = kFp8Block * (b0 + u) + 8 * lane;
     if (row >= a.n || e >= a.k) continue;
     *reinterpret_cast<kv_uint2*>(a.codes + row * a.codes_stride + e) = code;
