@@ -115,7 +115,10 @@ void launch_attend(AttendArgs a, const AttnLayout& layout, float* scratch, long 
     a.part_ml[which] = scratch + (long)l.max_parts * a.kv_heads * l.rows * D;
     scratch = a.part_ml[which] + 2L * l.max_parts * a.kv_heads * l.rows;
   }
-  if (layout.n_groups > 0) joins = (int)std::min<long>(kAttnJoiners, ((long)a.list[0].max_joins * a.list[0].rows + (long)a.list[1].max_joins * a.list[1].rows) / (1024 / D) * a.kv_heads);
+  if (layout.n_groups > 0) {                       // (every row of a group is joined)
+    const long bound = ((long)a.list[0].max_joins * a.list[0].rows + (long)a.list[1].max_joins * a.list[1].rows) / (1024 / D) * a.kv_heads;
+    joins = (int)std::min<long>(kAttnSharedJoiners, bound);
+  }
   a.joined = joins > 0;
   const dim3 grid((unsigned)((long)(a.list[0].max_items + a.list[1].max_items) * a.kv_heads));
   if (a.list[1].max_items > 0) hipLaunchKernelGGL((attend_mixed_kernel<T, KIND, D>), grid, dim3(256), 0, stream, a);
@@ -123,9 +126,8 @@ void launch_attend(AttendArgs a, const AttnLayout& layout, float* scratch, long 
   else if (a.list[0].rows == 16) hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 1, 4>), grid, dim3(256), 0, stream, a);
   else if (a.list[0].waves == 8) hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 2, 8>), grid, dim3(512), 0, stream, a);
   else hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 2, 4>), grid, dim3(256), 0, stream, a);
-  const dim3 joiners(joins < kAttnJoiners ? joins : kAttnJoiners);
-  if (layout.n_groups > 0) hipLaunchKernelGGL((attend_join_kernel<T, D, true>), joiners, dim3(256), 0, stream, a);
-  else if (joins > 0) hipLaunchKernelGGL((attend_join_kernel<T, D, false>), joiners, dim3(256), 0, stream, a);
+  if (layout.n_groups > 0) hipLaunchKernelGGL((attend_join_shared_kernel<T, D>), dim3(joins), dim3(256), 0, stream, a);
+  else if (joins > 0) hipLaunchKernelGGL((attend_join_kernel<T, D>), dim3(joins < kAttnJoiners ? joins : kAttnJoiners), dim3(256), 0, stream, a);
 }
 struct AttendLaunch {
   const AttendArgs& a;

@@ -211,6 +211,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const 
   const AttnList& l = a.list[which];
   if (l.max_items == 0) {
     if (lane < 2) plan[2 * which + lane] = 0;
+    if (SHARED && lane == 0) plan[4 + which] = 0;
     if constexpr (SHARED) __syncthreads();
     return;
   }
@@ -297,7 +298,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const 
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
   }
-  int n_items = 0, n_joins = 0, n_parts = 0;
+  int n_items = 0, n_joins = 0, n_parts = 0, fullest = 0;        // fullest: rows of a tile that is joined, at most
   int end_items = l.max_items, end_joins = l.max_joins;          // (all have a place: the cut leaves no more shares than the host has counted)
   for (int i0 = 0; i0 < tiles; i0 += 64) {
     // (of long lists a sequence's last tile, its longest, first)
@@ -329,6 +330,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const 
         j.prefix_list = rows <= a.short_rows ? 0 : 1;
         j.prefix_tile = tiles_ahead[j.prefix_list][t.home], j.prefix_row = (t.s.start - start[t.home]) * a.group;
       }
+      if (SHARED && joins) fullest = max(fullest, min(l.rows, t.s.n * a.group - t.tile * l.rows));
       if (joins) reinterpret_cast<AttnJoin*>(plan + l.joins)[join] = j;
       if (SHARED && t.home == -2) plan[l.prefixes + 2L * i] = part, plan[l.prefixes + 2L * i + 1] = splits;
     }
@@ -337,6 +339,11 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const 
 #pragma unroll
   for (int d = 32; d > 0; d /= 2) end_items = min(end_items, __shfl_xor(end_items, d)), end_joins = min(end_joins, __shfl_xor(end_joins, d));
   if (lane == 0) plan[2 * which] = min(n_items, end_items), plan[2 * which + 1] = min(n_joins, end_joins);
+  if constexpr (SHARED) {
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) fullest = max(fullest, __shfl_xor(fullest, d));
+    if (lane == 0) plan[4 + which] = fullest;
+  }
 }
 
 }  // namespace triteia_hip

@@ -902,9 +902,8 @@ __global__ __launch_bounds__(256, 2) void attend_mixed_kernel(AttendArgs a) {
 // between them, the shares: a group adds every n-th share, the groups' sums are added in their order.  The host knows bounds only, mostly far above
 // what there is to join, so a fixed number of workgroups walks what the plan says: one for every place of the bound took 10 to 15 us of a prompt's 180 to
 // 370 to find that nothing was cut.  grid up to kAttnJoiners, block 256
-// SHARED: a tile of a group has the shares of its group's prefix behind its own, in the place of the prefix's tiles that its rows have there.
 constexpr int kAttnJoiners = 1024;
-template <class T, int D, bool SHARED>
+template <class T, int D>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
   __shared__ attn_f4 sums[256];
@@ -915,7 +914,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
     const int which = next < short_units ? 0 : 1, unit = next - (which ? short_units : 0);
     const int rows = a.list[which].rows, pieces = rows / kGroups, piece = unit % pieces, index = unit / pieces / a.kv_heads, head = unit / pieces - index * a.kv_heads;
     const int* j = a.plan + a.list[which].joins + 8L * index;
-    const int q_start = j[0], n_tokens = j[1], tile = j[2], first = j[3], n_own = j[4];
+    const int q_start = j[0], n_tokens = j[1], tile = j[2], first = j[3], n_parts = j[4];
     const int r0 = kGroups * piece, live = min(kGroups, n_tokens * a.group - tile * rows - r0);
     if (live <= 0) continue;
     const float *part_o = a.part_o[which], *part_ml = a.part_ml[which];
@@ -923,27 +922,15 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
     while (wide < live) wide *= 2;
     const int i = group % wide, n = kGroups / wide;
     const long step = (long)a.kv_heads * rows, at = ((long)first * a.kv_heads + head) * rows + r0 + min(i, live - 1);
-    int n_parts = n_own;
-    const float *prefix_o = nullptr, *prefix_ml = nullptr;
-    long prefix_step = 0, prefix_at = 0;
-    if (SHARED && j[5] >= 0) {
-      const int prefix_rows = a.list[j[5]].rows, row = j[7] + tile * rows + r0 + min(i, live - 1);
-      const int* p = a.plan + a.list[j[5]].prefixes + 2L * (j[6] + row / prefix_rows);
-      prefix_o = a.part_o[j[5]], prefix_ml = a.part_ml[j[5]], prefix_step = (long)a.kv_heads * prefix_rows;
-      prefix_at = ((long)p[0] * a.kv_heads + head) * prefix_rows + row % prefix_rows, n_parts += p[1];
-    }
-    auto place = [&](int p) { return !SHARED || p < n_own ? at + p * step : prefix_at + (p - n_own) * prefix_step; };
-    auto ml = [&](int p) { return !SHARED || p < n_own ? part_ml : prefix_ml; };
-    auto o = [&](int p) { return !SHARED || p < n_own ? part_o : prefix_o; };
     float top = kAttnNone, sum = 0.f;
 #pragma unroll 4
-    for (int p = 0; p < n_parts; p++) top = fmaxf(top, ml(p)[2 * place(p)]);
+    for (int p = 0; p < n_parts; p++) top = fmaxf(top, part_ml[2 * (at + p * step)]);
     attn_f4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int p = group / wide; p < n_parts; p += n) {
-      const float f = __builtin_amdgcn_exp2f(ml(p)[2 * place(p)] - top);
-      sum += f * ml(p)[2 * place(p) + 1];
-      const attn_f4 y = *reinterpret_cast<const attn_f4*>(o(p) + place(p) * D + d);
+      const float f = __builtin_amdgcn_exp2f(part_ml[2 * (at + p * step)] - top);
+      sum += f * part_ml[2 * (at + p * step) + 1];
+      const attn_f4 y = *reinterpret_cast<const attn_f4*>(part_o + (at + p * step) * D + d);
 #pragma unroll
       for (int k = 0; k < 4; k++) x[k] = __builtin_fmaf(y[k], f, x[k]);
     }
@@ -955,6 +942,98 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
         x += sums[threadIdx.x + g * wide * kLanes];
         sum += totals[group + g * wide];
       }
+      const int row = tile * rows + r0 + group, token = row / a.group, g = row - token * a.group;
+      typedef T t4 __attribute__((ext_vector_type(4)));
+      t4 y;
+#pragma unroll
+      for (int k = 0; k < 4; k++) y[k] = sum == 0.f ? (T)0.f : (T)(x[k] / sum);
+      *reinterpret_cast<t4*>(static_cast<T*>(a.out) + ((long)(q_start + token) * (a.kv_heads * a.group) + head * a.group + g) * D + d) = y;
+    }
+    __syncthreads();
+  }
+}
+
+// The same for batches in groups that share a prefix: a tile of a group has the shares of its group's prefix behind its own, in the prefix's tiles that hold its rows.  Every
+// row is joined, so this is as long as its round trips: a lane group requests eight shares at once, statistics and sums together, and takes them in under a
+// running maximum; the plan says how many rows the fullest tile has, so that a unit has work.  (Two passes over the shares, one for the maxima, on 1024 workgroups took
+// 14 us for 64 requests of 64 heads and 23 for 96 of 32 + 32.)  grid up to kAttnSharedJoiners, block 256
+constexpr int kAttnSharedJoiners = 4096;
+template <class T, int D>
+__global__ __launch_bounds__(256) void attend_join_shared_kernel(AttendArgs a) {
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes, kAtOnce = 8;
+  __shared__ attn_f4 sums[256];
+  __shared__ float tops[kGroups], totals[kGroups];
+  int pieces[2], units[2];
+#pragma unroll
+  for (int which = 0; which < 2; which++) {
+    pieces[which] = (a.plan[4 + which] + kGroups - 1) / kGroups;
+    units[which] = a.plan[2 * which + 1] * a.kv_heads * pieces[which];
+  }
+  const int group = threadIdx.x / kLanes, d = 4 * (threadIdx.x % kLanes);
+  for (int next = blockIdx.x; next < units[0] + units[1]; next += gridDim.x) {
+    const int which = next < units[0] ? 0 : 1, unit = next - (which ? units[0] : 0);
+    const int rows = a.list[which].rows, piece = unit % pieces[which], index = unit / pieces[which] / a.kv_heads, head = unit / pieces[which] - index * a.kv_heads;
+    const int* j = a.plan + a.list[which].joins + 8L * index;
+    const int q_start = j[0], n_tokens = j[1], tile = j[2], first = j[3], n_own = j[4], prefix_list = j[5], prefix_tile = j[6], prefix_row = j[7];
+    const int r0 = kGroups * piece, live = min(min(kGroups, rows - r0), n_tokens * a.group - tile * rows - r0);
+    if (live <= 0) continue;
+    int wide = 1;                                  // rows side by side
+    while (wide < live) wide *= 2;
+    const int i = group % wide, n = kGroups / wide, mine = r0 + min(i, live - 1);
+    const long step = (long)a.kv_heads * rows, at = ((long)first * a.kv_heads + head) * rows + mine;
+    const float *own_o = a.part_o[which], *own_ml = a.part_ml[which], *prefix_o = own_o, *prefix_ml = own_ml;
+    int n_parts = n_own;
+    long prefix_step = 0, prefix_at = 0;
+    if (prefix_list >= 0) {
+      const int prefix_rows = a.list[prefix_list].rows, row = prefix_row + tile * rows + mine;
+      const int* p = a.plan + a.list[prefix_list].prefixes + 2L * (prefix_tile + row / prefix_rows);
+      prefix_o = a.part_o[prefix_list], prefix_ml = a.part_ml[prefix_list], prefix_step = (long)a.kv_heads * prefix_rows;
+      prefix_at = ((long)p[0] * a.kv_heads + head) * prefix_rows + row % prefix_rows, n_parts += p[1];
+    }
+    float top = kAttnNone, sum = 0.f;
+    attn_f4 x = {0.f, 0.f, 0.f, 0.f};
+    typedef float ml2 __attribute__((ext_vector_type(2)));
+    for (int p0 = group / wide; p0 < n_parts; p0 += kAtOnce * n) {
+      ml2 ml[kAtOnce];
+      attn_f4 o[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; k++) {
+        const int p = p0 + k * n;
+        const bool own = p < n_own;
+        const long place = own ? at + p * step : prefix_at + (p - n_own) * prefix_step;
+        ml[k] = ml2{kAttnNone, 0.f}, o[k] = attn_f4{0.f, 0.f, 0.f, 0.f};
+        if (p < n_parts) ml[k] = reinterpret_cast<const ml2*>(own ? own_ml : prefix_ml)[place], o[k] = *reinterpret_cast<const attn_f4*>((own ? own_o : prefix_o) + place * D + d);
+      }
+      float high = top;
+#pragma unroll
+      for (int k = 0; k < kAtOnce; k++) high = fmaxf(high, ml[k].x);
+      const float back = __builtin_amdgcn_exp2f(top - high);
+      sum *= back, x *= back, top = high;
+#pragma unroll
+      for (int k = 0; k < kAtOnce; k++) {
+        const float f = p0 + k * n < n_parts ? __builtin_amdgcn_exp2f(ml[k].x - top) : 0.f;
+        sum = __builtin_fmaf(f, ml[k].y, sum);
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = __builtin_fmaf(o[k][e], f, x[e]);
+      }
+    }
+    if (n > 1) {
+      sums[threadIdx.x] = x;
+      if (d == 0) tops[group] = top, totals[group] = sum;
+      __syncthreads();
+      if (group < live) {
+        float high = top;
+        for (int g = 1; g < n; g++) high = fmaxf(high, tops[group + g * wide]);
+        float f = __builtin_amdgcn_exp2f(top - high);
+        sum *= f, x *= f;
+        for (int g = 1; g < n; g++) {
+          f = __builtin_amdgcn_exp2f(tops[group + g * wide] - high);
+          sum = __builtin_fmaf(f, totals[group + g * wide], sum);
+          x += sums[threadIdx.x + g * wide * kLanes] * f;
+        }
+      }
+    }
+    if (group < live) {
       const int row = tile * rows + r0 + group, token = row / a.group, g = row - token * a.group;
       typedef T t4 __attribute__((ext_vector_type(4)));
       t4 y;
