@@ -42,12 +42,15 @@ class Shared(Batch):
                 self.pages[b, :whole], self.pages[b, whole:whole + mine] = shared, order[at:at + mine]
                 at += mine
                 k, v = (torch.cat([x, torch.randn((own, kv_heads, dim), generator=g) * big]) for x in first)
-                place = self.slots(b, torch.arange(kv))
-                ops().cache_write(self.cache, k.to(dtype).cuda(), v.to(dtype).cuda(), place)
-                for keep, raw, scale in ((self.k, self.cache.k, self.cache.k_scale), (self.v, self.cache.v, self.cache.v_scale)):
-                    x = rows_of(raw, page)[place.cpu()].double()
-                    keep.append(x if scale is None else x * rows_of(scale, page)[place.cpu()].double()[..., None])
+                ops().cache_write(self.cache, k.to(dtype).cuda(), v.to(dtype).cuda(), self.slots(b, torch.arange(kv)))
                 b += 1
+        # what the cache holds, from its own codes
+        for keep, raw, scale in ((self.k, self.cache.k, self.cache.k_scale), (self.v, self.cache.v, self.cache.v_scale)):
+            held, scales = rows_of(raw, page), None if scale is None else rows_of(scale, page)
+            for b, (_, kv) in enumerate(self.lengths):
+                place = self.slots(b, torch.arange(kv)).cpu()
+                x = held[place].double()
+                keep.append(x if scale is None else x * scales[place].double()[..., None])
         self.starts = [0]
         for n, _ in self.lengths:
             self.starts.append(self.starts[-1] + n)
@@ -56,26 +59,38 @@ class Shared(Batch):
     def groups(self):
         return dict(group_starts=torch.tensor(self.group_starts or [0], dtype=torch.int32).cuda(), prefix_lens=torch.tensor(self.prefix_lens, dtype=torch.int32).cuda())
 
+    def plan(self, max_q=None, causal=True, window=0, **groups):
+        q, cache, _, starts, lens = self.inputs()
+        return ops().attention_plan(cache, starts, lens, self.heads, q.shape[0], max_q, causal, window, **(groups or self.groups()))
+
     def attend(self, max_q=None, causal=True, window=0, scale=None, **groups):
         q, cache, pages, starts, lens = self.inputs()
-        plan = ops().attention_plan(cache, starts, lens, self.heads, q.shape[0], max_q, causal, window, **(groups or self.groups()))
-        return ops().paged_attention(q, cache, pages, starts, lens, plan=plan, causal=causal, window=window, scale=scale)
+        return ops().paged_attention(q, cache, pages, starts, lens, plan=self.plan(max_q, causal, window, **groups), causal=causal, window=window, scale=scale)
 
 
 DECODES = [(300, [(1, 1), (1, 15), (1, 70)]), (0, [(1, 40), (1, 3)]), (64, [(1, 1), (1, 64)]), (1100, [(1, 5), (1, 130), (1, 1), (1, 200), (1, 64), (1, 63), (1, 65)]),
-           (500, [(1, 20)]), (None, [(1, 90), (1, 1)])]
-CHUNKS = [(None, [(3, 100)]), (190, [(5, 5), (1, 40), (70, 70)]), (400, [(64, 128), (33, 33)]), (1000, [(200, 263), (129, 129), (1, 1), (40, 41)])]
-MANY = [(700, [(1, 1 + 7 * i % 90) for i in range(40)]), (65, [(1, 3)] * 30), (None, [(1, 100)] * 5)]
+           (500, [(1, 20)]), (None, [(1, 90), (1, 1), (1, 900)])]
+CHUNKS = [(None, [(3, 100)]), (190, [(5, 5), (1, 40), (70, 70), (2, 9)]), (400, [(64, 128), (33, 33), (1, 1), (1, 900)]), (1000, [(200, 263), (129, 129), (1, 1), (40, 41), (2, 30)])]
+MANY = [(1900, [(1, 1 + 7 * i % 90) for i in range(24)]), (130, [(1, 3)] * 30), (None, [(1, 100)] * 5)]
+PROMPTS = [(700, [(64, 128), (33, 33), (90, 100)]), (1000, [(200, 263), (129, 129)])]
+
+
+def shared(batch, plan):
+    """Whether the plan has every sequence of a group with a prefix joined from shares: the prefix's and its own."""
+    joins = int(plan.buffer.view(torch.int32)[[1, 3, 5]].sum())
+    at = [b for g, p in enumerate(batch.prefix_lens) if p >= 64 for b in range(batch.group_starts[g], batch.group_starts[g + 1])]
+    return joins >= sum(batch.lengths[b][0] > 0 for b in at) > 0
 
 
 @pytest.mark.parametrize("kind", list(KINDS))
 @pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("heads,kv_heads,page", [(4, 4, 16), (8, 2, 32), (20, 1, 64), (3, 1, 128)])
-@pytest.mark.parametrize("groups", [DECODES, CHUNKS, MANY], ids=["decodes", "chunks", "many"])
+@pytest.mark.parametrize("groups", [DECODES, CHUNKS, MANY, PROMPTS], ids=["decodes", "chunks", "many", "prompts"])
 def test_shared_prefix(kind, dtype, dim, heads, kv_heads, page, groups):
     batch = Shared(groups, heads, kv_heads, dim, page, kind, dtype)
     most = max(n for n, _ in batch.lengths)
+    assert groups is PROMPTS or shared(batch, batch.plan(most))
     batch.check(batch.attend(most))
     batch.check(batch.attend(most, causal=False, scale=0.2), causal=False, scale=0.2)
     batch.check(batch.attend(most, window=50), window=50)
@@ -93,11 +108,11 @@ def test_the_largest_number_of_new_tokens_is_a_hint(kind, most, groups):
 @pytest.mark.parametrize("most", [1, None])
 def test_groups_of_nothing(kind, most):
     """Sequences without new tokens, groups without sequences, new tokens that reach back into the prefix or ahead of the context, no tokens of their own, padding."""
-    batch = Shared([(200, [(0, 0), (1, 30), (0, 10), (1, 7)]), (300, []), (128, [(6, 2), (40, 3)]), (100, [(150, 30), (1, 1)]), (256, [(0, 9), (0, 1)]), (64, []),
+    batch = Shared([(1000, [(0, 0), (1, 30), (0, 10), (1, 7)]), (300, []), (128, [(6, 2), (40, 3)]), (100, [(150, 30), (1, 1)]), (256, [(0, 9), (0, 1)]), (64, []),
                     (None, [(2, 50)])], 6, 2, 64, 16, kind, padding=21)
     batch.check(batch.attend(most))
     batch.check(batch.attend(most, causal=False), causal=False)
-    cross = Shared([(320, [(3, 0), (1, 0), (20, 0)]), (70, [(1, 0), (2, 0)])], 6, 2, 64, 16, kind)
+    cross = Shared([(960, [(3, 0), (1, 0), (20, 0)]), (70, [(1, 0), (2, 0)])], 6, 2, 64, 16, kind)
     cross.check(cross.attend(most, causal=False), causal=False)                 # states that all rows see all of, and nothing else
     none = Shared([(None, [])], padding=3)
     assert not none.attend(most).any()
@@ -115,13 +130,35 @@ def test_prefixes_that_are_cut_into_shares(kind):
             batch.check(batch.attend(most, **how), **how)
 
 
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 32, 64), (30, 30, 128), (64, 32, 128)])
+def test_a_wavefront_for_each_sequence(kind, dtype, heads, kv_heads, dim):
+    """Enough sequences times heads of the cache that each one's own part is a wavefront's; a prompt, sequences that share little and long parts among them."""
+    batch = Shared([(1300, [(1, 1 + 37 * i % 300) for i in range(13)] + [(1, 700)]), (64, [(1, 9), (0, 5), (3, 70)]), (900, [(30, 40), (1, 1), (1, 64)]), (None, [(1, 900), (1, 20)])],
+                   heads, kv_heads, dim, 16, kind, dtype, padding=2)
+    assert shared(batch, batch.plan(1)) and len(batch.lengths) * kv_heads > 512
+    batch.check(batch.attend(1))
+    batch.check(batch.attend(30, causal=False, scale=0.2), causal=False, scale=0.2)
+
+
 @pytest.mark.parametrize("most", [1, None])
 def test_more_groups_and_tiles_than_a_wavefront_has_lanes(most):
-    groups = [(64 * (i % 3) + 5, [(1, 1 + i % 5)] * (1 + i % 4)) for i in range(150)]
-    batch = Shared(groups, 8, 1, 64, 16)
+    groups = [(64 * (15 + i % 3) + 5, [(1, 1 + i % 5)] * (4 + i % 3)) for i in range(75)]
+    batch = Shared(groups, 2, 1, 64, 16)
+    assert shared(batch, batch.plan(most))
     batch.check(batch.attend(most))
     batch = Shared([(130, [(20, 20)] * 6)] * 70, 8, 1, 64, 16)                  # more than 256 tiles
     batch.check(batch.attend(most))
+
+
+def test_sharing_that_does_not_pay():
+    """Short prefixes of a few requests are read again; the answer is the same."""
+    for groups, heads, kv_heads, pays in (([(512, [(1, 20)] * 16)], 64, 8, False), ([(4096, [(1, 20)] * 16)], 16, 8, True), ([(1024, [(1, 9), (1, 40)])], 8, 8, True),
+                                          ([(640, [(1, 10)] * 20)], 32, 32, True), ([(256, [(1, 10)] * 20)], 32, 8, False)):
+        batch = Shared(groups, heads, kv_heads, 64, 64)
+        assert shared(batch, batch.plan(None)) == pays, groups
+        batch.check(batch.attend(None))
 
 
 def test_a_prefix_is_what_the_pages_say():
@@ -139,16 +176,17 @@ def test_a_prefix_is_what_the_pages_say():
 def test_group_offsets_in_no_order(starts):
     """Each is taken as the largest ahead of it, inside the batch: any sequence is in one group at most, and every row is written.  (All share all of the prefix here, so that
     any grouping is right.)"""
-    batch = Shared([(300, [(1, 5), (2, 40), (1, 1), (3, 9), (1, 30), (1, 2), (1, 70)])], 4, 2, 64, 16)
-    for prefixes in ([300, 300, 300], [64, 0, 200]):
+    batch = Shared([(1000, [(1, 5), (2, 40), (1, 1), (3, 9), (1, 30), (1, 2), (1, 70)])], 4, 2, 64, 16)
+    for prefixes in ([1000, 1000, 1000], [64, 0, 800]):
         batch.check(batch.attend(3, group_starts=torch.tensor(starts, dtype=torch.int32).cuda(), prefix_lens=torch.tensor(prefixes, dtype=torch.int32).cuda()))
 
 
 def test_a_table_shorter_than_the_prefix():
     """Tokens behind the table's last column are not seen, of a prefix as of any context."""
-    batch = Shared([(640, [(1, 40), (2, 10)]), (320, [(1, 1), (1, 1)])], 4, 2, 64, 16)
+    batch = Shared([(1280, [(1, 40), (2, 10)]), (320, [(1, 1), (1, 1)])], 4, 2, 64, 16)
+    assert shared(batch, batch.plan(2, causal=False))
     q, cache, pages, starts, lens = batch.inputs()
-    for columns in (1, 3, 20, 30):
+    for columns in (1, 3, 20, 70):
         plan = ops().attention_plan(cache, starts, lens, 4, q.shape[0], 2, causal=False, **batch.groups())
         got = ops().paged_attention(q, cache, pages[:, :columns], starts, lens, plan=plan, causal=False)
         held = Batch.__new__(Batch)
@@ -162,10 +200,11 @@ def test_a_table_shorter_than_the_prefix():
 def test_what_is_no_number_reaches_the_rows_that_see_it(bad):
     """In the shared part all of the group, in a sequence's own part its own rows, behind the last token of a page none."""
     for most in (1, None):
-        batch = Shared([(256, [(1, 20), (2, 30), (1, 90)]), (128, [(1, 3), (1, 4)])], 4, 2, 64, 16)
+        batch = Shared([(1024, [(1, 20), (2, 30), (1, 90)]), (128, [(1, 3), (1, 4)])], 4, 2, 64, 16)
+        assert shared(batch, batch.plan(most))
         clean = batch.attend(most)
         batch.check(clean)
-        page, slot = divmod(int(batch.slots(1, torch.tensor([256 + 29]))), 16)      # the second sequence's newest token
+        page, slot = divmod(int(batch.slots(1, torch.tensor([1024 + 29]))), 16)      # the second sequence's newest token
         batch.cache.v[page, :, slot, 5] = bad
         got = batch.attend(most)
         assert not got[2, :, 5].isfinite().any() and torch.equal(got[[0, 1, 3, 4, 5]], clean[[0, 1, 3, 4, 5]])
@@ -202,7 +241,7 @@ def test_large_scores():
     """Sums of both parts meet under one maximum, however far apart their own are."""
     for big in (0.01, 30.0, 300.0):
         for kind in KINDS:
-            batch = Shared([(500, [(1, 60), (1, 3), (5, 90)])], 4, 2, 64, 16, kind, torch.bfloat16, big=big)
+            batch = Shared([(1000, [(1, 60), (1, 3), (5, 90)])], 4, 2, 64, 16, kind, torch.bfloat16, big=big)
             batch.q = (batch.q.float() * 0.2).to(batch.dtype)
             got = batch.attend(None)
             want, size, _ = batch.answer()

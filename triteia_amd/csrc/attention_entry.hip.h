@@ -107,26 +107,32 @@ struct ReadLaunch {
 template <class T, int KIND, int D>
 void launch_attend(AttendArgs a, const AttnLayout& layout, float* scratch, long table_tokens, hipStream_t stream) {
   int joins = 0;
-  for (int which = 0; which < 2; which++) {
+  const bool sharing = layout.list[2].max_items > 0;
+  for (int which = 0; which < kAttnLists; which++) {
     const AttnList& l = a.list[which] = layout.list[which];
     // (contexts that a table of so few tokens can hold are not cut)
-    if (table_tokens > (long)l.min_blocks * kAttnBlock) joins += l.max_joins * a.kv_heads * (l.rows / (1024 / D));
+    if (which < 2 && table_tokens > (long)l.min_blocks * kAttnBlock) joins += l.max_joins * a.kv_heads * (l.rows / (1024 / D));
     a.part_o[which] = scratch;
     a.part_ml[which] = scratch + (long)l.max_parts * a.kv_heads * l.rows * D;
     scratch = a.part_ml[which] + 2L * l.max_parts * a.kv_heads * l.rows;
   }
-  if (layout.n_groups > 0) {                       // (every row of a group is joined)
-    const long bound = ((long)a.list[0].max_joins * a.list[0].rows + (long)a.list[1].max_joins * a.list[1].rows) / (1024 / D) * a.kv_heads;
-    joins = (int)std::min<long>(kAttnSharedJoiners, bound);
+  if (sharing) {                                   // (every row of a group is joined)
+    const long bound = ((long)(a.list[0].max_joins + a.list[2].max_joins) * 16 + (long)a.list[1].max_joins * a.list[1].rows) / (1024 / D) * a.kv_heads;
+    joins = (int)std::min<long>(kAttnJoiners, bound);
   }
   a.joined = joins > 0;
   const dim3 grid((unsigned)((long)(a.list[0].max_items + a.list[1].max_items) * a.kv_heads));
-  if (a.list[1].max_items > 0) hipLaunchKernelGGL((attend_mixed_kernel<T, KIND, D>), grid, dim3(256), 0, stream, a);
+  if (sharing) {
+    const long own = (long)a.list[0].max_items * a.kv_heads;
+    const dim3 all((unsigned)((long)(a.list[2].max_items + a.list[1].max_items) * a.kv_heads + (layout.solo ? (own + 3) / 4 : own)));
+    if (layout.solo) hipLaunchKernelGGL((attend_groups_kernel<T, KIND, D, true>), all, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((attend_groups_kernel<T, KIND, D, false>), all, dim3(256), 0, stream, a);
+  } else if (a.list[1].max_items > 0) hipLaunchKernelGGL((attend_mixed_kernel<T, KIND, D>), grid, dim3(256), 0, stream, a);
   else if (a.list[0].rows == 16 && a.list[0].waves == 8) hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 1, 8>), grid, dim3(512), 0, stream, a);
   else if (a.list[0].rows == 16) hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 1, 4>), grid, dim3(256), 0, stream, a);
   else if (a.list[0].waves == 8) hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 2, 8>), grid, dim3(512), 0, stream, a);
   else hipLaunchKernelGGL((attend_rows_kernel<T, KIND, D, 2, 4>), grid, dim3(256), 0, stream, a);
-  if (layout.n_groups > 0) hipLaunchKernelGGL((attend_join_shared_kernel<T, D>), dim3(joins), dim3(256), 0, stream, a);
+  if (sharing) hipLaunchKernelGGL((attend_join_shared_kernel<T, D>), dim3(joins), dim3(256), 0, stream, a);
   else if (joins > 0) hipLaunchKernelGGL((attend_join_kernel<T, D>), dim3(joins < kAttnJoiners ? joins : kAttnJoiners), dim3(256), 0, stream, a);
 }
 struct AttendLaunch {
@@ -183,8 +189,9 @@ int attention_plan(const void* q_starts, const void* kv_lens, const void* group_
     return fail(TRITEIA_HIP_ERR_ARGUMENT, "attention_plan: a plan of %zu bytes, 16-byte aligned, is needed, got %zu", 4 * (size_t)l.ints, plan_bytes);
   DeviceGuard g(dev);
   if (!g.ok) return fail(TRITEIA_HIP_ERR_RUNTIME, "cannot select device %d", dev);
-  const auto kernel = n_groups > 0 ? attention_plan_kernel<true> : attention_plan_kernel<false>;
-  hipLaunchKernelGGL(kernel, dim3(1), dim3(kAttnPlanThreads), 0, static_cast<hipStream_t>(stream), static_cast<const int*>(q_starts), static_cast<const int*>(kv_lens),
+  const bool sharing = l.list[2].max_items > 0;
+  const auto kernel = sharing ? attention_plan_kernel<true> : attention_plan_kernel<false>;
+  hipLaunchKernelGGL(kernel, dim3(1), dim3(sharing ? 192 : kAttnPlanThreads), 0, static_cast<hipStream_t>(stream), static_cast<const int*>(q_starts), static_cast<const int*>(kv_lens),
                      static_cast<const int*>(group_starts), static_cast<const int*>(prefix_lens), l, static_cast<int*>(plan));
   return check_launch("attention_plan_kernel");
 }

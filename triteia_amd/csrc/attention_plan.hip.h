@@ -27,8 +27,15 @@ constexpr int kAttnWaves = 8;          // at most, of a workgroup with few rows
 constexpr int kAttnSorted = 256;       // lists of up to this many tiles begin with the longest
 constexpr int kAttnMaxSeqs = 4096;
 constexpr int kAttnMaxGroups = 1024;
+constexpr int kAttnSolo = 512;         // groups' sequences times heads of the cache above which each gets a wavefront
+constexpr int kAttnPrefixRows = 32;    // prefixes of up to so many rows are walked by all wavefronts of a workgroup
+constexpr int kAttnRowBlocks = 16;     // blocks of a share of few rows, at least
+constexpr int kAttnTileBlocks = 8;     // a share of a tile of 128 rows, at least
+constexpr int kAttnHalf = 30;           // blocks of a workgroup up to which half as many take the tiles of groups
+constexpr int kAttnOwnBlocks = 8;      // so are few rows' own parts of more than so many blocks, in batches with groups
 constexpr int kAttnMaxTokens = 0x7fffff80;   // a longer context is taken as this long, so that the end of its last block is still an int
-constexpr int kAttnPlanThreads = 128;
+constexpr int kAttnPlanThreads = 128;          // a wavefront for each list; of groups 192
+constexpr int kAttnLists = 3;          // few rows, tiles of 128 rows, and long walks of few rows (groups only)
 
 // One share of one tile.
 struct AttnItem {
@@ -52,8 +59,9 @@ struct AttnList {
 
 struct AttnLayout {
   int n_seqs, n_tokens, group, kv_heads, causal, window, n_groups;
+  int solo;              // short tiles: a wavefront each (groups only)
   int short_rows;        // sequences of more rows go to the long list; 0x7fffffff: there is none
-  AttnList list[2];      // short, long
+  AttnList list[kAttnLists];      // short, long, walks
   long ints;
 };
 
@@ -65,28 +73,30 @@ inline AttnLayout attn_layout(int n_seqs, int n_tokens, int heads, int kv_heads,
   const long live = n_seqs + 1 < n_tokens ? n_seqs + 1 : n_tokens;      // sequences with tokens, and the tokens behind them
   // (a group that shares has two sequences with tokens at least; its prefix has the rows of all of them)
   const long pairs = (n_seqs < n_tokens ? n_seqs : n_tokens) / 2, sharing = n_groups < pairs ? n_groups : pairs;
-  const bool only_short = most <= 32 && (sharing == 0 || rows <= 32);
-  AttnList &s = a.list[0], &l = a.list[1];
+  a.solo = sharing > 0 && a.group <= 16 && live * kv_heads > kAttnSolo;
+  const bool only_short = most <= 32 && sharing == 0;
+  AttnList &s = a.list[0], &l = a.list[1], &p = a.list[2];
   s.rows = only_short && most > 16 ? 32 : 16;
   a.short_rows = only_short ? 0x7fffffff : a.group <= 16 ? 16 : 0;       // (one token's heads fill more than a tile of 16: a long sequence)
   // A share is worth its scratch and its place in the joining launch from 1024 tokens on (short rows) or 512 (tiles: 26 sequences, two of 203 new
   // tokens on up to 2000, in e4m3, 59.5 / 49.2 / 62.7 us with 256 / 512 / 768; 3 of 100 on 3000 58.1 / 58.3 / 63.3, 8 of 300 on 300 36.1 / 21.4 / 21.5).
-  s.min_blocks = 16, s.rounds = 4, l.slots = 512, l.min_blocks = 8, l.rounds = 2;
+  s.min_blocks = kAttnRowBlocks, s.rounds = 4, l.slots = 512, l.min_blocks = kAttnTileBlocks, l.rounds = 2;
   l.rows = kAttnTileRows;
-  long tiles[2] = {only_short ? live + rows / s.rows : a.short_rows ? live : 0, only_short ? 0 : live + rows / l.rows};
+  p.rows = kAttnPrefixRows, p.slots = 512, p.min_blocks = kv_heads <= 8 ? 2 : 4, p.rounds = 2, p.waves = 4;
+  long tiles[kAttnLists] = {only_short ? live + rows / s.rows : a.short_rows ? live : 0, only_short ? 0 : live + rows / l.rows, 0};
   if (sharing > 0) {
-    if (only_short || a.short_rows) tiles[0] += sharing + (only_short ? rows / s.rows : 0);
-    if (!only_short) {
-      const long most_long = rows / (a.short_rows + 1);  // sequences of the long list
-      tiles[1] = (live < most_long ? live : most_long) + rows / l.rows + sharing + rows / l.rows;
-    }
+    const long most_long = rows / (a.short_rows + 1), most_wide = rows / (kAttnPrefixRows + 1);      // sequences and prefixes of the long list
+    tiles[1] = (live < most_long ? live : most_long) + rows / l.rows + (sharing < most_wide ? sharing : most_wide) + rows / l.rows;
+    tiles[2] = sharing + live;
+    l.min_blocks = 2;                  // (kAttnTileBlocks, and kAttnRowBlocks for walks, where it does not pay to share)
   }
   // Up to 128 workgroups with short rows: eight wavefronts, one a CU, so that a context is walked fast.  More: four, two a CU, one beginning or
   // ending while the other streams.  (us, eight / four: 32 of 500 tokens 8.0 / 8.7, 24 of 100000 cut into 256 / 512 215 / 220, 192 of up to 2000 in
   // e4m3 22.9 / 21.0, 2048 of up to 1000 112 / 100 and 81 / 58, 1280 of 34 21.5 / 13.2, 2048 of up to 4096 395 / 390.)
   s.waves = !only_short || tiles[0] * kv_heads > 128 ? 4 : kAttnWaves;
-  s.slots = only_short && s.waves == 4 ? 512 : 256, l.waves = 4;
-  for (int which = 0; which < 2; which++) {
+  s.slots = a.solo ? 2048 : only_short && s.waves == 4 ? 512 : 256, l.waves = 4;
+  if (a.solo) s.rounds = 2, s.min_blocks = 4;                 // (a wavefront takes 6 us for four blocks)
+  for (int which = 0; which < kAttnLists; which++) {
     AttnList& x = a.list[which];
     // (as the kernel cuts them: into the shares of whole rounds of workgroups; a cut tile has two at least)
     const long units = tiles[which] * kv_heads, whole = units < (long)x.rounds * x.slots ? units : (long)x.rounds * x.slots;
@@ -94,13 +104,13 @@ inline AttnLayout attn_layout(int n_seqs, int n_tokens, int heads, int kv_heads,
     x.max_joins = (int)(tiles[which] < shares / 2 ? tiles[which] : shares / 2);
     x.max_parts = (int)(tiles[which] > 0 ? shares : 0);
     x.max_items = (int)(tiles[which] > shares ? tiles[which] : shares);
-    if (n_groups > 0) x.max_joins = (int)tiles[which], x.max_parts = x.max_items;      // (a group's tiles are shares, cut or not)
+    if (sharing > 0) x.max_joins = (int)tiles[which], x.max_parts = x.max_items;      // (a group's tiles are shares, cut or not)
   }
-  long at = 8;
+  long at = sharing > 0 ? 16 : 8;
   for (AttnList& x : a.list) {
     x.items = at, at += 8L * x.max_items;
     x.joins = at, at += 8L * x.max_joins;
-    if (n_groups > 0) x.prefixes = at, at += 2L * x.max_joins;
+    if (sharing > 0) x.prefixes = at, at += 2L * x.max_joins;
   }
   a.ints = at;
   return a;
@@ -130,21 +140,24 @@ __device__ __forceinline__ void attn_range(const AttnSeq& s, int tile, int rows,
 template <bool SHARED>
 struct AttnGroups {
   static constexpr int kSize = SHARED ? kAttnMaxGroups + 1 : 1;
-  int start[kSize], first[kSize], least[kSize], live[kSize];
+  int start[kSize], first[kSize], least[kSize], few[kSize];     // few: sequences of half a tile's rows at most
+  unsigned long long saved, rows;                        // blocks that are not read again, rows to join
+  int longest;
   int home[SHARED ? kAttnMaxSeqs : 1];                   // a sequence's group, -1: none
 };
 
-// grid 1, block kAttnPlanThreads
+// grid 1, block kAttnPlanThreads, or 192 of groups
 template <bool SHARED>
-__global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const int* q_starts, const int* kv_lens, const int* group_starts, const int* prefix_lens,
+__global__ __launch_bounds__(SHARED ? 192 : kAttnPlanThreads) void attention_plan_kernel(const int* q_starts, const int* kv_lens, const int* group_starts, const int* prefix_lens,
                                                                           AttnLayout a, int* plan) {
   __shared__ int start[kAttnMaxSeqs + 1], count[kAttnMaxSeqs + 1], context[kAttnMaxSeqs + 1];
-  __shared__ int tiles_ahead[2][kAttnMaxSeqs + 1];       // of each sequence, in each list
-  __shared__ int order[2][kAttnSorted];
-  __shared__ int crossed[kAttnPlanThreads / 64];
+  constexpr int kThreads = SHARED ? 192 : kAttnPlanThreads, kLists = kThreads / 64;
+  __shared__ int tiles_ahead[kLists][kAttnMaxSeqs + 1];  // of each sequence, in each list
+  __shared__ int order[kLists][kAttnSorted];
+  __shared__ int crossed[kLists];
   __shared__ AttnGroups<SHARED> groups;
   bool back = false;                                     // an offset below the one ahead of it
-  for (int b = threadIdx.x; b <= a.n_seqs; b += kAttnPlanThreads) {
+  for (int b = threadIdx.x; b <= a.n_seqs; b += kThreads) {
     const bool rest = b == a.n_seqs;
     const int lo = b == 0 ? 0 : max(0, min(q_starts[b], a.n_tokens)), hi = rest ? a.n_tokens : max(0, min(q_starts[b + 1], a.n_tokens));
     back |= hi < lo;
@@ -155,7 +168,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const 
   __syncthreads();
   bool mend = false;
 #pragma unroll
-  for (int w = 0; w < kAttnPlanThreads / 64; w++) mend |= crossed[w] != 0;
+  for (int w = 0; w < kLists; w++) mend |= crossed[w] != 0;
   if (mend) {                                            // offsets in no order: each as the largest up to it, so that every token has one place
     if (threadIdx.x == 0) {
       for (int b = 1; b <= a.n_seqs; b++) {
@@ -166,24 +179,26 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const 
     }
     __syncthreads();
   }
+  bool pays = false;
   const int last = SHARED ? a.n_seqs + a.n_groups : a.n_seqs;      // of the sequences, the tokens behind them and the prefixes among them
   if constexpr (SHARED) {
     bool unordered = false;
-    for (int g = threadIdx.x; g <= a.n_groups; g += kAttnPlanThreads) {
+    for (int g = threadIdx.x; g <= a.n_groups; g += kThreads) {
       const int at = max(0, min(group_starts[g], a.n_seqs));
-      groups.start[g] = at, groups.least[g] = 0x7e000000, groups.live[g] = 0, groups.first[g] = 0x7fffffff;
+      groups.start[g] = at, groups.least[g] = 0x7e000000, groups.few[g] = 0, groups.first[g] = 0x7fffffff;
       if (g > 0) unordered |= at < max(0, min(group_starts[g - 1], a.n_seqs));
     }
     const bool any_unordered = __any(unordered);
+    if (threadIdx.x == 0) groups.saved = groups.rows = 0, groups.longest = 0;
     __syncthreads();                                     // (`crossed` has been read)
     if ((threadIdx.x & 63) == 0) crossed[threadIdx.x >> 6] = any_unordered;
     __syncthreads();
-    if ((crossed[0] | crossed[kAttnPlanThreads / 64 - 1]) != 0) {
+    if ((crossed[0] | crossed[1] | crossed[kLists - 1]) != 0) {
       if (threadIdx.x == 0)
         for (int g = 1; g <= a.n_groups; g++) groups.start[g] = max(groups.start[g], groups.start[g - 1]);
       __syncthreads();
     }
-    for (int b = threadIdx.x; b < a.n_seqs; b += kAttnPlanThreads) {
+    for (int b = threadIdx.x; b < a.n_seqs; b += kThreads) {
       int lo = -1, hi = a.n_groups;                      // the last group that starts at or ahead of sequence b
       while (lo < hi) {
         const int mid = (lo + hi + 1) / 2;
@@ -194,27 +209,45 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const 
       if (lo >= 0 && count[b] > 0) {
         atomicMin(&groups.least[lo], a.causal ? context[b] - count[b] : context[b]);
         atomicMin(&groups.first[lo], b);
-        atomicAdd(&groups.live[lo], 1);
+        if ((long)count[b] * a.group <= kAttnTileRows / 2) atomicAdd(&groups.few[lo], 1);
       }
     }
     __syncthreads();
-    for (int g = threadIdx.x; g < a.n_groups; g += kAttnPlanThreads) {
-      // (a window hides of the prefix from each row what it hides; nothing is shared then)
-      int prefix = groups.live[g] < 2 || a.window > 0 ? 0 : min(prefix_lens[g], groups.least[g]);
+    for (int g = threadIdx.x; g < a.n_groups; g += kThreads) {
+      // (a window hides of the prefix from each row what it hides; nothing is shared then.  Nor among prompts: tiles of 128 rows have the matrix cores busy either way.)
+      int prefix = groups.few[g] < 2 || a.window > 0 ? 0 : min(prefix_lens[g], groups.least[g]);
       prefix = max(prefix, 0) / kAttnBlock * kAttnBlock;
       const int b = a.n_seqs + 1 + g, from = start[groups.start[g]];
       start[b] = from, count[b] = prefix > 0 ? start[groups.start[g + 1]] - from : 0, context[b] = prefix;
+      if (prefix > 0) {
+        atomicAdd(&groups.saved, (unsigned long long)(groups.few[g] - 1) * (prefix / kAttnBlock) * a.kv_heads);
+        atomicAdd(&groups.rows, (unsigned long long)count[b] * a.group * a.kv_heads);
+        atomicMax(&groups.longest, prefix / kAttnBlock);
+      }
     }
+    __syncthreads();
+    // Whether it pays.  A block that is read again comes from the caches, 2 to 3 ns of the whole chip; sharing takes a second walk and a join of every row.  On 196 batches of 2 to
+    // 128 single tokens behind 128 to 8192 shared ones, over 8 and 32 heads of the cache, the choice is 0.4 % behind the better of both on average, 19 % at most: 64 requests of
+    // 64 heads behind 512 tokens 13.9 us each for itself and 19.0 shared, behind 2048 33.7 and 26.0, behind 8192 124 and 48.
+    pays = 10 * groups.saved >= 40000 + 6 * groups.rows || (groups.saved > 0 && groups.longest >= 12 && a.n_seqs * a.kv_heads <= 256);
+    if (!pays)
+      for (int g = threadIdx.x; g < a.n_groups; g += kThreads) count[a.n_seqs + 1 + g] = context[a.n_seqs + 1 + g] = 0;
     __syncthreads();
   }
   const int which = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const AttnList& l = a.list[which];
   if (l.max_items == 0) {
     if (lane < 2) plan[2 * which + lane] = 0;
-    if (SHARED && lane == 0) plan[4 + which] = 0;
+    if (SHARED && lane == 0) plan[6 + which] = 0;
     if constexpr (SHARED) __syncthreads();
     return;
   }
+  auto from_of = [&](int b) { return SHARED && b < a.n_seqs && groups.home[b] >= 0 ? context[a.n_seqs + 1 + groups.home[b]] : 0; };
+  auto list_of = [&](int b, long rows) {                         // of sequence b, the tokens behind the last or a prefix
+    if (SHARED && b > a.n_seqs) return rows <= kAttnPrefixRows ? 2 : 1;
+    if (SHARED && b < a.n_seqs && rows <= a.short_rows && context[b] - from_of(b) > kAttnOwnBlocks * kAttnBlock) return 2;
+    return rows <= a.short_rows ? 0 : 1;
+  };
   int* ahead = tiles_ahead[which];
   int tiles = 0;
   for (int b0 = 0; b0 <= last; b0 += 64) {
@@ -222,7 +255,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const 
     int mine = 0;
     if (b <= last) {
       const long rows = (long)count[b] * a.group;
-      if (rows > 0 && (rows <= a.short_rows) == (which == 0)) mine = (int)((rows + l.rows - 1) / l.rows);
+      if (rows > 0 && list_of(b, rows) == which) mine = (int)((rows + l.rows - 1) / l.rows);
     }
     int all;
     const int before = attn_scan(mine, &all);
@@ -266,7 +299,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const 
   int share = 0x7fffffff;
   const long units = (long)tiles * a.kv_heads;
   if (units < (long)l.rounds * l.slots) {
-    const int most = (int)((units + l.slots - 1) / l.slots * l.slots / a.kv_heads);        // shares of one head
+    int most = (int)((units + l.slots - 1) / l.slots * l.slots / a.kv_heads);              // shares of one head
     auto sum_of = [&](auto f) {                                  // f of every tile's blocks
       long sum = 0;
 #pragma unroll
@@ -277,7 +310,18 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const 
       return total;
     };
     const int total = sum_of([](int blocks) { return blocks; });
-    share = max(l.min_blocks, (total + most - 1) / max(most, 1));
+    if (pays) {                                                  // (one workgroup a CU and half the results to join, while they are short)
+      if (which > 0 && units <= l.slots / 2 && (long)total * a.kv_heads <= kAttnHalf * l.slots / 2) most = l.slots / 2 / a.kv_heads;
+    }
+    share = max(!SHARED || pays || which == 0 ? l.min_blocks : which == 1 ? kAttnTileBlocks : kAttnRowBlocks, (total + most - 1) / max(most, 1));
+    if (pays) {                                      // (a row's shares are joined: sixteen at most for this)
+      int longest = 0;
+#pragma unroll
+      for (int k = 0; k < kAttnSorted / 64; k++) longest = max(longest, mine[k]);
+#pragma unroll
+      for (int d = 32; d > 0; d /= 2) longest = max(longest, __shfl_xor(longest, d));
+      share = max(share, (longest + 15) / 16);
+    }
     while (share <= total && sum_of([&](int blocks) { return max(1, (blocks + share - 1) / share); }) > most) share += (share + 7) / 8;
   }
   // longest first, so that the last workgroups to run are short ones
@@ -326,8 +370,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const 
                           cut ? part + p : -1};
       AttnJoin j = {t.s.start, t.s.n, t.tile, part, splits, -1, 0, 0};
       if (SHARED && t.home > 0) {
-        const long rows = (long)count[t.home] * a.group;
-        j.prefix_list = rows <= a.short_rows ? 0 : 1;
+        j.prefix_list = list_of(t.home, (long)count[t.home] * a.group);
         j.prefix_tile = tiles_ahead[j.prefix_list][t.home], j.prefix_row = (t.s.start - start[t.home]) * a.group;
       }
       if (SHARED && joins) fullest = max(fullest, min(l.rows, t.s.n * a.group - t.tile * l.rows));
@@ -342,7 +385,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attention_plan_kernel(const 
   if constexpr (SHARED) {
 #pragma unroll
     for (int d = 32; d > 0; d /= 2) fullest = max(fullest, __shfl_xor(fullest, d));
-    if (lane == 0) plan[4 + which] = fullest;
+    if (lane == 0) plan[6 + which] = fullest;
   }
 }
 

@@ -42,8 +42,8 @@ struct AttendArgs {
   int group, kv_heads, causal, window;
   float scale_log2;                     // scale * log2(e)
   const int* plan;
-  AttnList list[2];
-  float *part_o[2], *part_ml[2];        // of each list: [parts][kv_heads][rows][D], [parts][kv_heads][rows][2]
+  AttnList list[kAttnLists];
+  float *part_o[kAttnLists], *part_ml[kAttnLists];        // of each list: [parts][kv_heads][rows][D], [parts][kv_heads][rows][2]
 };
 
 // The largest over lanes 32 apart, or 16 and 32 apart, in all of them: whole rows of lanes trade places on the vector ALU.
@@ -246,7 +246,7 @@ struct AttnRowsLds {
   alignas(16) float scales[KIND == kCacheSame ? 1 : WAVES][2][kSub];
 };
 
-template <class T, int KIND, int D, int NQ, int WAVES>
+template <class T, int KIND, int D, int NQ, int WAVES, int LIST = 0>
 __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int head, AttnRowsLds<KIND, D, NQ, WAVES>& shared) {
   using M = AttnMma<T>;
   using v8 = typename M::v8;
@@ -259,9 +259,9 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
   auto& meet_m = shared.meet_m;
   auto& meet_l = shared.meet_l;
   auto& scales = shared.scales;
-  AttnItem it = attn_item(a, 0, index);              // (requested together with the number of items)
-  if (index >= a.plan[0] || !attn_within(a, kRows, &it)) return;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  AttnItem it = attn_item(a, LIST, index);           // (requested together with the number of items)
+  if (index >= a.plan[2 * LIST] || !attn_within(a, kRows, &it)) return;
+  const int lane = threadIdx.x & 63, wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, h = lane >> 4;
   uint8_t* lds_k = lds + wave * 2 * kTile;
   uint8_t* lds_v = lds_k + kTile;
@@ -500,6 +500,29 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
     }
   }
 
+  if constexpr (WAVES == 1) {                // an item of its own: from the registers
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+      const float f = kNormed ? __builtin_ldexpf(1.f, -shift[n]) : 1.f;
+      float sum = l[n] * f;
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      const int r = 16 * n + col;
+      if (r > last_row) continue;
+      const AttnRow row = attn_row(a, it, kRows, r);
+      const long at = ((long)it.part * a.kv_heads + head) * (LIST == 2 ? kAttnPrefixRows : kRows) + r;
+      T* out = static_cast<T*>(a.out) + ((long)(it.q_start + row.token) * (a.kv_heads * a.group) + head * a.group + row.head) * D;
+#pragma unroll
+      for (int d = 0; d < D / 16; d++) {
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        const attn_f4 x = o[n][d] * f;
+        if (it.part >= 0) *reinterpret_cast<attn_f4*>(a.part_o[LIST] + at * D + 16 * d + 4 * h) = x;
+        else *reinterpret_cast<t4*>(out + 16 * d + 4 * h) = sum == 0.f ? t4{0, 0, 0, 0} : t4{(T)(x[0] / sum), (T)(x[1] / sum), (T)(x[2] / sum), (T)(x[3] / sum)};
+      }
+      if (it.part >= 0 && h == 0) a.part_ml[LIST][2 * at] = m[n], a.part_ml[LIST][2 * at + 1] = sum;
+    }
+    return;
+  }
   // the wavefronts' results: through LDS, the upper half's taken in by the lower half
 #pragma unroll
   for (int n = 0; n < NQ; n++) {
@@ -564,9 +587,9 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int index, int 
       for (int j = 0; j < 4; j++) y[j] = sum == 0.f ? (T)0.f : (T)(x[j] / sum);
       *reinterpret_cast<t4*>(static_cast<T*>(a.out) + ((long)(it.q_start + row.token) * (a.kv_heads * a.group) + head * a.group + row.head) * D + d) = y;
     } else {
-      const long at = ((long)it.part * a.kv_heads + head) * kRows + r;
-      *reinterpret_cast<attn_f4*>(a.part_o[0] + at * D + d) = x;
-      if (d == 0) a.part_ml[0][2 * at] = top, a.part_ml[0][2 * at + 1] = sum;
+      const long at = ((long)it.part * a.kv_heads + head) * (LIST == 2 ? kAttnPrefixRows : kRows) + r;
+      *reinterpret_cast<attn_f4*>(a.part_o[LIST] + at * D + d) = x;
+      if (d == 0) a.part_ml[LIST][2 * at] = top, a.part_ml[LIST][2 * at + 1] = sum;
     }
   }
 }
@@ -898,6 +921,33 @@ __global__ __launch_bounds__(256, 2) void attend_mixed_kernel(AttendArgs a) {
   else attend_rows<T, KIND, D, 1, 4>(a, index - a.list[1].max_items, head, shared.rows);
 }
 
+// Batches in groups: long walks of few rows (prefixes, and sequences that share little), tiles of 128 rows (prefixes of many, prompts), then the sequences' own parts.
+// SOLO: many of these, of few rows: a wavefront takes one and a head by itself, four of them a workgroup, and there is nothing to join between wavefronts.  (Of 220 tokens of a sequence's own a workgroup's
+// four wavefronts walk two sub-tiles each and spend the rest of their time on the way there and on joining.)
+// grid (list[2].max_items + list[1].max_items) * kv_heads + list[0].max_items * kv_heads (SOLO: a quarter of that, rounded up), block 256
+template <class T, int KIND, int D, bool SOLO>
+__global__ __launch_bounds__(256, 2) void attend_groups_kernel(AttendArgs a) {
+  __shared__ union {
+    AttnTileLds<D> tile;
+    AttnRowsLds<KIND, D, 2, 4> prefix;
+    AttnRowsLds<KIND, D, 1, 4> rows;
+    AttnRowsLds<KIND, D, 1, 1> solo[4];
+  } shared;
+  const int prefixes = a.list[2].max_items, tiles = prefixes + a.list[1].max_items, index = blockIdx.x / a.kv_heads, head = blockIdx.x - index * a.kv_heads;
+  if (index < prefixes) {
+    const int* p = a.plan + a.list[2].items + 8L * index;        // (one tile each; behind the last item it does not matter)
+    if (p[2] * a.group <= 16) attend_rows<T, KIND, D, 1, 4, 2>(a, index, head, shared.rows);
+    else attend_rows<T, KIND, D, 2, 4, 2>(a, index, head, shared.prefix);
+  } else if (index < tiles) {
+    attend_tile<T, KIND, D>(a, index - prefixes, head, shared.tile);
+  } else if constexpr (SOLO) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), unit = 4 * (blockIdx.x - tiles * a.kv_heads) + wave, own = unit / a.kv_heads;
+    if (own < a.list[0].max_items) attend_rows<T, KIND, D, 1, 1>(a, own, unit - own * a.kv_heads, shared.solo[wave]);
+  } else {
+    attend_rows<T, KIND, D, 1, 4>(a, index - tiles, head, shared.rows);
+  }
+}
+
 // Shares of one tile.  D / 4 lanes hold a row; a workgroup takes as many rows as it has such groups (or as many as there are, rounded up to a power of two) and,
 // between them, the shares: a group adds every n-th share, the groups' sums are added in their order.  The host knows bounds only, mostly far above
 // what there is to join, so a fixed number of workgroups walks what the plan says: one for every place of the bound took 10 to 15 us of a prompt's 180 to
@@ -955,24 +1005,24 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
 
 // The same for batches in groups that share a prefix: a tile of a group has the shares of its group's prefix behind its own, in the prefix's tiles that hold its rows.  Every
 // row is joined, so this is as long as its round trips: a lane group requests eight shares at once, statistics and sums together, and takes them in under a
-// running maximum; the plan says how many rows the fullest tile has, so that a unit has work.  (Two passes over the shares, one for the maxima, on 1024 workgroups took
-// 14 us for 64 requests of 64 heads and 23 for 96 of 32 + 32.)  grid up to kAttnSharedJoiners, block 256
-constexpr int kAttnSharedJoiners = 4096;
+// running maximum; the plan says how many rows the fullest tile has, so that a unit has work.  Two passes over the shares, one for the maxima, over all
+// places of the tiles took 14 us for 64 requests of 64 heads and 23 for 96 of 32 + 32, this 7 and 11.  grid up to kAttnJoiners, block 256
 template <class T, int D>
 __global__ __launch_bounds__(256) void attend_join_shared_kernel(AttendArgs a) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes, kAtOnce = 8;
   __shared__ attn_f4 sums[256];
   __shared__ float tops[kGroups], totals[kGroups];
-  int pieces[2], units[2];
+  int pieces[kAttnLists], units[kAttnLists];
 #pragma unroll
-  for (int which = 0; which < 2; which++) {
-    pieces[which] = (a.plan[4 + which] + kGroups - 1) / kGroups;
+  for (int which = 0; which < kAttnLists; which++) {
+    pieces[which] = (a.plan[6 + which] + kGroups - 1) / kGroups;
     units[which] = a.plan[2 * which + 1] * a.kv_heads * pieces[which];
   }
   const int group = threadIdx.x / kLanes, d = 4 * (threadIdx.x % kLanes);
-  for (int next = blockIdx.x; next < units[0] + units[1]; next += gridDim.x) {
-    const int which = next < units[0] ? 0 : 1, unit = next - (which ? units[0] : 0);
-    const int rows = a.list[which].rows, piece = unit % pieces[which], index = unit / pieces[which] / a.kv_heads, head = unit / pieces[which] - index * a.kv_heads;
+  for (int next = blockIdx.x; next < units[0] + units[1] + units[2]; next += gridDim.x) {
+    const int which = next < units[0] ? 0 : next < units[0] + units[1] ? 1 : 2, unit = next - (which > 0 ? units[0] : 0) - (which > 1 ? units[1] : 0);
+    const int per = which == 0 ? pieces[0] : which == 1 ? pieces[1] : pieces[2];
+    const int rows = a.list[which].rows, piece = unit % per, index = unit / per / a.kv_heads, head = unit / per - index * a.kv_heads;
     const int* j = a.plan + a.list[which].joins + 8L * index;
     const int q_start = j[0], n_tokens = j[1], tile = j[2], first = j[3], n_own = j[4], prefix_list = j[5], prefix_tile = j[6], prefix_row = j[7];
     const int r0 = kGroups * piece, live = min(min(kGroups, rows - r0), n_tokens * a.group - tile * rows - r0);
