@@ -133,3 +133,21 @@ def test_ops_refuse_the_cpu():
     for call in (lambda: ops.quantize_fp8(x), lambda: ops.dequantize_fp8(codes, scales), lambda: ops.matmul_fp8(x, codes, torch.ones(1, 2))):
         with pytest.raises(RuntimeError, match="GPU tensor"):
             call()
+
+
+def test_layer_keeps_the_types_of_its_base():
+    """Conversions of a whole model leave codes and scales what they are, and move them."""
+    from triteia_amd.python.nn import multi_delta_attention
+    model = torch.nn.Sequential(multi_delta_attention(256, 4, 2, 64, 1, with_base="fp8"))
+    layer = model[0].qkv_proj
+    layer.base_scale.fill_(0.1)
+    layer.base.view(torch.uint8).fill_(0x31)
+    for convert in (model.half, model.double, lambda: model.to(torch.bfloat16), lambda: model.to("cpu")):
+        convert()
+        assert layer.base.dtype == torch.float8_e4m3fn and bool((layer.base.view(torch.uint8) == 0x31).all())
+        assert torch.equal(layer.base_scale, torch.full((4, 2), 0.1)) and set(layer.state_dict()) == {"qweight", "meta", "scale", "base", "base_scale"}
+    assert layer.to("meta").base.dtype == torch.float8_e4m3fn and layer.base_scale.device.type == "meta"
+    for with_base in (None, False, True, 1):
+        from triteia_amd.python.nn import multi_delta_linear
+        dense = multi_delta_linear(256, 256, 1, with_base=with_base)
+        assert (dense.base is None) == (not with_base) and "base_scale" not in dense.state_dict()

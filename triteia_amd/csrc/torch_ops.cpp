@@ -103,21 +103,63 @@ bool packed_ok(const Tensor& q, const Tensor& meta, const Tensor& s, const Tenso
 // (what the routed product takes in one call, see triteia_hip_sbmm_2_4_routed_own)
 constexpr int64_t kMaxRoutedDeltas = 8192;
 
-// (under autocast the base product has autocast's type, whatever its inputs': another one than x's is refused by the Python path)
-bool base_ok(const Args& a, int i, const Tensor& x, int64_t k, int64_t m) {
-  return a.none(i) || (a.tensor(i) && on(a[i], x, x.scalar_type(), 2) && a[i].size(0) == m && a[i].size(1) == k &&
-                       !(at::autocast::is_autocast_enabled(at::kCUDA) && at::autocast::get_autocast_dtype(at::kCUDA) != x.scalar_type()));
-}
 // (a view that starts inside 16 bytes; a copy made by contiguous() does not)
 bool aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+
+int fp8_type(at::ScalarType t) { return t == at::kHalf ? 0 : t == at::kBFloat16 ? 1 : t == at::kFloat ? 2 : -1; }
+// [rows, elements] of adjacent elements whose rows start on 16 bytes
+bool fp8_rows_ok(const Tensor& t, int64_t rows, int64_t k) {
+  return t.dim() == 2 && t.size(0) == rows && t.size(1) == k && t.stride(1) == 1 && t.stride(0) >= 0 && t.stride(0) * t.element_size() % 16 == 0 && aligned(t);
+}
+bool fp8_scales_ok(const Tensor& t, int64_t rows, int64_t k) {
+  return t.scalar_type() == at::kFloat && t.dim() == 2 && t.size(0) == rows && t.size(1) == (k + 127) / 128 && t.stride(0) >= 0 && t.stride(1) >= 0;
+}
+
+// x [.., k] times a weight [m, k] in codes: `xs` scales of an x in codes, null of one in 16 bits.  Defined if it was launched.
+Tensor fp8_product(const Tensor& x, const Tensor& w, const Tensor& ws, const Tensor* xs, at::ScalarType type, int64_t tokens, const Place& at_) {
+  const int64_t k = w.size(1), m = w.size(0);
+  c10::SmallVector<int64_t, 5> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = m;
+  Tensor y = at::empty(shape, x.options().dtype(type));
+  const int x_type = xs ? 2 : fp8_type(x.scalar_type());
+  const size_t bytes = triteia_hip_fp8_scratch_bytes(tokens, m, k, x_type);
+  const Tensor scratch = bytes ? scratch_bytes(bytes, x) : Tensor();
+  return launched(triteia_hip_fp8_matmul(x.data_ptr(), x.dim() == 2 ? x.stride(0) : k, x_type, xs ? xs->data_ptr() : nullptr, xs ? xs->stride(0) : 0, xs ? xs->stride(1) : 0,
+                                         w.data_ptr(), w.stride(0), ws.data_ptr(), ws.stride(0), ws.stride(1), y.data_ptr(), fp8_type(type), tokens, m, k,
+                                         bytes ? scratch.data_ptr() : nullptr, bytes, at_.dev, at_.handle()))
+             ? y
+             : Tensor();
+}
+
+bool recorded(const Tensor& x, const Tensor& weight) {
+  return (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad())) || x._fw_grad(0).defined() || weight._fw_grad(0).defined();
+}
+
+// The base weight, argument i, if there is one: of x's type, or in codes with argument j their scales.
+// (under autocast the base product has autocast's type, whatever its inputs': another one than x's is refused by the Python path)
+bool base_ok(const Args& a, int i, const Tensor& x, int64_t k, int64_t m, int j = Args::kMax) {
+  const bool scaled = j < a.n && !a.none(j);
+  if (a.none(i)) return !scaled;
+  if (!a.tensor(i) || (at::autocast::is_autocast_enabled(at::kCUDA) && at::autocast::get_autocast_dtype(at::kCUDA) != x.scalar_type())) return false;
+  const Tensor& w = a[i];
+  if (!scaled) return on(w, x, x.scalar_type(), 2) && w.size(0) == m && w.size(1) == k;
+  if (!a.tensor(j)) return false;
+  const Tensor& ws = a[j];
+  return k % 16 == 0 && on(w, x, at::kFloat8_e4m3fn, 2) && on(ws, x, at::kFloat, 2) && fp8_rows_ok(w, m, k) && w.stride(0) <= (1 << 24) && fp8_scales_ok(ws, (m + 127) / 128, k) &&
+         !w.is_neg() && !ws.is_neg() && !x.is_neg() && !recorded(x, ws) && !recorded(x, w) && (!x.is_contiguous() || aligned(x));
+}
 
 // x [tokens, k] times the layer's dense weight, which base_ok has let pass: what the kernels add to.  A few hundred fp16 rows
 // run on the library's own kernel, everything else -- more tokens, other types, rows that are not aligned, a product that
 // autograd records, a process that has torch tune its products (torch.cuda.tunable) -- on torch's.
-Tensor base_product(const Tensor& x, const Tensor& weight, const Place& at_) {
+Tensor base_product(const Tensor& x, const Tensor& weight, const Place& at_, const Tensor* scale = nullptr) {
   const int64_t tokens = x.size(0), k = x.size(1), m = weight.size(0);
-  const bool recorded = (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad())) || x._fw_grad(0).defined() || weight._fw_grad(0).defined();
-  if (x.scalar_type() == at::kHalf && !recorded && sizes_ok({tokens, k, m}) && triteia_hip_dense_ok(tokens, m, k) &&
+  if (scale) {
+    Tensor y = fp8_product(x, weight, *scale, nullptr, x.scalar_type(), tokens, at_);
+    TORCH_CHECK(y.defined(), "triteia_hip: ", triteia_hip_last_error());
+    return y;
+  }
+  if (x.scalar_type() == at::kHalf && !recorded(x, weight) && sizes_ok({tokens, k, m}) && triteia_hip_dense_ok(tokens, m, k) &&
       !at::cuda::tunable::getTuningContext()->IsTunableOpEnabled() && x.is_contiguous() &&
       weight.stride(1) == 1 && weight.stride(0) >= k && weight.stride(0) % 8 == 0 && aligned(x) && aligned(weight) && !x.is_neg() && !weight.is_neg()) {
     Tensor y = at::empty({tokens, m}, x.options());
@@ -188,15 +230,18 @@ int routed(const Tensor& x, const Tensor& q, const Tensor& meta, const Tensor& s
                                          m, tokens, k, bytes ? ws.data_ptr() : nullptr, bytes, accumulate, at_.dev, at_.handle());
 }
 
-// sbmm(qweights, xs, metas, ss, indices, base or None): ops.sbmm_4bit_2_4_native
+// what base_ok has let pass at j
+const Tensor* scale_of(const Args& a, int j) { return a.tensor(j) ? &a[j] : nullptr; }
+
+// sbmm(qweights, xs, metas, ss, indices, base or None and, if it is in codes, its scales): ops.sbmm_4bit_2_4_native
 Tensor sbmm(const Args& a) {
-  if (a.n != 6) return {};
+  if (a.n != 6 && a.n != 7) return {};
   for (int i = 0; i < 5; i++)
     if (!a.tensor(i)) return {};
   const Tensor &q = a[0], &x = a[1], &meta = a[2], &s = a[3], &indices = a[4];
   if (!x.is_cuda() || x.dim() != 2 || x.scalar_type() != at::kHalf || s.dim() != 3) return {};
   const int64_t tokens = x.size(0), k = x.size(1), m = s.size(2);
-  if (!sizes_ok({tokens}) || q.size(0) > kMaxRoutedDeltas || !packed_ok(q, meta, s, x, q.size(0), k, m) || !base_ok(a, 5, x, k, m)) return {};
+  if (!sizes_ok({tokens}) || q.size(0) > kMaxRoutedDeltas || !packed_ok(q, meta, s, x, q.size(0), k, m) || !base_ok(a, 5, x, k, m, 6)) return {};
   if (indices.device() != x.device() || indices.dim() != 1 || indices.size(0) != tokens || !indices.is_contiguous() ||
       !at::isIntegralType(indices.scalar_type(), false))
     return {};
@@ -208,7 +253,7 @@ Tensor sbmm(const Args& a) {
     y = at::empty({tokens, m}, x.options());
     return launched(routed(xc, q, meta, s, idx, y, 0, 2, at_)) ? y : Tensor();
   }
-  y = base_product(xc, a[5], at_);
+  y = base_product(xc, a[5], at_, scale_of(a, 6));
   must_launch(routed(xc, q, meta, s, idx, y, 0, 1, at_));
   return y;
 }
@@ -318,16 +363,16 @@ class Beside {
 bool lora_hides(int64_t tokens, int64_t k, int64_t m) { return tokens >= 2048 && tokens * k >= (int64_t(1) << 35) / m; }
 bool captured() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
 
-// ldmm(indices, x, LwA, LwB, DeltaW, metas, ss, base or None): ops.ldmm.
+// ldmm(indices, x, LwA, LwB, DeltaW, metas, ss, base or None and, if it is in codes, its scales): ops.ldmm.
 Tensor ldmm(const Args& a) {
-  if (a.n != 8) return {};
+  if (a.n != 8 && a.n != 9) return {};
   for (int i = 0; i < 7; i++)
     if (!a.tensor(i)) return {};
   const Tensor &indices = a[0], &x = a[1], &A = a[2], &B = a[3], &q = a[4], &meta = a[5], &s = a[6];
   if (x.scalar_type() != at::kHalf || !lora_ok(A, B, x, indices) || s.dim() != 3) return {};
   const int64_t k = x.size(1), m = B.size(2);
   const size_t bytes = lora_bytes(A, x);
-  if (bytes == 0 || q.size(0) > kMaxRoutedDeltas || !packed_ok(q, meta, s, x, q.size(0), k, m) || !base_ok(a, 7, x, k, m)) return {};
+  if (bytes == 0 || q.size(0) > kMaxRoutedDeltas || !packed_ok(q, meta, s, x, q.size(0), k, m) || !base_ok(a, 7, x, k, m, 8)) return {};
   const Place at_(x);
   const Tensor xc = x.is_contiguous() ? x : x.contiguous();
   const Tensor idx = indices.scalar_type() == at::kInt ? indices : indices.to(at::kInt);
@@ -335,7 +380,7 @@ Tensor ldmm(const Args& a) {
   const bool large = base && lora_hides(x.size(0), k, m);      // (the pair on either one stream or two: the same bits in a graph)
   if (!large && lora_at_once(A, B, x)) {
     // (without a base weight the LoRA launch stores the adapters' rows and zeros in all others, the deltas' among them)
-    Tensor y = base ? base_product(xc, a[7], at_) : at::empty({x.size(0), m}, x.options());
+    Tensor y = base ? base_product(xc, a[7], at_, scale_of(a, 8)) : at::empty({x.size(0), m}, x.options());
     must_launch(lora_fused(y, xc, A, B, indices, 1.0, base, at_.dev, at_.handle()));
     must_launch(routed(xc, q, meta, s, idx, y, A.size(0), 1, at_));
     return y;
@@ -345,7 +390,7 @@ Tensor ldmm(const Args& a) {
     Tensor y;                  // (like the other buffers ahead of the stream: freed only after it has been joined)
     Beside side(at_);
     if (!launched(lora_shrink(xc, A, indices, scratch, true, at_.dev, side.handle()))) return {};
-    y = base_product(xc, a[7], at_);
+    y = base_product(xc, a[7], at_, scale_of(a, 8));
     side.follow();
     must_launch(lora_expand(y, A, B, scratch, 1.0, true, at_.dev, side.handle()));
     must_launch(routed(xc, q, meta, s, idx, y, A.size(0), 1, at_));
@@ -354,7 +399,7 @@ Tensor ldmm(const Args& a) {
   }
   if (!launched(lora_shrink(xc, A, indices, scratch, base, at_.dev, at_.handle()))) return {};
   // (without a base weight the expand stores the adapters' rows and zeros in all others, the deltas' among them)
-  Tensor y = base ? base_product(xc, a[7], at_) : at::empty({x.size(0), m}, x.options());
+  Tensor y = base ? base_product(xc, a[7], at_, scale_of(a, 8)) : at::empty({x.size(0), m}, x.options());
   must_launch(lora_expand(y, A, B, scratch, 1.0, base, at_.dev, at_.handle()));
   must_launch(routed(xc, q, meta, s, idx, y, A.size(0), 1, at_));
   return y;
@@ -634,15 +679,6 @@ Outputs shared_attention(const MoreArgs& a) { return a.n == 14 && a.whole(13) ? 
 
 // --- the base weight in 8 bits ---
 
-int fp8_type(at::ScalarType t) { return t == at::kHalf ? 0 : t == at::kBFloat16 ? 1 : t == at::kFloat ? 2 : -1; }
-// [rows, elements] of adjacent elements whose rows start on 16 bytes
-bool fp8_rows_ok(const Tensor& t, int64_t rows, int64_t k) {
-  return t.dim() == 2 && t.size(0) == rows && t.size(1) == k && t.stride(1) == 1 && t.stride(0) >= 0 && t.stride(0) * t.element_size() % 16 == 0 && aligned(t);
-}
-bool fp8_scales_ok(const Tensor& t, int64_t rows, int64_t k) {
-  return t.scalar_type() == at::kFloat && t.dim() == 2 && t.size(0) == rows && t.size(1) == (k + 127) / 128 && t.stride(0) >= 0 && t.stride(1) >= 0;
-}
-
 // quantize_fp8(x, rows of a scale)
 Outputs quantize_fp8(const MoreArgs& a) {
   if (a.n != 2 || !a.tensor(0) || !a.whole(1)) return {};
@@ -691,16 +727,9 @@ Outputs matmul_fp8(const MoreArgs& a) {
   if (codes ? x.dim() != 2 || !fp8_scales_ok(a[3], tokens, k) : x.dim() != 2 && !x.is_contiguous()) return {};
   if (x.dim() == 2 ? !fp8_rows_ok(x, tokens, k) : !aligned(x) || k % 8 != 0) return {};
   const Place at_(x);
-  c10::SmallVector<int64_t, 5> shape(x.sizes().begin(), x.sizes().end());
-  shape.back() = m;
   Outputs out;
-  out.first = at::empty(shape, x.options().dtype(type));
-  const int x_type = codes ? 2 : fp8_type(x.scalar_type());
-  const size_t bytes = triteia_hip_fp8_scratch_bytes(tokens, m, k, x_type);
-  const Tensor scratch = bytes ? scratch_bytes(bytes, x) : Tensor();
-  out.done = launched(triteia_hip_fp8_matmul(x.data_ptr(), x.dim() == 2 ? x.stride(0) : k, x_type, codes ? a[3].data_ptr() : nullptr, codes ? a[3].stride(0) : 0,
-                                             codes ? a[3].stride(1) : 0, w.data_ptr(), w.stride(0), ws.data_ptr(), ws.stride(0), ws.stride(1), out.first.data_ptr(),
-                                             fp8_type(type), tokens, m, k, bytes ? scratch.data_ptr() : nullptr, bytes, at_.dev, at_.handle()));
+  out.first = fp8_product(x, w, ws, codes ? &a[3] : nullptr, type, tokens, at_);
+  out.done = out.first.defined();
   return out;
 }
 

@@ -9,7 +9,7 @@ class multi_delta_attention(nn.Module):
     """qkv projection, rotary positions (with norms of queries and keys, if `qk_norm`), the write into the layer's paged cache, attention
     over it and the output projection, for a batch of sequences whose tokens each pick a variant of both projections (index -1: none).
 
-    Attention is causal over the whole context; heads have 64 or 128 elements.  `qkv_proj` and `o_proj` are `multi_delta_linear` layers; queries,
+    with_base: False, True (fp16) or "fp8", as for `multi_delta_linear`.  Attention is causal over the whole context; heads have 64 or 128 elements.  `qkv_proj` and `o_proj` are `multi_delta_linear` layers; queries,
     keys and values stay views of the former's output.  Every method runs on the current stream without a synchronisation and can be recorded into a graph."""
 
     def __init__(self, hidden, n_heads, n_kv_heads, head_dim, n_deltas, with_base=True, qk_norm=False, interleaved=False, eps=1e-6):

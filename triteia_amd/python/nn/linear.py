@@ -78,7 +78,8 @@ class multi_delta_linear(nn.Module):
     projection (the reference has the op, ops/matmul/sbmm.py:89-142, but no module around it).
 
     Buffers: qweight int32 [N, k/32, 2m], meta int16 [N, m, k/16], scale fp16 [N, 1, m],
-    base fp16 [m, k] (optional).  `forward(x, indices)` routes on the device; with
+    base fp16 [m, k] (optional), or with_base="fp8": base e4m3 [m, k] and base_scale float32 [m/128, k/128],
+    one for each block of 128 x 128 (`load_base` quantises into them).  `forward(x, indices)` routes on the device; with
     `plan=route_plan(indices, N)` the same routing is shared by all layers of a forward pass."""
 
     def __init__(self, infeatures, outfeatures, n_deltas, with_base=False):
@@ -89,7 +90,30 @@ class multi_delta_linear(nn.Module):
         self.register_buffer("qweight", torch.zeros((n_deltas, infeatures // 32, outfeatures * 2), dtype=torch.int32))
         self.register_buffer("meta", torch.zeros((n_deltas, outfeatures, infeatures // 16), dtype=torch.int16))
         self.register_buffer("scale", torch.zeros((n_deltas, 1, outfeatures), dtype=torch.float16))
-        self.register_buffer("base", torch.zeros((outfeatures, infeatures), dtype=torch.float16) if with_base else None)
+        assert not isinstance(with_base, str) or with_base == "fp8", f"with_base is False, True or 'fp8', got {with_base!r}"
+        fp8 = with_base == "fp8"
+        self.register_buffer("base", torch.zeros((outfeatures, infeatures), dtype=torch.float8_e4m3fn if fp8 else torch.float16) if with_base else None)
+        self.register_buffer("base_scale", torch.zeros((outfeatures // 128, infeatures // 128), dtype=torch.float32) if fp8 else None, persistent=fp8)
+
+    def _apply(self, fn, *args, **kwargs):
+        # (half(), to(dtype) and their like convert whatever torch counts as floating point: codes and their scales keep their types)
+        held = (self.base, self.base_scale)
+        super()._apply(fn, *args, **kwargs)
+        if held[1] is not None and (self.base.dtype != held[0].dtype or self.base_scale.dtype != held[1].dtype):
+            self.base, self.base_scale = (t.to(self.base.device) for t in held)
+        return self
+
+    @torch.no_grad()
+    def load_base(self, weight):
+        """Copy a dense weight [m, k] into the base, quantised on the GPU if it is held in 8 bits."""
+        assert self.base is not None and weight.shape == self.base.shape, f"a base of {None if self.base is None else tuple(self.base.shape)}, got {tuple(weight.shape)}"
+        if self.base_scale is None:
+            self.base.copy_(weight)
+            return
+        from triteia_amd.python.ops import quantize_fp8
+        codes, scales = quantize_fp8(weight.to(self.base.device), rows=128)
+        self.base.view(torch.uint8).copy_(codes.view(torch.uint8))
+        self.base_scale.copy_(scales)
 
     @torch.no_grad()
     def load_delta(self, i, module_or_qweight, meta=None, scale=None):
@@ -110,14 +134,16 @@ class multi_delta_linear(nn.Module):
 
     def forward(self, x, indices, plan=None):
         """x [..., k] fp16, indices int32 [tokens] in {-1, 0..N-1} (any order) -> [..., m]."""
-        from triteia_amd.python.capi import sbmm_2_4_planned, sbmm_2_4_routed
+        from triteia_amd.python.capi import matmul_fp8, sbmm_2_4_planned, sbmm_2_4_routed
         x2 = x.reshape(-1, x.shape[-1])
         x2 = x2 if x2.is_contiguous() else x2.contiguous()
         if plan is None:
-            y = native().sbmm(self.qweight, x2, self.meta, self.scale, indices, self.base)
+            y = native().sbmm(self.qweight, x2, self.meta, self.scale, indices, self.base, self.base_scale)
             if y is not None:
                 return y.view(x.shape[:-1] + (self.outfeatures,))
-        if self.base is not None:
+        if self.base_scale is not None:
+            y = matmul_fp8(x2, self.base, self.base_scale, None, None)
+        elif self.base is not None:
             y = torch.matmul(x2, self.base.t())
         else:
             y = torch.zeros((x2.shape[0], self.outfeatures), dtype=x.dtype, device=x.device)

@@ -5,7 +5,7 @@ delta indices[t] - M; -1 means base model only.
 """
 import torch
 
-from triteia_amd.python.capi import route_plan, routed_workspace, sbmm_2_4_routed, sgmv_routed
+from triteia_amd.python.capi import matmul_fp8, route_plan, routed_workspace, sbmm_2_4_routed, sgmv_routed
 from triteia_amd.python.capi._native import native
 from .lora import lora_forloop
 from .sbmm import sbmm_4bit_2_4_forloop
@@ -42,17 +42,24 @@ def baseline_ldmm(indices, x, LwA, LwB, DeltaW, metas, ss, base_weight=None, deb
     return y.to(x.dtype)
 
 
-def ldmm(indices, x, LwA, LwB, DeltaW, metas, ss, base_weight=None, debug=False):
+def _base(x, base_weight, base_scale):
+    return torch.matmul(x, base_weight.t()) if base_scale is None else matmul_fp8(x, base_weight, base_scale, None, None)
+
+
+def ldmm(indices, x, LwA, LwB, DeltaW, metas, ss, base_weight=None, debug=False, base_scale=None):
     """One routed LoRA pass (shrink + expand) for the LoRA tokens plus one routed sparse pass for
     the delta tokens, both accumulating in place into the base output; no gathers, no host
     synchronisation.  The reference routes the LoRA tokens through BGMV, which wants every
     adapter transposed on each call (ldmm.py:93-105); the kernels here read LwA / LwB as they are.
 
     indices int [B]; x [B, H1]; LwA [M, H1, R]; LwB [M, R, H2]; DeltaW / metas / ss the stacked
-    packed deltas.  Returns [B, H2] in x.dtype."""
+    packed deltas.  Returns [B, H2] in x.dtype.  base_scale: of a base_weight in e4m3, as
+    `quantize_fp8(w, rows=128)` leaves both (the product of `matmul_fp8`)."""
     # fp16 batches of up to 4096 tokens: the LoRA pair that routes by itself; what follows, with a routing plan for the
     # LoRA tokens, is for the others
-    y = native().ldmm(indices, x, LwA, LwB, DeltaW, metas, ss, base_weight)
+    if base_scale is not None and base_weight is None:
+        raise ValueError("base_scale without a base_weight")
+    y = native().ldmm(indices, x, LwA, LwB, DeltaW, metas, ss, base_weight, base_scale)
     if y is not None:
         return y
     x_ = x.to(torch.float16)
@@ -72,7 +79,7 @@ def ldmm(indices, x, LwA, LwB, DeltaW, metas, ss, base_weight=None, debug=False)
         side.wait_stream(cur)
         # (the GEMM is enqueued ahead of the side stream's work: recorded into a HIP graph in the other order, the
         # step measured 30 us longer on 256 tokens x 4096 x 11008; launched eagerly the order makes no difference)
-        y = torch.matmul(x_, base_weight.t())
+        y = _base(x_, base_weight, base_scale)
         try:
             with torch.cuda.stream(side):
                 plan = route_plan(idx32, M, workspace=ws)      # skips -1 and every index >= M (the delta tokens)
@@ -92,7 +99,7 @@ def ldmm(indices, x, LwA, LwB, DeltaW, metas, ss, base_weight=None, debug=False)
         sgmv_routed(y, v, B16, plan)
     else:
         if base_weight is not None:
-            y = torch.matmul(x_, base_weight.t())
+            y = _base(x_, base_weight, base_scale)
         else:
             y = torch.zeros(x_.shape[0], LwB.shape[2], dtype=x_.dtype, device=x_.device)
         if M > 0:

@@ -8,10 +8,12 @@ device and accepts any order.
 import torch
 
 from triteia_amd.python.capi._native import native
-from triteia_amd.python.capi import mul_2_4, sbmm_2_4, sbmm_2_4_multilaunch, sbmm_2_4_routed
+from triteia_amd.python.capi import matmul_fp8, mul_2_4, sbmm_2_4, sbmm_2_4_multilaunch, sbmm_2_4_routed
 
 
-def _base(xs, out_features, base_weight):
+def _base(xs, out_features, base_weight, base_scale=None):
+    if base_scale is not None:
+        return matmul_fp8(xs, base_weight, base_scale, None, None)
     if base_weight is not None:
         return torch.matmul(xs, base_weight.t())
     return torch.zeros(xs.shape[0], out_features, dtype=xs.dtype, device=xs.device)
@@ -66,14 +68,17 @@ def sbmm_4bit_2_4_multilaunch(qweights, xs, metas, ss, indices, base_weight=None
     return y
 
 
-def sbmm_4bit_2_4_native(qweights, xs, metas, ss, indices, base_weight=None):
+def sbmm_4bit_2_4_native(qweights, xs, metas, ss, indices, base_weight=None, base_scale=None):
     """Single-launch routed sbmm (sbmm.py:89-142): tokens are grouped by index on the device, each
     delta's weights are read once, and the result is accumulated straight into the base output.
-    No host synchronisation; indices may come in any order."""
-    y = native().sbmm(qweights, xs, metas, ss, indices, base_weight)
+    No host synchronisation; indices may come in any order.  base_scale: of a base_weight in e4m3,
+    as `quantize_fp8(w, rows=128)` leaves both (the product of `matmul_fp8`)."""
+    if base_scale is not None and base_weight is None:
+        raise ValueError("base_scale without a base_weight")
+    y = native().sbmm(qweights, xs, metas, ss, indices, base_weight, base_scale)
     if y is not None:
         return y
-    y = _base(xs, ss.shape[2], base_weight)
+    y = _base(xs, ss.shape[2], base_weight, base_scale)
     if indices.dtype != torch.int32:
         indices = indices.to(torch.int32)
     xs = xs if xs.is_contiguous() else xs.contiguous()
