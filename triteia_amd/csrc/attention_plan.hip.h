@@ -6,7 +6,7 @@
 // 64-token blocks, so that every list has work for the whole chip; a share's result goes to scratch and a tile's shares are joined by a launch behind.
 // Lengths stay on the device: what the host knows are upper bounds, from which it sizes the lists and the grids.
 //
-// One workgroup of two wavefronts, a list each, so that nothing but the sequences' lengths in LDS is waited for: sums over the lanes, a lane finds the
+// One workgroup of two wavefronts (with groups three), a list each, so that nothing but the sequences' lengths in LDS is waited for: sums over the lanes, a lane finds the
 // sequence of a tile by a binary search.  Tokens behind the last sequence get tiles without keys, whose rows are zeros.  Every number read from the
 // device is clamped and offsets that do not ascend are made to, so that every row has one tile and no list passes its end.
 //
@@ -15,7 +15,8 @@
 // new tokens of all of the group and whose context is the prefix, without a mask.  The group's own sequences begin behind it.  Each of their tiles is joined
 // from its own shares and the shares of the prefix's tiles that hold its rows.
 // Bound by latency: 6.4 us for one sequence, 8.2 for a step's 26 of which two are long (14.2 with 1024 threads on one list after the other, whose barriers
-// and shuffles were the time), 10.9 for 64, 15.7 for four prompts of 500 tokens and 64 heads over 8 (108 tiles), all of which are also put in order.
+// and shuffles were the time), 10.9 for 64, 15.7 for four prompts of 500 tokens and 64 heads over 8 (108 tiles), all of which are also put in order.  With groups: five
+// sequences of one 8.5, 64 12.7, 96 of six 18.5.
 #pragma once
 #include "lora_routed.hip.h"
 

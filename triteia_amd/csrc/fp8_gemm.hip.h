@@ -72,11 +72,11 @@ __device__ __forceinline__ void fp8_result(const Fp8Args& p, int share, int toke
 // NT x F: 16-token by 16-feature tiles of a wavefront; TW x FW wavefronts side by side.  Both operands go through LDS by direct loads, a ring of STAGES blocks.
 //
 // Few tiles are bound by the weights' way from HBM (64 tokens on 8192 x 28672 36 us, 6.5 TB/s; 53 before the walks were spread over K).  The large one, 256 x 256 on eight
-// wavefronts, is bound by LDS: a block's operands take 512 of its CU's cycles in and 1536 out, as many as its MFMAs, and the additions take every second slot of the vector
-// ALUs.  8000 tokens on 8192 x 28672 1600 to 1680 us, 2240 to 2350 TFLOP/s (1180 us without loads and additions, 1350 without loads, 1520 without additions; a library product
-// with one scale a tensor, without these additions, 1286).  On 4096 x 8192 x 8192 the matrix cores are busy 62 % of the time, wavefronts wait 29 %, and LDS has no conflicts.
+// wavefronts, by the matrix cores and what stands between their instructions: 8000 tokens on 8192 x 28672 1600 to 1680 us, 2240 to 2350 TFLOP/s; 1520 without the additions
+// (every second slot of the vector ALUs), 1350 without loads, 1180 without both.  Counted there: matrix cores busy 60 % of the cycles, at 1.9 GHz; LDS 27 %, no conflicts; wavefronts
+// wait 27 % of theirs.  (A library product with one scale a tensor, which has no additions, takes 1286.)
 // Measured and left: four wavefronts of 96 x 128 or 64 x 128, which read less of LDS (2246 and 2724 us: one wavefront a SIMD does not hide its own MFMAs), weights from L2 to
-// registers past LDS (3650), blocks two ahead, priorities.
+// registers past LDS (3650), requests two blocks ahead, priorities.
 template <int NT, int TW, int F, int FW, int STAGES>
 struct Fp8Tile {
   static constexpr int kTokens = 16 * NT * TW, kFeatures = 16 * F * FW;
