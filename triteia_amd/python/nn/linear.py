@@ -105,7 +105,7 @@ class multi_delta_linear(nn.Module):
 
     @torch.no_grad()
     def load_base(self, weight):
-        """Copy a dense weight [m, k] into the base, quantised on the GPU if it is held in 8 bits."""
+        """Copy a dense weight [m, k] into the base; one held in 8 bits is quantised on the GPU, from fp16 or bf16."""
         assert self.base is not None and weight.shape == self.base.shape, f"a base of {None if self.base is None else tuple(self.base.shape)}, got {tuple(weight.shape)}"
         if self.base_scale is None:
             self.base.copy_(weight)
