@@ -182,7 +182,7 @@ def sizes_of_every_tile():
     return {key: size for key, (_, size) in sorted(found.items())}
 
 
-@pytest.mark.parametrize("tile", [16016, 32016, 32032, 128016, 128032, 64064, 128064, 128128, 256128, 256256])
+@pytest.mark.parametrize("tile", [16016, 32016, 32032, 128016, 128032, 64064, 128064, 128096, 128128, 128160, 256096, 256128, 256192, 256224, 256256])
 def test_every_tile(tile):
     sizes = [size for key, size in sizes_of_every_tile().items() if key[0] == tile]
     assert sizes

@@ -41,12 +41,14 @@ struct Fp8Kernel {
   int tokens, features, beside, walkers;      // beside: workgroups that a CU holds; walkers: wavefronts that share the blocks
   float start, alone, shared;
 };
-// Fitted to 8000 timings of 20 tiles in graphs, on 8 layers from 1024 x 1024 to 8192 x 28672 with 1 to 2048 tokens, whole and with K in 2 to 16 shares, weights not in the caches.  On
-// these the rule's pick is 1.9 % behind the best of all that were timed on average, 19 % at most.
+// Fitted to 14000 timings of 27 tiles in graphs, on 8 layers from 1024 x 1024 to 8192 x 28672 with 1 to 6000 tokens, whole and with K in 2 to 16 shares, weights not in the caches.  Up to
+// 128 tokens the rule's pick is 0.3 % behind the best of all that were timed on average, 8 % at most; from 130 on 0.7 % and 8 %, and without the tiles of 96, 160, 192 and 224 tokens,
+// which leave fewer CUs idle in the last round, 5.3 % and 27 % (1500 on 8192 x 8192 110 -> 101 us, 800 on 2000 x 5000 23 -> 19).
 constexpr Fp8Kernel kFp8Kernels[] = {
     {16, 16, 2, 8, 3.644f, 0.306f, 0.369f},  {16, 32, 1, 8, 3.357f, 0.140f, 0.639f},  {32, 32, 1, 8, 3.500f, 0.885f, 0.414f},   {16, 128, 2, 1, 4.175f, 0.311f, 0.260f},
     {32, 128, 1, 1, 4.640f, 0.379f, 0.286f}, {64, 64, 2, 1, 4.963f, 0.354f, 0.255f},  {64, 128, 2, 1, 5.695f, 0.421f, 0.377f},
-    {128, 128, 1, 1, 5.864f, 0.626f, 0.091f}, {128, 256, 1, 1, 7.185f, 0.942f, 0.152f}, {256, 256, 1, 1, 7.492f, 1.662f, 0.189f}};
+    {96, 128, 1, 1, 5.076f, 0.395f, 0.544f}, {128, 128, 1, 1, 5.864f, 0.626f, 0.091f}, {160, 128, 1, 1, 5.627f, 0.727f, 0.326f}, {96, 256, 1, 1, 5.722f, 0.826f, 0.045f},
+    {128, 256, 1, 1, 7.185f, 0.942f, 0.152f}, {192, 256, 1, 1, 4.773f, 1.472f, 0.156f}, {224, 256, 1, 1, 5.354f, 1.552f, 0.361f}, {256, 256, 1, 1, 7.492f, 1.662f, 0.189f}};
 constexpr int kFp8KernelCount = sizeof(kFp8Kernels) / sizeof(kFp8Kernels[0]);
 constexpr int kFp8MaxSplits = 8;
 
@@ -111,8 +113,13 @@ int launch_fp8(const Fp8Args& a, int kernel, hipStream_t st) {
     case 4: return launch_fp8_tile<2, 1, 2, 4, 4>(a, st);
     case 5: return launch_fp8_tile<2, 2, 2, 2, 4>(a, st);
     case 6: return launch_fp8_tile<2, 2, 2, 4, 3>(a, st);
-    case 7: return launch_fp8_tile<4, 2, 2, 4, 3>(a, st);
-    case 8: return launch_fp8_tile<4, 2, 4, 4, 3>(a, st);
+    case 7: return launch_fp8_tile<3, 2, 2, 4, 3>(a, st);
+    case 8: return launch_fp8_tile<4, 2, 2, 4, 3>(a, st);
+    case 9: return launch_fp8_tile<5, 2, 2, 4, 3>(a, st);
+    case 10: return launch_fp8_tile<3, 2, 4, 4, 3>(a, st);
+    case 11: return launch_fp8_tile<4, 2, 4, 4, 3>(a, st);
+    case 12: return launch_fp8_tile<6, 2, 4, 4, 2>(a, st);
+    case 13: return launch_fp8_tile<7, 2, 4, 4, 2>(a, st);
     default: return launch_fp8_tile<8, 2, 4, 4, 2>(a, st);
   }
 }
