@@ -32,6 +32,8 @@ constexpr int kAttnSolo = 512;         // groups' sequences times heads of the c
 constexpr int kAttnPrefixRows = 32;    // prefixes of up to so many rows are walked by all wavefronts of a workgroup
 constexpr int kAttnRowBlocks = 16;     // blocks of a share of few rows, at least
 constexpr int kAttnTileBlocks = 8;     // a share of a tile of 128 rows, at least
+constexpr int kAttnRounds = 3;         // rounds of workgroups that groups' prompts are cut into, at most, if that leaves fewer slots idle
+constexpr int kAttnShareBlocks = 4;    // what a share costs ahead of its first block and in the join, in blocks
 constexpr int kAttnHalf = 30;           // blocks of a workgroup up to which half as many take the tiles of groups
 constexpr int kAttnOwnBlocks = 8;      // so are few rows' own parts of more than so many blocks, in batches with groups
 constexpr int kAttnMaxTokens = 0x7fffff80;   // a longer context is taken as this long, so that the end of its last block is still an int
@@ -101,7 +103,8 @@ inline AttnLayout attn_layout(int n_seqs, int n_tokens, int heads, int kv_heads,
     AttnList& x = a.list[which];
     // (as the kernel cuts them: into the shares of whole rounds of workgroups; a cut tile has two at least)
     const long units = tiles[which] * kv_heads, whole = units < (long)x.rounds * x.slots ? units : (long)x.rounds * x.slots;
-    const long shares = (whole + x.slots - 1) / x.slots * x.slots / kv_heads;
+    long shares = (whole + x.slots - 1) / x.slots * x.slots / kv_heads;
+    if (sharing > 0 && which == 1 && most > a.short_rows && tiles[1] > 0) shares = std::max(shares, (long)kAttnRounds * x.slots / kv_heads);
     x.max_joins = (int)(tiles[which] < shares / 2 ? tiles[which] : shares / 2);
     x.max_parts = (int)(tiles[which] > 0 ? shares : 0);
     x.max_items = (int)(tiles[which] > shares ? tiles[which] : shares);
@@ -314,16 +317,27 @@ __global__ __launch_bounds__(SHARED ? 192 : kAttnPlanThreads) void attention_pla
     if (pays) {                                                  // (one workgroup a CU and half the results to join, while they are short)
       if (which > 0 && units <= l.slots / 2 && (long)total * a.kv_heads <= kAttnHalf * l.slots / 2) most = l.slots / 2 / a.kv_heads;
     }
-    share = max(!SHARED || pays || which == 0 ? l.min_blocks : which == 1 ? kAttnTileBlocks : kAttnRowBlocks, (total + most - 1) / max(most, 1));
-    if (pays) {                                      // (a row's shares are joined: sixteen at most for this)
-      int longest = 0;
+    int longest = 0;
+    if constexpr (SHARED) {
 #pragma unroll
       for (int k = 0; k < kAttnSorted / 64; k++) longest = max(longest, mine[k]);
 #pragma unroll
       for (int d = 32; d > 0; d /= 2) longest = max(longest, __shfl_xor(longest, d));
-      share = max(share, (longest + 15) / 16);
     }
-    while (share <= total && sum_of([&](int blocks) { return max(1, (blocks + share - 1) / share); }) > most) share += (share + 7) / 8;
+    auto cut_into = [&](int shares) {
+      int blocks = max(!SHARED || pays || which == 0 ? l.min_blocks : which == 1 ? kAttnTileBlocks : kAttnRowBlocks, (total + shares - 1) / max(shares, 1));
+      if (pays) blocks = max(blocks, (longest + 15) / 16);       // (a row's shares are joined: sixteen at most for this)
+      while (blocks <= total && sum_of([&](int n) { return max(1, (n + blocks - 1) / blocks); }) > shares) blocks += (blocks + 7) / 8;
+      return blocks;
+    };
+    share = cut_into(most);
+    if (SHARED && !pays && which == 1 && tiles <= kAttnSorted) {  // (a batch without groups keeps its cut, and with it its bits)
+      int rounds = max(1, most * a.kv_heads / l.slots), least = rounds * (min(share, longest) + kAttnShareBlocks);
+      while (++rounds <= kAttnRounds && rounds * l.slots / a.kv_heads <= l.max_items) {
+        const int other = cut_into(rounds * l.slots / a.kv_heads), cost = rounds * (min(other, longest) + kAttnShareBlocks);
+        if (cost < least) least = cost, share = other;
+      }
+    }
   }
   // longest first, so that the last workgroups to run are short ones
   if (tiles <= kAttnSorted) {

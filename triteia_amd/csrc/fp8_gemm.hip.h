@@ -76,7 +76,7 @@ __device__ __forceinline__ void fp8_result(const Fp8Args& p, int share, int toke
 // (every second slot of the vector ALUs), 1350 without loads, 1180 without both.  Counted there: matrix cores busy 60 % of the cycles, at 1.9 GHz; LDS 27 %, no conflicts; wavefronts
 // wait 27 % of theirs.  (A library product with one scale a tensor, which has no additions, takes 1286.)
 // Measured and left: four wavefronts of 96 x 128 or 64 x 128, which read less of LDS (2246 and 2724 us: one wavefront a SIMD does not hide its own MFMAs), weights from L2 to
-// registers past LDS (3650), requests two blocks ahead, priorities.
+// registers past LDS (3650), 32 x 32 x 64 instructions (192 x 256 1960 -> 2200; 256 x 256 passes the registers), requests two blocks ahead, priorities.
 template <int NT, int TW, int F, int FW, int STAGES>
 struct Fp8Tile {
   static constexpr int kTokens = 16 * NT * TW, kFeatures = 16 * F * FW;
