@@ -131,6 +131,16 @@ def test_prefixes_that_are_cut_into_shares(kind):
 
 
 @pytest.mark.parametrize("kind", list(KINDS))
+def test_prompts_that_are_cut_into_two_rounds(kind):
+    """Prompts share nothing; 42 tiles over 8 heads are cut into more shares than the 64 of one round, and joined."""
+    batch = Shared([(1300, [(203, 203), (200, 251), (196, 199)]), (1280, [(203, 210), (193, 230), (200, 200)])], 32, 8, 64, 64, kind, torch.bfloat16, padding=3)
+    counts = batch.plan(203).buffer.view(torch.int32)[:6].tolist()
+    assert counts[3] == 42 and 64 < counts[2] <= 128 and counts[4:] == [0, 0], counts
+    batch.check(batch.attend(203))
+    batch.check(batch.attend(203, causal=False), causal=False)
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
 @pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("heads,kv_heads,dim", [(32, 32, 64), (30, 30, 128), (64, 32, 128)])
 def test_a_wavefront_for_each_sequence(kind, dtype, heads, kv_heads, dim):
