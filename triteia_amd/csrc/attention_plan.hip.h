@@ -147,6 +147,7 @@ struct AttnGroups {
   static constexpr int kSize = SHARED ? kAttnMaxGroups + 1 : 1;
   int start[kSize], first[kSize], least[kSize], few[kSize];     // few: sequences of half a tile's rows at most
   unsigned long long saved, rows;                        // blocks that are not read again, rows to join
+  int own;                                               // blocks of a head that the sequences' own parts have
   int longest;
   int home[SHARED ? kAttnMaxSeqs : 1];                   // a sequence's group, -1: none
 };
@@ -194,7 +195,7 @@ __global__ __launch_bounds__(SHARED ? 192 : kAttnPlanThreads) void attention_pla
       if (g > 0) unordered |= at < max(0, min(group_starts[g - 1], a.n_seqs));
     }
     const bool any_unordered = __any(unordered);
-    if (threadIdx.x == 0) groups.saved = groups.rows = 0, groups.longest = 0;
+    if (threadIdx.x == 0) groups.saved = groups.rows = 0, groups.longest = groups.own = 0;
     __syncthreads();                                     // (`crossed` has been read)
     if ((threadIdx.x & 63) == 0) crossed[threadIdx.x >> 6] = any_unordered;
     __syncthreads();
@@ -238,6 +239,13 @@ __global__ __launch_bounds__(SHARED ? 192 : kAttnPlanThreads) void attention_pla
     if (!pays)
       for (int g = threadIdx.x; g < a.n_groups; g += kThreads) count[a.n_seqs + 1 + g] = context[a.n_seqs + 1 + g] = 0;
     __syncthreads();
+    if (pays) {
+      int own = 0, all;
+      for (int b = threadIdx.x; b < a.n_seqs; b += kThreads)
+        if (count[b] > 0) own += min((context[b] - (groups.home[b] >= 0 ? context[a.n_seqs + 1 + groups.home[b]] : 0)) / kAttnBlock, 1 << 18);
+      attn_scan(own, &all);
+      if ((threadIdx.x & 63) == 0) atomicAdd(&groups.own, all);      // (read behind the next barrier)
+    }
   }
   const int which = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const AttnList& l = a.list[which];
@@ -315,8 +323,18 @@ __global__ __launch_bounds__(SHARED ? 192 : kAttnPlanThreads) void attention_pla
       return total;
     };
     const int total = sum_of([](int blocks) { return blocks; });
-    if (pays) {                                                  // (one workgroup a CU and half the results to join, while they are short)
-      if (which > 0 && units <= l.slots / 2 && (long)total * a.kv_heads <= kAttnHalf * l.slots / 2) most = l.slots / 2 / a.kv_heads;
+    if (pays && which > 0 && units <= l.slots / 2 && (long)total * a.kv_heads <= kAttnHalf * l.slots / 2) {
+      // Short walks leave slots to the own parts, and fewer results to join: half the slots.  Tiles: the more, the longer their walks and the less there is beside them.  (us with 3, 4, 5, 6 and
+      // 8 eighths of them: 64 requests of 64 heads over 8 behind 8200 tokens 61, 55, 51, 52, 61, of 32 + 32 heads 85, 93, 94, 95, 101; on 294 such batches of 32 to 128 requests 2.3 % behind
+      // the best of them on average, half the slots 5.2 %.)
+      const long walk = (long)total * a.kv_heads;
+      const long beside = SHARED ? 2L * groups.own * a.kv_heads : 0;
+      int eighths = 4;
+      if (which == 1) {
+        const bool some = walk * 2 >= 5L * l.slots / 2;
+        eighths = (walk >= 9L * l.slots / 2 ? 6 : some ? 5 : 3) - (beside >= walk) - (some && beside >= 5 * walk);
+      }
+      most = l.slots * eighths / 8 / a.kv_heads;
     }
     int longest = 0;
     if constexpr (SHARED) {
