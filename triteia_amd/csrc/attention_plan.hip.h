@@ -35,7 +35,7 @@ constexpr int kAttnTileBlocks = 8;     // a share of a tile of 128 rows, at leas
 // Rounds of workgroups that groups' prompts are cut into, at most, if that leaves fewer slots idle (42 tiles of 96 blocks over 8 heads, 336 workgroups on 512 slots, as 126 of 32 206 -> 180 us;
 // two groups of 3 prompts of 100 behind 12000, 64 heads over 8, 325 -> 274; three and four rounds give no more), and what a share costs ahead of its first block and in the join, in blocks.
 constexpr int kAttnRounds = 2, kAttnShareBlocks = 4;
-constexpr int kAttnHalf = 30;           // blocks of a workgroup up to which half as many take the tiles of groups
+constexpr int kAttnHalf = 30;          // blocks of a workgroup, on half of the slots, up to which a prefix is not given all of them
 constexpr int kAttnOwnBlocks = 8;      // so are few rows' own parts of more than so many blocks, in batches with groups
 constexpr int kAttnMaxTokens = 0x7fffff80;   // a longer context is taken as this long, so that the end of its last block is still an int
 constexpr int kAttnPlanThreads = 128;          // a wavefront for each list; of groups 192
