@@ -81,6 +81,33 @@ def test_base_in_8_bits_under_adapters_and_deltas(tokens):
     assert bool(((got.double() - rest - base).abs() <= bound).all())
 
 
+def test_one_row_of_any_stride_over_a_base_in_8_bits():
+    """A single row is adjacent elements whatever the strides of its view say: the newest token of a long sequence, a column."""
+    from triteia_amd.python.nn import multi_delta_linear
+    k, m, n, adapters, rank = 4096, 256, 3, 2, 16
+    layer = multi_delta_linear(k, m, n, with_base="fp8").cuda()
+    for buffer, value in zip((layer.qweight, layer.meta, layer.scale), to_gpu(*make_deltas(n, k, m, 3))):
+        buffer.copy_(value.view(buffer.shape))
+    layer.load_base(dense(m, k, 4))
+    rng = np.random.default_rng(8)
+    gA, gB = to_gpu((rng.standard_normal((adapters, k, rank)) * 0.05).astype(np.float16), (rng.standard_normal((adapters, rank, m)) * 0.05).astype(np.float16))
+    row = torch.from_numpy(activations(1, k, 5)).cuda()
+    hidden = torch.zeros(1, 4100, k, dtype=torch.float16, device="cuda")
+    hidden[:, -1] = row
+    views = hidden[:, -1], row.reshape(k, 1).t(), row.as_strided((1, k), (8, 1))
+    assert views[0].stride(0) > 1 << 24 and views[1].stride(0) == 1 and all(v.is_contiguous() and torch.equal(v, row) for v in views)
+    packed = layer.qweight, layer.meta, layer.scale
+    for index in (-1, 0, 2, 3):
+        idx = torch.tensor([index], dtype=torch.int32, device="cuda")
+        delta = idx.clamp(max=n - 1)
+        want = layer(row, delta), ops().ldmm(idx, row, gA, gB, *packed, layer.base, base_scale=layer.base_scale), ops().matmul_fp8(row, layer.base, layer.base_scale)
+        for x in views:
+            got = (ops().sbmm_4bit_2_4_native(packed[0], x, *packed[1:], delta, layer.base, layer.base_scale),
+                   ops().ldmm(idx, x, gA, gB, *packed, layer.base, base_scale=layer.base_scale), ops().matmul_fp8(x, layer.base, layer.base_scale))
+            assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(layer(x, delta), want[0])
+    assert torch.equal(layer(hidden[:, -1:], delta)[0], want[0])
+
+
 def test_refusals_of_the_base():
     from triteia_amd.python.nn import multi_delta_linear
     with pytest.raises(AssertionError, match="with_base"):

@@ -122,9 +122,10 @@ Tensor fp8_product(const Tensor& x, const Tensor& w, const Tensor& ws, const Ten
   shape.back() = m;
   Tensor y = at::empty(shape, x.options().dtype(type));
   const int x_type = xs ? 2 : fp8_type(x.scalar_type());
+  const int64_t x_stride = x.dim() == 2 && tokens > 1 ? x.stride(0) : k;      // (a single row's may be any number)
   const size_t bytes = triteia_hip_fp8_scratch_bytes(tokens, m, k, x_type);
   const Tensor scratch = bytes ? scratch_bytes(bytes, x) : Tensor();
-  return launched(triteia_hip_fp8_matmul(x.data_ptr(), x.dim() == 2 ? x.stride(0) : k, x_type, xs ? xs->data_ptr() : nullptr, xs ? xs->stride(0) : 0, xs ? xs->stride(1) : 0,
+  return launched(triteia_hip_fp8_matmul(x.data_ptr(), x_stride, x_type, xs ? xs->data_ptr() : nullptr, xs ? xs->stride(0) : 0, xs ? xs->stride(1) : 0,
                                          w.data_ptr(), w.stride(0), ws.data_ptr(), ws.stride(0), ws.stride(1), y.data_ptr(), fp8_type(type), tokens, m, k,
                                          bytes ? scratch.data_ptr() : nullptr, bytes, at_.dev, at_.handle()))
              ? y
