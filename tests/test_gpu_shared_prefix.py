@@ -152,6 +152,81 @@ def test_a_wavefront_for_each_sequence(kind, dtype, heads, kv_heads, dim):
     batch.check(batch.attend(30, causal=False, scale=0.2), causal=False, scale=0.2)
 
 
+MIXED = [(2048, [(1, 1 + 9 * i % 100) for i in range(40)])]
+
+
+@pytest.mark.parametrize("at", [0, 13, 40])
+def test_a_prompt_beside_requests_of_few_tokens(at):
+    """A prompt of a group walks its own context and leaves the others to share: as many tiles are joined as without it, wherever it stands."""
+    few = MIXED[0][1]
+    alone = Shared(MIXED, 8, 8, 64, 64)
+    mixed = Shared([(2048, few[:at] + [(1500, 1500)] + few[at:])], 8, 8, 64, 64)
+    joins = [batch.plan(most).buffer.view(torch.int32)[[1, 3, 5]].tolist() for batch, most in ((alone, 1), (mixed, 1500))]
+    assert joins[0][0] + joins[0][2] == len(few) == joins[1][0] + joins[1][2], joins
+    for most in (1, 1500):
+        mixed.check(mixed.attend(most))
+
+
+BETWEEN = [(1000, [(1, 30), (100, 120), (2, 5), (1, 1), (300, 310), (70, 70), (0, 9), (3, 200), (65, 90), (1, 2)]),
+           (800, [(80, 300), (1, 7), (257, 257), (66, 66), (129, 140), (4, 4), (1, 600), (70, 70)]), (640, [(70, 70), (1, 3), (2, 3), (80, 80)]), (600, [(100, 100), (1, 9), (67, 67)]), (900, [(1, 1), (1, 70)]),
+           (None, [(1, 50), (90, 90)])]
+PACKED = [(1024, [(15, 20), (270, 270), (16, 16), (14, 90), (90, 91), (64, 70), (64, 64), (1, 1), (99, 99), (260, 300), (60, 60)]), (700, [(64, 64), (666, 670), (64, 64), (1, 1)])]
+
+
+@pytest.mark.parametrize("many", [38, 40])
+def test_sequences_of_some_rows_share_while_they_are_few(many):
+    """Sequences of 65 to 256 rows are in the prefix as long as they have 8192 rows together."""
+    some = [(210, 220 + i) for i in range(many)]
+    batch = Shared([(768, [*some[:20], (1, 9), (1, 200), (0, 3), (3, 3), (2, 2), *some[20:]])], 2, 2, 64, 64)
+    counts = batch.plan(210).buffer.view(torch.int32)[:6].tolist()
+    assert counts[1] == 4 and (counts[4] > 0) == (many == 40), counts           # (a prefix of 7 rows is in the list of long walks, one of thousands among the tiles)
+    for most in (1, 210):
+        batch.check(batch.attend(most))
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 4, 128), (8, 2, 64), (20, 1, 128), (48, 48, 64)])
+@pytest.mark.parametrize("groups", [BETWEEN, PACKED], ids=["between", "packed"])
+def test_prompts_between_requests_of_few_tokens(kind, dtype, heads, kv_heads, dim, groups):
+    """The rows that share are not adjacent: in prefixes of few rows, of several tiles, in more than one group, with groups beside them whose rows are."""
+    batch = Shared(groups, heads, kv_heads, dim, 16, kind, dtype, padding=3)
+    for most in (1, 666):
+        batch.check(batch.attend(most))
+    batch.check(batch.attend(666, causal=False, scale=0.2), causal=False, scale=0.2)
+    few = [n for _, seqs in groups for n, _ in seqs if 0 < n * heads // kv_heads <= 64]
+    joins = batch.plan(666).buffer.view(torch.int32)[[1, 3, 5]].tolist()
+    assert len(few) < 2 or sum(joins) >= 2, joins
+
+
+def test_prompts_that_come_and_go_between_replays():
+    """Which sequences are prompts is the device's to say: one graph, whose offsets change between replays."""
+    batch = Shared([(700, [(1, 100), (170, 200), (2, 100), (1, 100), (166, 200), (3, 100)]), (900, [(1, 100), (1, 100), (180, 200), (1, 100)])], 4, 2, 64, 16)
+    q, cache, pages, starts, lens = batch.inputs()
+    groups = batch.groups()
+
+    def call():
+        plan = ops().attention_plan(cache, starts, lens, batch.heads, q.shape[0], 180, **groups)
+        return ops().paged_attention(q, cache, pages, starts, lens, plan=plan)
+
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    total = batch.starts[-1]
+    for new in ([n for n, _ in batch.lengths], [170, 1, 1, 66, 2, 3, 180, 1, 1, 1], [1] * 10, [20, 30, 1, 2, 60, 2, 1, 1, 50, 1], [1, 1, 129, 1, 128, 1, 2, 150, 1, 64], [n for n, _ in batch.lengths]):
+        batch.lengths = [(n, kv) for n, (_, kv) in zip(new, batch.lengths)]
+        batch.starts = [sum(new[:i]) for i in range(len(new) + 1)]
+        assert batch.starts[-1] <= total
+        starts.copy_(torch.tensor(batch.starts, dtype=torch.int32))
+        torch.cuda.synchronize()
+        graph.replay()
+        alone = call()
+        torch.cuda.synchronize()
+        assert torch.equal(alone, out)
+        batch.check(alone)
+
+
 @pytest.mark.parametrize("most", [1, None])
 def test_more_groups_and_tiles_than_a_wavefront_has_lanes(most):
     groups = [(64 * (15 + i % 3) + 5, [(1, 1 + i % 5)] * (4 + i % 3)) for i in range(75)]

@@ -11,12 +11,15 @@
 // device is clamped and offsets that do not ascend are made to, so that every row has one tile and no list passes its end.
 //
 // Sequences in groups that share their first tokens (SHARED): group g is sequences group_starts[g] .. group_starts[g + 1] - 1, whose tables begin with the
-// same pages.  Of prefix_lens[g] tokens, those that every row of the group sees, in whole blocks, are attended to once: by one more sequence, whose rows are the
-// new tokens of all of the group and whose context is the prefix, without a mask.  The group's own sequences begin behind it.  Each of their tiles is joined
-// from its own shares and the shares of the prefix's tiles that hold its rows.
+// same pages.  Its sequences of up to 64 rows share, and those of up to 256 as long as a batch has few of them: of prefix_lens[g] tokens, those that all of their rows see, in whole
+// blocks, are attended to once, by one more sequence, whose rows are all of their new tokens and whose context is the prefix, without a mask.  They themselves begin behind it, and each of
+// their tiles is joined from its own shares and the shares of the prefix's tiles that hold its rows.  Prompts of the group walk their whole context: their tiles have the matrix cores busy
+// either way, and in the prefix each of their rows is written in 32 bits and joined.  (us with them in the prefix or, where that does not pay, nothing shared, and without them: 64 requests of one token
+// and one of 1000 behind 8192, 64 heads over 8, 539 and 424, three of 100 263 and 168; 48 and one of 3000 behind 2000, 32 + 32 heads, 366 and 260.  But one of 200 rows, 20 requests beside it, 51 and 61.)
+// Where prompts stand between the others the prefix's rows are not adjacent, and the plan has a list of their tokens (`map`).
 // Bound by latency: 6.4 us for one sequence, 8.2 for a step's 26 of which two are long (14.2 with 1024 threads on one list after the other, whose barriers
 // and shuffles were the time), 10.9 for 64, 15.7 for four prompts of 500 tokens and 64 heads over 8 (108 tiles), all of which are also put in order.  With groups: five
-// sequences of one 8.5, 64 12.7, 96 of six 18.5.
+// sequences of one 9.2, 64 13.3, 96 of six 18.9.
 #pragma once
 #include "lora_routed.hip.h"
 
@@ -29,6 +32,8 @@ constexpr int kAttnSorted = 256;       // lists of up to this many tiles begin w
 constexpr int kAttnMaxSeqs = 4096;
 constexpr int kAttnMaxGroups = 1024;
 constexpr int kAttnSolo = 512;         // groups' sequences times heads of the cache above which each gets a wavefront
+constexpr int kAttnSharedRows = kAttnTileRows / 2;      // sequences of up to so many rows share a prefix,
+constexpr int kAttnMostRows = 2 * kAttnTileRows, kAttnMoreRows = 8192;      // and of up to so many, if those of more than kAttnSharedRows have so many together
 constexpr int kAttnPrefixRows = 32;    // prefixes of up to so many rows are walked by all wavefronts of a workgroup
 constexpr int kAttnRowBlocks = 16;     // blocks of a share of few rows, at least
 constexpr int kAttnTileBlocks = 8;     // a share of a tile of 128 rows, at least
@@ -43,7 +48,7 @@ constexpr int kAttnLists = 3;          // few rows, tiles of 128 rows, and long 
 
 // One share of one tile.
 struct AttnItem {
-  int seq, q_start, n_tokens, kv_len, tile, kv_begin, kv_end, part;   // part: of the scratch, -1: the whole tile
+  int seq, q_start, n_tokens, kv_len, tile, kv_begin, kv_end, part;   // q_start: the first token, below zero of a list of them (attn_token); part: of the scratch, -1: the whole tile
 };
 // A tile of several shares, or of a group: the list of the group's prefix (-1: none), the prefix's first tile there and its row of the tile's sequence's first.
 struct AttnJoin {
@@ -66,6 +71,8 @@ struct AttnLayout {
   int solo;              // short tiles: a wavefront each (groups only)
   int short_rows;        // sequences of more rows go to the long list; 0x7fffffff: there is none
   AttnList list[kAttnLists];      // short, long, walks
+  int shared_rows;       // of prefixes, at most
+  long map;              // tokens of prefixes whose rows are not adjacent (groups only)
   long ints;
 };
 
@@ -77,6 +84,7 @@ inline AttnLayout attn_layout(int n_seqs, int n_tokens, int heads, int kv_heads,
   const long live = n_seqs + 1 < n_tokens ? n_seqs + 1 : n_tokens;      // sequences with tokens, and the tokens behind them
   // (a group that shares has two sequences with tokens at least; its prefix has the rows of all of them)
   const long pairs = (n_seqs < n_tokens ? n_seqs : n_tokens) / 2, sharing = n_groups < pairs ? n_groups : pairs;
+  a.shared_rows = (int)std::min(rows, (long)n_seqs * kAttnSharedRows + kAttnMoreRows);
   a.solo = sharing > 0 && a.group <= 16 && live * kv_heads > kAttnSolo;
   const bool only_short = most <= 32 && sharing == 0;
   AttnList &s = a.list[0], &l = a.list[1], &p = a.list[2];
@@ -117,6 +125,8 @@ inline AttnLayout attn_layout(int n_seqs, int n_tokens, int heads, int kv_heads,
     x.joins = at, at += 8L * x.max_joins;
     if (sharing > 0) x.prefixes = at, at += 2L * x.max_joins;
   }
+  a.map = at;
+  if (sharing > 0) at += a.shared_rows / a.group;
   a.ints = at;
   return a;
 }
@@ -145,11 +155,16 @@ __device__ __forceinline__ void attn_range(const AttnSeq& s, int tile, int rows,
 template <bool SHARED>
 struct AttnGroups {
   static constexpr int kSize = SHARED ? kAttnMaxGroups + 1 : 1;
-  int start[kSize], first[kSize], least[kSize], few[kSize];     // few: sequences of half a tile's rows at most
+  int start[kSize], first[kSize], least[kSize], few[kSize], tokens[kSize];      // of the sequences that share; few: those of up to kAttnSharedRows rows
+  int mixed[kSize];                                      // prompts among the group's sequences
+  int more;                                              // rows of sequences that share if they fit
+  int listed;                                            // whether some prefix's tokens are in the plan's list
   unsigned long long saved, rows;                        // blocks that are not read again, rows to join
+  int prompts, wide;                                     // tiles of 128 rows: of sequences that share nothing, of prefixes
   int own;                                               // blocks of a head that the sequences' own parts have
   int longest;
-  int home[SHARED ? kAttnMaxSeqs : 1];                   // a sequence's group, -1: none
+  int home[SHARED ? kAttnMaxSeqs : 1];                   // the group that a sequence shares with, -1: none
+  int place[SHARED ? kAttnMaxSeqs : 1];                  // of its tokens among those that are listed
 };
 
 // grid 1, block kAttnPlanThreads, or 192 of groups
@@ -191,11 +206,11 @@ __global__ __launch_bounds__(SHARED ? 192 : kAttnPlanThreads) void attention_pla
     bool unordered = false;
     for (int g = threadIdx.x; g <= a.n_groups; g += kThreads) {
       const int at = max(0, min(group_starts[g], a.n_seqs));
-      groups.start[g] = at, groups.least[g] = 0x7e000000, groups.few[g] = 0, groups.first[g] = 0x7fffffff;
+      groups.start[g] = at, groups.least[g] = 0x7e000000, groups.few[g] = groups.tokens[g] = groups.mixed[g] = 0, groups.first[g] = 0x7fffffff;
       if (g > 0) unordered |= at < max(0, min(group_starts[g - 1], a.n_seqs));
     }
     const bool any_unordered = __any(unordered);
-    if (threadIdx.x == 0) groups.saved = groups.rows = 0, groups.longest = groups.own = 0;
+    if (threadIdx.x == 0) groups.saved = groups.rows = 0, groups.longest = groups.own = groups.listed = groups.prompts = groups.wide = groups.more = 0;
     __syncthreads();                                     // (`crossed` has been read)
     if ((threadIdx.x & 63) == 0) crossed[threadIdx.x >> 6] = any_unordered;
     __syncthreads();
@@ -210,25 +225,44 @@ __global__ __launch_bounds__(SHARED ? 192 : kAttnPlanThreads) void attention_pla
         const int mid = (lo + hi + 1) / 2;
         if (groups.start[mid] <= b) lo = mid; else hi = mid - 1;
       }
-      if (lo == a.n_groups) lo = -1;                     // behind the last
+      if (lo == a.n_groups || count[b] == 0) lo = -1;    // behind the last
       groups.home[b] = lo;
-      if (lo >= 0 && count[b] > 0) {
-        atomicMin(&groups.least[lo], a.causal ? context[b] - count[b] : context[b]);
-        atomicMin(&groups.first[lo], b);
-        if ((long)count[b] * a.group <= kAttnTileRows / 2) atomicAdd(&groups.few[lo], 1);
+      const long rows = (long)count[b] * a.group;
+      if (lo >= 0 && rows > kAttnSharedRows && rows <= kAttnMostRows) atomicAdd(&groups.more, (int)rows);
+    }
+    __syncthreads();
+    const int most_rows = groups.more <= kAttnMoreRows ? kAttnMostRows : kAttnSharedRows;
+    for (int b = threadIdx.x; b < a.n_seqs; b += kThreads) {
+      const int home = groups.home[b];
+      const long rows = (long)count[b] * a.group;
+      if (home >= 0 && rows <= most_rows) {
+        atomicMin(&groups.least[home], a.causal ? context[b] - count[b] : context[b]);
+        atomicMin(&groups.first[home], b);
+        atomicAdd(&groups.tokens[home], count[b]);
+        if (rows <= kAttnSharedRows) atomicAdd(&groups.few[home], 1);
+      } else {
+        if (home >= 0) groups.home[b] = -1, groups.mixed[home] = 1;
+        if (rows > a.short_rows) atomicAdd(&groups.prompts, (int)((rows + kAttnTileRows - 1) / kAttnTileRows));
       }
     }
     __syncthreads();
     for (int g = threadIdx.x; g < a.n_groups; g += kThreads) {
-      // (a window hides of the prefix from each row what it hides; nothing is shared then.  Nor among prompts: tiles of 128 rows have the matrix cores busy either way.)
+      // (a window hides of the prefix from each row what it hides; nothing is shared then)
       int prefix = groups.few[g] < 2 || a.window > 0 ? 0 : min(prefix_lens[g], groups.least[g]);
       prefix = max(prefix, 0) / kAttnBlock * kAttnBlock;
-      const int b = a.n_seqs + 1 + g, from = start[groups.start[g]];
-      start[b] = from, count[b] = prefix > 0 ? start[groups.start[g + 1]] - from : 0, context[b] = prefix;
+      const int b = a.n_seqs + 1 + g;
+      start[b] = count[b] = 0, context[b] = prefix;
       if (prefix > 0) {
+        start[b] = start[groups.first[g]], count[b] = groups.tokens[g];
+        if (groups.mixed[g]) {
+          int end = groups.start[g + 1] - 1;             // the last that shares
+          while (groups.home[end] != g) end--;
+          if (start[end] + count[end] - start[b] != count[b]) start[b] = -1, groups.listed = 1;      // (not adjacent: placed below)
+        }
         atomicAdd(&groups.saved, (unsigned long long)(groups.few[g] - 1) * (prefix / kAttnBlock) * a.kv_heads);
         atomicAdd(&groups.rows, (unsigned long long)count[b] * a.group * a.kv_heads);
         atomicMax(&groups.longest, prefix / kAttnBlock);
+        if ((long)count[b] * a.group > kAttnPrefixRows) atomicAdd(&groups.wide, (count[b] * a.group + kAttnTileRows - 1) / kAttnTileRows);
       }
     }
     __syncthreads();
@@ -236,9 +270,32 @@ __global__ __launch_bounds__(SHARED ? 192 : kAttnPlanThreads) void attention_pla
     // 128 single tokens behind 128 to 8192 shared ones, over 8 and 32 heads of the cache, the choice is 0.4 % behind the better of both on average, 19 % at most: 64 requests of
     // 64 heads behind 512 tokens 13.9 us each for itself and 19.0 shared, behind 2048 33.7 and 26.0, behind 8192 124 and 48.
     pays = 10 * groups.saved >= 40000 + 6 * groups.rows || (groups.saved > 0 && groups.longest >= 12 && a.n_seqs * a.kv_heads <= 256);
+    // Not where prompts fill whole rounds of workgroups and the prefixes' tiles would begin another: 64 requests and a prompt of 2048 behind 8192 774 us, shared 885; 32 and one of 1000 behind
+    // 4096 219 and 260.
+    const uint32_t slots = a.list[1].slots, prompts = (uint32_t)groups.prompts * a.kv_heads, with = prompts + (uint32_t)groups.wide * a.kv_heads;      // (below 2^31)
+    if (4L * prompts >= 3L * with && (with + slots - 1) / slots > (prompts + slots - 1) / slots) pays = false;
     if (!pays)
       for (int g = threadIdx.x; g < a.n_groups; g += kThreads) count[a.n_seqs + 1 + g] = context[a.n_seqs + 1 + g] = 0;
     __syncthreads();
+    if (pays && groups.listed) {
+      if (threadIdx.x < 64) {
+        int listed = 0, all;
+        for (int b0 = 0; b0 < a.n_seqs; b0 += 64) {
+          const int b = b0 + threadIdx.x, home = b < a.n_seqs ? groups.home[b] : -1;
+          const int before = attn_scan(home >= 0 && start[a.n_seqs + 1 + home] < 0 ? count[b] : 0, &all);
+          if (b < a.n_seqs) groups.place[b] = listed + before;
+          listed += all;
+        }
+      }
+      __syncthreads();
+      for (int b = threadIdx.x; b < a.n_seqs; b += kThreads)
+        if (groups.home[b] >= 0 && start[a.n_seqs + 1 + groups.home[b]] < 0)
+          for (int i = 0; i < count[b]; i++) plan[a.map + groups.place[b] + i] = start[b] + i;
+      __syncthreads();
+      // (what attn_token reads: below zero, the plan's index)
+      for (int g = threadIdx.x; g < a.n_groups; g += kThreads)
+        if (start[a.n_seqs + 1 + g] < 0) start[a.n_seqs + 1 + g] = ~(int)(a.map + groups.place[groups.first[g]]);
+    }
     if (pays) {
       int own = 0, all;
       for (int b = threadIdx.x; b < a.n_seqs; b += kThreads)
@@ -257,7 +314,7 @@ __global__ __launch_bounds__(SHARED ? 192 : kAttnPlanThreads) void attention_pla
   }
   auto from_of = [&](int b) { return SHARED && b < a.n_seqs && groups.home[b] >= 0 ? context[a.n_seqs + 1 + groups.home[b]] : 0; };
   auto list_of = [&](int b, long rows) {                         // of sequence b, the tokens behind the last or a prefix
-    if (SHARED && b > a.n_seqs) return rows <= kAttnPrefixRows ? 2 : 1;
+    if (SHARED && b > a.n_seqs) return rows <= kAttnPrefixRows && start[b] >= 0 ? 2 : 1;      // (tiles only take their tokens from a list)
     if (SHARED && b < a.n_seqs && rows <= a.short_rows && context[b] - from_of(b) > kAttnOwnBlocks * kAttnBlock) return 2;
     return rows <= a.short_rows ? 0 : 1;
   };
@@ -405,7 +462,8 @@ __global__ __launch_bounds__(SHARED ? 192 : kAttnPlanThreads) void attention_pla
       AttnJoin j = {t.s.start, t.s.n, t.tile, part, splits, -1, 0, 0};
       if (SHARED && t.home > 0) {
         j.prefix_list = list_of(t.home, (long)count[t.home] * a.group);
-        j.prefix_tile = tiles_ahead[j.prefix_list][t.home], j.prefix_row = (t.s.start - start[t.home]) * a.group;
+        const int ahead_of = start[t.home] < 0 ? groups.place[t.seq] - groups.place[groups.first[t.home - a.n_seqs - 1]] : t.s.start - start[t.home];
+        j.prefix_tile = tiles_ahead[j.prefix_list][t.home], j.prefix_row = ahead_of * a.group;
       }
       if (SHARED && joins) fullest = max(fullest, min(l.rows, t.s.n * a.group - t.tile * l.rows));
       if (joins) reinterpret_cast<AttnJoin*>(plan + l.joins)[join] = j;

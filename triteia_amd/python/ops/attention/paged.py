@@ -15,8 +15,9 @@ def attention_plan(cache, q_starts, kv_lens, n_heads, n_tokens, max_q=None, caus
 
     Sequences that share a prefix: group g is sequences group_starts[g] .. group_starts[g + 1] - 1 (int32 [groups + 1], ascending; those ahead of the first and behind the last are
     in none), whose contexts begin with the same prefix_lens[g] tokens (int32 [groups]) on the same pages.  What all new tokens of a group see of its prefix is read and
-    multiplied once for all of them, in whole blocks of 64; the results are those of every sequence by itself, in another order of sums.  A group of one
-    sequence, a prefix of 0 and a batch with a `window` share nothing."""
+    multiplied once for all of them, in whole blocks of 64; the results are those of every sequence by itself, in another order of sums.  Prompts among them (of more than 256 new tokens times
+    heads / kv_heads, of more than 64 in a batch with many such) go through their whole context by themselves.  A group of one sequence, of prompts, a prefix of 0 and a batch with a `window` share
+    nothing."""
     return capi.attention_plan(q_starts, kv_lens, n_tokens, n_heads, cache.kv_heads, max_q, causal, window, group_starts, prefix_lens)
 
 
