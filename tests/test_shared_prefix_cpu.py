@@ -55,6 +55,28 @@ def test_sizes():
     assert lib.triteia_hip_shared_plan_bytes(4, 1025, 4, 4, 2, 1) == 0 and lib.triteia_hip_shared_scratch_bytes(4, 1025, 4, 4, 2, 1, 64) == 0
 
 
+@pytest.mark.parametrize("heads,kv_heads", [(64, 8), (32, 32), (32, 4), (20, 1)])
+@pytest.mark.parametrize("seqs,groups", [(1, 1), (8, 1), (16, 3), (64, 1), (200, 20)])
+def test_scratch_of_prompts(heads, kv_heads, seqs, groups):
+    """Prompts share nothing, and no number of their tokens takes more: beside the scratch without groups there is that of the rows that may share, 64 a sequence and 4096, in tiles of 128, and of
+    the tiles that a sequence or a group leaves part empty, each for the rows themselves and for the prefix."""
+    lib, dim, group = _ffi.lib(), 128, heads // kv_heads
+    rows = 64 * seqs + 4096
+    tiles = 2 * rows // 128 + 2 * (seqs + groups + 1)
+    allowed = 4 * kv_heads * (dim + 2) * (128 * tiles + 48 * (seqs + groups + 1)) + 2 * 1024 * 32 * (dim + 2) * 4
+    for max_q in (1, 4096):
+        sizes = []
+        for tokens in (8192, 32768, 131072, 1 << 20):
+            held = lib.triteia_hip_shared_scratch_bytes(seqs, groups, tokens, heads, kv_heads, max_q, dim)
+            alone = lib.triteia_hip_attention_scratch_bytes(seqs, tokens, heads, kv_heads, 4096, dim)
+            assert 0 < held <= alone + allowed, (tokens, held, alone, allowed)
+            if group * tokens >= rows + 128 * seqs:
+                sizes.append(held)
+        assert max(sizes) <= 1.02 * min(sizes), sizes
+    eight = lib.triteia_hip_shared_scratch_bytes(8, 1, 131072, 64, 8, 131072, 128), lib.triteia_hip_attention_scratch_bytes(8, 131072, 64, 8, 131072, 128)
+    assert eight[0] <= 1.2 * eight[1], eight
+
+
 class Subclass(torch.Tensor):
     """Any subclass: it may give every operation another meaning."""
 

@@ -33,7 +33,7 @@ constexpr int kAttnMaxSeqs = 4096;
 constexpr int kAttnMaxGroups = 1024;
 constexpr int kAttnSolo = 512;         // groups' sequences times heads of the cache above which each gets a wavefront
 constexpr int kAttnSharedRows = kAttnTileRows / 2;      // sequences of up to so many rows share a prefix,
-constexpr int kAttnMostRows = 2 * kAttnTileRows, kAttnMoreRows = 8192;      // and of up to so many, if those of more than kAttnSharedRows have so many together
+constexpr int kAttnMostRows = 2 * kAttnTileRows, kAttnMoreRows = 4096;      // and of up to so many, if those of more than kAttnSharedRows have so many together
 constexpr int kAttnPrefixRows = 32;    // prefixes of up to so many rows are walked by all wavefronts of a workgroup
 constexpr int kAttnRowBlocks = 16;     // blocks of a share of few rows, at least
 constexpr int kAttnTileBlocks = 8;     // a share of a tile of 128 rows, at least
@@ -96,9 +96,13 @@ inline AttnLayout attn_layout(int n_seqs, int n_tokens, int heads, int kv_heads,
   l.rows = kAttnTileRows;
   p.rows = kAttnPrefixRows, p.slots = 512, p.min_blocks = kv_heads <= 8 ? 2 : 4, p.rounds = 2, p.waves = 4;
   long tiles[kAttnLists] = {only_short ? live + rows / s.rows : a.short_rows ? live : 0, only_short ? 0 : live + rows / l.rows, 0};
+  long joined = 0, kept = 0;            // tiles of the long list that share a prefix, those and the prefixes'
   if (sharing > 0) {
-    const long most_long = rows / (a.short_rows + 1), most_wide = rows / (kAttnPrefixRows + 1);      // sequences and prefixes of the long list
-    tiles[1] = (live < most_long ? live : most_long) + rows / l.rows + (sharing < most_wide ? sharing : most_wide) + rows / l.rows;
+    // (sequences and prefixes of the long list: of more rows than the others take.  A short prefix whose tokens are listed has a prompt in its group, and with it more rows than that.)
+    joined = std::min(live, (long)a.shared_rows / (a.short_rows + 1)) + a.shared_rows / l.rows;
+    const long prefixes = std::min(sharing, rows / (kAttnPrefixRows + 1)) + a.shared_rows / l.rows;
+    kept = joined + prefixes;
+    tiles[1] = std::min(live, rows / (a.short_rows + 1)) + rows / l.rows + prefixes;
     tiles[2] = sharing + live;
     l.min_blocks = 2;                  // (kAttnTileBlocks, and kAttnRowBlocks for walks, where it does not pay to share)
   }
@@ -117,13 +121,17 @@ inline AttnLayout attn_layout(int n_seqs, int n_tokens, int heads, int kv_heads,
     x.max_joins = (int)(tiles[which] < shares / 2 ? tiles[which] : shares / 2);
     x.max_parts = (int)(tiles[which] > 0 ? shares : 0);
     x.max_items = (int)(tiles[which] > shares ? tiles[which] : shares);
-    if (sharing > 0) x.max_joins = (int)tiles[which], x.max_parts = x.max_items;      // (a group's tiles are shares, cut or not)
+    // (of a group tiles are shares, cut or not.  Of the long list those are few, whatever prompts there are beside them: 8 sequences of 64 heads over 8 with 32768 new tokens have
+    // 80 MB of scratch, 70 without groups; a place for every row, twice, was 2.2 GB.)
+    if (sharing > 0 && which != 1) x.max_joins = (int)tiles[which], x.max_parts = x.max_items;
+    if (sharing > 0 && which == 1) x.max_parts = (int)std::max(shares, kept), x.max_joins = (int)std::min(tiles[1], joined + x.max_parts / 2);
   }
   long at = sharing > 0 ? 16 : 8;
-  for (AttnList& x : a.list) {
+  for (int which = 0; which < kAttnLists; which++) {
+    AttnList& x = a.list[which];
     x.items = at, at += 8L * x.max_items;
     x.joins = at, at += 8L * x.max_joins;
-    if (sharing > 0) x.prefixes = at, at += 2L * x.max_joins;
+    if (sharing > 0) x.prefixes = at, at += 2L * tiles[which];
   }
   a.map = at;
   if (sharing > 0) at += a.shared_rows / a.group;
@@ -409,7 +417,7 @@ __global__ __launch_bounds__(SHARED ? 192 : kAttnPlanThreads) void attention_pla
     share = cut_into(most);
     if (SHARED && !pays && which == 1 && tiles <= kAttnSorted) {  // (a batch without groups keeps its cut, and with it its bits)
       int rounds = max(1, most * a.kv_heads / l.slots), least = rounds * (min(share, longest) + kAttnShareBlocks);
-      while (++rounds <= kAttnRounds && rounds * l.slots / a.kv_heads <= l.max_items) {
+      while (++rounds <= kAttnRounds && rounds * l.slots / a.kv_heads <= l.max_parts) {
         const int other = cut_into(rounds * l.slots / a.kv_heads), cost = rounds * (min(other, longest) + kAttnShareBlocks);
         if (cost < least) least = cost, share = other;
       }
@@ -452,7 +460,7 @@ __global__ __launch_bounds__(SHARED ? 192 : kAttnPlanThreads) void attention_pla
     const bool cut = splits > 1 || (SHARED && i >= 0 && t.home != -1), joins = cut && t.home != -2;
     const int join = n_joins + attn_scan(joins, &all_joins);
     const int part = n_parts + attn_scan(cut ? splits : 0, &all_parts);
-    if (i >= 0 && (item + splits > l.max_items || (joins && join >= l.max_joins))) {
+    if (i >= 0 && (item + splits > l.max_items || (joins && join >= l.max_joins) || (cut && part + splits > l.max_parts))) {
       end_items = min(end_items, item), end_joins = min(end_joins, join);
     } else if (i >= 0) {
       AttnItem* out = reinterpret_cast<AttnItem*>(plan + l.items) + item;
