@@ -134,7 +134,14 @@ def ptr(t):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)
 
 
+def require_no_trace():
+    """torch.jit.trace records torch's operations: of a kernel launched beside them it would keep the empty output."""
+    if torch.jit.is_tracing():
+        raise RuntimeError("this op launches a kernel of its own, which a trace does not record: call it outside of torch.jit.trace (or capture a graph)")
+
+
 def require_gpu(**tensors):
+    require_no_trace()
     dev = None
     for name, t in tensors.items():
         if not isinstance(t, torch.Tensor):

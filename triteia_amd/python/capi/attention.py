@@ -22,6 +22,7 @@ def _check(err):
 
 def _require(like=None, optional=(), **tensors):
     """GPU tensors of one device, in any layout, that record no gradient in either direction; those named in `optional` may be None."""
+    _ffi.require_no_trace()
     for name, t in tensors.items():
         if t is None and name in optional:
             continue
