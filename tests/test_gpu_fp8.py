@@ -197,6 +197,43 @@ def test_every_tile(tile):
         assert torch.equal(*twice)
 
 
+@pytest.mark.parametrize("tile", [16016, 32016, 32032, 128016, 128032, 64064, 128064, 128096, 128128, 128160, 256096, 256128, 256192, 256224, 256256])
+def test_every_tile_adds_every_product(tile):
+    """Whole numbers of -8 to 8 under scales of powers of two that change from block to block: products of up to 64, whole, lie within the 13 bits that the instruction keeps, and sums of up to 11024 of them
+    times 4, in quarters, within 24.  So every sum is exact, and one product left out, taken twice or under another block's scale shows in its element.
+
+    And random codes in norm: of eight products seven are off by less than 2^-13 of the largest, each with a sign of its own: sqrt(7 / 3) 2^-13 of it in the mean, whose square is at most the sum
+    of all eight's, so the result is off by that part of its norm, below 2^-12.  One product in 4096 left out everywhere is 2^-6."""
+    for tokens, k, m in [size for key, size in sizes_of_every_tile().items() if key[0] == tile]:
+        g = torch.Generator("cuda").manual_seed(tokens + k + m)
+        pick = lambda lo, hi, *shape: torch.randint(lo, hi + 1, shape, generator=g, device="cuda").float()  # noqa: E731
+        blocks = -(-k // 128)
+        x, w = pick(-8, 8, tokens, k).to(E4M3), pick(-8, 8, m, k).to(E4M3)
+        xs, ws = torch.exp2(pick(-1, 1, tokens, blocks)), torch.exp2(pick(-1, 1, -(-m // 128), blocks))
+        want = values(x, xs, 1) @ values(w, ws, 128).t()
+        assert torch.equal(want, want.float().double()) and torch.equal(ops().matmul_fp8(x, w, ws, x_scale=xs, dtype=torch.float32).double(), want)
+        for dtype in HALF:
+            assert torch.equal(ops().matmul_fp8(x, w, ws, x_scale=xs, dtype=dtype), want.float().to(dtype))
+        x, xs = ops().quantize_fp8(torch.randn(tokens, k, generator=g, device="cuda").half())
+        w, ws = ops().quantize_fp8(torch.randn(m, k, generator=g, device="cuda").half(), rows=128)
+        want = values(x, xs, 1) @ values(w, ws, 128).t()
+        off = (ops().matmul_fp8(x, w, ws, x_scale=xs, dtype=torch.float32).double() - want).norm() / want.norm()
+        assert float(off) <= 2.0 ** -12, (tokens, k, m, float(off))
+
+
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_what_cancels_in_eight_products(tokens):
+    """Small products beside large ones that cancel: kept to 2^-13 of the largest in its eight, and whole in another."""
+    one, w, x = torch.ones(1, 1, device="cuda"), torch.zeros(16, 128, device="cuda"), torch.zeros(tokens, 128, device="cuda")
+    x[:, 8:10], w[:, 8], w[:, 9] = 448.0, 448.0, -448.0
+    for a, b in ((2.0, 2.0), (3.0, 4.0), (15.0, 15.0), (0.25, 0.5), (-7.0, 8.0)):
+        for place, bound in ((10, 2.0 ** -13 * 448 * 448), (15, 2.0 ** -13 * 448 * 448), (7, 0.0), (16, 0.0), (127, 0.0)):
+            near_x, near_w = x.clone(), w.clone()
+            near_x[:, place], near_w[:, place] = a, b
+            got = ops().matmul_fp8(near_x.to(E4M3), near_w.to(E4M3), one, x_scale=one.expand(tokens, 1), dtype=torch.float32)
+            assert bool(((got - a * b).abs() <= bound).all()), (a, b, place, got[0, 0])
+
+
 @pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("tokens", [1, 3, 4, 5, 8])
 def test_few_tokens_quantised_on_the_way(tokens, dtype):
