@@ -12,8 +12,8 @@ int check_fp8(const char* what, int n, int k) {
 }
 int fp8_blocks(int k) { return (k + kFp8Block - 1) / kFp8Block; }
 
-// 16 rows x U blocks a workgroup of the quantiser: one block while all of them fit side by side, four of a large tensor, requested together.  (us, one / four, on rows of 8192: 128 2.5 / 3.2,
-// 512 4.05 / 4.18, 1024 6.17 / 5.97, 8000 34.8 / 32.4.)
+// 16 rows x U blocks a workgroup of the quantiser: one block while all of them fit side by side, four of a large tensor, requested together.  (us, one / four, on rows of 8192 in
+// fp16, four tensors in turn and the same one again: 128 2.4 / 3.2 and 2.4 / 3.1, 512 4.4 / 4.8 and 3.9 / 4.1, 1024 7.2 / 7.3 and 5.9 / 5.8, 8000 41 / 37.5 and 33 / 32.)
 long fp8_groups(int n, int k, int u) { return (n + 15L) / 16 * ((fp8_blocks(k) + u - 1) / u); }
 constexpr int kFp8Wide = 4;
 int fp8_width(int n, int k) { return fp8_groups(n, k, 1) > 2048 ? kFp8Wide : 1; }
@@ -61,7 +61,9 @@ Fp8Pick pick_fp8(int tokens, int m, int k) {
   const int blocks = fp8_blocks(k);
   for (int i = 0; i < kFp8KernelCount; i++) {
     const Fp8Kernel& c = kFp8Kernels[i];
-    if (c.walkers > 1 && c.features > 16 && tokens <= 16) continue;      // (4096 x 11008 on 16 features a workgroup 10.9 us, on 32 12.1)
+    // (The fitted costs would give 32 features a workgroup to large layers.  1 to 16 tokens in codes on 16 features and on 32, us, weights not in the caches: 4096 x 4096 6.1 to 6.6 and
+    // 6.7 to 7.8, 4096 x 11008 11.6 to 12.6 and 13.2 to 14.3, 11008 x 4096 12.0 to 13.0 and 13.2 to 15.4, 4096 x 12288 12.3 to 13.4 and 13.5 to 14.7; on 8192 x 8192 14.0 to 15.5 and 13.9 to 14.1.)
+    if (c.walkers > 1 && c.features > 16 && tokens <= 16) continue;
     const long tiles = ((tokens + c.tokens - 1L) / c.tokens) * ((m + c.features - 1L) / c.features);
     for (int splits = 1; splits <= kFp8MaxSplits; splits *= 2) {
       if (splits > 1 && (tiles * splits > 512 || blocks / splits < 8 || (c.walkers > 1 && (splits > 2 || tiles > 96)))) break;
@@ -77,8 +79,9 @@ Fp8Pick pick_fp8(int tokens, int m, int k) {
   }
   return best;
 }
-// Rows of W lie a power of two apart, and walks in lockstep read the same few channels: 64 tokens on 8192 x 28672 53 us, spread 43.  From 512 tokens on, and on small layers,
-// there is nothing to spread (2048 tokens on 4096 x 4096 39.0 and 39.4).
+// Rows of W lie a power of two apart, and walks in lockstep read the same few channels of HBM: in codes on 8192 x 28672, weights not in the caches, one token 52 us and spread 41, 64 56 and 48, 256
+// 83 and 81; 16 on 4096 x 22016 24 and 19, on 4096 x 11008 13.2 and 12.6.  From 512 tokens on, on small layers and on weights that the Infinity Cache holds there is nothing to spread (512 131 and 131; 4096 x 4096
+// 6.6 and 6.6; one token on 8192 x 28672 again and again 36.4 and 36.7).
 bool fp8_rotates(int tokens, int m, int k) { return tokens <= 512 && (long)m * k >= (1L << 25); }
 
 long fp8_units(const Fp8Args& a, int tokens, int features) { return ((a.m + features - 1L) / features) * ((a.tokens + tokens - 1L) / tokens) * a.splits; }

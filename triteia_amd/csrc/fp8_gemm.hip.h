@@ -71,10 +71,11 @@ __device__ __forceinline__ void fp8_result(const Fp8Args& p, int share, int toke
 
 // NT x F: 16-token by 16-feature tiles of a wavefront; TW x FW wavefronts side by side.  Both operands go through LDS by direct loads, a ring of STAGES blocks.
 //
-// Few tiles are bound by the weights' way from HBM (64 tokens on 8192 x 28672 36 us, 6.5 TB/s; 53 before the walks were spread over K).  The large one, 256 x 256 on eight
+// Few tiles are bound by the weights' way from HBM: 64 tokens in codes on 8192 x 28672, four weights in turn, 48 us (4.9 TB/s; 56 before the walks were spread over K); the same weight
+// again and again, which the Infinity Cache holds, 36 either way.  The large one, 256 x 256 on eight
 // wavefronts, by the matrix cores and what stands between their instructions: 8000 tokens on 8192 x 28672 1600 to 1680 us, 2240 to 2350 TFLOP/s; 1520 without the additions
 // (every second slot of the vector ALUs), 1350 without loads, 1180 without both.  Counted there: matrix cores busy 60 % of the cycles, at 1.9 GHz; LDS 27 %, no conflicts; wavefronts
-// wait 27 % of theirs.  (A library product with one scale a tensor, which has no additions, takes 1286.)
+// wait 27 % of theirs; 2.8 GB read beyond L2, 0.3 of them once, at 1.7 TB/s.  (A library product with one scale a tensor, which has no additions, takes 1286.)
 // Measured and left: four wavefronts of 96 x 128 or 64 x 128, which read less of LDS (2246 and 2724 us: one wavefront a SIMD does not hide its own MFMAs), weights from L2 to
 // registers past LDS (3650), 32 x 32 x 64 instructions (192 x 256 1960 -> 2200; 256 x 256 passes the registers), requests two blocks ahead, priorities.
 template <int NT, int TW, int F, int FW, int STAGES>

@@ -3,8 +3,8 @@
 // A block of magnitudes below 1e-30 is zeros with scale 0; one that holds a NaN or an infinity gets the scale NaN, so that all of it
 // reads back as NaN.  Scale and quotient are rounded as 32-bit divisions round.
 //
-// Bound by memory: 16 lanes of 16 bytes hold a row of a block, so that a maximum over it is four lane moves.  8000 x 8192 in bf16 35 us and back 29 (5.7 and 6.8 TB/s; a large
-// copy reaches 5.3), 11008 x 4096 in blocks of 128 x 128 23 and 20 (6.0 and 6.6), 13 x 4096 2.3 and 2.2, which is a launch.
+// Bound by memory: 16 lanes of 16 bytes hold a row of a block, so that a maximum over it is four lane moves.  8000 x 8192 in bf16, four tensors in turn, 38 us and back 38 (5.2 TB/s; a
+// large copy reaches 5.3), the same one again, parts of which the caches hold, 32 to 35 and 29; 11008 x 4096 in blocks of 128 x 128 again and again 23 and 20, 13 x 4096 2.3 and 2.2, which is a launch.
 #pragma once
 #include "kv_cache.hip.h"
 
