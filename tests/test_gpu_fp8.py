@@ -288,6 +288,35 @@ def test_product_layouts():
     assert torch.equal(ops().matmul_fp8(one, w, ws), ops().matmul_fp8(one.contiguous(), w, ws))
 
 
+def test_single_rows_of_any_stride():
+    """A row of adjacent elements, whatever its view's stride says: of x, of codes and of a weight with one feature."""
+    k = 4096
+    w, ws = (t.cuda() for t in weight(256, k, seed=2))
+    x = randn(1, k, seed=3, dtype=torch.float16).cuda()
+    x8, xs = ops().quantize_fp8(x)
+
+    def views(t):
+        far = torch.zeros(1, (1 << 25) // k + 4, k, dtype=torch.uint8, device="cuda").view(torch.uint8)
+        raw = t.view(torch.uint8) if t.dtype == E4M3 else None
+        if raw is None:
+            far = torch.zeros(1, (1 << 25) // k + 4, k, dtype=t.dtype, device="cuda")
+            far[:, -1] = t
+            return t, far[:, -1], t.reshape(k, 1).t(), t.as_strided((1, k), (24, 1))
+        far[:, -1] = raw
+        return t, far.view(E4M3)[:, -1], raw.reshape(k, 1).t().view(E4M3), raw.as_strided((1, k), (24, 1)).view(E4M3)
+
+    want, one = ops().matmul_fp8(x, w, ws), ops().matmul_fp8(x, w[:1], ws[:1])
+    assert torch.equal(one, want[:, :1])
+    for view in views(x):
+        assert view.stride(1) == 1 and torch.equal(ops().matmul_fp8(view, w, ws), want)
+        codes, scales = ops().quantize_fp8(view)
+        assert torch.equal(codes.view(torch.uint8), x8.view(torch.uint8)) and torch.equal(scales, xs)
+    for view in views(x8):
+        assert torch.equal(ops().matmul_fp8(view, w, ws, x_scale=xs, dtype=torch.float16), want) and torch.equal(ops().dequantize_fp8(view, xs), ops().dequantize_fp8(x8, xs))
+    for view in views(w[:1].clone()):
+        assert torch.equal(ops().matmul_fp8(x, view, ws[:1]), one)
+
+
 def test_product_without_tokens_or_features():
     w, ws = (t.cuda() for t in weight(130, 256))
     assert ops().matmul_fp8(torch.zeros(0, 256, dtype=torch.float16, device="cuda"), w, ws).shape == (0, 130)

@@ -80,7 +80,8 @@ def matmul_fp8(x, weight, weight_scale, x_scale, dtype):
         raise RuntimeError(f"weight must be [features, elements] in torch.float8_e4m3fn, got {tuple(weight.shape)} in {weight.dtype}")
     m, k = weight.shape
     _width("weight", k)
-    if m and (weight.stride(1) != 1 or not 0 <= weight.stride(0) <= 1 << 24 or weight.stride(0) % 16 or weight.data_ptr() % 16 or weight.is_neg()):
+    w_stride = weight.stride(0) if m > 1 else k                        # (a single row's may be any number)
+    if m and (weight.stride(1) != 1 or not 0 <= w_stride <= 1 << 24 or w_stride % 16 or weight.data_ptr() % 16 or weight.is_neg()):
         raise RuntimeError(f"weight's rows must be of adjacent elements, start on 16 bytes and lie up to 2^24 elements apart, got strides {weight.stride()}")
     weight_scale = _scales("weight_scale", weight_scale, _blocks(m), k)
     codes = x.dtype == torch.float8_e4m3fn
@@ -105,6 +106,6 @@ def matmul_fp8(x, weight, weight_scale, x_scale, dtype):
     nbytes = _ffi.lib().triteia_hip_fp8_scratch_bytes(tokens, m, k, x_type)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
     _check(_ffi.lib().triteia_hip_fp8_matmul(
-        _ffi.ptr(x), x.stride(0), x_type, _ffi.ptr(x_scale), *(x_scale.stride() if codes else (0, 0)), _ffi.ptr(weight), weight.stride(0), _ffi.ptr(weight_scale),
+        _ffi.ptr(x), x.stride(0), x_type, _ffi.ptr(x_scale), *(x_scale.stride() if codes else (0, 0)), _ffi.ptr(weight), w_stride, _ffi.ptr(weight_scale),
         *weight_scale.stride(), _ffi.ptr(out), _TYPES[dtype], tokens, m, k, _ffi.ptr(scratch), nbytes, _ffi.device_index(x), _ffi.stream_of(x)))
     return out
