@@ -1,6 +1,7 @@
 """A trace follows torch's operations.  A kernel launched beside them leaves it an output that nothing fills, so every op refuses to be recorded into one."""
 import pytest
 import torch
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from triteia_amd.python import capi, ops
 
@@ -40,5 +41,7 @@ CALLS = {
 def test_no_op_is_recorded_into_a_trace(name):
     with pytest.raises(RuntimeError, match="trace"):
         torch.jit.trace(CALLS[name], (x,), check_trace=False)
+    with pytest.raises(RuntimeError, match="trace"):
+        make_fx(CALLS[name])(x)
     with pytest.raises(RuntimeError, match="GPU tensor"):              # the same call outside of one
         CALLS[name](x)

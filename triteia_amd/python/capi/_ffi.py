@@ -135,9 +135,9 @@ def ptr(t):
 
 
 def require_no_trace():
-    """torch.jit.trace records torch's operations: of a kernel launched beside them it would keep the empty output."""
-    if torch.jit.is_tracing():
-        raise RuntimeError("this op launches a kernel of its own, which a trace does not record: call it outside of torch.jit.trace (or capture a graph)")
+    """torch.jit.trace and make_fx record torch's operations: of a kernel launched beside them they would keep the empty output."""
+    if torch.jit.is_tracing() or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise RuntimeError("this op launches a kernel of its own, which a trace does not record: call it outside of torch.jit.trace and make_fx (or capture a graph)")
 
 
 def require_gpu(**tensors):
