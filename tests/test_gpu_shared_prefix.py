@@ -199,6 +199,38 @@ def test_prompts_between_requests_of_few_tokens(kind, dtype, heads, kv_heads, di
     assert len(few) < 2 or sum(joins) >= 2, joins
 
 
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("groups", [BETWEEN, PACKED], ids=["between", "packed"])
+def test_plan_and_scratch_of_nan_with_prompts(kind, groups):
+    """What a plan or a kernel reads without its having been written shows: both begin as NaN, and as the plan's largest numbers; twice, with the same bits."""
+    from triteia_amd.python.capi import _ffi
+    batch = Shared(groups, 8, 2, 128, 16, kind, padding=9)
+    q, cache, pages, starts, lens = batch.inputs()
+    at = batch.groups()
+    sizes = (len(batch.lengths), len(batch.prefix_lens), q.shape[0], 8, 2)
+    lib, most, where = _ffi.lib(), 666, (_ffi.device_index(q), _ffi.stream_of(q))
+    plan_bytes, nbytes = lib.triteia_hip_shared_plan_bytes(*sizes, most), lib.triteia_hip_shared_scratch_bytes(*sizes, most, cache.dim)
+    outs = []
+    for fill in (0xff, 0x7f):
+        out, scratch, plan = (torch.full_like(q, math.nan), *(torch.full((n,), fill, dtype=torch.uint8, device="cuda") for n in (nbytes, plan_bytes)))
+        codes = [lib.triteia_hip_shared_plan(_ffi.ptr(starts), _ffi.ptr(lens), _ffi.ptr(at["group_starts"]), _ffi.ptr(at["prefix_lens"]), *sizes, most, 1, 0, _ffi.ptr(plan), plan_bytes, *where),
+                 lib.triteia_hip_shared_attention(
+                     _ffi.ptr(q), q.stride(0), q.stride(1), _ffi.ptr(out), *cache._pointers(), cache._strides, cache.n_pages, cache.page, cache.kind, _ffi.ptr(pages), pages.stride(0),
+                     pages.shape[1], _ffi.ptr(plan), plan_bytes, *sizes, cache.dim, most, 1, 0, cache.dim ** -0.5, _ffi.ptr(scratch), nbytes, 0, *where)]
+        assert codes == [0, 0], _ffi.last_error()
+        outs.append(out)
+    batch.check(outs[0])
+    assert torch.equal(*outs)
+
+
+def test_prompts_in_hundreds_of_groups():
+    groups = [(1024, [(1, 1 + i % 30), (65 + i % 7, 65 + i % 40), (1 + i % 3, 9)]) for i in range(400)]
+    batch = Shared(groups, 1, 1, 64, 64)
+    joins = batch.plan(1).buffer.view(torch.int32)[[1, 3, 5]].tolist()
+    assert joins[0] >= 800, joins
+    batch.check(batch.attend(1))
+
+
 def test_prompts_that_come_and_go_between_replays():
     """Which sequences are prompts is the device's to say: one graph, whose offsets change between replays."""
     batch = Shared([(700, [(1, 100), (170, 200), (2, 100), (1, 100), (166, 200), (3, 100)]), (900, [(1, 100), (1, 100), (180, 200), (1, 100)])], 4, 2, 64, 16)

@@ -270,7 +270,7 @@ __global__ __launch_bounds__(SHARED ? 192 : kAttnPlanThreads) void attention_pla
         atomicAdd(&groups.saved, (unsigned long long)(groups.few[g] - 1) * (prefix / kAttnBlock) * a.kv_heads);
         atomicAdd(&groups.rows, (unsigned long long)count[b] * a.group * a.kv_heads);
         atomicMax(&groups.longest, prefix / kAttnBlock);
-        if ((long)count[b] * a.group > kAttnPrefixRows) atomicAdd(&groups.wide, (count[b] * a.group + kAttnTileRows - 1) / kAttnTileRows);
+        if (count[b] * a.group > kAttnPrefixRows || start[b] < 0) atomicAdd(&groups.wide, (count[b] * a.group + kAttnTileRows - 1) / kAttnTileRows);
       }
     }
     __syncthreads();
