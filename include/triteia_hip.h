@@ -394,7 +394,7 @@ TRITEIA_HIP_API int triteia_hip_paged_attention(const void* q, long q_token, lon
 /* The same for sequences in groups that share their first tokens: group g is sequences group_starts[g] .. group_starts[g + 1] - 1 (int32 [n_groups + 1], ascending;
  * sequences ahead of the first and behind the last are in none), whose rows of `pages` name the same pages for the first prefix_lens[g] tokens (int32 [n_groups]).  Of
  * those, the tokens that all rows of a group see are read and multiplied once for all of the group; prompts (sequences of more than 256 new tokens times heads / kv_heads,
- * of more than 64 where those between have more than 4096 together) are no part of that and go through their whole context.  Any prefix_lens are right as long as the pages are the same;
+ * of more than 64 where those between have more than 6144 together) are no part of that and go through their whole context.  Any prefix_lens are right as long as the pages are the same;
  * with a window nothing is shared.  Up to 1024 groups, n_seqs + n_groups up to 4096.  A plan, and the call on it, with the same n_groups. */
 TRITEIA_HIP_API size_t triteia_hip_shared_plan_bytes(int n_seqs, int n_groups, int n_tokens, int heads, int kv_heads, int max_q);
 TRITEIA_HIP_API size_t triteia_hip_shared_scratch_bytes(int n_seqs, int n_groups, int n_tokens, int heads, int kv_heads, int max_q, int dim);

@@ -173,13 +173,13 @@ BETWEEN = [(1000, [(1, 30), (100, 120), (2, 5), (1, 1), (300, 310), (70, 70), (0
 PACKED = [(1024, [(15, 20), (270, 270), (16, 16), (14, 90), (90, 91), (64, 70), (64, 64), (1, 1), (99, 99), (260, 300), (60, 60)]), (700, [(64, 64), (666, 670), (64, 64), (1, 1)])]
 
 
-@pytest.mark.parametrize("many", [19, 20])
+@pytest.mark.parametrize("many", [29, 30])
 def test_sequences_of_some_rows_share_while_they_are_few(many):
-    """Sequences of 65 to 256 rows are in the prefix as long as they have 4096 rows together."""
+    """Sequences of 65 to 256 rows are in the prefix as long as they have 6144 rows together."""
     some = [(210, 220 + i) for i in range(many)]
     batch = Shared([(768, [*some[:9], (1, 9), (1, 200), (0, 3), (3, 3), (2, 2), *some[9:]])], 2, 2, 64, 64)
     counts = batch.plan(210).buffer.view(torch.int32)[:6].tolist()
-    assert counts[1] == 4 and (counts[4] > 0) == (many == 20), counts           # (a prefix of 7 rows is in the list of long walks, one of thousands among the tiles)
+    assert counts[1] == 4 and (counts[4] > 0) == (many == 30), counts           # (a prefix of 7 rows is in the list of long walks, one of thousands among the tiles)
     for most in (1, 210):
         batch.check(batch.attend(most))
 

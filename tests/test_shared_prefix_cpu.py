@@ -58,10 +58,10 @@ def test_sizes():
 @pytest.mark.parametrize("heads,kv_heads", [(64, 8), (32, 32), (32, 4), (20, 1)])
 @pytest.mark.parametrize("seqs,groups", [(1, 1), (8, 1), (16, 3), (64, 1), (200, 20)])
 def test_scratch_of_prompts(heads, kv_heads, seqs, groups):
-    """Prompts share nothing, and no number of their tokens takes more: beside the scratch without groups there is that of the rows that may share, 64 a sequence and 4096, in tiles of 128, and of
+    """Prompts share nothing, and no number of their tokens takes more: beside the scratch without groups there is that of the rows that may share, 64 a sequence and 6144, in tiles of 128, and of
     the tiles that a sequence or a group leaves part empty, each for the rows themselves and for the prefix."""
     lib, dim, group = _ffi.lib(), 128, heads // kv_heads
-    rows = 64 * seqs + 4096
+    rows = 64 * seqs + 6144
     tiles = 2 * rows // 128 + 2 * (seqs + groups + 1)
     allowed = 4 * kv_heads * (dim + 2) * (128 * tiles + 48 * (seqs + groups + 1)) + 2 * 1024 * 32 * (dim + 2) * 4
     for max_q in (1, 4096):

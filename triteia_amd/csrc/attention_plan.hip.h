@@ -33,7 +33,9 @@ constexpr int kAttnMaxSeqs = 4096;
 constexpr int kAttnMaxGroups = 1024;
 constexpr int kAttnSolo = 512;         // groups' sequences times heads of the cache above which each gets a wavefront
 constexpr int kAttnSharedRows = kAttnTileRows / 2;      // sequences of up to so many rows share a prefix,
-constexpr int kAttnMostRows = 2 * kAttnTileRows, kAttnMoreRows = 4096;      // and of up to so many, if those of more than kAttnSharedRows have so many together
+// and of up to so many, if those of more than kAttnSharedRows have so many together.  (us, in the prefix and not: 64 of 80 rows beside 64 of 8 behind 4096, 64 heads over 8, 178 and 217, 32 of 160 beside
+// 96 of 8 189 and 250; but 100 of 80 beside 100 of 4 behind 1500, 32 heads over 8, 175 and 146, and their scratch grows.)
+constexpr int kAttnMostRows = 2 * kAttnTileRows, kAttnMoreRows = 6144;
 constexpr int kAttnPrefixRows = 32;    // prefixes of up to so many rows are walked by all wavefronts of a workgroup
 constexpr int kAttnRowBlocks = 16;     // blocks of a share of few rows, at least
 constexpr int kAttnTileBlocks = 8;     // a share of a tile of 128 rows, at least
